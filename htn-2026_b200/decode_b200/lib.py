@@ -113,6 +113,17 @@ PROTOTYPES = {
     "qd_prefill_qk_rope_at": (c_int, [c_void_p, c_int64, c_int, c_int64, c_int64, c_int, c_int, c_void_p, c_void_p,
                                       c_float, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64,
                                       c_int64, c_int64, c_void_p]),
+    "qd_paged_rope_append": (c_int, [c_void_p, c_int64, c_int, c_int64, c_int, c_int, c_int, c_void_p, c_void_p,
+                                     c_float, c_void_p, c_void_p, c_int64, c_int64, c_int, c_void_p, c_void_p, c_int,
+                                     c_void_p, c_int64, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int,
+                                     c_int64, c_int64, c_void_p, c_int, c_void_p]),
+    "qd_paged_attn_plan": (c_int, [c_int, c_int, c_int, c_int, P_INT, P_I64]),
+    "qd_paged_attn": (c_int, [c_void_p, c_int64, c_int, c_int64, c_int, c_int, c_int, c_void_p, c_void_p, c_int64,
+                              c_int, c_int64, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int, c_float,
+                              c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p, c_int64, c_void_p, c_int,
+                              c_void_p]),
+    "qd_sample": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                          c_void_p, c_void_p, c_int, c_void_p]),
 }
 
 QD_OK, QD_ERR_ARG, QD_ERR_SCRATCH, QD_ERR_CUDA, QD_ERR_UNSUPPORTED = 0, 1, 2, 3, 4
@@ -120,7 +131,9 @@ QD_EPI_STORE, QD_EPI_RES, QD_EPI_SWIGLU, QD_EPI_SWIGLU_PACKED, QD_EPI_RES_SUMS, 
 DEVERR = {1: "wait for a weight block timed out", 2: "wait for a free ring slot timed out",
           4: "drain of in-flight copies timed out", 8: "token id out of range",
           16: "decode position outside the cache", 32: "a wait for another CTA's results timed out",
-          64: "dynamic shared memory misaligned (kernel did nothing)"}
+          64: "dynamic shared memory misaligned (kernel did nothing)",
+          128: "page outside the pool, or a request longer than its page table row"}
+QD_BF16, QD_FP16, QD_FP32 = 0, 1, 2
 
 
 class QDError(RuntimeError):

@@ -49,7 +49,15 @@ enum {
   QD_DEVERR_TOKEN = 8,
   QD_DEVERR_POS = 16,
   QD_DEVERR_DEP = 32,
-  QD_DEVERR_SMEM = 64 /* a kernel found its dynamic shared memory misaligned and did nothing */
+  QD_DEVERR_SMEM = 64, /* a kernel found its dynamic shared memory misaligned and did nothing */
+  QD_DEVERR_PAGE = 128 /* a page table names a page outside the pool, or a request outgrows its table row */
+};
+
+/* element types of the paged-cache and sampling entry points */
+enum {
+  QD_BF16 = 0,
+  QD_FP16 = 1,
+  QD_FP32 = 2
 };
 
 /* Library identification and the last error message of the calling thread. */
@@ -407,6 +415,71 @@ int qd_prefill_attn(const void* q, int64_t ldq, int batch, int64_t S, int64_t q_
 int qd_prefill_attn_rows(const void* q, int64_t ldq, int batch, int64_t S, int64_t q_begin, int nq_heads,
                          int nkv_heads, const void* k_cache, const void* v_cache, int64_t cap, int64_t cs_b,
                          int64_t cs_h, float scale, void* out, int64_t ldo, int* err, cudaStream_t stream);
+
+/* ---------------------------------------------------------------- paged K/V cache
+ * A ragged batch over a cache of pages (no counterpart in the reference, whose cache is one slab per
+ * sequence). Request i < batch has the token rows cu_tokens[i] .. cu_tokens[i + 1] - 1 of the token-major
+ * arrays (device int32 [batch + 1], ascending from 0; rows from cu_tokens[batch] on belong to nobody and
+ * are left alone) and, with them, kv_len[i] cached positions (device int32 [batch]): its new token j of n
+ * is at position kv_len[i] - n + j. Position p of request i is row p % page_size of page
+ * page_table[i * ld_table + p / page_size] (device int32, max_pages entries a row; entries past the last
+ * needed one are never read). The pools k_pages / v_pages hold [n_pages][nkv_heads][page_size][head_dim]
+ * elements of `dtype` (QD_BF16 or QD_FP16) at page stride ps_page and head stride ps_head (elements), rows
+ * contiguous. head_dim is 64 or 128; page_size 16, 32, 64 or 128; nq_heads a multiple of nkv_heads; every
+ * pointer 16-byte aligned and every stride of 16-bit elements a multiple of 8.
+ *
+ * qd_paged_rope_append: for every new token, from its row of qkv [tokens][(nq + 2 nkv) * head_dim] (row
+ * stride ldqkv):  q_out[t][h] = rope(norm(q_h)) (row stride ldq),  K row = rope(norm(k_h)),  V row = v_h
+ * with norm(x) = x * rsqrt(mean(x^2) + eps) * w (left out where q_norm, k_norm are null: both or none) and
+ * rope turning the pairs (x[r], x[r + rot_half]), r < rot_half, by the angle of the token's position; the
+ * elements from 2 * rot_half on pass through. cos / sin are fp32 [n_pos][rot_half] tables (row stride
+ * ld_cs, a multiple of 4); rot_half a multiple of 8 up to head_dim / 2. All arithmetic is fp32 and rounds
+ * once, on the store. A token whose position is negative or not below n_pos writes nothing and flags
+ * QD_DEVERR_POS in *err (err may be null); one whose page is not in the pool or whose position is past its
+ * table row writes q_out alone and flags QD_DEVERR_PAGE. */
+int qd_paged_rope_append(const void* qkv, int64_t ldqkv, int dtype, int64_t tokens, int nq_heads, int nkv_heads,
+                         int head_dim, const void* q_norm, const void* k_norm, float eps, const float* cos,
+                         const float* sin, int64_t ld_cs, int64_t n_pos, int rot_half, const int32_t* cu_tokens,
+                         const int32_t* kv_len, int batch, const int32_t* page_table, int64_t ld_table, int max_pages,
+                         void* q_out, int64_t ldq, void* k_pages, void* v_pages, int64_t n_pages, int page_size,
+                         int64_t ps_page, int64_t ps_head, int* err, int pdl, cudaStream_t stream);
+
+/* qd_paged_attn: causal grouped-query attention of every new token over its request's pages (the new
+ * tokens' own rows are already in them): for the token at position p, query head h and the keys
+ * 0 .. min(p, kv_len - 1) of KV head h / (nq / nkv),
+ *   out[t][h] = softmax(q k^T * scale) v   (row stride ldo),   lse[t][h] = log sum exp(q k^T * scale)
+ * (lse fp32, row stride ld_lse, may be null). A token that sees no key (kv_len smaller than the number of
+ * new tokens) gets zeros and lse = -inf. One call serves single tokens, chunks of a prompt and whole
+ * prompts side by side. Scores, softmax statistics and sums are fp32; probabilities are rounded to `dtype`
+ * before the product with V. Cache rows at and past kv_len are never used, whatever they hold. A request
+ * that outgrows its table row (kv_len > max_pages * page_size) is cut to it and flags QD_DEVERR_PAGE, as
+ * does a page outside the pool (its keys then read as zeros). qd_paged_attn_plan gives the grid
+ * (grid_hint <= 0: one CTA per SM) and the scratch size, which depend on neither batch nor lengths. */
+int qd_paged_attn_plan(int nq_heads, int nkv_heads, int head_dim, int grid_hint, int* grid, int64_t* scratch_bytes);
+int qd_paged_attn(const void* q, int64_t ldq, int dtype, int64_t tokens, int nq_heads, int nkv_heads, int head_dim,
+                  const void* k_pages, const void* v_pages, int64_t n_pages, int page_size, int64_t ps_page,
+                  int64_t ps_head, const int32_t* cu_tokens, const int32_t* kv_len, int batch,
+                  const int32_t* page_table, int64_t ld_table, int max_pages, float scale, void* out, int64_t ldo,
+                  float* lse, int64_t ld_lse, int grid, void* scratch, int64_t scratch_bytes, int* err, int pdl,
+                  cudaStream_t stream);
+
+/* ---------------------------------------------------------------- sampling
+ * One token per row of logits [rows][vocab] (QD_BF16, QD_FP16 or QD_FP32; row stride ld), drawn with the
+ * row's uniform number u in [0, 1). The tokens are ordered by logit, the largest first and equal logits by
+ * index; with m the largest logit, d = (l - m) * (1 / temperature), and the weight of a token is expf(d),
+ * rounded to a multiple of 2^-40 (so that sums of weights are exact and no order of addition matters). Kept are
+ *   the first top_k tokens                                           (top_k <= 0: all)
+ *   of them the fewest whose weights reach top_p of those tokens' sum (top_p >= 1: all; at least one)
+ *   of them those with d >= log(min_p)                               (min_p <= 0: all; min_p > 1 counts as 1)
+ * and the token drawn is the first, in order of index, at which the running sum of kept weights exceeds
+ * u * (their sum). logprob (may be null) = d - log(sum of the kept weights): the logarithm of the drawn
+ * token's share. temperature, top_k, top_p, min_p are device arrays with an entry per row; each may be
+ * null (temperature 1, the filter off). A temperature that is not at least 1e-5 (0, negative, NaN) takes
+ * the largest logit (the lowest index on ties), logprob 0. A NaN logit counts as -inf; +inf logits share
+ * the whole weight; a row with nothing above -inf gives token -1 and logprob -inf. vocab <= 2^18. */
+int qd_sample(const void* logits, int dtype, int64_t ld, int64_t rows, int64_t vocab, const float* temperature,
+              const int32_t* top_k, const float* top_p, const float* min_p, const float* u, int64_t* tok,
+              float* logprob, int pdl, cudaStream_t stream);
 
 #ifdef __cplusplus
 }

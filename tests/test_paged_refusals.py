@@ -1,0 +1,117 @@
+"""What the paged-cache and sampling entry points refuse, and with which code: host checks, so no GPU is
+needed (every call here must return before its launch). The wrappers' own checks of types and shapes are at
+the end."""
+
+import ctypes
+
+import pytest
+import torch
+
+P = 1 << 20  # stands for a 16-byte aligned device pointer: never dereferenced on the host
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from decode_b200 import build, lib as L
+
+    build.build()
+    return L.load()
+
+
+def _append_args(**kw):
+    a = dict(qkv=P, ldqkv=48 * 128, dtype=0, tokens=4, nq=32, nkv=8, dim=128, qn=P, kn=P, eps=1e-6, cos=P, sin=P, ld_cs=64,
+             n_pos=100, half=64, cu=P, kv=P, batch=2, table=P, ld_table=3, max_pages=3, q_out=P, ldq=4096, k=P, v=P, pages=9,
+             page=16, ps_page=8 * 16 * 128, ps_head=16 * 128, err=None, pdl=0, stream=None)
+    assert set(kw) <= set(a)
+    return list({**a, **kw}.values())
+
+
+def _attn_args(**kw):
+    a = dict(q=P, ldq=4096, dtype=0, tokens=4, nq=32, nkv=8, dim=128, k=P, v=P, pages=9, page=16, ps_page=8 * 16 * 128,
+             ps_head=16 * 128, cu=P, kv=P, batch=2, table=P, ld_table=3, max_pages=3, scale=0.1, out=P, ldo=4096, lse=P, ld_lse=32,
+             grid=148, scratch=P, bytes=1 << 40, err=None, pdl=0, stream=None)
+    assert set(kw) <= set(a)
+    return list({**a, **kw}.values())
+
+
+def _sample_args(**kw):
+    a = dict(logits=P, dtype=0, ld=1000, rows=2, vocab=1000, temperature=None, top_k=None, top_p=None, min_p=None, u=P, tok=P,
+             logprob=None, pdl=0, stream=None)
+    assert set(kw) <= set(a)
+    return list({**a, **kw}.values())
+
+
+SHARED = [({"dtype": 2}, 4), ({"dtype": 9}, 4), ({"dim": 96}, 4), ({"page": 24}, 4), ({"page": 256}, 4), ({"page": 0}, 4),
+          ({"nkv": 0}, 1), ({"nq": 30}, 1), ({"nq": 4}, 1), ({"batch": 0}, 1), ({"max_pages": 0}, 1), ({"ld_table": 2}, 1),
+          ({"pages": 0}, 1), ({"tokens": -1}, 1), ({"tokens": 1 << 31}, 1), ({"k": None}, 1), ({"v": P + 8}, 1), ({"cu": None}, 1),
+          ({"kv": None}, 1), ({"table": None}, 1), ({"ps_head": 1000}, 1), ({"ps_head": 2052}, 1), ({"ps_page": 17}, 1)]
+
+
+@pytest.mark.parametrize("change,code", SHARED + [
+    ({"qkv": None}, 1), ({"qkv": P + 2}, 1), ({"q_out": None}, 1), ({"ldqkv": 48 * 128 - 8}, 1), ({"ldqkv": 48 * 128 + 4}, 1),
+    ({"ldq": 4088}, 1), ({"kn": None}, 1), ({"qn": None}, 1), ({"qn": P + 4}, 1), ({"cos": None}, 1), ({"sin": P + 8}, 1),
+    ({"half": 4}, 1), ({"half": 12}, 1), ({"half": 72}, 1), ({"ld_cs": 32}, 1), ({"ld_cs": 66}, 1), ({"n_pos": 0}, 1)])
+def test_append_refuses(lib, change, code):
+    assert lib.qd_paged_rope_append(*_append_args(**change)) == code, change
+    assert lib.qd_last_error()
+
+
+@pytest.mark.parametrize("change,code", SHARED + [
+    ({"q": None}, 1), ({"q": P + 2}, 1), ({"out": None}, 1), ({"out": P + 8}, 1), ({"ldq": 4095}, 1), ({"ldo": 4088}, 1),
+    ({"ld_lse": 31}, 1), ({"scale": 0.0}, 1), ({"scale": float("nan")}, 1), ({"grid": 0}, 2), ({"scratch": None}, 2),
+    ({"bytes": 8}, 2)])
+def test_attention_refuses(lib, change, code):
+    assert lib.qd_paged_attn(*_attn_args(**change)) == code, change
+    assert lib.qd_last_error()
+
+
+@pytest.mark.parametrize("change,code", [
+    ({"dtype": 3}, 4), ({"logits": None}, 1), ({"u": None}, 1), ({"tok": None}, 1), ({"rows": -1}, 1), ({"vocab": 0}, 1),
+    ({"ld": 999}, 1), ({"vocab": (1 << 18) + 1, "ld": 1 << 19}, 4), ({"logits": P + 1}, 1), ({"dtype": 2, "logits": P + 2}, 1)])
+def test_sample_refuses(lib, change, code):
+    assert lib.qd_sample(*_sample_args(**change)) == code, change
+    assert lib.qd_last_error()
+
+
+def test_nothing_to_do_is_not_an_error(lib):
+    assert lib.qd_paged_rope_append(*_append_args(tokens=0)) == 0
+    assert lib.qd_paged_attn(*_attn_args(tokens=0)) == 0
+    assert lib.qd_sample(*_sample_args(rows=0)) == 0
+
+
+def test_attention_plan(lib):
+    grid, nbytes = ctypes.c_int(0), ctypes.c_int64(0)
+    assert lib.qd_paged_attn_plan(32, 8, 128, 5, ctypes.byref(grid), ctypes.byref(nbytes)) == 0
+    assert grid.value == 5 and nbytes.value > 0
+    assert lib.qd_paged_attn_plan(32, 7, 128, 0, ctypes.byref(grid), ctypes.byref(nbytes)) == 4
+    assert lib.qd_paged_attn_plan(32, 8, 80, 0, ctypes.byref(grid), ctypes.byref(nbytes)) == 4
+    assert lib.qd_paged_attn_plan(32, 8, 128, 0, None, ctypes.byref(nbytes)) == 1
+
+
+def test_wrappers_refuse_cpu_tensors_and_wrong_types():
+    from decode_b200 import paged, sample
+
+    k, v = paged.new_pools(3, 2, 16, 128, "cpu")
+    cu, kv, table = torch.tensor([0, 1], dtype=torch.int32), torch.tensor([1], dtype=torch.int32), torch.zeros((1, 1), dtype=torch.int32)
+    cos, sin = paged.rope_table(4, 128, 1e4, "cpu")
+    qkv, q = torch.zeros((1, 8 * 128), dtype=torch.bfloat16), torch.zeros((1, 4, 128), dtype=torch.bfloat16)
+    with pytest.raises(AssertionError):
+        paged.rope_append(qkv, cu, kv, table, 4, 2, cos, sin, q, k, v)
+    with pytest.raises(AssertionError):
+        paged.rope_append(qkv.float(), cu, kv, table, 4, 2, cos, sin, q, k, v)
+    with pytest.raises(AssertionError):
+        sample.sample(torch.zeros((1, 10)), torch.zeros((1,)), torch.zeros((1,), dtype=torch.int64))
+    with pytest.raises(AssertionError):
+        sample.sample(torch.zeros((1, 10), dtype=torch.float64), torch.zeros((1,)), torch.zeros((1,), dtype=torch.int64))
+
+
+def test_rope_table_is_the_angles_in_64_bits():
+    from decode_b200 import paged
+
+    cos, sin = paged.rope_table(70000, 128, 5e6, "cpu")
+    assert cos.shape == (70000, 64) and cos.dtype == torch.float32
+    p, r = 69999, 3
+    angle = p * 5e6 ** (-2 * r / 128)
+    import math
+
+    assert abs(float(cos[p, r]) - math.cos(angle)) < 1e-7 and abs(float(sin[p, r]) - math.sin(angle)) < 1e-7
