@@ -47,7 +47,7 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __gr
 
   const int i = warp_find_request(a.b.cu, a.b.batch, (int)t, lane);
   if (i >= a.b.batch) return;  // a row that belongs to no request
-  const int pos = __ldg(a.b.kv_len + i) - __ldg(a.b.cu + i + 1) + (int)t;
+  const int pos = ld_i32(a.b.kv_len + i) - ld_i32(a.b.cu + i + 1) + (int)t;
   if (pos < 0 || pos >= a.n_pos) {
     if (lane == 0) flag_error(a.b.err, QD_DEVERR_POS);
     return;
@@ -57,7 +57,7 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __gr
     dst = a.q_out + (t * a.ldq + (int64_t)h * D) * 2;
   } else {
     const int entry = pos >> a.b.page_shift;
-    const int page = entry < a.b.max_pages ? __ldg(a.b.table + i * a.b.ld_table + entry) : -1;
+    const int page = entry < a.b.max_pages ? ld_i32(a.b.table + i * a.b.ld_table + entry) : -1;
     const bool in = page >= 0 && page < a.b.n_pages;
     if (!in && c == 0) flag_error(a.b.err, QD_DEVERR_PAGE);
     const int kvh = h < a.b.nq + a.b.nkv ? h - a.b.nq : h - a.b.nq - a.b.nkv;

@@ -27,6 +27,7 @@ template <typename T>
 struct Elem;
 template <>
 struct Elem<__nv_bfloat16> {
+  static constexpr bool kBf16 = true;
   static __device__ __forceinline__ float2 unpack(uint32_t u) { return make_float2(bf_lo(u), bf_hi(u)); }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
@@ -35,6 +36,7 @@ struct Elem<__nv_bfloat16> {
 };
 template <>
 struct Elem<__half> {
+  static constexpr bool kBf16 = false;
   static __device__ __forceinline__ float2 unpack(uint32_t u) {
     return __half22float2(*reinterpret_cast<const __half2*>(&u));
   }
@@ -43,6 +45,9 @@ struct Elem<__half> {
     return *reinterpret_cast<const uint32_t*>(&v);
   }
 };
+
+// The batch's arrays may come from the kernel before: L2 loads, never moved above the wait for it.
+__device__ __forceinline__ int ld_i32(const int32_t* p) { return __ldcg(p); }
 
 __device__ __forceinline__ void flag_error(int* err, int code) {
   if (err) atomicOr(err, code);
@@ -56,7 +61,7 @@ __device__ __forceinline__ int warp_find_request(const int32_t* cu, int batch, i
   while (n > 0) {
     const int step = (n + 31) >> 5;
     const int i = lo + (lane + 1) * step;  // cu[i] <= t: at least i requests end at or before t
-    const bool past = i <= lo + n && __ldg(cu + i) <= t;
+    const bool past = i <= lo + n && ld_i32(cu + i) <= t;
     const int k = __popc(__ballot_sync(0xffffffffu, past));
     const int end = lo + n;
     lo += k * step;
