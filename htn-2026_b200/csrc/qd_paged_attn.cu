@@ -2,15 +2,22 @@
 //
 // Rows. The query heads of one KV head share its keys, so a tile of 128 MMA rows holds tpt = 128 / group
 // tokens x group heads (row = token * group + head), and a work unit is (request, tile pair, KV head): up to
-// two such tiles (A, B) that read the same key blocks. A single token fills one tile's first group rows.
-// Per block of 128 keys, for each tile x:
+// two such tiles (A, B) that read the same key blocks. Per block of 128 keys, for each tile x:
 //   S_x = Q_x K^T   tcgen05.mma M = 128 rows, N = 128 keys, fp32 in tensor memory
 //   softmax         a warpgroup per tile, thread = row: running maximum and sum in fp32,
 //                   P = exp2(s * scale * log2 e - m) written over S_x as 16-bit pairs
 //   O_x += P_x V    M = 128 rows, N = head_dim, P from tensor memory, V an MN-major operand
-// While one warpgroup turns its S into P the tensor cores run the other tile's products. The maximum only
-// moves when a row's grows by more than 2^8 (then the warp rescales O_x in tensor memory): O / l does not
-// depend on which maximum is used, and 2^8 leaves the fp32 sums and the 16-bit P far from overflow.
+// While one warpgroup turns its S into P the tensor cores run the other tile's products. A unit of one tile
+// keeps both busy too: A takes its even blocks, B its odd ones, and A's warps add O_B to O_A at the end, each
+// with its own maximum. The maximum only moves when a row's grows by more than 2^8 (then the warp rescales
+// O_x in tensor memory): O / l does not depend on which maximum is used, and 2^8 leaves the fp32 sums and the
+// 16-bit P far from overflow.
+//
+// Few rows. With at most 16 rows (a single token of up to 16 heads a group, or a few tokens) most of a
+// 128-row tile would be exponentials of nothing, so the products are turned round: S^T = K Q^T (M = 128
+// keys, N = 16 rows) puts a key in every thread, which has one score per row to deal with; the rows' maxima
+// are reduced over the warpgroup, P goes to shared memory as the K-major operand of O^T += V^T P^T (M =
+// head_dim, N = 16 rows). Even and odd blocks alternate between the warpgroups as above.
 //
 // Keys and values come page by page: a box of a page's rows x 64 dims per copy (TMA, 128-byte swizzle), the
 // lanes of the producer warp issuing one each, into a ring of slots that K and V blocks take in turn. Rows
@@ -22,6 +29,8 @@
 // leaves fp32 partials (O, m, l) in the scratch, and the CTA that finishes last (a ticket per cut unit)
 // joins them in the order of the keys, so results repeat bit for bit. Every CTA finds its place on the line
 // from cu_tokens and kv_len itself: no planning launch, and no length is needed on the host.
+#include <climits>
+
 #include "qd_host.h"
 #include "qd_paged_dev.cuh"
 #include "qd_umma.cuh"
@@ -33,15 +42,17 @@ constexpr int kPgThreads = 384;  // warps 0-3 softmax A, 4-7 softmax B, 8 produc
 constexpr int kPgSoftmaxRegs = 208, kPgOtherRegs = 88;
 constexpr int kPgKeys = 128;     // keys per block
 constexpr int kPgBox = 128 * 128;  // [128 rows][64 dims] of 16 bits
+constexpr int kFewRows = 16;       // rows of a few-row unit (MMA N)
+constexpr int kFewP = 2 * kFewRows * 128;  // its P: 2 halves of 64 keys x 16 rows of 128 B
 constexpr int kPgUnitCost = 1;     // a unit's fixed cost (Q, epilogue) in key blocks, for the split
 
 struct alignas(64) PagedAttnArgs {
-  CUtensorMap tq, tq1, tk, tv;  // tq: a whole tile's rows; tq1: one token's
+  CUtensorMap tq, tqf, tq1, tk, tv;  // q boxes: a whole tile's tokens, as many as make 16 rows, one
   PagedBatch b;
   char* out;
   float* lse;
   int64_t ldo, ld_lse;
-  int group, tpt;            // heads per KV head, tokens per tile
+  int group, tpt, tpf;        // heads per KV head, tokens per tile and per 16 rows (0: a group is larger)
   int period, period_blocks;  // ceil sums over tile pairs repeat every `period` pairs, `period_blocks` blocks on
   float scale_log2;
   float* partials;  // [2 * grid slots][2 tiles][D / 4][128] float4, then [slots][2][128] float2
@@ -54,13 +65,22 @@ struct PgLayout {
   static constexpr int kSlots = D == 128 ? 5 : 10;
   static constexpr int q = 0;
   static constexpr int kv = q + 2 * kItem;
-  static constexpr int bars = kv + kSlots * kItem;
-  // qfull[2], qempty[2], sfull[2], pfull[2], odone[2], ofree[2], group[2], segfull[4], segempty[4],
+  static constexpr int p = kv + kSlots * kItem;  // P of few-row units (head_dim 128: in their Q region)
+  static constexpr int bars = p + (D == 64 ? 2 * kFewP : 0);
+  // qfull[2], qempty[2], sfull[2], pfull[2], odone[2], ofree[2], group[2], segfull[4], segempty[4], join, -,
   // full[slots], empty[slots]
-  static constexpr int nbars = 22 + 2 * kSlots;
+  static constexpr int nbars = 24 + 2 * kSlots;
   static constexpr int seg = bars + nbars * 8;  // segment ring
   static constexpr int misc = seg + 4 * 64;     // tmem slot, abort, line start, flags, drain counts
-  static constexpr int total = misc + 192;
+  static constexpr int ml = misc + 192;         // at a unit's end: (m, l) of the odd blocks' rows [128], or the
+                                                // warps' sums of few-row units [2 groups][16 rows][4 warps]
+  static constexpr int mx = ml + 1024;          // the warps' maxima of few-row units [2 groups][16][4]
+  static constexpr int mb = mx + 1024;          // the odd blocks' maxima of few-row units [16]
+  static constexpr int total = mb + 128;
+  // where warpgroup x's P of a few-row unit in Q region `reg` is: Q takes the first 4 KiB of each 64-dim half
+  static __device__ __forceinline__ int few_p(int reg, int x) {
+    return D == 128 ? q + reg * kItem + 4096 + x * kPgBox : p + x * kFewP;
+  }
 };
 
 // A CTA's piece of a unit: what every warp needs to know of it.
@@ -68,6 +88,7 @@ struct PgSeg {
   int row0, ntok, pos0, kv;  // first token row, tokens, the first's position, keys of the request
   int head, j0, nb;          // KV head, first key block, blocks; nb = 0 ends the CTA's list
   int whole;                 // this piece is the whole unit (no partials)
+  int few;                   // one tile of at most 16 rows
   int slot, c0, nc;          // partial slot, first CTA and number of CTAs of the unit
   int region;                // Q region of a single tile, or -1: both tiles
 };
@@ -90,6 +111,39 @@ __device__ __forceinline__ float pg_ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
+}
+
+template <int N>
+struct Const {
+  static constexpr int value = N;
+};
+
+// maximum over the warp (NaN where a lane has one only if all have)
+__device__ __forceinline__ float redux_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ void tmem_wait_ld8(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])::"memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n"
+      "tcgen05.wait::st.sync.aligned;" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16};\n"
+      "tcgen05.wait::st.sync.aligned;" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
 }
 
 // One request on the line of key blocks.
@@ -117,20 +171,99 @@ __device__ __forceinline__ int pg_blocks(const PagedAttnArgs& a, const PgReq& r,
 }
 // sum of pg_blocks over the request's pairs. Where nothing is cut the terms are ceil((pos0 + 2 tpt k) / 128),
 // which grow by period_blocks every `period` pairs: one pass over a period suffices.
-__device__ __forceinline__ int64_t pg_sum_blocks(const PagedAttnArgs& a, const PgReq& r) {
-  if (r.pairs == 0) return 0;
-  if (r.pairs == 1) return pg_blocks(a, r, 0);
-  int64_t sum = 0;
+__device__ __forceinline__ int pg_sum_blocks(const PagedAttnArgs& a, const PgReq& r) {
+  if (r.pairs <= 1) return r.pairs ? pg_blocks(a, r, 0) : 0;
+  int sum = 0;
   if (r.pos0 >= 0 && r.kv == r.pos0 + r.n) {
     const int m = r.pairs - 1, q = m / a.period, rest = m - q * a.period;
+#pragma unroll 1
     for (int j = 1; j <= min(a.period, m); ++j) {
-      const int64_t cnt = q + (j <= rest);
+      const int cnt = q + (j <= rest);
       sum += cnt * ((r.pos0 + 2 * a.tpt * j + kPgKeys - 1) / kPgKeys) + a.period_blocks * (cnt * (cnt - 1) / 2);
     }
     return sum + pg_blocks(a, r, m);
   }
+#pragma unroll 1
   for (int k = 0; k < r.pairs; ++k) sum += pg_blocks(a, r, k);
   return sum;
+}
+// The line of `total` places over `ctas` CTAs: the first total % ctas take one more than the others.
+struct PgLine {
+  unsigned total, ctas, each, more;
+  __device__ __forceinline__ unsigned begin(unsigned c) const { return c * each + min(c, more); }
+  __device__ __forceinline__ unsigned owner(unsigned at) const {
+    const unsigned big = more * (each + 1);
+    return at < big ? at / (each + 1) : more + (at - big) / each;
+  }
+};
+
+// Joins a cut unit's pieces of one tile (x): 128 threads, thread r. kItems float4 of the output at a time, with
+// kPieces pieces' loads in flight for each. Out of line: it keeps its registers out of the main loop's way.
+template <typename T, int D, int kItems, int kPieces>
+__device__ __forceinline__ void pg_join_items(const PagedAttnArgs& a, const PgSeg& g, int x, int r, int rows, int t0) {
+  const float4* const po = reinterpret_cast<const float4*>(a.partials);
+  const float2* const pm = reinterpret_cast<const float2*>(a.partials + (int64_t)2 * gridDim.x * 2 * D * 128);
+  const int total = rows * (D / 4);
+#pragma unroll 1
+  for (int e0 = r; e0 < total; e0 += 128 * kItems) {
+    int row[kItems], c4[kItems];
+    float M[kItems], L[kItems];
+    float4 acc[kItems];
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      const int e = min(e0 + 128 * i, total - 1);
+      c4[i] = e / rows;
+      row[i] = e - c4[i] * rows;
+      M[i] = -INFINITY;
+      L[i] = 0.f;
+      acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll 1
+    for (int q0 = 0; q0 < g.nc; q0 += kPieces) {
+      float2 ml[kPieces][kItems];
+      float4 v[kPieces][kItems];
+#pragma unroll
+      for (int q = 0; q < kPieces; ++q) {
+        const int qq = min(q0 + q, g.nc - 1);  // past the last piece: the last again, not counted
+        const int64_t slot = (2 * (g.c0 + qq) + (qq == 0 ? 1 : 0)) * 2 + x;
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) {
+          ml[q][i] = __ldcg(pm + slot * 128 + row[i]);
+          v[q][i] = __ldcg(po + (slot * (D / 4) + c4[i]) * 128 + row[i]);
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < kPieces; ++q)
+#pragma unroll
+        for (int i = 0; i < kItems; ++i)
+          if (q0 + q < g.nc && ml[q][i].y > 0.f) {  // a piece in which the row saw no key counts for nothing
+            const float mn = fmaxf(M[i], ml[q][i].x), fa = exp2f(M[i] - mn), fb = exp2f(ml[q][i].x - mn);
+            M[i] = mn;
+            L[i] = L[i] * fa + ml[q][i].y * fb;
+            acc[i].x = acc[i].x * fa + v[q][i].x * fb;
+            acc[i].y = acc[i].y * fa + v[q][i].y * fb;
+            acc[i].z = acc[i].z * fa + v[q][i].z * fb;
+            acc[i].w = acc[i].w * fa + v[q][i].w * fb;
+          }
+    }
+#pragma unroll
+    for (int i = 0; i < kItems; ++i)
+      if (e0 + 128 * i < total) {
+        const float inv = L[i] > 0.f ? 1.0f / L[i] : 0.f;
+        const int tok = row[i] / a.group, t2 = g.row0 + t0 + tok, h2 = g.head * a.group + row[i] - tok * a.group;
+        *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + t2 * a.ldo + (int64_t)h2 * D + 4 * c4[i]) =
+            make_uint2(Elem<T>::pack(acc[i].x * inv, acc[i].y * inv), Elem<T>::pack(acc[i].z * inv, acc[i].w * inv));
+        if (c4[i] == 0 && a.lse)
+          a.lse[t2 * a.ld_lse + h2] = L[i] > 0.f ? (M[i] + __log2f(L[i])) * 0.69314718055994531f : -INFINITY;
+      }
+  }
+}
+template <typename T, int D>
+__device__ __noinline__ void pg_join(const PagedAttnArgs& a, const PgSeg& g, int x, int r, int rows, int t0) {
+  if (rows * (D / 4) > 256)
+    pg_join_items<T, D, 8, 2>(a, g, x, r, rows, t0);
+  else
+    pg_join_items<T, D, 1, 8>(a, g, x, r, rows, t0);
 }
 
 template <typename T, int D>
@@ -153,12 +286,13 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
   auto group = [&](int x) { return bars + 96 + 8u * x; };
   auto segfull = [&](int k) { return bars + 112 + 8u * (k & 3); };
   auto segempty = [&](int k) { return bars + 144 + 8u * (k & 3); };
-  auto full = [&](int s) { return bars + 176 + 8u * s; };
-  auto empty = [&](int s) { return bars + 176 + 8u * (kSlots + s); };
+  const uint32_t join = bars + 176;
+  auto full = [&](int s) { return bars + 192 + 8u * s; };
+  auto empty = [&](int s) { return bars + 192 + 8u * (kSlots + s); };
   PgSeg* segs = reinterpret_cast<PgSeg*>(smem + Lay::seg);
   int* misc = reinterpret_cast<int*>(smem + Lay::misc);
   int* abort = misc + 1;
-  int64_t* scan = reinterpret_cast<int64_t*>(misc + 16);  // warp totals [12]
+  int* scan = misc + 16;  // warp totals [12]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   constexpr int unit_cost = kPgUnitCost;
   if (tid == 0) {
@@ -171,6 +305,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
       mbar_init(ofree(x), 4);
       mbar_init(group(x), 4);
     }
+    mbar_init(join, 4);
     for (int k = 0; k < 4; ++k) {
       mbar_init(segfull(k), 1);
       mbar_init(segempty(k), 9);  // the MMA warp and eight softmax warps
@@ -185,20 +320,22 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
   if (warp == 9) tmem_alloc(smem_u32(misc), 512);
 
   // ---- this CTA's place on the line: a prefix sum over the requests, and a walk from the one it starts in
-  int64_t mine = 0;
+  // (in 32 bits: 2^31 key blocks would be hours of work)
+  int mine = 0;
   const int per = (a.b.batch + kPgThreads - 1) / kPgThreads;
   const int i0 = min(tid * per, a.b.batch), i1 = min(i0 + per, a.b.batch);
+  PgReq r = {};
   bool cut = false;
   for (int i = i0; i < i1; ++i) {
-    const PgReq r = pg_request(a, i);
+    r = pg_request(a, i);
     cut |= r.kv != r.pos0 + r.n && r.n > 0;
-    mine += a.b.nkv * ((int64_t)unit_cost * r.pairs + pg_sum_blocks(a, r));
+    mine += a.b.nkv * (unit_cost * r.pairs + pg_sum_blocks(a, r));
   }
   if (cut && blockIdx.x == 0) flag_error(a.b.err, QD_DEVERR_PAGE);
-  int64_t incl = mine;
+  int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+    const int v = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += v;
   }
   if (lane == 31) scan[warp] = incl;
@@ -206,36 +343,41 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
   __syncthreads();
   tc_fence_after();
   grid_dep_launch();
-  int64_t before = 0, W = 0;
+  int before = incl - mine;
+  PgLine line;
+  line.total = 0;
+#pragma unroll
   for (int w = 0; w < kPgThreads / 32; ++w) {
-    if (w < warp) before += scan[w];
-    W += scan[w];
+    const int v = scan[w];
+    if (w < warp) before += v;
+    line.total += v;
   }
-  before += incl - mine;
-  // with less than one piece per CTA the first W CTAs take one each, and the rest nothing
-  const int G = (int)min((int64_t)gridDim.x, W), cta = blockIdx.x;
-  const int64_t begin = cta < G ? part_begin(W, G, cta) : W, end = cta < G ? part_begin(W, G, cta + 1) : W;
-  if (mine > 0 && begin >= before && begin < before + mine && begin < end) {
-    int64_t w = begin - before;
-    int i = i0;
-    PgReq r = pg_request(a, i);
-    for (;;) {
-      const int64_t c = a.b.nkv * ((int64_t)unit_cost * r.pairs + pg_sum_blocks(a, r));
-      if (w < c) break;
-      w -= c;
-      r = pg_request(a, ++i);
+  // with less than one place per CTA the first ones take one each, and the rest nothing
+  line.ctas = min((unsigned)gridDim.x, line.total);
+  line.each = line.ctas ? line.total / line.ctas : 0;
+  line.more = line.total - line.each * line.ctas;
+  const int cta = blockIdx.x;
+  const int begin = cta < (int)line.ctas ? (int)line.begin(cta) : 0;
+  const int end = cta < (int)line.ctas ? (int)line.begin(cta + 1) : 0;
+  if (begin < end && begin >= before && begin < before + mine) {
+    int w = begin - before, i = i0;
+    if (per > 1) {
+      for (r = pg_request(a, i);; r = pg_request(a, ++i)) {
+        const int c = a.b.nkv * (unit_cost * r.pairs + pg_sum_blocks(a, r));
+        if (w < c) break;
+        w -= c;
+      }
     }
-    int k = 0;
-    for (;; ++k) {
-      const int64_t c = (int64_t)a.b.nkv * (unit_cost + pg_blocks(a, r, k));
-      if (w < c) break;
-      w -= c;
+    int k = 0, len = unit_cost + pg_blocks(a, r, 0);
+    while (w >= a.b.nkv * len) {
+      w -= a.b.nkv * len;
+      len = unit_cost + pg_blocks(a, r, ++k);
     }
-    const int len = unit_cost + pg_blocks(a, r, k);
     misc[2] = i;
     misc[3] = k;
-    misc[4] = (int)(w / len);  // KV head
-    misc[5] = (int)(w % len);  // place in the unit
+    misc[4] = w / len;  // KV head
+    misc[5] = w % len;  // place in the unit
+    *reinterpret_cast<PgReq*>(smem + Lay::mx) = r;
   }
   __syncthreads();
   const uint32_t tmem = (uint32_t)misc[0];
@@ -247,26 +389,31 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
   if (warp == 8) {
     // ------------------------------------------------------------ producer: all lanes walk the line
     const uint64_t pol = policy_evict_normal();
-    int64_t at = begin;
-    int i = misc[2], k = misc[3], h = misc[4], o = misc[5];
-    const int box_rows = min(a.b.page_size, kPgKeys);
-    const int boxes = kPgKeys / box_rows * kHalves, box_bytes = box_rows * 128;
+    int at = begin, i = misc[2], k = misc[3], h = misc[4], o = misc[5];
+    const int boxes = (kPgKeys >> a.b.page_shift) * kHalves, box_bytes = a.b.page_size * 128;
     const int my_page = lane / kHalves, my_half = lane % kHalves;
-    int seg = 0, item = 0, next_region = 0, qfills[2] = {0, 0};
+    int seg = 0, items = 0, slot = 0, next_region = 0, qfills[2] = {0, 0};
+    uint32_t phase = 1;  // of empty(slot): a ring's first round passes at once
     bool ok = true;
-    PgReq r = {};
-    if (at < end) r = pg_request(a, i);
+    r = *reinterpret_cast<const PgReq*>(smem + Lay::mx);
+    __syncwarp();
+    // this lane's page of block j of the current request; -2: no box (past the last key)
+    auto page_of = [&](int j) {
+      const int key = j * kPgKeys + (my_page << a.b.page_shift);
+      if (lane >= boxes || key >= r.kv) return -2;
+      return max(ld_i32(a.b.table + i * a.b.ld_table + (key >> a.b.page_shift)), -1);
+    };
     while (at < end && ok) {
       const int nblk = pg_blocks(a, r, k);
-      const int take = (int)min(end - at, (int64_t)(unit_cost + nblk - o));
+      const int take = min(end - at, unit_cost + nblk - o);
       const int j0 = max(o - unit_cost, 0), j1 = max(o + take - unit_cost, 0);
       if (j1 > j0) {
-        const int64_t first = at - o + unit_cost;  // place of the unit's first block
-        const int c0 = part_owner(W, G, first), c1 = part_owner(W, G, first + nblk - 1);
+        int page = page_of(j0);
+        const int first = at - o + unit_cost;  // place of the unit's first block
         const int t0 = k * 2 * a.tpt, ntok = min(2 * a.tpt, r.n - t0);
-        const bool two = ntok > a.tpt;
+        const bool two = ntok > a.tpt, few = ntok <= a.tpf;
         const int ra = two ? 0 : next_region;
-        // Q: the regions this unit takes, once their last users' S products are done
+        // Q: the regions this unit takes, once their last users are done
         for (int x = 0; x <= (two ? 1 : 0) && ok; ++x) {
           const int reg = two ? x : ra;
           if (qfills[reg] > 0 && !mbar_wait_abort(qempty(reg), (qfills[reg] - 1) & 1, a.b.err, kErrWaitEmpty, abort))
@@ -276,6 +423,18 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         if (lane == 0) {
+          for (int x = 0; x <= (two ? 1 : 0); ++x) {
+            const int reg = two ? x : ra;
+            const bool one = ntok - x * a.tpt == 1;
+            const CUtensorMap* map = one ? &a.tq1 : few ? &a.tqf : &a.tq;
+            mbar_arrive_expect_tx(qfull(reg), kHalves * a.group * (one ? 1 : few ? a.tpf : a.tpt) * 128);
+#pragma unroll
+            for (int hf = 0; hf < kHalves; ++hf)
+              pg_tma_4d(sb + Lay::q + reg * Lay::kItem + hf * kPgBox, map, 64 * hf, 0, h, r.row0 + t0 + x * a.tpt,
+                        qfull(reg), pol);
+            misc[6 + reg] = qfills[reg] + 1;
+          }
+          const int c0 = line.owner(first), c1 = line.owner(first + nblk - 1);
           PgSeg* s = segs + (seg & 3);
           s->row0 = r.row0 + t0;
           s->ntok = ntok;
@@ -285,58 +444,44 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
           s->j0 = j0;
           s->nb = j1 - j0;
           s->whole = j0 == 0 && j1 == nblk;
+          s->few = few;
           s->slot = 2 * cta + (j0 > 0 ? 0 : 1);
           s->c0 = c0;
           s->nc = c1 - c0 + 1;
           s->region = two ? -1 : ra;
           mbar_arrive(segfull(seg));
-          for (int x = 0; x <= (two ? 1 : 0); ++x) {
-            const int reg = two ? x : ra;
-            const bool one = ntok - x * a.tpt == 1;
-            mbar_arrive_expect_tx(qfull(reg), kHalves * a.group * (one ? 1 : a.tpt) * 128);
-#pragma unroll
-            for (int hf = 0; hf < kHalves; ++hf)
-              pg_tma_4d(sb + Lay::q + reg * Lay::kItem + hf * kPgBox, one ? &a.tq1 : &a.tq, 64 * hf, 0, h,
-                        r.row0 + t0 + x * a.tpt, qfull(reg), pol);
-            misc[6 + reg] = qfills[reg] + 1;
-          }
         }
         for (int x = 0; x <= (two ? 1 : 0); ++x) ++qfills[two ? x : ra];
         next_region = two ? 0 : 1 - ra;
         ++seg;
         // K and V blocks in turn
-        const int32_t* trow = a.b.table + i * a.b.ld_table;
-        auto page_of = [&](int j) {  // this lane's page of block j; -2: no box (past the last key)
-          const int key = j * kPgKeys + my_page * box_rows;
-          return lane < boxes && key < r.kv ? ld_i32(trow + (key >> a.b.page_shift)) : -2;
-        };
-        int page = page_of(j0);
         for (int j = j0; j < j1 && ok; ++j) {
           const int next = j + 1 < j1 ? page_of(j + 1) : -2;
-          const int key = j * kPgKeys + my_page * box_rows;
-          const bool need = lane < boxes && key < r.kv;
+          const bool need = page != -2;
           const int n_need = __popc(__ballot_sync(0xffffffffu, need));
           if (need && (page < 0 || page >= a.b.n_pages)) {
             flag_error(a.b.err, QD_DEVERR_PAGE);
             page = -1;  // outside the tensor map: the copy fills zeros
           }
-          for (int kv = 0; kv < 2; ++kv, ++item) {
-            const int s = item % kSlots;
-            if (item >= kSlots) {
-              const bool got = mbar_wait_abort(empty(s), (item / kSlots - 1) & 1, a.b.err, kErrWaitEmpty, abort);
-              if (!__all_sync(0xffffffffu, got)) {
-                ok = false;
-                break;
-              }
+          const uint32_t at_page = sb + Lay::kv + my_half * kPgBox + my_page * box_bytes;
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv) {
+            const bool got = mbar_wait_abort(empty(slot), phase, a.b.err, kErrWaitEmpty, abort);
+            if (!__all_sync(0xffffffffu, got)) {
+              ok = false;
+              break;
             }
             if (lane == 0) {
-              mbar_arrive_expect_tx(full(s), n_need * box_bytes);
-              misc[8] = item + 1;
+              mbar_arrive_expect_tx(full(slot), n_need * box_bytes);
+              misc[8] = ++items;
             }
             __syncwarp();
             if (need)
-              pg_tma_4d(sb + Lay::kv + s * Lay::kItem + my_half * kPgBox + my_page * box_bytes, kv ? &a.tv : &a.tk,
-                        64 * my_half, 0, h, page, full(s), pol);
+              pg_tma_4d(at_page + slot * Lay::kItem, kv ? &a.tv : &a.tk, 64 * my_half, 0, h, page, full(slot), pol);
+            if (++slot == kSlots) {
+              slot = 0;
+              phase ^= 1;
+            }
           }
           page = next;
         }
@@ -359,15 +504,169 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
       mbar_arrive(segfull(seg));
     }
   } else if (warp == 9) {
-    // ------------------------------------------------------------ MMA: lane 0 waits and issues
+    // ------------------------------------------------------------ MMA: one elected lane waits and issues
     constexpr uint32_t kTypes = (7u << 7) | (7u << 10), kind = Elem<T>::kBf16 ? (1u << 7) | (1u << 10) : 0u;
     constexpr uint32_t id_s = (umma_idesc_bf16(kPgKeys) & ~kTypes) | kind;
     constexpr uint32_t id_o = (umma_idesc_bf16(D, false, true) & ~kTypes) | kind;
-    int item = 0, uses[2] = {0, 0}, sc[2] = {0, 0}, pc[2] = {0, 0}, units[2] = {0, 0};
+    constexpr uint32_t id_sf = (umma_idesc_bf16(kFewRows) & ~kTypes) | kind;
+    constexpr uint32_t id_of = (umma_idesc_bf16(kFewRows, true, false) & ~kTypes) | kind;
+    // operand descriptors: a start address in units of 16 B below, strides above; steps are plain additions
+    const uint64_t d_q = umma_desc_sw128(sb + Lay::q), d_k = umma_desc_sw128(sb + Lay::kv);
+    const uint64_t d_v = umma_desc_sw128(sb + Lay::kv, kPgBox, 1024);
+    // few rows, head_dim 64: the 64 upper rows of O^T repeat the lower ones (block stride 0)
+    const uint64_t d_vf = umma_desc_sw128(sb + Lay::kv, D == 128 ? kPgBox : 0, 1024);
+    constexpr uint64_t kItem16 = Lay::kItem >> 4;
+    int slot = 0, pc[2] = {0, 0}, units[2] = {0, 0};
+    uint32_t phase = 0, quse = 0;  // of full(slot); bit r: the phase of qfull(r)
+    const bool leader = elect_one();
     bool ok = true;
     auto wait = [&](uint32_t bar, int parity) {
       if (ok) ok = mbar_wait_abort(bar, parity & 1, a.b.err, kErrWaitFull, abort);
     };
+    struct Ring {
+      int slot;
+      uint32_t phase;
+    };
+    auto ahead = [&](int n) {  // the item n places on
+      const int t = slot + n;
+      return t >= kSlots ? Ring{t - kSlots, phase ^ 1u} : Ring{t, phase};
+    };
+    auto advance = [&](int n) {
+      const Ring t = ahead(n);
+      slot = t.slot;
+      phase = t.phase;
+    };
+    // S_x = Q K^T; its columns held the P that O_x has taken in
+    auto issue_s = [&](auto xc, auto fewc, int reg, Ring k) __attribute__((always_inline)) {
+      constexpr int x = decltype(xc)::value;
+      constexpr bool few = decltype(fewc)::value != 0;
+      if (pc[x] > 0) wait(odone(x), pc[x] - 1);
+      wait(full(k.slot), k.phase);
+      tc_fence_after();
+      if (ok) {
+        const uint64_t q = d_q + reg * kItem16, kt = d_k + k.slot * kItem16;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) {  // 16 dims per MMA: +32 B inside a 64-dim half, the next half after 4
+          const uint64_t step = ((d >> 2) * kPgBox + (d & 3) * 32) >> 4;
+          umma_f16(tS(x), (few ? kt : q) + step, (few ? q : kt) + step, few ? id_sf : id_s, d > 0 ? 1u : 0u);
+        }
+      }
+      umma_commit(sfull(x));
+    };
+    // O_x += P_x V
+    auto issue_pv = [&](auto xc, auto fewc, int reg, Ring v, bool first) __attribute__((always_inline)) {
+      constexpr int x = decltype(xc)::value;
+      constexpr bool few = decltype(fewc)::value != 0;
+      if (first && units[x] > 0) wait(ofree(x), units[x] - 1);
+      wait(pfull(x), pc[x]);
+      ++pc[x];
+      tc_fence_after();
+      if (ok) {
+        const uint64_t vt = (few ? d_vf : d_v) + v.slot * kItem16;
+        const uint64_t pt = umma_desc_sw128(sb + Lay::few_p(reg, x));
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {  // 16 keys per MMA: 8 columns of P pairs; V two 8-key atoms
+          const uint32_t acc = kk ? 1u : first ? 0u : 1u;
+          if (few)
+            umma_f16(tO(x), vt + kk * (2048 >> 4), pt + (((kk >> 2) * (kFewP / 2) + (kk & 3) * 32) >> 4), id_of, acc);
+          else
+            umma_f16_ts(tO(x), tS(x) + 8 * kk, vt + kk * (2048 >> 4), id_o, acc);
+        }
+      }
+      umma_commit(odone(x));
+    };
+    // `rows` of V are keys; the ones past them hold anything and are zeroed (the whole warp comes here)
+    auto zero_v = [&](int rows, Ring v) {
+      if (leader) wait(full(v.slot), v.phase);
+      __syncwarp();
+      char* const vt = smem + Lay::kv + v.slot * Lay::kItem;
+#pragma unroll 1
+      for (int c = max(rows, 0) * 8 + lane; c < kPgKeys * 8; c += 32)
+#pragma unroll
+        for (int hf = 0; hf < kHalves; ++hf) *reinterpret_cast<uint4*>(vt + hf * kPgBox + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+      fence_proxy_async_smem();
+      __syncwarp();
+    };
+    const Const<0> c0;
+    const Const<1> c1;
+    // two tiles over the same blocks: K_0, then V_j, K_j+1 in the ring's order
+    auto pair_unit = [&](const PgSeg& g) {
+      if (leader) {
+        wait(qfull(0), quse);
+        wait(qfull(1), quse >> 1);
+        issue_s(c0, c0, 0, ahead(0));
+        issue_s(c1, c0, 1, ahead(0));
+        umma_commit(empty(slot));
+      }
+#pragma unroll 1
+      for (int j = 0; j < g.nb; ++j) {
+        const Ring v = ahead(1), k = ahead(2);
+        const int rows = g.kv - (g.j0 + j) * kPgKeys;
+        if (rows < kPgKeys) zero_v(rows, v);
+        if (leader) {
+          const bool more = j + 1 < g.nb;
+          wait(full(v.slot), v.phase);
+          issue_pv(c0, c0, 0, v, j == 0);
+          if (more) issue_s(c0, c0, 0, k);
+          issue_pv(c1, c0, 0, v, j == 0);
+          umma_commit(empty(v.slot));
+          if (more) {
+            issue_s(c1, c0, 1, k);
+            umma_commit(empty(k.slot));
+          }
+          if (j + 2 == g.nb || g.nb == 1) {  // the last S products are on their way
+            umma_commit(qempty(0));
+            umma_commit(qempty(1));
+          }
+        }
+        advance(2);
+        __syncwarp();
+      }
+      quse ^= 3;
+      ++units[0];
+      ++units[1];
+    };
+    // one tile: its even blocks in S_A, O_A, its odd ones in S_B, O_B; K_j+2 is asked for after V_j
+    auto single_unit = [&](const PgSeg& g, auto fewc) {
+      constexpr bool few = decltype(fewc)::value != 0;
+      const int reg = g.region;
+      if (leader) {
+        wait(qfull(reg), quse >> reg);
+        issue_s(c0, fewc, reg, ahead(0));
+        umma_commit(empty(slot));
+        if (g.nb > 1) {
+          issue_s(c1, fewc, reg, ahead(2));
+          umma_commit(empty(ahead(2).slot));
+        }
+      }
+      auto block = [&](auto xc, int j) __attribute__((always_inline)) {
+        const Ring v = ahead(1), k = ahead(4);
+        const int rows = g.kv - (g.j0 + j) * kPgKeys;
+        if (rows < kPgKeys) zero_v(rows, v);
+        if (leader) {
+          wait(full(v.slot), v.phase);
+          issue_pv(xc, fewc, reg, v, j < 2);
+          umma_commit(empty(v.slot));
+          if (j + 2 < g.nb) {
+            issue_s(xc, fewc, reg, k);
+            umma_commit(empty(k.slot));
+          }
+          // the region is free after the last S products; a few-row unit's P is in it too
+          if (few ? j + 1 == g.nb : (j + 3 == g.nb || (g.nb < 3 && j == 0))) umma_commit(qempty(reg));
+        }
+        advance(2);
+        __syncwarp();
+      };
+#pragma unroll 1
+      for (int j = 0; j < g.nb; j += 2) {
+        block(c0, j);
+        if (j + 1 < g.nb) block(c1, j + 1);
+      }
+      quse ^= 1u << reg;
+      ++units[0];
+      if (g.nb > 1) ++units[1];
+    };
+#pragma unroll 1
     for (int seg = 0;; ++seg) {
       wait(segfull(seg), seg >> 2);
       if (!__all_sync(0xffffffffu, ok)) break;
@@ -375,84 +674,24 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
       __syncwarp();
       if (lane == 0) mbar_arrive(segempty(seg));
       if (g.nb == 0) break;
-      const int nx = g.region < 0 ? 2 : 1, reg0 = g.region < 0 ? 0 : g.region;
-      auto issue_s = [&](int x, int it) {  // S_x = Q_x K^T; its columns held the P that O_x has taken in
-        if (sc[x] > 0) wait(odone(x), sc[x] - 1);
-        ++sc[x];
-        tc_fence_after();
-        if (ok) {
-          const uint32_t q = sb + Lay::q + (reg0 + x) * Lay::kItem, kt = sb + Lay::kv + it % kSlots * Lay::kItem;
-#pragma unroll
-          for (int d = 0; d < D / 16; ++d)  // 16 dims per MMA: +32 B inside a 64-dim half, the next half after 4
-            umma_bf16(tS(x), umma_desc_sw128(q + (d >> 2) * kPgBox + (d & 3) * 32),
-                      umma_desc_sw128(kt + (d >> 2) * kPgBox + (d & 3) * 32), id_s, d > 0 ? 1u : 0u);
-        }
-        umma_commit(sfull(x));
-      };
-      auto issue_pv = [&](int x, int it, bool first) {  // O_x += P_x V
-        if (first && units[x] > 0) wait(ofree(x), units[x] - 1);
-        wait(pfull(x), pc[x]);
-        ++pc[x];
-        tc_fence_after();
-        if (ok) {
-          const uint32_t v = sb + Lay::kv + it % kSlots * Lay::kItem;
-#pragma unroll
-          for (int kk = 0; kk < 8; ++kk)  // 16 keys per MMA: 8 columns of P pairs; V two 8-key atoms
-            umma_bf16_ts(tO(x), tS(x) + 8 * kk, umma_desc_sw128(v + kk * 2048, kPgBox, 1024), id_o,
-                         (first && kk == 0) ? 0u : 1u);
-        }
-        umma_commit(odone(x));
-      };
-      if (lane == 0) {
-        for (int x = 0; x < nx; ++x) wait(qfull(reg0 + x), uses[reg0 + x]);
-        wait(full(item % kSlots), item / kSlots);
-        for (int x = 0; x < nx; ++x) issue_s(x, item);
-        umma_commit(empty(item % kSlots));
-        if (g.nb == 1)
-          for (int x = 0; x < nx; ++x) umma_commit(qempty(reg0 + x));
-      }
-      for (int x = 0; x < nx; ++x) ++uses[reg0 + x];
-      for (int j = 0; j < g.nb; ++j, item += 2) {
-        const int vi = item + 1, ki = item + 2;
-        const int rows = g.kv - (g.j0 + j) * kPgKeys;
-        if (lane == 0) wait(full(vi % kSlots), vi / kSlots);
-        __syncwarp();
-        if (rows < kPgKeys) {  // V rows past the last key hold anything: zero them
-          char* v = smem + Lay::kv + vi % kSlots * Lay::kItem;
-          for (int c = max(rows, 0) * 8 + lane; c < kPgKeys * 8; c += 32)
-#pragma unroll
-            for (int hf = 0; hf < kHalves; ++hf)
-              *reinterpret_cast<uint4*>(v + hf * kPgBox + c * 16) = make_uint4(0u, 0u, 0u, 0u);
-          fence_proxy_async_smem();
-          __syncwarp();
-        }
-        if (lane == 0) {
-          for (int x = 0; x < nx; ++x) {
-            issue_pv(x, vi, j == 0);
-            if (x == nx - 1) umma_commit(empty(vi % kSlots));
-            if (j + 1 < g.nb) {
-              if (x == 0) wait(full(ki % kSlots), ki / kSlots);
-              issue_s(x, ki);
-              if (x == nx - 1) umma_commit(empty(ki % kSlots));
-              if (j + 2 == g.nb) umma_commit(qempty(reg0 + x));
-            }
-          }
-        }
-        __syncwarp();
-      }
-      for (int x = 0; x < nx; ++x) ++units[x];
+      if (g.region < 0)
+        pair_unit(g);
+      else if (g.few)
+        single_unit(g, c1);
+      else
+        single_unit(g, c0);
       if (!__all_sync(0xffffffffu, ok)) break;
     }
-    if (lane == 0)  // no MMA may still run when its memory is given back
+    if (leader)  // no MMA may still run when its memory is given back
       for (int x = 0; x < 2; ++x)
         if (pc[x] > 0) mbar_wait(odone(x), (pc[x] - 1) & 1, a.b.err, kErrDrain);
   }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPgSoftmaxRegs));
     // ------------------------------------------------------------ softmax and epilogue: warpgroup x = tile x
-    const int x = warp >> 2, r = 32 * (warp & 3) + lane;
+    const int x = warp >> 2, r = 32 * (warp & 3) + lane;  // (r: the row, no longer the request)
     const uint32_t lane_off = (uint32_t)(32 * (warp & 3)) << 16;
-    int cnt = 0, meets = 0;
+    int cnt = 0, meets = 0, joins = 0;
     bool ok = true;
     auto wait = [&](uint32_t bar, int parity) {
       if (ok) ok = mbar_wait_abort(bar, parity & 1, a.b.err, kErrWaitFull, abort);
@@ -467,6 +706,179 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
     float2* const pm = reinterpret_cast<float2*>(a.partials + (int64_t)2 * gridDim.x * 2 * D * 128);
     auto part_o = [&](int slot, int c4, int row) { return po + ((int64_t)(slot * 2 + x) * (D / 4) + c4) * 128 + row; };
     auto part_m = [&](int slot, int row) { return pm + (slot * 2 + x) * 128 + row; };
+    // A cut unit: whoever finishes last joins the pieces, in the order of their keys. The pieces' stores are
+    // made visible by the barrier and the ticket (release is cumulative).
+    auto finish = [&](const PgSeg& g, int rows, int t0) __attribute__((always_inline)) {
+      meet();
+      if (!ok) return;
+      if (r == 0) {
+        const bool last = atom_add_acq_rel(a.tickets + 2 * g.c0 + x, 1) == g.nc - 1;
+        if (last) a.tickets[2 * g.c0 + x] = 0;
+        misc[10 + x] = last;
+      }
+      meet();
+      if (!ok || !misc[10 + x]) return;
+      pg_join<T, D>(a, g, x, r, rows, t0);
+    };
+    // A unit of at most kC rows on this warpgroup's blocks: thread r has key r of the block (and, of O^T, dim r).
+    auto few_rows = [&](auto cols, const PgSeg& g, int rows, bool joined) __attribute__((always_inline)) {
+      constexpr int kC = decltype(cols)::value;
+      auto load_cols = [&](uint32_t taddr, uint32_t* v) {
+        if constexpr (kC == 8) {
+          tmem_ld8(taddr, reinterpret_cast<float*>(v));
+          tmem_wait_ld8(v);
+        } else {
+          tmem_ld16_raw(taddr, v);
+          tmem_wait_ld16(v);
+        }
+      };
+      float4* const mx = reinterpret_cast<float4*>(smem + Lay::mx) + x * kFewRows;
+      float4* const sums = reinterpret_cast<float4*>(smem + Lay::ml);
+      float* const mb = reinterpret_cast<float*>(smem + Lay::mb);
+      char* const p_row = smem + Lay::few_p(g.region, x) + (r >> 6) * (kFewP / 2) + (r & 7) * 2;
+      const int chunk = (r & 63) >> 3, wg = warp & 3;
+      float m[kC], l[kC];
+#pragma unroll
+      for (int c = 0; c < kC; ++c) {
+        m[c] = -INFINITY;
+        l[c] = 0.f;
+      }
+      for (int j = x; j < g.nb; j += 2, ++cnt) {
+        wait(sfull(x), cnt);
+        if (!ok) return;
+        tc_fence_after();
+        uint32_t sv[kC];
+        load_cols(tS(x) + lane_off, sv);
+        const int key0 = (g.j0 + j) * kPgKeys;
+        if (key0 + kPgKeys > min(g.kv, g.pos0 + 1)) {  // some row sees only a part of this block
+          const int key = key0 + r;
+          int lim = g.pos0 + 1, next = a.group;  // of the row's token
+#pragma unroll
+          for (int c = 0; c < kC; ++c) {
+            if (c == next) {
+              ++lim;
+              next += a.group;
+            }
+            if (key >= min(lim, g.kv)) sv[c] = __float_as_uint(-INFINITY);
+          }
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < kC; ++c)
+          if (c < rows) {
+            const float v = redux_max(__uint_as_float(sv[c]));
+            if (lane == c) top = v;
+          }
+        if (lane < rows) reinterpret_cast<float*>(mx + lane)[wg] = top;
+        meet();
+        if (!ok) return;
+        bool grow = false;
+        float mn[kC];
+#pragma unroll
+        for (int c = 0; c < kC; ++c)
+          if (c < rows) {
+            const float4 v = mx[c];
+            mn[c] = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) * a.scale_log2;
+            grow |= mn[c] > m[c] + 8.f;
+          }
+        if (grow) {  // the same in every thread of the warpgroup
+          uint32_t o[kC];
+          if (j > x) load_cols(tO(x) + lane_off, o);
+#pragma unroll
+          for (int c = 0; c < kC; ++c)
+            if (c < rows) {
+              const float m_to = fmaxf(m[c], mn[c]);
+              const float alpha = m_to == -INFINITY ? 1.f : exp2f(m[c] - m_to);
+              o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
+              l[c] *= alpha;
+              m[c] = m_to;
+            }
+          if (j > x) {
+            if constexpr (kC == 8)
+              tmem_st8(tO(x) + lane_off, o);
+            else
+              tmem_st16(tO(x) + lane_off, o);
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < kC; ++c)
+          if (c < rows) {
+            const float p = pg_ex2(fmaf(__uint_as_float(sv[c]), a.scale_log2, m[c] == -INFINITY ? 0.f : -m[c]));
+            l[c] += p;
+            const uint32_t w = Elem<T>::pack(p, 0.f);
+            *reinterpret_cast<uint16_t*>(p_row + c * 128 + ((chunk ^ (c & 7)) << 4)) = (uint16_t)w;
+          }
+        tc_fence_before();
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(pfull(x));
+      }
+      wait(odone(x), cnt - 1);
+      if (!ok) return;
+      tc_fence_after();
+      {  // the warps' sums of every row, side by side
+        float mine = 0.f;
+#pragma unroll
+        for (int c = 0; c < kC; ++c)
+          if (c < rows) {
+            const float v = warp_sum(l[c]);
+            if (lane == c) mine = v;
+          }
+        if (lane < rows) reinterpret_cast<float*>(sums + x * kFewRows + lane)[wg] = mine;
+      }
+      if (x == 1) {  // tile A's warps (same lanes of tensor memory) take O_B from here
+#pragma unroll
+        for (int c = 0; c < kC; ++c)
+          if (r == c) mb[c] = m[c];
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(join);
+        return;
+      }
+      meet();
+      if (ok && joined) wait(join, joins++);
+      if (!ok) return;
+      tc_fence_after();
+      uint32_t o[kC], ob[kC];
+      load_cols(tO(0) + lane_off, o);
+      if (joined) load_cols(tO(1) + lane_off, ob);
+      int tok = g.row0, head = 0;
+#pragma unroll
+      for (int c = 0; c < kC; ++c)
+        if (c < rows) {
+          const float4 s = sums[c];
+          float L = (s.x + s.y) + (s.z + s.w), M = m[c], v = __uint_as_float(o[c]);
+          if (joined) {
+            const float4 sbv = sums[kFewRows + c];
+            const float m2 = mb[c], mn = fmaxf(M, m2);
+            const float fa = mn == -INFINITY ? 1.f : exp2f(M - mn), fb = mn == -INFINITY ? 0.f : exp2f(m2 - mn);
+            L = L * fa + ((sbv.x + sbv.y) + (sbv.z + sbv.w)) * fb;
+            v = v * fa + __uint_as_float(ob[c]) * fb;
+            M = mn;
+          }
+          const int hq = g.head * a.group + head;
+          if (g.whole) {
+            const float inv = L > 0.f ? 1.0f / L : 0.f;
+            if (r < D)
+              reinterpret_cast<uint16_t*>(a.out)[tok * a.ldo + (int64_t)hq * D + r] = (uint16_t)Elem<T>::pack(v * inv, 0.f);
+            if (r == c && a.lse)
+              a.lse[tok * a.ld_lse + hq] = L > 0.f ? (M + __log2f(L)) * 0.69314718055994531f : -INFINITY;
+          } else {
+            if (r < D) __stcg(reinterpret_cast<float*>(part_o(g.slot, r >> 2, c)) + (r & 3), v);
+            if (r == c) __stcg(part_m(g.slot, c), make_float2(M, L));
+          }
+          if (++head == a.group) {
+            head = 0;
+            ++tok;
+          }
+        }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(ofree(0));
+        if (joined) mbar_arrive(ofree(1));
+      }
+    };
     for (int seg = 0;; ++seg) {
       wait(segfull(seg), seg >> 2);
       if (!ok) break;
@@ -474,15 +886,30 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
       __syncwarp();
       if (lane == 0) mbar_arrive(segempty(seg));
       if (g.nb == 0) break;
-      if (x == 1 && g.region >= 0) continue;  // a single tile
-      const int ntok = min(a.tpt, g.ntok - x * a.tpt), rows = ntok * a.group;
-      const int my_tok = r / a.group, tok = g.row0 + x * a.tpt + my_tok;
+      const bool two = g.region < 0, joined = !two && g.nb > 1;
+      if (x == 1 && !two && !joined) continue;  // one tile, one block
+      const int t0 = two ? x * a.tpt : 0;       // this tile's first token
+      const int ntok = min(a.tpt, g.ntok - t0), rows = ntok * a.group;
+      const int my_tok = r / a.group, tok = g.row0 + t0 + my_tok;
       const int head = g.head * a.group + r - my_tok * a.group;
-      // keys this row sees: up to its own position; none for the MMA rows past the last token
-      const int lim = r < rows ? min(g.kv, g.pos0 + x * a.tpt + my_tok + 1) : 0;
+      // keys this row sees: up to its own position (MMA rows past the last token hold anything)
+      const int lim = r < rows ? min(g.kv, g.pos0 + t0 + my_tok + 1) : INT_MAX;
       const bool idle = (r & ~31) >= rows;  // no row of this warp is a token's
       float m_used = -INFINITY, l = 0.f;
-      for (int j = 0; j < g.nb; ++j, ++cnt) {
+      const int jf = two ? 0 : x;
+      if (g.few) {
+        if (rows <= 8)
+          few_rows(Const<8>(), g, rows, joined);
+        else
+          few_rows(Const<kFewRows>(), g, rows, joined);
+        if (!ok) break;
+        if (x == 1 || g.whole) continue;
+        finish(g, rows, t0);
+        if (!ok) break;
+        continue;
+      }
+      const int step = two ? 1 : 2;  // one tile: the even blocks, or the odd ones
+      for (int j = jf; j < g.nb; j += step, ++cnt) {
         wait(sfull(x), cnt);
         if (!ok) break;
         tc_fence_after();
@@ -508,7 +935,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
           if (__any_sync(0xffffffffu, m_new > m_used + 8.f)) {
             const float m_to = fmaxf(m_used, m_new);
             const float alpha = m_to == -INFINITY ? 1.f : exp2f(m_used - m_to);
-            if (j > 0) {
+            if (j > jf) {
 #pragma unroll 1
               for (int c4 = 0; c4 < D / 32; ++c4) {
                 uint32_t o[32];
@@ -541,93 +968,78 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
       wait(odone(x), cnt - 1);
       if (!ok) break;
       tc_fence_after();
-      T* const orow = reinterpret_cast<T*>(a.out) + tok * a.ldo + (int64_t)head * D;
-      if (g.whole) {
-        const float inv = l > 0.f ? 1.0f / l : 0.f;
-        if (!idle) {
-#pragma unroll 1
-          for (int c4 = 0; c4 < D / 32; ++c4) {
-            uint32_t o[32];
-            tmem_ld32(tO(x) + lane_off + 32 * c4, o);
-            if (r < rows) {
-              uint4* d4 = reinterpret_cast<uint4*>(orow + 32 * c4);
-#pragma unroll
-              for (int c = 0; c < 4; ++c) {
-                uint32_t w[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  w[e] = Elem<T>::pack(__uint_as_float(o[8 * c + 2 * e]) * inv, __uint_as_float(o[8 * c + 2 * e + 1]) * inv);
-                d4[c] = make_uint4(w[0], w[1], w[2], w[3]);
-              }
-            }
-          }
-          if (r < rows && a.lse)
-            a.lse[tok * a.ld_lse + head] = l > 0.f ? (m_used + __log2f(l)) * 0.69314718055994531f : -INFINITY;
+      float2* const ml = reinterpret_cast<float2*>(smem + Lay::ml);
+      if (joined && x == 1) {  // the odd blocks: tile A's warps (same lanes of tensor memory) take O_B from here
+        ml[r] = make_float2(m_used, l);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(join);
+        continue;
+      }
+      float fa = 1.f, fb = 0.f;
+      if (joined) {
+        wait(join, joins++);
+        if (!ok) break;
+        tc_fence_after();
+        const float2 o = ml[r];
+        const float m = fmaxf(m_used, o.x);
+        if (m != -INFINITY) {
+          fa = exp2f(m_used - m);
+          fb = exp2f(o.x - m);
         }
-      } else if (!idle) {
+        l = l * fa + o.y * fb;
+        m_used = m;
+      }
+      if (!idle) {
+        // a whole unit's rows go out normalised, a piece's as they are
+        const float norm = !g.whole ? 1.f : l > 0.f ? 1.0f / l : 0.f;
+        fa *= norm;
+        fb *= norm;
+        T* const orow = reinterpret_cast<T*>(a.out) + tok * a.ldo + (int64_t)head * D;
 #pragma unroll 1
         for (int c4 = 0; c4 < D / 32; ++c4) {
           uint32_t o[32];
           tmem_ld32(tO(x) + lane_off + 32 * c4, o);
-          if (r < rows)
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fa);
+          if (joined) {
+            uint32_t ob[32];
+            tmem_ld32(tO(1) + lane_off + 32 * c4, ob);
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              o[e] = __float_as_uint(fmaf(__uint_as_float(ob[e]), fb, __uint_as_float(o[e])));
+          }
+          if (r < rows && g.whole) {
+            uint4* d4 = reinterpret_cast<uint4*>(orow + 32 * c4);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                w[e] = Elem<T>::pack(__uint_as_float(o[8 * c + 2 * e]), __uint_as_float(o[8 * c + 2 * e + 1]));
+              d4[c] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          } else if (r < rows) {
 #pragma unroll
             for (int c = 0; c < 8; ++c)
               __stcg(part_o(g.slot, 8 * c4 + c, r),
                      make_float4(__uint_as_float(o[4 * c]), __uint_as_float(o[4 * c + 1]), __uint_as_float(o[4 * c + 2]),
                                  __uint_as_float(o[4 * c + 3])));
+          }
         }
-        if (r < rows) __stcg(part_m(g.slot, r), make_float2(m_used, l));
+        if (r < rows && !g.whole) __stcg(part_m(g.slot, r), make_float2(m_used, l));
+        if (r < rows && g.whole && a.lse)
+          a.lse[tok * a.ld_lse + head] = l > 0.f ? (m_used + __log2f(l)) * 0.69314718055994531f : -INFINITY;
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(ofree(x));
+      if (lane == 0) {
+        mbar_arrive(ofree(x));
+        if (joined) mbar_arrive(ofree(1));
+      }
       if (g.whole) continue;
-      // ---- the unit is cut: whoever finishes last joins the pieces, in the order of their keys
-      __threadfence();
-      meet();
+      finish(g, rows, t0);
       if (!ok) break;
-      if (r == 0) {
-        const bool last = atom_add_acq_rel(a.tickets + 2 * g.c0 + x, 1) == g.nc - 1;
-        if (last) a.tickets[2 * g.c0 + x] = 0;
-        misc[10 + x] = last;
-      }
-      meet();
-      if (!ok) break;
-      if (!misc[10 + x]) continue;
-      __threadfence();
-      auto slot_of = [&](int q) { return 2 * (g.c0 + q) + (q == 0 ? 1 : 0); };
-      for (int e = r; e < rows * (D / 4); e += 128) {
-        const int row = e % rows, c4 = e / rows;
-        float M = -INFINITY, L = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int q0 = 0; q0 < g.nc; q0 += 8) {
-          float2 ml[8];
-          float4 v[8];
-#pragma unroll
-          for (int q = 0; q < 8; ++q)
-            if (q0 + q < g.nc) {
-              ml[q] = __ldcg(part_m(slot_of(q0 + q), row));
-              v[q] = __ldcg(part_o(slot_of(q0 + q), c4, row));
-            }
-#pragma unroll
-          for (int q = 0; q < 8; ++q)
-            if (q0 + q < g.nc && ml[q].y > 0.f) {  // a piece in which the row saw no key counts for nothing
-              const float mn = fmaxf(M, ml[q].x), fa = exp2f(M - mn), fb = exp2f(ml[q].x - mn);
-              M = mn;
-              L = L * fa + ml[q].y * fb;
-              acc.x = acc.x * fa + v[q].x * fb;
-              acc.y = acc.y * fa + v[q].y * fb;
-              acc.z = acc.z * fa + v[q].z * fb;
-              acc.w = acc.w * fa + v[q].w * fb;
-            }
-        }
-        const float inv = L > 0.f ? 1.0f / L : 0.f;
-        const int t2 = g.row0 + x * a.tpt + row / a.group, h2 = g.head * a.group + row % a.group;
-        *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + t2 * a.ldo + (int64_t)h2 * D + 4 * c4) =
-            make_uint2(Elem<T>::pack(acc.x * inv, acc.y * inv), Elem<T>::pack(acc.z * inv, acc.w * inv));
-        if (c4 == 0 && a.lse)
-          a.lse[t2 * a.ld_lse + h2] = L > 0.f ? (M + __log2f(L)) * 0.69314718055994531f : -INFINITY;
-      }
     }
   }
   tc_fence_before();
@@ -693,6 +1105,7 @@ extern "C" int qd_paged_attn(const void* q, int64_t ldq, int dtype, int64_t toke
   if (!encode) return set_error(QD_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
   a.group = nq_heads / nkv_heads;
   a.tpt = 128 / a.group;
+  a.tpf = kFewRows / a.group;
   const CUtensorMapDataType type = dtype == QD_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const cuuint32_t estr[4] = {1, 1, 1, 1};
   auto map4 = [&](CUtensorMap* m, const void* base, const cuuint64_t* dims, const cuuint64_t* strides,
@@ -705,7 +1118,8 @@ extern "C" int qd_paged_attn(const void* q, int64_t ldq, int dtype, int64_t toke
     const cuuint64_t dims[4] = {(cuuint64_t)head_dim, (cuuint64_t)a.group, (cuuint64_t)nkv_heads, (cuuint64_t)tokens};
     const cuuint64_t strides[3] = {(cuuint64_t)head_dim * 2, (cuuint64_t)a.group * head_dim * 2, (cuuint64_t)ldq * 2};
     const cuuint32_t box[4] = {64, (cuuint32_t)a.group, 1, (cuuint32_t)a.tpt}, box1[4] = {64, (cuuint32_t)a.group, 1, 1};
-    if (!map4(&a.tq, q, dims, strides, box) || !map4(&a.tq1, q, dims, strides, box1))
+    const cuuint32_t boxf[4] = {64, (cuuint32_t)a.group, 1, (cuuint32_t)(a.tpf > 0 ? a.tpf : 1)};
+    if (!map4(&a.tq, q, dims, strides, box) || !map4(&a.tqf, q, dims, strides, boxf) || !map4(&a.tq1, q, dims, strides, box1))
       return set_error(QD_ERR_CUDA, "cuTensorMapEncodeTiled failed for q");
   }
   {
