@@ -68,8 +68,8 @@ struct PgLayout {
   static constexpr int p = kv + kSlots * kItem;  // P of few-row units (head_dim 128: in their Q region)
   static constexpr int bars = p + (D == 64 ? 2 * kFewP : 0);
   // qfull[2], qempty[2], sfull[2], pfull[2], odone[2], ofree[2], group[2], segfull[4], segempty[4], join, -,
-  // full[slots], empty[slots]
-  static constexpr int nbars = 24 + 2 * kSlots;
+  // sload[2], full[slots], empty[slots]
+  static constexpr int nbars = 26 + 2 * kSlots;
   static constexpr int seg = bars + nbars * 8;  // segment ring
   static constexpr int misc = seg + 4 * 64;     // tmem slot, abort, line start, flags, drain counts
   static constexpr int ml = misc + 192;         // at a unit's end: (m, l) of the odd blocks' rows [128], or the
@@ -124,18 +124,21 @@ __device__ __forceinline__ float redux_max(float v) {
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
   return r;
 }
-__device__ __forceinline__ void tmem_wait_ld8(uint32_t* r) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])::"memory");
-}
-__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
+__device__ __forceinline__ void tmem_ld4_wait(uint32_t taddr, uint32_t* r) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n"
-      "tcgen05.wait::st.sync.aligned;" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+      "tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+      : "r"(taddr)
       : "memory");
 }
-
+__device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};\n"
+      "tcgen05.wait::st.sync.aligned;" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+      : "memory");
+}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
@@ -143,6 +146,16 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
       "tcgen05.wait::st.sync.aligned;" ::"r"(taddr),
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+// 128 consecutive columns of this thread's lane in one load, waited
+__device__ __forceinline__ void tmem_ld128(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x128.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63, %64, %65, %66, %67, %68, %69, %70, %71, %72, %73, %74, %75, %76, %77, %78, %79, %80, %81, %82, %83, %84, %85, %86, %87, %88, %89, %90, %91, %92, %93, %94, %95, %96, %97, %98, %99, %100, %101, %102, %103, %104, %105, %106, %107, %108, %109, %110, %111, %112, %113, %114, %115, %116, %117, %118, %119, %120, %121, %122, %123, %124, %125, %126, %127}, [%128];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]), "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]), "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]), "=r"(r[80]), "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]), "=r"(r[88]), "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]), "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]), "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]), "=r"(r[111]), "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]), "=r"(r[118]), "=r"(r[119]), "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
+      : "r"(taddr)
       : "memory");
 }
 
@@ -198,7 +211,7 @@ struct PgLine {
 };
 
 // Joins a cut unit's pieces of one tile (x): 128 threads, thread r. kItems float4 of the output at a time, with
-// kPieces pieces' loads in flight for each. Out of line: it keeps its registers out of the main loop's way.
+// kPieces pieces' loads in flight for each.
 template <typename T, int D, int kItems, int kPieces>
 __device__ __forceinline__ void pg_join_items(const PagedAttnArgs& a, const PgSeg& g, int x, int r, int rows, int t0) {
   const float4* const po = reinterpret_cast<const float4*>(a.partials);
@@ -259,11 +272,11 @@ __device__ __forceinline__ void pg_join_items(const PagedAttnArgs& a, const PgSe
   }
 }
 template <typename T, int D>
-__device__ __noinline__ void pg_join(const PagedAttnArgs& a, const PgSeg& g, int x, int r, int rows, int t0) {
+__device__ __forceinline__ void pg_join(const PagedAttnArgs& a, const PgSeg& g, int x, int r, int rows, int t0) {
   if (rows * (D / 4) > 256)
-    pg_join_items<T, D, 8, 2>(a, g, x, r, rows, t0);
+    pg_join_items<T, D, 2, 2>(a, g, x, r, rows, t0);
   else
-    pg_join_items<T, D, 1, 8>(a, g, x, r, rows, t0);
+    pg_join_items<T, D, 1, 4>(a, g, x, r, rows, t0);
 }
 
 template <typename T, int D>
@@ -287,8 +300,9 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
   auto segfull = [&](int k) { return bars + 112 + 8u * (k & 3); };
   auto segempty = [&](int k) { return bars + 144 + 8u * (k & 3); };
   const uint32_t join = bars + 176;
-  auto full = [&](int s) { return bars + 192 + 8u * s; };
-  auto empty = [&](int s) { return bars + 192 + 8u * (kSlots + s); };
+  auto sload = [&](int x) { return bars + 192 + 8u * x; };
+  auto full = [&](int s) { return bars + 208 + 8u * s; };
+  auto empty = [&](int s) { return bars + 208 + 8u * (kSlots + s); };
   PgSeg* segs = reinterpret_cast<PgSeg*>(smem + Lay::seg);
   int* misc = reinterpret_cast<int*>(smem + Lay::misc);
   int* abort = misc + 1;
@@ -304,6 +318,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
       mbar_init(odone(x), 1);
       mbar_init(ofree(x), 4);
       mbar_init(group(x), 4);
+      mbar_init(sload(x), 4);
     }
     mbar_init(join, 4);
     for (int k = 0; k < 4; ++k) {
@@ -518,6 +533,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
     constexpr uint64_t kItem16 = Lay::kItem >> 4;
     int slot = 0, pc[2] = {0, 0}, units[2] = {0, 0};
     uint32_t phase = 0, quse = 0;  // of full(slot); bit r: the phase of qfull(r)
+    int pairs = 0;                 // blocks of units of two tiles so far
     const bool leader = elect_one();
     bool ok = true;
     auto wait = [&](uint32_t bar, int parity) {
@@ -536,11 +552,14 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
       slot = t.slot;
       phase = t.phase;
     };
-    // S_x = Q K^T; its columns held the P that O_x has taken in
+    // every product that reads P has been done
+    auto wait_pv = [&](int x) {
+      if (pc[x] > 0) wait(odone(x), pc[x] - 1);
+    };
+    // S_x = Q K^T
     auto issue_s = [&](auto xc, auto fewc, int reg, Ring k) __attribute__((always_inline)) {
       constexpr int x = decltype(xc)::value;
       constexpr bool few = decltype(fewc)::value != 0;
-      if (pc[x] > 0) wait(odone(x), pc[x] - 1);
       wait(full(k.slot), k.phase);
       tc_fence_after();
       if (ok) {
@@ -554,9 +573,9 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
       umma_commit(sfull(x));
     };
     // O_x += P_x V
-    auto issue_pv = [&](auto xc, auto fewc, int reg, Ring v, bool first) __attribute__((always_inline)) {
+    auto issue_pv = [&](auto xc, auto modec, int reg, Ring v, bool first) __attribute__((always_inline)) {
       constexpr int x = decltype(xc)::value;
-      constexpr bool few = decltype(fewc)::value != 0;
+      constexpr bool few = decltype(modec)::value == 1, pair = decltype(modec)::value == 2;
       if (first && units[x] > 0) wait(ofree(x), units[x] - 1);
       wait(pfull(x), pc[x]);
       ++pc[x];
@@ -570,7 +589,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
           if (few)
             umma_f16(tO(x), vt + kk * (2048 >> 4), pt + (((kk >> 2) * (kFewP / 2) + (kk & 3) * 32) >> 4), id_of, acc);
           else
-            umma_f16_ts(tO(x), tS(x) + 8 * kk, vt + kk * (2048 >> 4), id_o, acc);
+            umma_f16_ts(tO(x), tS(pair ? 1 - x : x) + 8 * kk, vt + kk * (2048 >> 4), id_o, acc);
         }
       }
       umma_commit(odone(x));
@@ -589,40 +608,56 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
     };
     const Const<0> c0;
     const Const<1> c1;
-    // two tiles over the same blocks: K_0, then V_j, K_j+1 in the ring's order
+    const Const<2> c2;
+    // Two tiles over the same blocks. Each tile's P goes over the other's S, which that has long loaded: so the
+    // next S of a tile does not wait for its own P to be used up, and S_A runs a block ahead:
+    //   S_A 0, S_B 0, S_A 1;  PV_A j, S_B j+1, PV_B j, S_A j+2
     auto pair_unit = [&](const PgSeg& g) {
       if (leader) {
         wait(qfull(0), quse);
         wait(qfull(1), quse >> 1);
+        wait_pv(0);
+        wait_pv(1);
         issue_s(c0, c0, 0, ahead(0));
         issue_s(c1, c0, 1, ahead(0));
         umma_commit(empty(slot));
+        if (g.nb > 1) {
+          wait(sload(0), pairs);
+          issue_s(c0, c0, 0, ahead(2));
+        } else {
+          umma_commit(qempty(0));
+          umma_commit(qempty(1));
+        }
       }
 #pragma unroll 1
       for (int j = 0; j < g.nb; ++j) {
-        const Ring v = ahead(1), k = ahead(2);
+        const Ring v = ahead(1), k1 = ahead(2), k2 = ahead(4);
         const int rows = g.kv - (g.j0 + j) * kPgKeys;
         if (rows < kPgKeys) zero_v(rows, v);
         if (leader) {
-          const bool more = j + 1 < g.nb;
           wait(full(v.slot), v.phase);
-          issue_pv(c0, c0, 0, v, j == 0);
-          if (more) issue_s(c0, c0, 0, k);
-          issue_pv(c1, c0, 0, v, j == 0);
-          umma_commit(empty(v.slot));
-          if (more) {
-            issue_s(c1, c0, 1, k);
-            umma_commit(empty(k.slot));
+          issue_pv(c0, c2, 0, v, j == 0);
+          if (j + 1 < g.nb) {
+            wait_pv(0);  // S_B's columns hold P_A
+            issue_s(c1, c0, 1, k1);
+            umma_commit(empty(k1.slot));
+            if (j + 2 == g.nb) {
+              umma_commit(qempty(0));
+              umma_commit(qempty(1));
+            }
           }
-          if (j + 2 == g.nb || g.nb == 1) {  // the last S products are on their way
-            umma_commit(qempty(0));
-            umma_commit(qempty(1));
+          issue_pv(c1, c2, 0, v, j == 0);
+          umma_commit(empty(v.slot));
+          if (j + 2 < g.nb) {
+            wait_pv(1);
+            issue_s(c0, c0, 0, k2);
           }
         }
         advance(2);
         __syncwarp();
       }
       quse ^= 3;
+      pairs += g.nb;
       ++units[0];
       ++units[1];
     };
@@ -632,6 +667,8 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
       const int reg = g.region;
       if (leader) {
         wait(qfull(reg), quse >> reg);
+        wait_pv(0);
+        wait_pv(1);
         issue_s(c0, fewc, reg, ahead(0));
         umma_commit(empty(slot));
         if (g.nb > 1) {
@@ -648,6 +685,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
           issue_pv(xc, fewc, reg, v, j < 2);
           umma_commit(empty(v.slot));
           if (j + 2 < g.nb) {
+            wait_pv(decltype(xc)::value);
             issue_s(xc, fewc, reg, k);
             umma_commit(empty(k.slot));
           }
@@ -691,7 +729,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
     // ------------------------------------------------------------ softmax and epilogue: warpgroup x = tile x
     const int x = warp >> 2, r = 32 * (warp & 3) + lane;  // (r: the row, no longer the request)
     const uint32_t lane_off = (uint32_t)(32 * (warp & 3)) << 16;
-    int cnt = 0, meets = 0, joins = 0;
+    int cnt = 0, pairs = 0, meets = 0, joins = 0;
     bool ok = true;
     auto wait = [&](uint32_t bar, int parity) {
       if (ok) ok = mbar_wait_abort(bar, parity & 1, a.b.err, kErrWaitFull, abort);
@@ -720,14 +758,14 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
       if (!ok || !misc[10 + x]) return;
       pg_join<T, D>(a, g, x, r, rows, t0);
     };
-    // A unit of at most kC rows on this warpgroup's blocks: thread r has key r of the block (and, of O^T, dim r).
+    // A unit of at most kC rows on this warpgroup's blocks: thread r has key r of the block (and, of O^T, dim r);
+    // what there is one of per row (maximum, factors) is lane c's for row c, the same in all four warps.
     auto few_rows = [&](auto cols, const PgSeg& g, int rows, bool joined) __attribute__((always_inline)) {
       constexpr int kC = decltype(cols)::value;
       auto load_cols = [&](uint32_t taddr, uint32_t* v) {
-        if constexpr (kC == 8) {
-          tmem_ld8(taddr, reinterpret_cast<float*>(v));
-          tmem_wait_ld8(v);
-        } else {
+        if constexpr (kC == 4)
+          tmem_ld4_wait(taddr, v);
+        else {
           tmem_ld16_raw(taddr, v);
           tmem_wait_ld16(v);
         }
@@ -737,12 +775,11 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
       float* const mb = reinterpret_cast<float*>(smem + Lay::mb);
       char* const p_row = smem + Lay::few_p(g.region, x) + (r >> 6) * (kFewP / 2) + (r & 7) * 2;
       const int chunk = (r & 63) >> 3, wg = warp & 3;
-      float m[kC], l[kC];
+      float m = -INFINITY;  // of row `lane`
+      float l[kC];          // of every row, this thread's keys
 #pragma unroll
-      for (int c = 0; c < kC; ++c) {
-        m[c] = -INFINITY;
-        l[c] = 0.f;
-      }
+      for (int c = 0; c < kC; ++c) l[c] = 0.f;
+#pragma unroll 1
       for (int j = x; j < g.nb; j += 2, ++cnt) {
         wait(sfull(x), cnt);
         if (!ok) return;
@@ -764,50 +801,44 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
         }
         float top = -INFINITY;
 #pragma unroll
-        for (int c = 0; c < kC; ++c)
-          if (c < rows) {
-            const float v = redux_max(__uint_as_float(sv[c]));
-            if (lane == c) top = v;
-          }
+        for (int c = 0; c < kC; ++c) {
+          const float v = redux_max(__uint_as_float(sv[c]));
+          top = lane == c ? v : top;
+        }
         if (lane < rows) reinterpret_cast<float*>(mx + lane)[wg] = top;
         meet();
         if (!ok) return;
-        bool grow = false;
-        float mn[kC];
-#pragma unroll
-        for (int c = 0; c < kC; ++c)
-          if (c < rows) {
-            const float4 v = mx[c];
-            mn[c] = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) * a.scale_log2;
-            grow |= mn[c] > m[c] + 8.f;
-          }
-        if (grow) {  // the same in every thread of the warpgroup
-          uint32_t o[kC];
-          if (j > x) load_cols(tO(x) + lane_off, o);
-#pragma unroll
-          for (int c = 0; c < kC; ++c)
-            if (c < rows) {
-              const float m_to = fmaxf(m[c], mn[c]);
-              const float alpha = m_to == -INFINITY ? 1.f : exp2f(m[c] - m_to);
-              o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
-              l[c] *= alpha;
-              m[c] = m_to;
-            }
+        float mn = -INFINITY;
+        if (lane < rows) {
+          const float4 v = mx[lane];
+          mn = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) * a.scale_log2;
+        }
+        if (__any_sync(0xffffffffu, mn > m + 8.f)) {  // the same in every warp of the group
+          const float m_to = fmaxf(m, mn), alpha = m_to == -INFINITY ? 1.f : exp2f(m - m_to);
+          m = m_to;
           if (j > x) {
-            if constexpr (kC == 8)
-              tmem_st8(tO(x) + lane_off, o);
+            uint32_t o[kC];
+            load_cols(tO(x) + lane_off, o);
+#pragma unroll
+            for (int c = 0; c < kC; ++c) {
+              const float f = __shfl_sync(0xffffffffu, alpha, c);
+              o[c] = __float_as_uint(__uint_as_float(o[c]) * f);
+              l[c] *= f;
+            }
+            if constexpr (kC == 4)
+              tmem_st4(tO(x) + lane_off, o);
             else
               tmem_st16(tO(x) + lane_off, o);
           }
         }
+        const float nm = m == -INFINITY ? 0.f : -m;
 #pragma unroll
-        for (int c = 0; c < kC; ++c)
-          if (c < rows) {
-            const float p = pg_ex2(fmaf(__uint_as_float(sv[c]), a.scale_log2, m[c] == -INFINITY ? 0.f : -m[c]));
-            l[c] += p;
-            const uint32_t w = Elem<T>::pack(p, 0.f);
-            *reinterpret_cast<uint16_t*>(p_row + c * 128 + ((chunk ^ (c & 7)) << 4)) = (uint16_t)w;
-          }
+        for (int c = 0; c < kC; ++c) {
+          const float p = pg_ex2(fmaf(__uint_as_float(sv[c]), a.scale_log2, __shfl_sync(0xffffffffu, nm, c)));
+          l[c] += p;
+          const uint32_t w = Elem<T>::pack(p, 0.f);
+          *reinterpret_cast<uint16_t*>(p_row + c * 128 + ((chunk ^ (c & 7)) << 4)) = (uint16_t)w;
+        }
         tc_fence_before();
         fence_proxy_async_smem();
         __syncwarp();
@@ -817,19 +848,17 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
       if (!ok) return;
       tc_fence_after();
       {  // the warps' sums of every row, side by side
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+          for (int c = 0; c < kC; ++c) l[c] += __shfl_xor_sync(0xffffffffu, l[c], o);
         float mine = 0.f;
 #pragma unroll
-        for (int c = 0; c < kC; ++c)
-          if (c < rows) {
-            const float v = warp_sum(l[c]);
-            if (lane == c) mine = v;
-          }
+        for (int c = 0; c < kC; ++c) mine = lane == c ? l[c] : mine;
         if (lane < rows) reinterpret_cast<float*>(sums + x * kFewRows + lane)[wg] = mine;
       }
       if (x == 1) {  // tile A's warps (same lanes of tensor memory) take O_B from here
-#pragma unroll
-        for (int c = 0; c < kC; ++c)
-          if (r == c) mb[c] = m[c];
+        if (wg == 0 && lane < rows) mb[lane] = m;
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(join);
@@ -842,36 +871,44 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
       uint32_t o[kC], ob[kC];
       load_cols(tO(0) + lane_off, o);
       if (joined) load_cols(tO(1) + lane_off, ob);
-      int tok = g.row0, head = 0;
-#pragma unroll
-      for (int c = 0; c < kC; ++c)
-        if (c < rows) {
-          const float4 s = sums[c];
-          float L = (s.x + s.y) + (s.z + s.w), M = m[c], v = __uint_as_float(o[c]);
-          if (joined) {
-            const float4 sbv = sums[kFewRows + c];
-            const float m2 = mb[c], mn = fmaxf(M, m2);
-            const float fa = mn == -INFINITY ? 1.f : exp2f(M - mn), fb = mn == -INFINITY ? 0.f : exp2f(m2 - mn);
-            L = L * fa + ((sbv.x + sbv.y) + (sbv.z + sbv.w)) * fb;
-            v = v * fa + __uint_as_float(ob[c]) * fb;
-            M = mn;
-          }
-          const int hq = g.head * a.group + head;
-          if (g.whole) {
-            const float inv = L > 0.f ? 1.0f / L : 0.f;
-            if (r < D)
-              reinterpret_cast<uint16_t*>(a.out)[tok * a.ldo + (int64_t)hq * D + r] = (uint16_t)Elem<T>::pack(v * inv, 0.f);
-            if (r == c && a.lse)
-              a.lse[tok * a.ld_lse + hq] = L > 0.f ? (M + __log2f(L)) * 0.69314718055994531f : -INFINITY;
-          } else {
-            if (r < D) __stcg(reinterpret_cast<float*>(part_o(g.slot, r >> 2, c)) + (r & 3), v);
-            if (r == c) __stcg(part_m(g.slot, c), make_float2(M, L));
-          }
-          if (++head == a.group) {
-            head = 0;
-            ++tok;
-          }
+      float fa = 1.f, fb = 0.f;
+      int64_t row_at = 0;  // of row `lane`, in elements
+      if (lane < rows) {
+        const float4 s = sums[lane];
+        float L = (s.x + s.y) + (s.z + s.w), M = m;
+        if (joined) {
+          const float4 s2 = sums[kFewRows + lane];
+          const float m2 = mb[lane], mn = fmaxf(M, m2);
+          fa = mn == -INFINITY ? 1.f : exp2f(M - mn);
+          fb = mn == -INFINITY ? 0.f : exp2f(m2 - mn);
+          L = L * fa + ((s2.x + s2.y) + (s2.z + s2.w)) * fb;
+          M = mn;
         }
+        const int tok = lane / a.group, hq = g.head * a.group + lane - tok * a.group;
+        row_at = (g.row0 + tok) * a.ldo + (int64_t)hq * D;
+        if (g.whole) {
+          const float inv = L > 0.f ? 1.0f / L : 0.f;
+          fa *= inv;
+          fb *= inv;
+          if (wg == 0 && a.lse)
+            a.lse[(g.row0 + tok) * a.ld_lse + hq] = L > 0.f ? (M + __log2f(L)) * 0.69314718055994531f : -INFINITY;
+        } else if (wg == 0) {
+          __stcg(part_m(g.slot, lane), make_float2(M, L));
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < kC; ++c) {
+        float v = __uint_as_float(o[c]) * __shfl_sync(0xffffffffu, fa, c);
+        const float f = __shfl_sync(0xffffffffu, fb, c);
+        const int64_t to = __shfl_sync(0xffffffffu, row_at, c);
+        if (joined) v = fmaf(__uint_as_float(ob[c]), f, v);
+        if (c < rows && r < D) {
+          if (g.whole)
+            reinterpret_cast<uint16_t*>(a.out)[to + r] = (uint16_t)Elem<T>::pack(v, 0.f);
+          else
+            __stcg(reinterpret_cast<float*>(part_o(g.slot, r >> 2, c)) + (r & 3), v);
+        }
+      }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
@@ -898,8 +935,8 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
       float m_used = -INFINITY, l = 0.f;
       const int jf = two ? 0 : x;
       if (g.few) {
-        if (rows <= 8)
-          few_rows(Const<8>(), g, rows, joined);
+        if (rows <= 4)
+          few_rows(Const<4>(), g, rows, joined);
         else
           few_rows(Const<kFewRows>(), g, rows, joined);
         if (!ok) break;
@@ -913,10 +950,14 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
         wait(sfull(x), cnt);
         if (!ok) break;
         tc_fence_after();
+        uint32_t sv[128];
+        if (!idle) tmem_ld128(tS(x) + lane_off, sv);
+        if (two) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(sload(x));
+        }
         if (!idle) {
-          uint32_t sv[128];
-          tmem_ld64(tS(x) + lane_off, sv);
-          tmem_ld64(tS(x) + lane_off + 64, sv + 64);
           const int left = lim - (g.j0 + j) * kPgKeys;
           if (__any_sync(0xffffffffu, left < kPgKeys)) {
 #pragma unroll
@@ -930,12 +971,13 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
             for (int c = 0; c < 4; ++c)
               m4[c] = pg_max3(m4[c], __uint_as_float(sv[e + 2 * c]), __uint_as_float(sv[e + 2 * c + 1]));
           const float m_new = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * a.scale_log2;
-          // warp-uniform (tensor-memory loads and stores are warp-collective); O_x holds every block before
-          // this one: S_x was issued after their products had completed
+          // warp-uniform (tensor-memory loads and stores are warp-collective)
           if (__any_sync(0xffffffffu, m_new > m_used + 8.f)) {
             const float m_to = fmaxf(m_used, m_new);
             const float alpha = m_to == -INFINITY ? 1.f : exp2f(m_used - m_to);
             if (j > jf) {
+              wait(odone(x), cnt - 1);  // O_x with every block before this one
+              tc_fence_after();
 #pragma unroll 1
               for (int c4 = 0; c4 < D / 32; ++c4) {
                 uint32_t o[32];
@@ -959,12 +1001,17 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
             sv[c] = Elem<T>::pack(p0, p1);
           }
           l += ((ls[0] + ls[1]) + (ls[2] + ls[3])) + ((ls[4] + ls[5]) + (ls[6] + ls[7]));
-          tmem_st64(tS(x) + lane_off, sv);
+          if (two) {  // over the other tile's S, once that has loaded it (B: the one A is ahead with)
+            wait(sload(1 - x), pairs + j + (x == 1 && j + 1 < g.nb ? 1 : 0));
+            tc_fence_after();
+          }
+          tmem_st64(tS(two ? 1 - x : x) + lane_off, sv);
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(pfull(x));
       }
+      if (two) pairs += g.nb;
       wait(odone(x), cnt - 1);
       if (!ok) break;
       tc_fence_after();
