@@ -38,13 +38,13 @@
 namespace qd {
 
 constexpr int kPgThreads = 384;  // warps 0-3 softmax A, 4-7 softmax B, 8 producer, 9 MMA, 10-11 only start up
-// registers per thread after the start: 2 * 208 + 88 = 3 * 168, what the launch gave the three warpgroups
-constexpr int kPgSoftmaxRegs = 208, kPgOtherRegs = 88;
+// registers per thread after the start: 2 * 224 + 56 = 3 * 168, what the launch gave the three warpgroups
+constexpr int kPgSoftmaxRegs = 224, kPgOtherRegs = 56;
 constexpr int kPgKeys = 128;     // keys per block
 constexpr int kPgBox = 128 * 128;  // [128 rows][64 dims] of 16 bits
 constexpr int kFewRows = 16;       // rows of a few-row unit (MMA N)
 constexpr int kFewP = 2 * kFewRows * 128;  // its P: 2 halves of 64 keys x 16 rows of 128 B
-constexpr int kPgUnitCost = 1;     // a unit's fixed cost (Q, epilogue) in key blocks, for the split
+constexpr int kPgUnitCost = 2;     // a unit's fixed cost (Q, epilogue) in key blocks, for the split
 
 struct alignas(64) PagedAttnArgs {
   CUtensorMap tq, tqf, tq1, tk, tv;  // q boxes: a whole tile's tokens, as many as make 16 rows, one
@@ -53,9 +53,12 @@ struct alignas(64) PagedAttnArgs {
   float* lse;
   int64_t ldo, ld_lse;
   int group, tpt, tpf;        // heads per KV head, tokens per tile and per 16 rows (0: a group is larger)
+  int inv_group;              // row / group = row * inv_group >> 16 for the rows of a tile
   int period, period_blocks;  // ceil sums over tile pairs repeat every `period` pairs, `period_blocks` blocks on
   float scale_log2;
-  float* partials;  // [2 * grid slots][2 tiles][D / 4][128] float4, then [slots][2][128] float2
+  // [2 * grid slots][2 tiles] of 128 x D floats ([D / 4][128 rows][4], few-row units [rows][D]), then the rows'
+  // (m, l) [slots][2][128]
+  float* partials;
   int* tickets;     // [grid][2]
 };
 
@@ -149,16 +152,16 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
       : "memory");
 }
 
-// 128 consecutive columns of this thread's lane in one load, waited
-__device__ __forceinline__ void tmem_ld128(uint32_t taddr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x128.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63, %64, %65, %66, %67, %68, %69, %70, %71, %72, %73, %74, %75, %76, %77, %78, %79, %80, %81, %82, %83, %84, %85, %86, %87, %88, %89, %90, %91, %92, %93, %94, %95, %96, %97, %98, %99, %100, %101, %102, %103, %104, %105, %106, %107, %108, %109, %110, %111, %112, %113, %114, %115, %116, %117, %118, %119, %120, %121, %122, %123, %124, %125, %126, %127}, [%128];\n"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]), "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]), "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]), "=r"(r[80]), "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]), "=r"(r[88]), "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]), "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]), "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]), "=r"(r[111]), "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]), "=r"(r[118]), "=r"(r[119]), "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
-      : "r"(taddr)
-      : "memory");
+// 64 consecutive columns of this thread's lane, not waited for; and the wait, which ties the registers
+__device__ __forceinline__ void tmem_ld64_raw(uint32_t taddr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+               : "r"(taddr));
 }
-
+__device__ __forceinline__ void tmem_wait_ld64(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]), "+r"(r[32]), "+r"(r[33]), "+r"(r[34]), "+r"(r[35]), "+r"(r[36]), "+r"(r[37]), "+r"(r[38]), "+r"(r[39]), "+r"(r[40]), "+r"(r[41]), "+r"(r[42]), "+r"(r[43]), "+r"(r[44]), "+r"(r[45]), "+r"(r[46]), "+r"(r[47]), "+r"(r[48]), "+r"(r[49]), "+r"(r[50]), "+r"(r[51]), "+r"(r[52]), "+r"(r[53]), "+r"(r[54]), "+r"(r[55]), "+r"(r[56]), "+r"(r[57]), "+r"(r[58]), "+r"(r[59]), "+r"(r[60]), "+r"(r[61]), "+r"(r[62]), "+r"(r[63])::"memory");
+}
 // One request on the line of key blocks.
 struct PgReq {
   int row0, n, pos0, kv;  // token rows, the first one's position, keys (cut to the table row)
@@ -210,45 +213,42 @@ struct PgLine {
   }
 };
 
-// Joins a cut unit's pieces of one tile (x): 128 threads, thread r. kItems float4 of the output at a time, with
-// kPieces pieces' loads in flight for each.
-template <typename T, int D, int kItems, int kPieces>
-__device__ __forceinline__ void pg_join_items(const PagedAttnArgs& a, const PgSeg& g, int x, int r, int rows, int t0) {
-  const float4* const po = reinterpret_cast<const float4*>(a.partials);
-  const float2* const pm = reinterpret_cast<const float2*>(a.partials + (int64_t)2 * gridDim.x * 2 * D * 128);
-  const int total = rows * (D / 4);
+// Joins a cut few-row unit's pieces (rows of D floats) in the order of their keys: four warps, a row per D / 4
+// lanes, kRows such rows at a time with kPieces pieces' loads in flight for each.
+template <typename T, int D, int kRows, int kPieces>
+__device__ __forceinline__ void pg_join_few(const PagedAttnArgs& a, const PgSeg& g, int r, int rows) {
+  constexpr int kAt = 128 / (D / 4);  // rows under way per step of kRows
+  const int c4 = r % (D / 4), first = r / (D / 4);
+  const float2* const pm = reinterpret_cast<const float2*>(a.partials + (int64_t)2 * gridDim.x * 2 * 128 * D);
 #pragma unroll 1
-  for (int e0 = r; e0 < total; e0 += 128 * kItems) {
-    int row[kItems], c4[kItems];
-    float M[kItems], L[kItems];
-    float4 acc[kItems];
+  for (int r0 = first; r0 < rows; r0 += kAt * kRows) {
+    float M[kRows], L[kRows];
+    float4 acc[kRows];
 #pragma unroll
-    for (int i = 0; i < kItems; ++i) {
-      const int e = min(e0 + 128 * i, total - 1);
-      c4[i] = e / rows;
-      row[i] = e - c4[i] * rows;
+    for (int i = 0; i < kRows; ++i) {
       M[i] = -INFINITY;
       L[i] = 0.f;
       acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
 #pragma unroll 1
     for (int q0 = 0; q0 < g.nc; q0 += kPieces) {
-      float2 ml[kPieces][kItems];
-      float4 v[kPieces][kItems];
+      float2 ml[kPieces][kRows];
+      float4 v[kPieces][kRows];
 #pragma unroll
       for (int q = 0; q < kPieces; ++q) {
         const int qq = min(q0 + q, g.nc - 1);  // past the last piece: the last again, not counted
-        const int64_t slot = (2 * (g.c0 + qq) + (qq == 0 ? 1 : 0)) * 2 + x;
+        const int64_t at = ((2 * (g.c0 + qq) + (qq == 0 ? 1 : 0)) * 2) * 128;
 #pragma unroll
-        for (int i = 0; i < kItems; ++i) {
-          ml[q][i] = __ldcg(pm + slot * 128 + row[i]);
-          v[q][i] = __ldcg(po + (slot * (D / 4) + c4[i]) * 128 + row[i]);
+        for (int i = 0; i < kRows; ++i) {
+          const int64_t row = at + min(r0 + kAt * i, rows - 1);
+          ml[q][i] = __ldcg(pm + row);
+          v[q][i] = __ldcg(reinterpret_cast<const float4*>(a.partials + row * D) + c4);
         }
       }
 #pragma unroll
       for (int q = 0; q < kPieces; ++q)
 #pragma unroll
-        for (int i = 0; i < kItems; ++i)
+        for (int i = 0; i < kRows; ++i)
           if (q0 + q < g.nc && ml[q][i].y > 0.f) {  // a piece in which the row saw no key counts for nothing
             const float mn = fmaxf(M[i], ml[q][i].x), fa = exp2f(M[i] - mn), fb = exp2f(ml[q][i].x - mn);
             M[i] = mn;
@@ -260,23 +260,18 @@ __device__ __forceinline__ void pg_join_items(const PagedAttnArgs& a, const PgSe
           }
     }
 #pragma unroll
-    for (int i = 0; i < kItems; ++i)
-      if (e0 + 128 * i < total) {
+    for (int i = 0; i < kRows; ++i) {
+      const int row = r0 + kAt * i;
+      if (row < rows) {
         const float inv = L[i] > 0.f ? 1.0f / L[i] : 0.f;
-        const int tok = row[i] / a.group, t2 = g.row0 + t0 + tok, h2 = g.head * a.group + row[i] - tok * a.group;
-        *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + t2 * a.ldo + (int64_t)h2 * D + 4 * c4[i]) =
+        const int tok = (row * a.inv_group) >> 16, t2 = g.row0 + tok, h2 = g.head * a.group + row - tok * a.group;
+        *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + t2 * a.ldo + (int64_t)h2 * D + 4 * c4) =
             make_uint2(Elem<T>::pack(acc[i].x * inv, acc[i].y * inv), Elem<T>::pack(acc[i].z * inv, acc[i].w * inv));
-        if (c4[i] == 0 && a.lse)
+        if (c4 == 0 && a.lse)
           a.lse[t2 * a.ld_lse + h2] = L[i] > 0.f ? (M[i] + __log2f(L[i])) * 0.69314718055994531f : -INFINITY;
       }
+    }
   }
-}
-template <typename T, int D>
-__device__ __forceinline__ void pg_join(const PagedAttnArgs& a, const PgSeg& g, int x, int r, int rows, int t0) {
-  if (rows * (D / 4) > 256)
-    pg_join_items<T, D, 2, 2>(a, g, x, r, rows, t0);
-  else
-    pg_join_items<T, D, 1, 4>(a, g, x, r, rows, t0);
 }
 
 template <typename T, int D>
@@ -525,12 +520,12 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
     constexpr uint32_t id_o = (umma_idesc_bf16(D, false, true) & ~kTypes) | kind;
     constexpr uint32_t id_sf = (umma_idesc_bf16(kFewRows) & ~kTypes) | kind;
     constexpr uint32_t id_of = (umma_idesc_bf16(kFewRows, true, false) & ~kTypes) | kind;
-    // operand descriptors: a start address in units of 16 B below, strides above; steps are plain additions
-    const uint64_t d_q = umma_desc_sw128(sb + Lay::q), d_k = umma_desc_sw128(sb + Lay::kv);
-    const uint64_t d_v = umma_desc_sw128(sb + Lay::kv, kPgBox, 1024);
+    // low words of the operand descriptors: a start address in units of 16 B, so steps are plain additions
+    const uint32_t d_q = umma_desc_lo(sb + Lay::q), d_k = umma_desc_lo(sb + Lay::kv);
+    const uint32_t d_v = umma_desc_lo(sb + Lay::kv, kPgBox);
     // few rows, head_dim 64: the 64 upper rows of O^T repeat the lower ones (block stride 0)
-    const uint64_t d_vf = umma_desc_sw128(sb + Lay::kv, D == 128 ? kPgBox : 0, 1024);
-    constexpr uint64_t kItem16 = Lay::kItem >> 4;
+    const uint32_t d_vf = umma_desc_lo(sb + Lay::kv, D == 128 ? kPgBox : 0);
+    constexpr uint32_t kItem16 = Lay::kItem >> 4;
     int slot = 0, pc[2] = {0, 0}, units[2] = {0, 0};
     uint32_t phase = 0, quse = 0;  // of full(slot); bit r: the phase of qfull(r)
     int pairs = 0;                 // blocks of units of two tiles so far
@@ -563,10 +558,10 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
       wait(full(k.slot), k.phase);
       tc_fence_after();
       if (ok) {
-        const uint64_t q = d_q + reg * kItem16, kt = d_k + k.slot * kItem16;
+        const uint32_t q = d_q + reg * kItem16, kt = d_k + k.slot * kItem16;
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) {  // 16 dims per MMA: +32 B inside a 64-dim half, the next half after 4
-          const uint64_t step = ((d >> 2) * kPgBox + (d & 3) * 32) >> 4;
+          const uint32_t step = ((d >> 2) * kPgBox + (d & 3) * 32) >> 4;
           umma_f16(tS(x), (few ? kt : q) + step, (few ? q : kt) + step, few ? id_sf : id_s, d > 0 ? 1u : 0u);
         }
       }
@@ -577,12 +572,11 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
       constexpr int x = decltype(xc)::value;
       constexpr bool few = decltype(modec)::value == 1, pair = decltype(modec)::value == 2;
       if (first && units[x] > 0) wait(ofree(x), units[x] - 1);
+      const uint32_t vt = (few ? d_vf : d_v) + v.slot * kItem16;
+      const uint32_t pt = umma_desc_lo(sb + Lay::few_p(reg, x));
       wait(pfull(x), pc[x]);
-      ++pc[x];
       tc_fence_after();
       if (ok) {
-        const uint64_t vt = (few ? d_vf : d_v) + v.slot * kItem16;
-        const uint64_t pt = umma_desc_sw128(sb + Lay::few_p(reg, x));
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk) {  // 16 keys per MMA: 8 columns of P pairs; V two 8-key atoms
           const uint32_t acc = kk ? 1u : first ? 0u : 1u;
@@ -592,6 +586,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
             umma_f16_ts(tO(x), tS(pair ? 1 - x : x) + 8 * kk, vt + kk * (2048 >> 4), id_o, acc);
         }
       }
+      ++pc[x];
       umma_commit(odone(x));
     };
     // `rows` of V are keys; the ones past them hold anything and are zeroed (the whole warp comes here)
@@ -620,8 +615,8 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
         wait_pv(1);
         issue_s(c0, c0, 0, ahead(0));
         issue_s(c1, c0, 1, ahead(0));
-        umma_commit(empty(slot));
         if (g.nb > 1) {
+          umma_commit(empty(slot));
           wait(sload(0), pairs);
           issue_s(c0, c0, 0, ahead(2));
         } else {
@@ -640,14 +635,15 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
           if (j + 1 < g.nb) {
             wait_pv(0);  // S_B's columns hold P_A
             issue_s(c1, c0, 1, k1);
-            umma_commit(empty(k1.slot));
             if (j + 2 == g.nb) {
               umma_commit(qempty(0));
               umma_commit(qempty(1));
+            } else {
+              umma_commit(empty(k1.slot));
             }
           }
           issue_pv(c1, c2, 0, v, j == 0);
-          umma_commit(empty(v.slot));
+          if (j + 1 < g.nb) umma_commit(empty(v.slot));  // the last K and V slots: the softmax warps' to give back
           if (j + 2 < g.nb) {
             wait_pv(1);
             issue_s(c0, c0, 0, k2);
@@ -683,7 +679,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
         if (leader) {
           wait(full(v.slot), v.phase);
           issue_pv(xc, fewc, reg, v, j < 2);
-          umma_commit(empty(v.slot));
+          if (few || j + 1 < g.nb) umma_commit(empty(v.slot));  // else the softmax warps' to give back
           if (j + 2 < g.nb) {
             wait_pv(decltype(xc)::value);
             issue_s(xc, fewc, reg, k);
@@ -729,7 +725,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
     // ------------------------------------------------------------ softmax and epilogue: warpgroup x = tile x
     const int x = warp >> 2, r = 32 * (warp & 3) + lane;  // (r: the row, no longer the request)
     const uint32_t lane_off = (uint32_t)(32 * (warp & 3)) << 16;
-    int cnt = 0, pairs = 0, meets = 0, joins = 0;
+    int cnt = 0, pairs = 0, blocks = 0, meets = 0, joins = 0;  // blocks: of all units so far
     bool ok = true;
     auto wait = [&](uint32_t bar, int parity) {
       if (ok) ok = mbar_wait_abort(bar, parity & 1, a.b.err, kErrWaitFull, abort);
@@ -740,23 +736,25 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
       if (lane == 0) mbar_arrive(group(x));
       wait(group(x), meets++);
     };
-    float4* const po = reinterpret_cast<float4*>(a.partials);
-    float2* const pm = reinterpret_cast<float2*>(a.partials + (int64_t)2 * gridDim.x * 2 * D * 128);
-    auto part_o = [&](int slot, int c4, int row) { return po + ((int64_t)(slot * 2 + x) * (D / 4) + c4) * 128 + row; };
+    float2* const pm = reinterpret_cast<float2*>(a.partials + (int64_t)2 * gridDim.x * 2 * 128 * D);
+    // a few-row piece's row, and four dims of a tile's rows
+    auto part_o = [&](int slot, int row) { return a.partials + ((int64_t)slot * 2 * 128 + row) * D; };
+    auto part_c = [&](int slot, int c4) {
+      return reinterpret_cast<float4*>(a.partials) + ((int64_t)(slot * 2 + x) * (D / 4) + c4) * 128;
+    };
     auto part_m = [&](int slot, int row) { return pm + (slot * 2 + x) * 128 + row; };
-    // A cut unit: whoever finishes last joins the pieces, in the order of their keys. The pieces' stores are
-    // made visible by the barrier and the ticket (release is cumulative).
-    auto finish = [&](const PgSeg& g, int rows, int t0) __attribute__((always_inline)) {
+    // A cut unit: whoever finishes last (true) joins the pieces. Their stores are made visible by the barrier
+    // and the ticket (release is cumulative).
+    auto is_last = [&](const PgSeg& g) {
       meet();
-      if (!ok) return;
+      if (!ok) return false;
       if (r == 0) {
         const bool last = atom_add_acq_rel(a.tickets + 2 * g.c0 + x, 1) == g.nc - 1;
         if (last) a.tickets[2 * g.c0 + x] = 0;
         misc[10 + x] = last;
       }
       meet();
-      if (!ok || !misc[10 + x]) return;
-      pg_join<T, D>(a, g, x, r, rows, t0);
+      return ok && misc[10 + x] != 0;
     };
     // A unit of at most kC rows on this warpgroup's blocks: thread r has key r of the block (and, of O^T, dim r);
     // what there is one of per row (maximum, factors) is lane c's for row c, the same in all four warps.
@@ -884,7 +882,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
           L = L * fa + ((s2.x + s2.y) + (s2.z + s2.w)) * fb;
           M = mn;
         }
-        const int tok = lane / a.group, hq = g.head * a.group + lane - tok * a.group;
+        const int tok = (lane * a.inv_group) >> 16, hq = g.head * a.group + lane - tok * a.group;
         row_at = (g.row0 + tok) * a.ldo + (int64_t)hq * D;
         if (g.whole) {
           const float inv = L > 0.f ? 1.0f / L : 0.f;
@@ -906,7 +904,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
           if (g.whole)
             reinterpret_cast<uint16_t*>(a.out)[to + r] = (uint16_t)Elem<T>::pack(v, 0.f);
           else
-            __stcg(reinterpret_cast<float*>(part_o(g.slot, r >> 2, c)) + (r & 3), v);
+            __stcg(part_o(g.slot, c) + r, v);
         }
       }
       tc_fence_before();
@@ -923,11 +921,12 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
       __syncwarp();
       if (lane == 0) mbar_arrive(segempty(seg));
       if (g.nb == 0) break;
+      blocks += g.nb;
       const bool two = g.region < 0, joined = !two && g.nb > 1;
       if (x == 1 && !two && !joined) continue;  // one tile, one block
       const int t0 = two ? x * a.tpt : 0;       // this tile's first token
       const int ntok = min(a.tpt, g.ntok - t0), rows = ntok * a.group;
-      const int my_tok = r / a.group, tok = g.row0 + t0 + my_tok;
+      const int my_tok = (r * a.inv_group) >> 16, tok = g.row0 + t0 + my_tok;
       const int head = g.head * a.group + r - my_tok * a.group;
       // keys this row sees: up to its own position (MMA rows past the last token hold anything)
       const int lim = r < rows ? min(g.kv, g.pos0 + t0 + my_tok + 1) : INT_MAX;
@@ -941,7 +940,12 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
           few_rows(Const<kFewRows>(), g, rows, joined);
         if (!ok) break;
         if (x == 1 || g.whole) continue;
-        finish(g, rows, t0);
+        if (is_last(g)) {
+          if (rows <= 4)
+            pg_join_few<T, D, 1, 4>(a, g, r, rows);
+          else
+            pg_join_few<T, D, 2, 2>(a, g, r, rows);
+        }
         if (!ok) break;
         continue;
       }
@@ -951,26 +955,38 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
         if (!ok) break;
         tc_fence_after();
         uint32_t sv[128];
-        if (!idle) tmem_ld128(tS(x) + lane_off, sv);
+        if (!idle) {
+          tmem_ld64(tS(x) + lane_off, sv);
+          tmem_ld64_raw(tS(x) + lane_off + 64, sv + 64);
+        }
+        const int left = lim - (g.j0 + j) * kPgKeys;
+        float m_new = -INFINITY;
+        if (!idle) {
+          const bool part = __any_sync(0xffffffffu, left < kPgKeys);
+          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            uint32_t* const v = sv + 64 * hf;
+            if (hf) tmem_wait_ld64(v);
+            if (part) {
+#pragma unroll
+              for (int e = 0; e < 64; ++e)
+                if (64 * hf + e >= left) v[e] = __float_as_uint(-INFINITY);
+            }
+#pragma unroll
+            for (int e = 0; e < 64; e += 8)
+#pragma unroll
+              for (int c = 0; c < 4; ++c)
+                m4[c] = pg_max3(m4[c], __uint_as_float(v[e + 2 * c]), __uint_as_float(v[e + 2 * c + 1]));
+          }
+          m_new = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * a.scale_log2;
+        }
         if (two) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(sload(x));
         }
         if (!idle) {
-          const int left = lim - (g.j0 + j) * kPgKeys;
-          if (__any_sync(0xffffffffu, left < kPgKeys)) {
-#pragma unroll
-            for (int e = 0; e < 128; ++e)
-              if (e >= left) sv[e] = __float_as_uint(-INFINITY);
-          }
-          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int e = 0; e < 128; e += 8)
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-              m4[c] = pg_max3(m4[c], __uint_as_float(sv[e + 2 * c]), __uint_as_float(sv[e + 2 * c + 1]));
-          const float m_new = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * a.scale_log2;
           // warp-uniform (tensor-memory loads and stores are warp-collective)
           if (__any_sync(0xffffffffu, m_new > m_used + 8.f)) {
             const float m_to = fmaxf(m_used, m_new);
@@ -990,17 +1006,19 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
             l *= alpha;
             m_used = m_to;
           }
+        }
+        if (!idle) {
           const float nm = m_used == -INFINITY ? 0.f : -m_used;  // a row that has seen no key yet: P = 0
-          float ls[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+          float ls[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int c = 0; c < 64; ++c) {  // P pair c = keys 2c, 2c + 1, packed in place over the scores
             const float p0 = pg_ex2(fmaf(__uint_as_float(sv[2 * c]), a.scale_log2, nm));
             const float p1 = pg_ex2(fmaf(__uint_as_float(sv[2 * c + 1]), a.scale_log2, nm));
-            ls[(2 * c) & 7] += p0;
-            ls[(2 * c + 1) & 7] += p1;
+            ls[(2 * c) & 3] += p0;
+            ls[(2 * c + 1) & 3] += p1;
             sv[c] = Elem<T>::pack(p0, p1);
           }
-          l += ((ls[0] + ls[1]) + (ls[2] + ls[3])) + ((ls[4] + ls[5]) + (ls[6] + ls[7]));
+          l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
           if (two) {  // over the other tile's S, once that has loaded it (B: the one A is ahead with)
             wait(sload(1 - x), pairs + j + (x == 1 && j + 1 < g.nb ? 1 : 0));
             tc_fence_after();
@@ -1037,12 +1055,29 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
         l = l * fa + o.y * fb;
         m_used = m;
       }
+      // Rows go out through the shared memory of the unit's last V block (tile B: K block), which is still this
+      // warpgroup's: thread r lays down row r, 16-byte chunks swizzled by row, and whole rows are stored from
+      // there (row by row from the registers would be partial sectors, 32 lines an instruction: 7 k cycles).
+      const int it = 2 * blocks - 1 - (two ? x : 0), slot = it % kSlots;
+      char* const stage = smem + Lay::kv + slot * Lay::kItem;
+      auto lay_down = [&](int c, const uint32_t* w) {  // dims 8 c .. 8 c + 7, packed
+        *reinterpret_cast<uint4*>(stage + r * (2 * D) + ((c ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+      };
+      auto store_rows = [&]() {
+        meet();
+#pragma unroll 1
+        for (int i = r; i < rows * (D / 8); i += 128) {
+          const int row = i / (D / 8), c = i % (D / 8), rt = (row * a.inv_group) >> 16;
+          const uint4 v = *reinterpret_cast<const uint4*>(stage + row * (2 * D) + ((c ^ (row & 7)) << 4));
+          T* const to = reinterpret_cast<T*>(a.out) + (g.row0 + t0 + rt) * a.ldo +
+                        (int64_t)(g.head * a.group + row - rt * a.group) * D + 8 * c;
+          *reinterpret_cast<uint4*>(to) = v;
+        }
+      };
+      const float norm = !g.whole ? 1.f : l > 0.f ? 1.0f / l : 0.f;  // a piece's rows stay as they are
+      fa *= norm;
+      fb *= norm;
       if (!idle) {
-        // a whole unit's rows go out normalised, a piece's as they are
-        const float norm = !g.whole ? 1.f : l > 0.f ? 1.0f / l : 0.f;
-        fa *= norm;
-        fb *= norm;
-        T* const orow = reinterpret_cast<T*>(a.out) + tok * a.ldo + (int64_t)head * D;
 #pragma unroll 1
         for (int c4 = 0; c4 < D / 32; ++c4) {
           uint32_t o[32];
@@ -1056,27 +1091,19 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
             for (int e = 0; e < 32; ++e)
               o[e] = __float_as_uint(fmaf(__uint_as_float(ob[e]), fb, __uint_as_float(o[e])));
           }
-          if (r < rows && g.whole) {
-            uint4* d4 = reinterpret_cast<uint4*>(orow + 32 * c4);
+          if (g.whole) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              uint32_t w[4];
+            for (int e = 0; e < 16; ++e) o[e] = Elem<T>::pack(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1]));
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                w[e] = Elem<T>::pack(__uint_as_float(o[8 * c + 2 * e]), __uint_as_float(o[8 * c + 2 * e + 1]));
-              d4[c] = make_uint4(w[0], w[1], w[2], w[3]);
-            }
+            for (int c = 0; c < 4; ++c) lay_down(4 * c4 + c, o + 4 * c);
           } else if (r < rows) {
 #pragma unroll
             for (int c = 0; c < 8; ++c)
-              __stcg(part_o(g.slot, 8 * c4 + c, r),
-                     make_float4(__uint_as_float(o[4 * c]), __uint_as_float(o[4 * c + 1]), __uint_as_float(o[4 * c + 2]),
-                                 __uint_as_float(o[4 * c + 3])));
+              __stcg(part_c(g.slot, 8 * c4 + c) + r, make_float4(__uint_as_float(o[4 * c]), __uint_as_float(o[4 * c + 1]),
+                                                                 __uint_as_float(o[4 * c + 2]), __uint_as_float(o[4 * c + 3])));
           }
         }
         if (r < rows && !g.whole) __stcg(part_m(g.slot, r), make_float2(m_used, l));
-        if (r < rows && g.whole && a.lse)
-          a.lse[tok * a.ld_lse + head] = l > 0.f ? (m_used + __log2f(l)) * 0.69314718055994531f : -INFINITY;
       }
       tc_fence_before();
       __syncwarp();
@@ -1084,9 +1111,65 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
         mbar_arrive(ofree(x));
         if (joined) mbar_arrive(ofree(1));
       }
-      if (g.whole) continue;
-      finish(g, rows, t0);
+      bool out_rows = g.whole;
+      if (!g.whole && is_last(g)) {  // join the pieces in the order of their keys: thread = row
+        out_rows = true;
+        float M = -INFINITY, L = 0.f;
+        const int row = min(r, rows - 1);
+        auto slot_of = [&](int q) { return 2 * (g.c0 + q) + (q == 0 ? 1 : 0); };
+#pragma unroll 1
+        for (int q = 0; q < g.nc; ++q) M = fmaxf(M, __ldcg(part_m(slot_of(q), row)).x);
+        const float base = M == -INFINITY ? 0.f : M;
+#pragma unroll 1
+        for (int q = 0; q < g.nc; ++q) {
+          const float2 ml = __ldcg(part_m(slot_of(q), row));
+          L += ml.y * exp2f(ml.x - base);
+        }
+        const float inv = L > 0.f ? 1.0f / L : 0.f;
+#pragma unroll 1
+        for (int c8 = 0; c8 < D / 8; c8 += 2) {  // 16 dims at a time
+          float acc[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+#pragma unroll 1
+          for (int q = 0; q < g.nc; q += 2) {
+            const int q1 = min(q + 1, g.nc - 1);
+            float4 v[2][4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              v[0][c] = __ldcg(part_c(slot_of(q), 2 * c8 + c) + row);
+              v[1][c] = __ldcg(part_c(slot_of(q1), 2 * c8 + c) + row);
+            }
+            const float w0 = exp2f(__ldcg(part_m(slot_of(q), row)).x - base) * inv;
+            const float w1 = q + 1 < g.nc ? exp2f(__ldcg(part_m(slot_of(q1), row)).x - base) * inv : 0.f;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              acc[4 * c] = fmaf(v[1][c].x, w1, fmaf(v[0][c].x, w0, acc[4 * c]));
+              acc[4 * c + 1] = fmaf(v[1][c].y, w1, fmaf(v[0][c].y, w0, acc[4 * c + 1]));
+              acc[4 * c + 2] = fmaf(v[1][c].z, w1, fmaf(v[0][c].z, w0, acc[4 * c + 2]));
+              acc[4 * c + 3] = fmaf(v[1][c].w, w1, fmaf(v[0][c].w, w0, acc[4 * c + 3]));
+            }
+          }
+          uint32_t w[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w[e] = Elem<T>::pack(acc[2 * e], acc[2 * e + 1]);
+          lay_down(c8, w);
+          lay_down(c8 + 1, w + 4);
+        }
+        m_used = M;
+        l = L;
+      }
       if (!ok) break;
+      if (out_rows) {
+        store_rows();
+        if (!ok) break;
+        if (r < rows && a.lse)
+          a.lse[tok * a.ld_lse + head] = l > 0.f ? (m_used + __log2f(l)) * 0.69314718055994531f : -INFINITY;
+      }
+      fence_proxy_async_smem();  // the slot's next contents come by TMA
+      meet();
+      if (!ok) break;
+      if (r == 0) mbar_arrive(empty(slot));
     }
   }
   tc_fence_before();
@@ -1144,8 +1227,8 @@ extern "C" int qd_paged_attn(const void* q, int64_t ldq, int dtype, int64_t toke
     return set_error(QD_ERR_ARG, "paged attention: q / out / lse null, misaligned or with a bad stride (%lld, %lld, %lld), or scale %g",
                      (long long)ldq, (long long)ldo, (long long)ld_lse, (double)scale);
   const PagedAttnPlan plan = paged_attn_plan(grid < 1 ? 1 : grid, head_dim);
-  if (grid < 1 || !scratch || scratch_bytes < plan.bytes || !aligned16(scratch))
-    return set_error(QD_ERR_SCRATCH, "paged attention: grid %d needs %lld B of 16-byte aligned scratch (have %lld)", grid,
+  if (grid < 1 || !scratch || scratch_bytes < plan.bytes || (reinterpret_cast<uintptr_t>(scratch) & 31))
+    return set_error(QD_ERR_SCRATCH, "paged attention: grid %d needs %lld B of 32-byte aligned scratch (have %lld)", grid,
                      (long long)plan.bytes, (long long)scratch_bytes);
   if (tokens == 0) return QD_OK;
   const PFN_cuTensorMapEncodeTiled_v12000 encode = tensor_map_encoder();
@@ -1153,6 +1236,7 @@ extern "C" int qd_paged_attn(const void* q, int64_t ldq, int dtype, int64_t toke
   a.group = nq_heads / nkv_heads;
   a.tpt = 128 / a.group;
   a.tpf = kFewRows / a.group;
+  a.inv_group = 65536 / a.group + 1;  // exact: the excess is below 128 / 65536, a fraction's distance to 1 at least 1 / 128
   const CUtensorMapDataType type = dtype == QD_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const cuuint32_t estr[4] = {1, 1, 1, 1};
   auto map4 = [&](CUtensorMap* m, const void* base, const cuuint64_t* dims, const cuuint64_t* strides,
