@@ -10,10 +10,10 @@
 // sums by warp are sums in index order. Values that all CTAs need go to every CTA's memory (distributed
 // shared memory) behind a cluster barrier.
 //   1  load, largest logit
-//   2  (top-k or top-p) a histogram of number and weight over 2048 equal steps of d down to the weights that
-//      round to 0, summed over the cluster by shares of bins: the bin in which the prefix ends is exact
-//   3  the tokens of that bin, a few hundred, are gathered into one CTA, which finds the last one kept; a
-//      bin of more than that (many ties, a high temperature) is cut again, by key, first
+//   2  (top-k or top-p) a histogram of number and weight over up to 2048 equal steps of d down to the weights
+//      that round to 0, summed over the cluster by shares of bins: the bin in which the prefix ends is exact
+//   3  the tokens of that bin, a few hundred, are gathered into one CTA, which sorts them and finds the last
+//      one kept; a bin of more than 512 (many ties, a high temperature) is cut again, by key, first
 //   4  the kept weight of every warp, the warp in which u falls, and a walk through its tokens
 // Without top-k and top-p only 1 and 4 are left, and the weights are computed once. What bounds it: the
 // instructions per logit (exponential, conversion, 64-bit sums; shared-memory atomics in 2) for many rows,
@@ -30,7 +30,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kSampleThreads = 512, kSampleWarps = kSampleThreads / 32;
 constexpr int kSampleBins = 2048;
-constexpr int kSampleList = 512;                // tokens that one CTA resolves by comparing each with each
+constexpr int kSampleList = kSampleThreads;     // tokens that one CTA sorts, one a thread
 constexpr float kSampleOne = 1099511627776.0f;  // 2^40
 constexpr float kSampleDeep = 28.5f;            // e^-28.42 = 2^-41: beyond, weights round to 0
 constexpr int64_t kSampleMaxVocab = 1 << 18;    // 2^18 weights of 2^40 stay below 2^63
@@ -102,20 +102,32 @@ __device__ __forceinline__ uint32_t logit_key(float l) {
 __device__ __forceinline__ float key_logit(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
-// d = (l - m) / temperature of the definition (NaN for a NaN logit: below every bound), and the weight in
-// units of 2^-40
-__device__ __forceinline__ float logit_depth(float l, float m, float inv_t) {
-  return l == m ? 0.f : l == -INFINITY ? l : __fmul_rn(__fsub_rn(l, m), inv_t);
+// d = (l - m) / temperature of the definition, for a finite m (NaN for a NaN logit: below every bound)
+__device__ __forceinline__ float logit_depth(float l, float m, float inv_t) { return __fmul_rn(__fsub_rn(l, m), inv_t); }
+// w = expf(d) <= 1 as a whole number of 2^-40: hi = floor(w 2^20) and lo = the rest, rounded to even, each in
+// the low bits of a float of 2^23 (adding 2^23 rounds to a whole number). Six instructions and no carry where
+// a 64-bit conversion and addition take some twenty; the bits above are taken off once per sum.
+constexpr uint32_t kHalfBits = 0x4b000000u;
+__device__ __forceinline__ void weight_halves(float w, uint32_t& hi, uint32_t& lo) {
+  const float h = __fmaf_rd(w, 1048576.0f, 8388608.0f);
+  const float rest = __fmaf_rn(w, 1048576.0f, -(h - 8388608.0f));
+  hi = __float_as_uint(h);
+  lo = __float_as_uint(__fmaf_rn(rest, 1048576.0f, 8388608.0f));
 }
-__device__ __forceinline__ uint64_t depth_weight(float d) { return __float2ull_rn(expf(d) * kSampleOne); }
-__device__ __forceinline__ int depth_bin(float d) {
-  return min((int)(-d * (kSampleBins / kSampleDeep)), kSampleBins - 1);
+__device__ __forceinline__ uint64_t depth_weight(float d) {
+  uint32_t hi, lo;
+  weight_halves(expf(d), hi, lo);
+  return ((uint64_t)(hi - kHalfBits) << 20) + (lo - kHalfBits);
 }
+__device__ __forceinline__ int depth_bin(float d, float per_d, int bins) { return min((int)(-d * per_d), bins - 1); }
 
+// 64-bit sum over the warp by 16-bit pieces: four reduction instructions in place of ten dependent shuffles
 __device__ __forceinline__ uint64_t warp_sum64(uint64_t v) {
+  uint64_t s = 0;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+  for (int i = 0; i < 4; ++i)
+    s += (uint64_t)__reduce_add_sync(0xffffffffu, (uint32_t)(v >> (16 * i)) & 0xffffu) << (16 * i);
+  return s;
 }
 __device__ __forceinline__ uint64_t warp_scan64(uint64_t v, int lane) {  // inclusive
 #pragma unroll
@@ -134,15 +146,15 @@ struct Bracket {
   uint64_t count, weight;
   int bin, n;
 };
-// The cluster's bins of which this thread has the sums: up to 4, `count` and `weight` before the first.
+// The bin of which this thread has the cluster's sums (none: 0), and the sums before it.
 struct BinSums {
-  uint32_t n[4];
-  uint64_t w[4], count, weight, total_count, total_weight;
+  uint32_t n;
+  uint64_t w, count, weight, total_count, total_weight;
 };
 
 struct SampleShared {
   uint32_t cnt[kSampleBins], lo[kSampleBins], hi[kSampleBins];  // this CTA's histogram
-  uint64_t list[kSampleList], list_w[kSampleList];              // gathered tokens (key, ~index), their weights
+  uint64_t list[kSampleList];                                   // gathered tokens (key, ~index)
   Pair64 xch[2][kSampleMaxCluster];                             // a value of every CTA, two exchanges in turn
   uint64_t warp_a[kSampleWarps], warp_b[kSampleWarps];
   Bracket found;
@@ -153,7 +165,7 @@ struct SampleShared {
 constexpr int kSampleShared = (sizeof(SampleShared) + 15) / 16 * 16;
 
 template <typename T>
-__global__ void __launch_bounds__(kSampleThreads) sample_kernel(const __grid_constant__ SampleArgs a) {
+__global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_constant__ SampleArgs a) {
   constexpr int kVec = Vec<T>::n;
   extern __shared__ __align__(16) char smem_raw[];
   SampleShared& sh = *reinterpret_cast<SampleShared*>(smem_raw);
@@ -219,17 +231,22 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const __grid_con
   }
   __syncthreads();
   int turn = 0;
-  // (va, vb) of thread 0 to every CTA of the cluster; all threads pass the barrier
+  // (va, vb), known to warp 0, to every CTA of the cluster; all threads pass the barrier
   auto exchange = [&](uint64_t va, uint64_t vb) {
-    if (tid == 0)
-      for (int c = 0; c < C; ++c) *cluster.map_shared_rank(&sh.xch[turn][rank], c) = Pair64{va, vb};
+    if (tid < C) *cluster.map_shared_rank(&sh.xch[turn][rank], tid) = Pair64{va, vb};
     cluster.sync();
     const Pair64* r = sh.xch[turn];
     turn ^= 1;
     return r;
   };
-  if (tid == 0)
-    for (int w = 1; w < kSampleWarps; ++w) best = sh.warp_a[w] > best ? sh.warp_a[w] : best;
+  if (warp == 0) {
+    best = lane < kSampleWarps ? sh.warp_a[lane] : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const uint64_t c = __shfl_xor_sync(0xffffffffu, best, o);
+      best = c > best ? c : best;
+    }
+  }
   {
     const Pair64* r = exchange(best, 0);
     best = 0;
@@ -242,62 +259,75 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const __grid_con
       a.tok[row] = m == -INFINITY ? -1 : (int64_t)(uint32_t)~(uint32_t)best;
       if (a.logprob) a.logprob[row] = m == -INFINITY ? m : 0.f;
     }
-    cluster.sync();  // no CTA may leave while another still writes to it
-    return;
+    return;  // (nothing of a CTA's memory is used by others after its last barrier)
   }
-  // +inf logits: the others weigh nothing at any temperature
-  const float inv_t = m == INFINITY ? 1.f : __fdiv_rn(1.f, temp);
+  // +inf logits share everything at any temperature: ties at the top, of which the filters keep the first
+  const bool top_inf = m == INFINITY;
+  // (an infinite temperature's 1 / T = 0 would make NaN of masked logits: any d that rounds to weight 1 will do)
+  const float inv_t = fmaxf(__fdiv_rn(1.f, temp), 1e-38f);
 
-  // f(logit, index) over this warp's logits
+  // f(kVec logits, index of the first) over this warp's vectors
   auto each = [&](auto f) {
 #pragma unroll 1
     for (int i = lane; i < vecs; i += 32) {
       float v[kVec];
       Vec<T>::get(mine[i], v);
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) f(v[j], first + i * kVec + j);
+      f(v, first + i * kVec);
     }
   };
-
 
   const int k = a.top_k ? a.top_k[row] : 0;
   const float p = a.top_p ? a.top_p[row] : 1.f;
   const bool cut_k = k > 0 && k < n, cut_p = p < 1.f;
-  float thr = -INFINITY;  // kept: logits above it ...
-  uint64_t take = 0;      // ... and this many of those equal to it
+  float thr = top_inf ? INFINITY : -INFINITY;  // kept: logits above it ...
+  uint64_t take = 0;                           // ... and this many of those equal to it
 
-  if (cut_k || cut_p) {
-    const int bins = kSampleBins / C, per = (bins + kSampleThreads - 1) / kSampleThreads;  // per: 1 to 4
+  if ((cut_k || cut_p) && !top_inf) {
+    const int bins = min(kSampleBins, kSampleThreads * C), share = bins / C;  // a CTA's share: a bin a thread
+    const float per_d = bins / kSampleDeep;
     auto clear = [&]() {
-      for (int i = tid; i < kSampleBins; i += kSampleThreads) sh.cnt[i] = sh.lo[i] = sh.hi[i] = 0;
+      for (int i = tid; i < bins; i += kSampleThreads) sh.cnt[i] = sh.lo[i] = sh.hi[i] = 0;
       __syncthreads();
     };
-    auto count_in = [&](int bin, float d) {
-      atomicAdd(&sh.cnt[bin], 1u);
+    // four tokens into the bins (-1: none), their weights with the carry from the low words' old values; the
+    // additions of all four are under way together
+    auto count_in = [&](const int* bin, const float* d) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (bin[j] >= 0) atomicAdd(&sh.cnt[bin[j]], 1u);
       if (!cut_p) return;  // numbers are enough
-      const uint64_t w = depth_weight(d);
-      const uint32_t w_lo = (uint32_t)w, old = atomicAdd(&sh.lo[bin], w_lo);
-      const uint32_t w_hi = (uint32_t)(w >> 32) + (old + w_lo < old ? 1u : 0u);  // with the carry
-      if (w_hi) atomicAdd(&sh.hi[bin], w_hi);
+      uint64_t w[4];
+      uint32_t old[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = depth_weight(d[j]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (bin[j] >= 0) old[j] = atomicAdd(&sh.lo[bin[j]], (uint32_t)w[j]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t hi = (uint32_t)(w[j] >> 32) + (old[j] + (uint32_t)w[j] < old[j] ? 1u : 0u);
+        if (bin[j] >= 0 && hi) atomicAdd(&sh.hi[bin[j]], hi);
+      }
     };
     // the cluster's histograms added up, each CTA a share of the bins, and the sums before this thread's
     auto sum_bins = [&]() {
       cluster.sync();
       BinSums s;
       uint64_t c = 0, w = 0;
+      if (tid < share) {
+        const int b = rank * share + tid;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s.n[j] = 0;
-        s.w[j] = 0;
-        const int b = rank * bins + tid * per + j;
-        if (j < per && tid * per + j < bins)
-          for (int q = 0; q < C; ++q) {
-            s.n[j] += *cluster.map_shared_rank(&sh.cnt[b], q);
-            s.w[j] += *cluster.map_shared_rank(&sh.lo[b], q) + ((uint64_t)*cluster.map_shared_rank(&sh.hi[b], q) << 32);
-          }
-        c += s.n[j];
-        w += s.w[j];
+        for (int q = 0; q < kSampleMaxCluster; ++q)
+          if (q < C) c += *cluster.map_shared_rank(&sh.cnt[b], q);
+        if (cut_p) {
+#pragma unroll
+          for (int q = 0; q < kSampleMaxCluster; ++q)
+            if (q < C)
+              w += *cluster.map_shared_rank(&sh.lo[b], q) + ((uint64_t)*cluster.map_shared_rank(&sh.hi[b], q) << 32);
+        }
       }
+      s.n = (uint32_t)c;
+      s.w = w;
       const uint64_t ci = warp_scan64(c, lane), wi = warp_scan64(w, lane);
       if (lane == 31) {
         sh.warp_a[warp] = ci;
@@ -306,15 +336,11 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const __grid_con
       __syncthreads();
       s.count = ci - c;
       s.weight = wi - w;
-      uint64_t ct = 0, wt = 0;
-      for (int q = 0; q < kSampleWarps; ++q) {
-        if (q < warp) {
-          s.count += sh.warp_a[q];
-          s.weight += sh.warp_b[q];
-        }
-        ct += sh.warp_a[q];
-        wt += sh.warp_b[q];
-      }
+      uint64_t ct = lane < kSampleWarps ? sh.warp_a[lane] : 0, wt = lane < kSampleWarps ? sh.warp_b[lane] : 0;
+      s.count += warp_sum64(lane < warp ? ct : 0);
+      s.weight += warp_sum64(lane < warp ? wt : 0);
+      ct = warp_sum64(ct);
+      wt = warp_sum64(wt);
       const Pair64* r = exchange(ct, wt);
       s.total_count = s.total_weight = 0;
       for (int q = 0; q < C; ++q) {
@@ -329,16 +355,11 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const __grid_con
     };
     // the bin in which the prefix of `want` tokens (of weight `want`) ends, given what lies above all bins
     auto find = [&](const BinSums& s, uint64_t want, bool by_weight, uint64_t count0, uint64_t weight0) {
-      uint64_t c = count0 + s.count, w = weight0 + s.weight;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint64_t before = by_weight ? w : c, here = by_weight ? s.w[j] : s.n[j];
-        if (before < want && want <= before + here)
-          for (int q = 0; q < C; ++q)
-            *cluster.map_shared_rank(&sh.found, q) = Bracket{c, w, rank * bins + tid * per + j, (int)s.n[j]};
-        c += s.n[j];
-        w += s.w[j];
-      }
+      const uint64_t c = count0 + s.count, w = weight0 + s.weight;
+      const uint64_t before = by_weight ? w : c, here = by_weight ? s.w : s.n;
+      if (before < want && want <= before + here)
+        for (int q = 0; q < C; ++q)
+          *cluster.map_shared_rank(&sh.found, q) = Bracket{c, w, rank * share + tid, (int)s.n};
       cluster.sync();
       return sh.found;
     };
@@ -347,13 +368,25 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const __grid_con
       Bracket br = find(s0, want, by_weight, 0, 0);
       const int step = br.bin;
       uint32_t k_lo = 0, k_hi = 0;  // by key, once the bracket is narrower than the step
-      auto inside = [&](float l) {
-        if (!(l > -INFINITY)) return false;
-        if (k_hi) return logit_key(l) >= k_lo && logit_key(l) <= k_hi;
-        const float d = logit_depth(l, m, inv_t);
-        return d >= -kSampleDeep && depth_bin(d) == step;
+      // logits of the step lie in between these, by more than the roundings of d (2^-20 of it and of l, m)
+      // (a temperature that has no such bounds in fp32 gets none)
+      const bool bounded = temp < 1e30f;
+      const float slop = 1e-5f * (fabsf(m) + kSampleDeep * temp), width = kSampleDeep / bins;
+      const float l_top = bounded ? m - step * width * temp + slop : INFINITY;
+      const float l_low = bounded && step < bins - 1 ? m - (step + 1) * width * temp - slop : -INFINITY;
+      auto may_be = [&](const float* v) {
+        bool any = false;
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) any |= v[j] >= l_low && v[j] <= l_top;
+        return any;
       };
-      while (br.n > kSampleList) {
+      auto inside = [&](float l) {
+        const float d = logit_depth(l, m, inv_t);
+        const uint32_t key = logit_key(l);
+        return l > -INFINITY && (k_hi ? key >= k_lo && key <= k_hi : d >= -kSampleDeep && depth_bin(d, per_d, bins) == step);
+      };
+      // a round leaves a 512th or less of the keys' range: 32 bits take four
+      for (int round = 0; round < 4 && br.n > kSampleList; ++round) {
         if (!k_hi) {  // the keys in this step
           if (tid == 0) {
             sh.key_min = 0xffffffffu;
@@ -361,10 +394,13 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const __grid_con
           }
           __syncthreads();
           uint32_t lo = 0xffffffffu, hi = 0;
-          each([&](float l, int) {
-            if (inside(l)) {
-              lo = min(lo, logit_key(l));
-              hi = max(hi, logit_key(l));
+          each([&](const float* v, int) {
+            if (!may_be(v)) return;
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) {
+              const bool in = inside(v[j]);
+              lo = min(lo, in ? logit_key(v[j]) : 0xffffffffu);
+              hi = max(hi, in ? logit_key(v[j]) : 0u);
             }
           });
           lo = __reduce_min_sync(0xffffffffu, lo);
@@ -383,10 +419,23 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const __grid_con
         }
         if (k_lo == k_hi) break;  // equal logits: arithmetic
         int shift = 0;
-        while (((k_hi - k_lo) >> shift) >= (uint32_t)kSampleBins) ++shift;
+        while (((k_hi - k_lo) >> shift) >= (uint32_t)bins) ++shift;
         clear();
-        each([&](float l, int) {
-          if (inside(l)) count_in((int)((k_hi - logit_key(l)) >> shift), logit_depth(l, m, inv_t));
+        each([&](const float* v, int) {
+          if (!may_be(v)) return;
+#pragma unroll
+          for (int h = 0; h < kVec; h += 4) {
+            int bin[4];
+            float d[4];
+            bool any = false;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              d[j] = logit_depth(v[h + j], m, inv_t);
+              bin[j] = inside(v[h + j]) ? (int)((k_hi - logit_key(v[h + j])) >> shift) : -1;
+              any |= bin[j] >= 0;
+            }
+            if (any) count_in(bin, d);
+          }
         });
         const BinSums s = sum_bins();
         br = find(s, want, by_weight, br.count, br.weight);
@@ -400,34 +449,56 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const __grid_con
         take = by_weight ? (want - br.weight + w1 - 1) / w1 : want - br.count;
         weight = br.weight + take * w1;
       } else {
-        // the bracket's tokens into the first CTA, where each is compared with each
+        // the bracket's tokens into the first CTA, in any order
         uint64_t* const list = cluster.map_shared_rank(sh.list, 0);
         int* const list_n = cluster.map_shared_rank(&sh.list_n, 0);
-        each([&](float l, int i) {
-          if (inside(l)) list[atomicAdd(list_n, 1)] = ((uint64_t)logit_key(l) << 32) | (uint32_t)~i;
+        each([&](const float* v, int i) {
+          if (!may_be(v)) return;
+          unsigned in = 0;
+#pragma unroll
+          for (int j = 0; j < kVec; ++j) in |= (unsigned)inside(v[j]) << j;
+          if (in) {
+            int to = atomicAdd(list_n, __popc(in));
+#pragma unroll
+            for (int j = 0; j < kVec; ++j)
+              if (in >> j & 1u) list[to++] = ((uint64_t)logit_key(v[j]) << 32) | (uint32_t)~(i + j);
+          }
         });
         cluster.sync();
         if (rank == 0) {
-          const uint64_t me = tid < br.n ? sh.list[tid] : 0;
-          const uint64_t w = tid < br.n ? depth_weight(logit_depth(key_logit((uint32_t)(me >> 32)), m, inv_t)) : 0;
-          sh.list_w[tid] = w;
-          __syncthreads();
-          if (tid < br.n) {
-            uint64_t c_up = br.count, w_up = br.weight;
-            uint32_t ties = 0;
-#pragma unroll 4
-            for (int j = 0; j < br.n; ++j) {
-              const uint64_t o = sh.list[j];
-              if (o > me) {
-                ++c_up;
-                w_up += sh.list_w[j];
-                ties += (o >> 32) == (me >> 32);
+          // sorted by (key, ~index) downwards, a token a thread: bitonic, by shuffles within a warp
+          uint64_t me = tid < br.n ? sh.list[tid] : 0;
+          for (int size = 2; size < 2 * br.n; size *= 2) {  // (a sorted block holds what the others pad with 0)
+            for (int step = size / 2; step > 0; step /= 2) {
+              uint64_t o;
+              if (step >= 32) {
+                __syncthreads();
+                sh.list[tid] = me;
+                __syncthreads();
+                o = sh.list[tid ^ step];
+              } else {
+                o = __shfl_xor_sync(0xffffffffu, me, step);
               }
+              const bool keep_max = ((tid & step) == 0) == ((tid & size) == 0);
+              me = (me > o) == keep_max ? me : o;
             }
-            if (by_weight ? w_up < want && want <= w_up + w : c_up + 1 == want)
-              for (int q = 0; q < C; ++q)
-                *cluster.map_shared_rank(&sh.cut, q) = Pair64{w_up + w, (me & 0xffffffff00000000ull) | (ties + 1)};
           }
+          const uint64_t w = me ? depth_weight(logit_depth(key_logit((uint32_t)(me >> 32)), m, inv_t)) : 0;
+          uint64_t upto = warp_scan64(w, lane);
+          if (lane == 31) sh.warp_a[warp] = upto;
+          __syncthreads();
+          const uint64_t others = lane < kSampleWarps ? sh.warp_a[lane] : 0;
+          upto += br.weight + warp_sum64(lane < warp ? others : 0);
+          if (tid < br.n && (by_weight ? upto - w < want && want <= upto : br.count + tid + 1 == want)) {
+            sh.cut = Pair64{upto, me};
+            sh.list_n = tid;  // the place of the last one kept
+          }
+          __syncthreads();
+          const Pair64 last = sh.cut;
+          const int place = sh.list_n;
+          const int ties = __syncthreads_count(tid <= place && (me >> 32) == (last.b >> 32));
+          if (tid < C)
+            *cluster.map_shared_rank(&sh.cut, tid) = Pair64{last.a, (last.b & 0xffffffff00000000ull) | (unsigned)ties};
           if (tid == 0) sh.list_n = 0;
         }
         cluster.sync();
@@ -440,10 +511,17 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const __grid_con
 
     // ---- 2, 3: the histogram over steps of d, and the cuts
     clear();
-    each([&](float l, int) {
-      if (l > -INFINITY) {
-        const float d = logit_depth(l, m, inv_t);
-        if (d >= -kSampleDeep) count_in(depth_bin(d), d);
+    each([&](const float* v, int) {
+#pragma unroll
+      for (int h = 0; h < kVec; h += 4) {
+        int bin[4];
+        float d[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          d[j] = logit_depth(v[h + j], m, inv_t);
+          bin[j] = v[h + j] > -INFINITY && d[j] >= -kSampleDeep ? depth_bin(d[j], per_d, bins) : -1;
+        }
+        count_in(bin, d);
       }
     });
     const BinSums s = sum_bins();
@@ -459,24 +537,41 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const __grid_con
   // ---- 4: the kept weights, ties counted apart (they all weigh the same)
   const float mp = a.min_p ? a.min_p[row] : 0.f;
   const float floor_d = mp > 0.f ? logf(fminf(mp, 1.f)) : -INFINITY;
-  const bool tied = thr > -INFINITY && logit_depth(thr, m, inv_t) >= floor_d;
-  const uint64_t w1 = tied ? depth_weight(logit_depth(thr, m, inv_t)) : 0;
-  auto kept = [&](float l) {  // the weight of a logit above the threshold, 0 of others
-    if (!(l > thr)) return (uint64_t)0;
-    const float d = logit_depth(l, m, inv_t);
-    return d >= floor_d ? depth_weight(d) : (uint64_t)0;
-  };
+  const bool tied = top_inf || (thr > -INFINITY && logit_depth(thr, m, inv_t) >= floor_d);
+  const uint64_t w1 = top_inf ? (uint64_t)1 << 40 : tied ? depth_weight(logit_depth(thr, m, inv_t)) : 0;
   auto taken = [&](uint64_t before, uint64_t here) {  // the weight of `here` ties that come after `before` others
     return before >= take ? (uint64_t)0 : min(here, take - before) * w1;
   };
+  // expf(d) of a logit above the threshold, 0 of others
+  auto kept = [&](float l) {
+    const float d = logit_depth(l, m, inv_t);
+    return l > thr && d >= floor_d ? expf(d) : 0.f;
+  };
+  // adds a vector's kept weights in halves, and its ties
+  auto add_kept = [&](const float* v, uint32_t& hi, uint32_t& lo, uint32_t& eq) {
+    bool any = false;
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) any |= v[j] >= thr;
+    if (any) {
+      uint32_t h[kVec], l[kVec];
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) weight_halves(kept(v[j]), h[j], l[j]);
+      if (tied)
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) eq += v[j] == thr;
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) {
+        hi += h[j] - kHalfBits;
+        lo += l[j] - kHalfBits;
+      }
+    }
+  };
   {
-    uint64_t w = 0;
-    uint32_t eq = 0;
-    each([&](float l, int) {
-      w += kept(l);
-      eq += tied && l == thr;
-    });
-    w = warp_sum64(w);
+    // halves of up to 2^20 a logit: 32 bits hold the sums of a lane's 512 vectors (2^18 logits over 128 or
+    // more warps), and of the warp in 64
+    uint32_t hi = 0, lo = 0, eq = 0;
+    each([&](const float* v, int) { add_kept(v, hi, lo, eq); });
+    const uint64_t w = warp_sum64(((uint64_t)hi << 20) + lo);
     eq = __reduce_add_sync(0xffffffffu, eq);
     if (lane == 0) {
       sh.warp_a[warp] = w;
@@ -485,15 +580,22 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const __grid_con
   }
   __syncthreads();
   uint64_t sum_w = 0, sum_eq = 0;
-  if (tid == 0)
-    for (int q = 0; q < kSampleWarps; ++q) {
-      sum_w += sh.warp_a[q];
-      sum_eq += sh.warp_b[q];
-    }
+  if (warp == 0) {
+    sum_w = warp_sum64(lane < kSampleWarps ? sh.warp_a[lane] : 0);
+    sum_eq = __reduce_add_sync(0xffffffffu, lane < kSampleWarps ? (uint32_t)sh.warp_b[lane] : 0u);
+  }
   const Pair64* r = exchange(sum_w, sum_eq);
+  if (top_inf) {
+    for (int c = 0; c < C; ++c) take += r[c].b;
+    if (cut_k) take = min(take, (uint64_t)k);
+    if (cut_p) {
+      const double want = ceil((double)p * (double)(int64_t)(take * w1));
+      take = want > (double)w1 ? ((uint64_t)want + w1 - 1) / w1 : 1;
+    }
+  }
   uint64_t total = 0, seen = 0, run = 0, seen0 = 0, here = 0;  // run, seen0: before this CTA; here: its weight
   for (int c = 0; c < C; ++c) {
-    const uint64_t w = r[c].a + taken(seen, r[c].b);
+    const uint64_t w = r[c].a + (tied ? taken(seen, r[c].b) : 0);
     if (c == rank) {
       run = total;
       seen0 = seen;
@@ -509,52 +611,52 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const __grid_con
     // the warp's part in which the running sum passes `at`: lane q looks at part q
     uint64_t eq = lane < kSampleWarps ? sh.warp_b[lane] : 0, w = lane < kSampleWarps ? sh.warp_a[lane] : 0;
     uint64_t eq_before = seen0 + warp_scan64(eq, lane) - eq;
-    w += taken(eq_before, eq);
+    if (tied) w += taken(eq_before, eq);
     uint64_t incl = run + warp_scan64(w, lane);
     const int q = __ffs(__ballot_sync(0xffffffffu, incl > at)) - 1;
     run = __shfl_sync(0xffffffffu, incl - w, q);
     seen = __shfl_sync(0xffffffffu, eq_before, q);
     const uint4* const from = part + q * vecs;
     const int base = (rank * kSampleWarps + q) * a.per_warp;
+    // 32 vectors at a time up to the one in which the sum passes, then its lane, then that lane's logits
     for (int i0 = 0; i0 < vecs; i0 += 32) {
-      float v[kVec];
       const int i = i0 + lane;
-      uint64_t wl = 0, el = 0;
+      uint32_t hi = 0, lo = 0, el = 0;
       if (i < vecs) {
+        float v[kVec];
         Vec<T>::get(from[i], v);
-#pragma unroll
-        for (int j = 0; j < kVec; ++j) {
-          wl += kept(v[j]);
-          el += tied && v[j] == thr;
-        }
+        add_kept(v, hi, lo, el);
       }
-      const uint64_t e_before = seen + warp_scan64(el, lane) - el;
-      const uint64_t wt = wl + taken(e_before, el), upto = run + warp_scan64(wt, lane);
-      const unsigned past = __ballot_sync(0xffffffffu, upto > at);
-      if (past) {
-        if (lane == __ffs(past) - 1) {
-          uint64_t sum = upto - wt, e = e_before;
-          bool done = false;
-#pragma unroll
-          for (int j = 0; j < kVec; ++j) {
-            const bool tie = tied && v[j] == thr;
-            sum += tie ? taken(e, 1) : kept(v[j]);
-            e += tie;
-            if (!done && sum > at) {
-              done = true;
-              a.tok[row] = base + i * kVec + j;
-              if (a.logprob)
-                a.logprob[row] = logit_depth(v[j], m, inv_t) - logf((float)(int64_t)total * (1.f / kSampleOne));
-            }
-          }
-        }
-        break;
+      const uint64_t wl = ((uint64_t)hi << 20) + lo;
+      const uint32_t el_all = __reduce_add_sync(0xffffffffu, el);
+      const uint64_t w_all = warp_sum64(wl) + (el_all ? taken(seen, el_all) : 0);
+      if (run + w_all <= at) {
+        run += w_all;
+        seen += el_all;
+        continue;
       }
-      run = __shfl_sync(0xffffffffu, upto, 31);
-      seen = __shfl_sync(0xffffffffu, e_before + el, 31);
+      uint64_t e_before = seen;
+      if (el_all) e_before += warp_scan64(el, lane) - el;
+      const uint64_t wt = wl + (el_all ? taken(e_before, el) : 0), upto = run + warp_scan64(wt, lane);
+      const int at_lane = __ffs(__ballot_sync(0xffffffffu, upto > at)) - 1;
+      run = __shfl_sync(0xffffffffu, upto - wt, at_lane);
+      seen = __shfl_sync(0xffffffffu, e_before, at_lane);
+      const int iv = i0 + at_lane;  // the vector; lane j takes its logit j
+      const float l = lane < kVec ? Vec<T>::one(reinterpret_cast<const T*>(from + iv)[lane]) : -INFINITY;
+      const bool tie = tied && l == thr;
+      const unsigned ties = __ballot_sync(0xffffffffu, tie);
+      uint32_t wh, wo;
+      weight_halves(kept(l), wh, wo);
+      const uint64_t wj = tie ? taken(seen + __popc(ties & ((1u << lane) - 1u)), 1)
+                              : ((uint64_t)(wh - kHalfBits) << 20) + (wo - kHalfBits);
+      const unsigned past = __ballot_sync(0xffffffffu, run + warp_scan64(wj, lane) > at);
+      if (lane == __ffs(past) - 1) {
+        a.tok[row] = base + iv * kVec + lane;
+        if (a.logprob) a.logprob[row] = (top_inf ? 0.f : logit_depth(l, m, inv_t)) - logf((float)(int64_t)total * (1.f / kSampleOne));
+      }
+      break;
     }
   }
-  cluster.sync();  // no CTA may leave while another still reads or writes its memory
 }
 
 }  // namespace qd
@@ -576,11 +678,16 @@ extern "C" int qd_sample(const void* logits, int dtype, int64_t ld, int64_t rows
   if (reinterpret_cast<uintptr_t>(logits) % (dtype == QD_FP32 ? 4 : 2))
     return set_error(QD_ERR_ARG, "sample: misaligned logits");
   if (rows == 0) return QD_OK;
-  // The cluster: 4096 logits a CTA are enough to pay for its barriers (151,936 logits: 8 CTAs).
+  // The cluster: the fewest CTAs of which two fit an SM (so that one's loads and barriers hide behind the
+  // other's arithmetic) and which fill the SMs, but at most one for 4096 logits. Measured on 64 / 256 rows of
+  // 151,936 BF16 logits: see the kernel.
+  const int size = dtype == QD_FP32 ? 4 : 2;
   int cluster = 1;
-  while (cluster < kSampleMaxCluster && vocab >= (int64_t)8192 * cluster) cluster *= 2;
+  while (cluster < kSampleMaxCluster && vocab >= (int64_t)8192 * cluster &&
+         (rows * cluster < host_sm_count() || kSampleShared + vocab * size / cluster > 110 * 1024))
+    cluster *= 2;
   SampleArgs a = {logits, ld, vocab, temperature, top_k, top_p, min_p, u, tok, logprob, 0, 0};
-  const int size = dtype == QD_FP32 ? 4 : 2, parts = cluster * kSampleWarps;
+  const int parts = cluster * kSampleWarps;
   a.per_warp = (int)((vocab + parts - 1) / parts + 7) / 8 * 8;
   a.wide = aligned16(logits) && ld * size % 16 == 0;
   const int smem = kSampleShared + a.per_warp * kSampleWarps * size;
