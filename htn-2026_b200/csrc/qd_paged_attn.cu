@@ -70,8 +70,8 @@ struct PgLayout {
   static constexpr int kv = q + 2 * kItem;
   static constexpr int p = kv + kSlots * kItem;  // P of few-row units (head_dim 128: in their Q region)
   static constexpr int bars = p + (D == 64 ? 2 * kFewP : 0);
-  // qfull[2], qempty[2], sfull[2], pfull[2], odone[2], ofree[2], group[2], segfull[4], segempty[4], join, -,
-  // sload[2], full[slots], empty[slots]
+  // qfull[2], qempty[2], sfull[2], pfull[2], odone[2], ofree[2], group[2], segfull[4], segempty[4], join,
+  // sload A odd, A even, B, full[slots], empty[slots]
   static constexpr int nbars = 26 + 2 * kSlots;
   static constexpr int seg = bars + nbars * 8;  // segment ring
   static constexpr int misc = seg + 4 * 64;     // tmem slot, abort, line start, flags, drain counts
@@ -295,7 +295,10 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
   auto segfull = [&](int k) { return bars + 112 + 8u * (k & 3); };
   auto segempty = [&](int k) { return bars + 144 + 8u * (k & 3); };
   const uint32_t join = bars + 176;
-  auto sload = [&](int x) { return bars + 192 + 8u * x; };
+  // S_A's loads alternate between two barriers: B waits for one that may be two phases away from the last it
+  // knows of, and a parity wait two phases ahead (or behind) of a barrier answers wrongly
+  auto sload_a = [&](int n) { return bars + ((n & 1) ? 184 : 192); };
+  const uint32_t sload_b = bars + 200;
   auto full = [&](int s) { return bars + 208 + 8u * s; };
   auto empty = [&](int s) { return bars + 208 + 8u * (kSlots + s); };
   PgSeg* segs = reinterpret_cast<PgSeg*>(smem + Lay::seg);
@@ -313,9 +316,10 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
       mbar_init(odone(x), 1);
       mbar_init(ofree(x), 4);
       mbar_init(group(x), 4);
-      mbar_init(sload(x), 4);
+      mbar_init(x ? sload_b : sload_a(0), 4);
     }
     mbar_init(join, 4);
+    mbar_init(sload_a(1), 4);
     for (int k = 0; k < 4; ++k) {
       mbar_init(segfull(k), 1);
       mbar_init(segempty(k), 9);  // the MMA warp and eight softmax warps
@@ -617,7 +621,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
         issue_s(c1, c0, 1, ahead(0));
         if (g.nb > 1) {
           umma_commit(empty(slot));
-          wait(sload(0), pairs);
+          wait(sload_a(pairs), pairs >> 1);
           issue_s(c0, c0, 0, ahead(2));
         } else {
           umma_commit(qempty(0));
@@ -980,11 +984,12 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
                 m4[c] = pg_max3(m4[c], __uint_as_float(v[e + 2 * c]), __uint_as_float(v[e + 2 * c + 1]));
           }
           m_new = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * a.scale_log2;
+          if (r >= rows) m_new = -INFINITY;  // what a row holds that is no token's must not move its warp's maxima
         }
         if (two) {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(sload(x));
+          if (lane == 0) mbar_arrive(x ? sload_b : sload_a(pairs + j));
         }
         if (!idle) {
           // warp-uniform (tensor-memory loads and stores are warp-collective)
@@ -1019,8 +1024,15 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
             sv[c] = Elem<T>::pack(p0, p1);
           }
           l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
-          if (two) {  // over the other tile's S, once that has loaded it (B: the one A is ahead with)
-            wait(sload(1 - x), pairs + j + (x == 1 && j + 1 < g.nb ? 1 : 0));
+          if (two) {  // over the other tile's S, once that has loaded it (B: the one A is ahead with, whose
+                      // products were issued after B's last P was used up)
+            const int n = pairs + min(j + 1, g.nb - 1);  // the S_A that A has by now
+            if (x == 0)
+              wait(sload_b, pairs + j);
+            else if (j == 0 || j + 1 < g.nb)
+              wait(sload_a(n), n >> 1);
+            else  // no S_A comes after B's last P but one, which has to be used up before the last
+              wait(odone(1), cnt - 1);
             tc_fence_after();
           }
           tmem_st64(tS(two ? 1 - x : x) + lane_off, sv);
@@ -1028,6 +1040,8 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(pfull(x));
+        // the next S may come before this P is complete: a warp without rows must not arrive twice for it
+        if (idle && two) wait(pfull(x), cnt);
       }
       if (two) pairs += g.nb;
       wait(odone(x), cnt - 1);
@@ -1055,10 +1069,11 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
         l = l * fa + o.y * fb;
         m_used = m;
       }
-      // Rows go out through the shared memory of the unit's last V block (tile B: K block), which is still this
-      // warpgroup's: thread r lays down row r, 16-byte chunks swizzled by row, and whole rows are stored from
-      // there (row by row from the registers would be partial sectors, 32 lines an instruction: 7 k cycles).
-      const int it = 2 * blocks - 1 - (two ? x : 0), slot = it % kSlots;
+      // Rows go out through the shared memory of the unit's last V block (of two tiles, A: its last K block, whose
+      // products were issued before those that this warpgroup has waited for; V is B's, which comes last): thread
+      // r lays down row r, 16-byte chunks swizzled by row, and whole rows are stored from there (row by row from
+      // the registers would be partial sectors, 32 lines an instruction: 7 k cycles).
+      const int it = 2 * blocks - 1 - (two ? 1 - x : 0), slot = it % kSlots;
       char* const stage = smem + Lay::kv + slot * Lay::kItem;
       auto lay_down = [&](int c, const uint32_t* w) {  // dims 8 c .. 8 c + 7, packed
         *reinterpret_cast<uint4*>(stage + r * (2 * D) + ((c ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);

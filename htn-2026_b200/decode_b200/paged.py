@@ -22,8 +22,10 @@ import math
 import torch
 
 from . import lib as L
-from .ops import _ptr, _stream
 
+# the current stream's handle of a device, without the Stream object that torch.cuda.current_stream() makes
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+I32, F32 = torch.int32, torch.float32
 TYPES = {torch.bfloat16: L.QD_BF16, torch.float16: L.QD_FP16}
 
 
@@ -41,14 +43,28 @@ def rope_table(positions: int, head_dim: int, theta: float, device):
 
 
 def _check_batch(dtype, k_pages, v_pages, cu_tokens, kv_len, page_table):
-    assert dtype in TYPES, f"expected BF16 or FP16 tensors, got {dtype}"
-    assert k_pages.dtype == dtype and v_pages.dtype == dtype and k_pages.is_cuda and v_pages.is_cuda
-    assert k_pages.dim() == 4 and k_pages.shape == v_pages.shape and k_pages.stride() == v_pages.stride()
-    assert k_pages.stride(3) == 1 and k_pages.stride(2) == k_pages.shape[3], "rows of a page must be contiguous"
-    assert cu_tokens.dtype == kv_len.dtype == page_table.dtype == torch.int32
+    """(pool shape, pool strides, batch, table row stride, table columns); each property is read once, since a
+    call for a few tokens takes the GPU less time than reading it twice takes the host."""
+    shape, strides, table = k_pages.shape, k_pages.stride(), page_table.shape
+    assert k_pages.dtype is dtype and v_pages.dtype is dtype and k_pages.is_cuda and v_pages.is_cuda
+    assert v_pages.shape == shape and v_pages.stride() == strides and len(shape) == 4
+    assert strides[3] == 1 and strides[2] == shape[3], "rows of a page must be contiguous"
+    assert cu_tokens.dtype is I32 and kv_len.dtype is I32 and page_table.dtype is I32
     assert cu_tokens.is_cuda and kv_len.is_cuda and page_table.is_cuda
-    assert cu_tokens.is_contiguous() and kv_len.is_contiguous() and page_table.stride(-1) == 1
-    assert kv_len.numel() == page_table.shape[0] and cu_tokens.numel() == kv_len.numel() + 1
+    ld_table, step = page_table.stride()
+    assert cu_tokens.is_contiguous() and kv_len.is_contiguous() and (step == 1 or table[1] == 1)
+    assert kv_len.shape == table[:1] and cu_tokens.shape == (table[0] + 1,)
+    return shape, strides, table[0], max(ld_table, table[1]) if table[0] == 1 else ld_table, table[1]
+
+
+def _rows(t, tokens: int, heads: int, D: int) -> int:
+    """Row stride of a [tokens, heads, D] or [tokens, heads * D] tensor with contiguous rows."""
+    strides = t.stride()
+    if len(strides) == 3:
+        assert t.shape == (tokens, heads, D) and strides[2] == 1 and (strides[1] == D or heads == 1)
+    else:
+        assert t.shape == (tokens, heads * D) and strides[1] == 1
+    return max(strides[0], heads * D) if tokens <= 1 else strides[0]
 
 
 def rope_append(qkv, cu_tokens, kv_len, page_table, nq: int, nkv: int, cos, sin, q_out, k_pages, v_pages, q_norm=None,
@@ -56,21 +72,22 @@ def rope_append(qkv, cu_tokens, kv_len, page_table, nq: int, nkv: int, cos, sin,
     """q_out[t] = rope(norm(q)) and K = rope(norm(k)), V into the pages, for every new token t
     (qd_paged_rope_append). qkv [tokens, (nq + 2 nkv) * head_dim]; q_out [tokens, nq, head_dim] or
     [tokens, nq * head_dim]; cos / sin fp32 [positions, pairs turned] (`rope_table`)."""
-    D = k_pages.shape[3]
-    _check_batch(qkv.dtype, k_pages, v_pages, cu_tokens, kv_len, page_table)
-    assert qkv.is_cuda and qkv.dim() == 2 and qkv.shape[1] == (nq + 2 * nkv) * D and qkv.stride(1) == 1
-    assert q_out.dtype == qkv.dtype and q_out.shape[0] == qkv.shape[0] and q_out.numel() == qkv.shape[0] * nq * D
-    assert q_out.stride(-1) == 1 and (q_out.dim() == 2 or q_out.stride(1) == D)
-    assert k_pages.shape[1] == nkv
-    assert cos.dtype == sin.dtype == torch.float32 and cos.shape == sin.shape and cos.stride() == sin.stride()
-    assert cos.stride(1) == 1
-    for w in (q_norm, k_norm):
-        assert w is None or (w.dtype == qkv.dtype and w.numel() == D and w.is_contiguous())
-    L.call("qd_paged_rope_append", qkv.data_ptr(), qkv.stride(0), TYPES[qkv.dtype], qkv.shape[0], nq, nkv, D,
-           _ptr(q_norm), _ptr(k_norm), eps, cos.data_ptr(), sin.data_ptr(), cos.stride(0), cos.shape[0], cos.shape[1],
-           cu_tokens.data_ptr(), kv_len.data_ptr(), kv_len.numel(), page_table.data_ptr(), page_table.stride(0),
-           page_table.shape[1], q_out.data_ptr(), q_out.stride(0), k_pages.data_ptr(), v_pages.data_ptr(),
-           k_pages.shape[0], k_pages.shape[2], k_pages.stride(0), k_pages.stride(1), _ptr(err), int(pdl), _stream())
+    dtype = qkv.dtype
+    assert dtype in TYPES, f"expected BF16 or FP16 tensors, got {dtype}"
+    pool, ps, batch, ld_table, max_pages = _check_batch(dtype, k_pages, v_pages, cu_tokens, kv_len, page_table)
+    D, tokens = pool[3], qkv.shape[0]
+    assert qkv.is_cuda and q_out.is_cuda and q_out.dtype is dtype and pool[1] == nkv
+    ldqkv, ldq = _rows(qkv, tokens, nq + 2 * nkv, D), _rows(q_out, tokens, nq, D)
+    angles, ld = cos.shape, cos.stride()
+    assert cos.dtype is F32 and sin.dtype is F32 and sin.shape == angles and sin.stride() == ld and ld[1] == 1
+    if q_norm is not None or k_norm is not None:
+        for w in (q_norm, k_norm):
+            assert w is not None and w.dtype is dtype and w.shape == (D,) and w.is_contiguous()
+    L.call("qd_paged_rope_append", qkv.data_ptr(), ldqkv, TYPES[dtype], tokens, nq, nkv, D,
+           q_norm.data_ptr() if q_norm is not None else None, k_norm.data_ptr() if k_norm is not None else None, eps,
+           cos.data_ptr(), sin.data_ptr(), ld[0], angles[0], angles[1], cu_tokens.data_ptr(), kv_len.data_ptr(), batch,
+           page_table.data_ptr(), ld_table, max_pages, q_out.data_ptr(), ldq, k_pages.data_ptr(), v_pages.data_ptr(),
+           pool[0], pool[2], ps[0], ps[1], None if err is None else err.data_ptr(), pdl, _raw_stream(qkv.get_device()))
     return q_out
 
 
@@ -86,25 +103,28 @@ class PagedAttention:
         g, nbytes = ctypes.c_int(0), ctypes.c_int64(0)
         L.call("qd_paged_attn_plan", nq, nkv, head_dim, grid, ctypes.byref(g), ctypes.byref(nbytes))
         self.grid = g.value
-        self.scratch = torch.zeros((max(1, nbytes.value),), dtype=torch.uint8, device=device)
+        self.scratch = torch.zeros((nbytes.value,), dtype=torch.uint8, device=device)
+        self.scratch_bytes = nbytes.value
         self.scale = 1.0 / math.sqrt(head_dim)
 
     def __call__(self, q, k_pages, v_pages, cu_tokens, kv_len, page_table, out, lse=None, scale: float | None = None,
                  err=None, pdl: bool = True):
         """q, out [tokens, nq, head_dim] or [tokens, nq * head_dim]; lse (optional) fp32 [tokens, nq]."""
-        nq, D = self.nq, self.head_dim
-        _check_batch(q.dtype, k_pages, v_pages, cu_tokens, kv_len, page_table)
-        assert q.dtype == out.dtype == self.dtype and q.is_cuda and out.is_cuda
-        assert q.numel() == out.numel() == q.shape[0] * nq * D and out.shape[0] == q.shape[0]
-        assert q.stride(-1) == 1 and out.stride(-1) == 1
-        assert (q.dim() == 2 or q.stride(1) == D) and (out.dim() == 2 or out.stride(1) == D)
-        assert k_pages.shape[1] == self.nkv and k_pages.shape[3] == D
+        nq, D, dtype = self.nq, self.head_dim, self.dtype
+        pool, ps, batch, ld_table, max_pages = _check_batch(dtype, k_pages, v_pages, cu_tokens, kv_len, page_table)
+        tokens = q.shape[0]
+        assert q.dtype is dtype and out.dtype is dtype and q.is_cuda and out.is_cuda
+        assert pool[1] == self.nkv and pool[3] == D
+        ldq, ldo = _rows(q, tokens, nq, D), _rows(out, tokens, nq, D)
+        lse_ptr, ld_lse = None, 0
         if lse is not None:
-            assert lse.dtype == torch.float32 and lse.shape == (q.shape[0], nq) and lse.stride(1) == 1
-        L.call("qd_paged_attn", q.data_ptr(), q.stride(0), TYPES[self.dtype], q.shape[0], nq, self.nkv, D,
-               k_pages.data_ptr(), v_pages.data_ptr(), k_pages.shape[0], k_pages.shape[2], k_pages.stride(0),
-               k_pages.stride(1), cu_tokens.data_ptr(), kv_len.data_ptr(), kv_len.numel(), page_table.data_ptr(),
-               page_table.stride(0), page_table.shape[1], self.scale if scale is None else scale, out.data_ptr(),
-               out.stride(0), _ptr(lse), lse.stride(0) if lse is not None else 0, self.grid, self.scratch.data_ptr(),
-               self.scratch.numel(), _ptr(err), int(pdl), _stream())
+            assert lse.dtype is F32 and lse.is_cuda and lse.shape == (tokens, nq)
+            ld_lse, step = lse.stride()
+            assert step == 1 or nq == 1
+            lse_ptr, ld_lse = lse.data_ptr(), max(ld_lse, nq) if tokens <= 1 else ld_lse
+        L.call("qd_paged_attn", q.data_ptr(), ldq, TYPES[dtype], tokens, nq, self.nkv, D, k_pages.data_ptr(),
+               v_pages.data_ptr(), pool[0], pool[2], ps[0], ps[1], cu_tokens.data_ptr(), kv_len.data_ptr(), batch,
+               page_table.data_ptr(), ld_table, max_pages, self.scale if scale is None else scale, out.data_ptr(), ldo,
+               lse_ptr, ld_lse, self.grid, self.scratch.data_ptr(), self.scratch_bytes,
+               None if err is None else err.data_ptr(), pdl, _raw_stream(q.get_device()))
         return out

@@ -5,9 +5,18 @@ from __future__ import annotations
 import torch
 
 from . import lib as L
-from .ops import _ptr, _stream
 
+# the current stream's handle of a device, without the Stream object that torch.cuda.current_stream() makes
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+F32 = torch.float32
 TYPES = {torch.bfloat16: L.QD_BF16, torch.float16: L.QD_FP16, torch.float32: L.QD_FP32}
+
+
+def _row_values(t, dtype, shape):
+    if t is None:
+        return None
+    assert t.dtype is dtype and t.shape == shape and t.is_cuda and t.is_contiguous()
+    return t.data_ptr()
 
 
 def sample(logits, u, tok, temperature=None, top_k=None, top_p=None, min_p=None, logprob=None, vocab: int | None = None,
@@ -17,15 +26,14 @@ def sample(logits, u, tok, temperature=None, top_k=None, top_p=None, min_p=None,
     fp32 with unit column stride; u fp32 [rows]; tok int64 [rows]; logprob (optional) fp32 [rows].
     temperature / top_p / min_p fp32 [rows] and top_k int32 [rows] are per row; None leaves that step out.
     Graph-capturable; launches on the current torch CUDA stream."""
-    rows = logits.shape[0]
-    assert logits.is_cuda and logits.dtype in TYPES and logits.dim() == 2 and logits.stride(1) == 1
-    n = logits.shape[1] if vocab is None else vocab
-    assert n <= logits.shape[1]
-    assert u.dtype == torch.float32 and u.numel() == rows and u.is_contiguous() and u.is_cuda
-    assert tok.dtype == torch.int64 and tok.numel() == rows and tok.is_contiguous() and tok.is_cuda
-    for x, t in ((temperature, torch.float32), (top_k, torch.int32), (top_p, torch.float32), (min_p, torch.float32),
-                 (logprob, torch.float32)):
-        assert x is None or (x.dtype == t and x.numel() == rows and x.is_contiguous() and x.is_cuda)
-    L.call("qd_sample", logits.data_ptr(), TYPES[logits.dtype], logits.stride(0), rows, n, _ptr(temperature),
-           _ptr(top_k), _ptr(top_p), _ptr(min_p), u.data_ptr(), tok.data_ptr(), _ptr(logprob), int(pdl), _stream())
+    shape, dtype = logits.shape, logits.dtype
+    ld, step = logits.stride()
+    rows, n = shape[0], shape[1] if vocab is None else vocab
+    assert logits.is_cuda and dtype in TYPES and (step == 1 or shape[1] == 1) and n <= shape[1]
+    one = shape[:1]
+    assert u.dtype is F32 and u.shape == one and u.is_cuda and u.is_contiguous()
+    assert tok.dtype is torch.int64 and tok.shape == one and tok.is_cuda and tok.is_contiguous()
+    L.call("qd_sample", logits.data_ptr(), TYPES[dtype], max(ld, n) if rows <= 1 else ld, rows, n,
+           _row_values(temperature, F32, one), _row_values(top_k, torch.int32, one), _row_values(top_p, F32, one),
+           _row_values(min_p, F32, one), u.data_ptr(), tok.data_ptr(), _row_values(logprob, F32, one), pdl, _raw_stream(logits.get_device()))
     return tok

@@ -95,3 +95,25 @@ def append(b: Batch, cos, sin, q_norm, k_norm, eps):
         q_out[t], q_tol[t] = parts[0]
         keys[i, pos], values[i, pos] = parts[1], b.qkv.view(b.tokens, -1, dim)[t, nq + nkv:]
     return q_out, q_tol, keys, values
+
+
+def attention_on_gpu(b: Batch, device):
+    """`attention` for large batches: the same sums and bounds, a request at a time on the device."""
+    scale, u = 1 / math.sqrt(b.dim), UNIT[b.dtype]
+    out = torch.zeros((b.tokens, b.nq, b.dim), dtype=torch.float64, device=device)
+    tol, lse = out.clone(), torch.full((b.tokens, b.nq), -math.inf, dtype=torch.float64, device=device)
+    lse_tol = torch.zeros_like(lse)
+    for i, (n, kv) in enumerate(b.spec):
+        t = slice(int(b.cu[i]), int(b.cu[i]) + n)
+        last = torch.arange(kv - n, kv, device=device)
+        dead = torch.arange(kv, device=device)[None, :] > last[:, None]
+        for h in range(b.nq):
+            g = h // (b.nq // b.nkv)
+            q, k, v = b.q[t, h].to(device).double(), b.k[i][:, g].to(device).double(), b.v[i][:, g].to(device).double()
+            s = (q @ k.T * scale).masked_fill(dead, -math.inf)
+            p = torch.softmax(s, -1)
+            out[t, h], lse[t, h] = p @ v, torch.logsumexp(s, -1)
+            ds = b.dim * 2.0 ** -24 * (q.abs() @ k.abs().T * scale).amax(-1) + 2.0 ** -20
+            tol[t, h] = u * out[t, h].abs() + (1.01 * u + 2 * ds[:, None]) * (p @ v.abs()) + kv * 2.0 ** -25 * v.abs().amax()
+            lse_tol[t, h] = 2 * ds + 2.0 ** -21 * lse[t, h].abs()
+    return out, lse, tol, lse_tol

@@ -97,6 +97,26 @@ def test_attention_one_request_split_over_every_sm():
     _check(b, out, lse)
 
 
+@pytest.mark.parametrize("spec,nq,nkv,dim,page,dtype", [
+    ([(1500, 4000)], 8, 2, 128, 64, BF16), ([(1, 900), (700, 701), (300, 2000), (1, 3000)], 16, 4, 128, 16, BF16),
+    ([(301, 777), (277, 512), (290, 300)], 14, 2, 64, 32, FP16), ([(2000, 2000)], 4, 4, 128, 128, BF16),
+    ([(40, 3000), (30, 2500), (25, 700)], 32, 8, 128, 32, BF16), ([(9, 5000)] * 5, 8, 2, 64, 16, FP16)])
+def test_attention_large(spec, nq, nkv, dim, page, dtype):
+    """Units of many blocks, cut and whole, with every SM busy; several runs, since what could go wrong here
+    (memory given back too early) shows only sometimes."""
+    b = R.Batch(spec, nq, nkv, dim, page, dtype, seed=17, device=DEV)
+    ref, ref_lse, tol, lse_tol = R.attention_on_gpu(b, DEV)
+    first, err = None, _err()
+    for _ in range(8):
+        out, lse = _attend(b, err=err)
+        assert int(err.item()) == 0
+        d = (out.double() - ref).abs()
+        assert bool((d <= tol).all()), (int((~(d <= tol)).sum()), float(d.max()))
+        assert bool(((lse.double() - ref_lse).abs() <= lse_tol).all())
+        first = out if first is None else first
+        assert torch.equal(out, first)
+
+
 def test_attention_padding_rows_scale_and_no_lse():
     b = R.Batch([(2, 40), (1, 17)], 8, 2, 128, 16, pad_tokens=3, seed=2, device=DEV)
     out, lse = _attend(b, scale=0.3)
