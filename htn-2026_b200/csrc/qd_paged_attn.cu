@@ -44,7 +44,11 @@ constexpr int kPgKeys = 128;     // keys per block
 constexpr int kPgBox = 128 * 128;  // [128 rows][64 dims] of 16 bits
 constexpr int kFewRows = 16;       // rows of a few-row unit (MMA N)
 constexpr int kFewP = 2 * kFewRows * 128;  // its P: 2 halves of 64 keys x 16 rows of 128 B
-constexpr int kPgUnitCost = 2;     // a unit's fixed cost (Q, epilogue) in key blocks, for the split
+// The line of work, in places: a key block of a pair of tiles takes 3, one of a single tile (or few rows) 2, and
+// a unit's fixed cost (Q, its rows' way out) 7; measured, 2.1 us, 1.4 us and some 5 us. A CTA takes whole blocks.
+constexpr int kPgPairCost = 3, kPgBlockCost = 2, kPgUnitCost = 7;
+constexpr int kPgPiece = 12;  // places that a CTA takes at least, where units are whole tiles
+constexpr int kPgWhole = 8;   // key blocks up to which units of tiles are left whole, when there are CTAs for all
 
 struct alignas(64) PagedAttnArgs {
   CUtensorMap tq, tqf, tq1, tk, tv;  // q boxes: a whole tile's tokens, as many as make 16 rows, one
@@ -185,10 +189,17 @@ __device__ __forceinline__ int pg_blocks(const PagedAttnArgs& a, const PgReq& r,
   const int keys = min(r.kv, r.pos0 + min(r.n, (k + 1) * 2 * a.tpt));
   return max((keys + kPgKeys - 1) / kPgKeys, 1);
 }
-// sum of pg_blocks over the request's pairs. Where nothing is cut the terms are ceil((pos0 + 2 tpt k) / 128),
-// which grow by period_blocks every `period` pairs: one pass over a period suffices.
-__device__ __forceinline__ int pg_sum_blocks(const PagedAttnArgs& a, const PgReq& r) {
-  if (r.pairs <= 1) return r.pairs ? pg_blocks(a, r, 0) : 0;
+// places of a key block of tile pair k
+__device__ __forceinline__ int pg_weight(const PagedAttnArgs& a, const PgReq& r, int k) {
+  return r.n - k * 2 * a.tpt > a.tpt ? kPgPairCost : kPgBlockCost;
+}
+__device__ __forceinline__ int pg_cost(const PagedAttnArgs& a, const PgReq& r, int k) {
+  return kPgUnitCost + pg_weight(a, r, k) * pg_blocks(a, r, k);
+}
+// sum of pg_cost over the request's pairs. Where nothing is cut the terms are ceil((pos0 + 2 tpt k) / 128),
+// which grow by period_blocks every `period` pairs: one pass over a period suffices (all but the last are pairs).
+__device__ __forceinline__ int pg_sum_cost(const PagedAttnArgs& a, const PgReq& r) {
+  if (r.pairs <= 1) return r.pairs ? pg_cost(a, r, 0) : 0;
   int sum = 0;
   if (r.pos0 >= 0 && r.kv == r.pos0 + r.n) {
     const int m = r.pairs - 1, q = m / a.period, rest = m - q * a.period;
@@ -197,10 +208,10 @@ __device__ __forceinline__ int pg_sum_blocks(const PagedAttnArgs& a, const PgReq
       const int cnt = q + (j <= rest);
       sum += cnt * ((r.pos0 + 2 * a.tpt * j + kPgKeys - 1) / kPgKeys) + a.period_blocks * (cnt * (cnt - 1) / 2);
     }
-    return sum + pg_blocks(a, r, m);
+    return kPgUnitCost * m + kPgPairCost * sum + pg_cost(a, r, m);
   }
 #pragma unroll 1
-  for (int k = 0; k < r.pairs; ++k) sum += pg_blocks(a, r, k);
+  for (int k = 0; k < r.pairs; ++k) sum += pg_cost(a, r, k);
   return sum;
 }
 // The line of `total` places over `ctas` CTAs: the first total % ctas take one more than the others.
@@ -304,9 +315,8 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
   PgSeg* segs = reinterpret_cast<PgSeg*>(smem + Lay::seg);
   int* misc = reinterpret_cast<int*>(smem + Lay::misc);
   int* abort = misc + 1;
-  int* scan = misc + 16;  // warp totals [12]
+  int* scan = misc + 16;  // warp totals [2][12]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  constexpr int unit_cost = kPgUnitCost;
   if (tid == 0) {
     for (int x = 0; x < 2; ++x) {
       mbar_init(qfull(x), 1);
@@ -335,28 +345,48 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
 
   // ---- this CTA's place on the line: a prefix sum over the requests, and a walk from the one it starts in
   // (in 32 bits: 2^31 key blocks would be hours of work)
-  int mine = 0;
+  int mine = 0, mine_u = 0;  // places, and units
   const int per = (a.b.batch + kPgThreads - 1) / kPgThreads;
   const int i0 = min(tid * per, a.b.batch), i1 = min(i0 + per, a.b.batch);
   PgReq r = {};
-  bool cut = false;
+  bool cut = false, tiles = false, longer = false;
   for (int i = i0; i < i1; ++i) {
     r = pg_request(a, i);
+    tiles |= r.n > a.tpf;
     cut |= r.kv != r.pos0 + r.n && r.n > 0;
-    mine += a.b.nkv * (unit_cost * r.pairs + pg_sum_blocks(a, r));
+    mine += a.b.nkv * pg_sum_cost(a, r);
+    mine_u += a.b.nkv * r.pairs;
+    longer |= r.pairs && pg_blocks(a, r, r.pairs - 1) > kPgWhole;
   }
   if (cut && blockIdx.x == 0) flag_error(a.b.err, QD_DEVERR_PAGE);
-  int incl = mine;
+  int incl = mine, incl_u = mine_u;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += v;
+    const int v = __shfl_up_sync(0xffffffffu, incl, o), u = __shfl_up_sync(0xffffffffu, incl_u, o);
+    if (lane >= o) {
+      incl += v;
+      incl_u += u;
+    }
   }
-  if (lane == 31) scan[warp] = incl;
+  if (lane == 31) {
+    scan[warp] = incl;
+    scan[12 + warp] = incl_u;
+  }
   tc_fence_before();
-  __syncthreads();
+  tiles = __syncthreads_or(tiles);
+  longer = __syncthreads_or(longer);
   tc_fence_after();
   grid_dep_launch();
+  int units = 0;
+#pragma unroll
+  for (int w = 0; w < kPgThreads / 32; ++w) units += scan[12 + w];
+  // Units of tiles that are few and short are not cut: a place each, and a CTA each
+  const bool whole = tiles && !longer && units <= (int)gridDim.x;
+  if (whole) {
+    mine = mine_u;
+    incl = incl_u;
+    scan += 12;
+  }
   int before = incl - mine;
   PgLine line;
   line.total = 0;
@@ -366,8 +396,11 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
     if (w < warp) before += v;
     line.total += v;
   }
-  // with less than one place per CTA the first ones take one each, and the rest nothing
-  line.ctas = min((unsigned)gridDim.x, line.total);
+  // With little work the first CTAs take kPgPiece places each (a block, if all units have few rows), the rest
+  // nothing: joining the pieces of a tile of 128 rows costs about as much as some blocks of keys. No CTA takes
+  // less than a block, so that every one between the first and the last of a cut unit has some of it.
+  const unsigned least = whole ? 1 : tiles ? kPgPiece : kPgBlockCost;
+  line.ctas = min((unsigned)gridDim.x, max(line.total / least, min(line.total, 1u)));
   line.each = line.ctas ? line.total / line.ctas : 0;
   line.more = line.total - line.each * line.ctas;
   const int cta = blockIdx.x;
@@ -377,15 +410,16 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
     int w = begin - before, i = i0;
     if (per > 1) {
       for (r = pg_request(a, i);; r = pg_request(a, ++i)) {
-        const int c = a.b.nkv * (unit_cost * r.pairs + pg_sum_blocks(a, r));
+        const int c = a.b.nkv * (whole ? r.pairs : pg_sum_cost(a, r));
         if (w < c) break;
         w -= c;
       }
     }
-    int k = 0, len = unit_cost + pg_blocks(a, r, 0);
+    int k = 0, len = whole ? 1 : pg_cost(a, r, 0);
     while (w >= a.b.nkv * len) {
       w -= a.b.nkv * len;
-      len = unit_cost + pg_blocks(a, r, ++k);
+      ++k;
+      len = whole ? 1 : pg_cost(a, r, k);
     }
     misc[2] = i;
     misc[3] = k;
@@ -418,12 +452,14 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
       return max(ld_i32(a.b.table + i * a.b.ld_table + (key >> a.b.page_shift)), -1);
     };
     while (at < end && ok) {
-      const int nblk = pg_blocks(a, r, k);
-      const int take = min(end - at, unit_cost + nblk - o);
-      const int j0 = max(o - unit_cost, 0), j1 = max(o + take - unit_cost, 0);
+      const int nblk = pg_blocks(a, r, k), wt = pg_weight(a, r, k), len = whole ? 1 : kPgUnitCost + wt * nblk;
+      const int take = min(end - at, len - o);
+      // the blocks whose first places are among these
+      const int j0 = whole ? 0 : (max(o - kPgUnitCost, 0) + wt - 1) / wt;
+      const int j1 = whole ? nblk : (max(o + take - kPgUnitCost, 0) + wt - 1) / wt;
       if (j1 > j0) {
         int page = page_of(j0);
-        const int first = at - o + unit_cost;  // place of the unit's first block
+        const int first = at - o + kPgUnitCost;  // place of the unit's first block
         const int t0 = k * 2 * a.tpt, ntok = min(2 * a.tpt, r.n - t0);
         const bool two = ntok > a.tpt, few = ntok <= a.tpf;
         const int ra = two ? 0 : next_region;
@@ -448,7 +484,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
                         qfull(reg), pol);
             misc[6 + reg] = qfills[reg] + 1;
           }
-          const int c0 = line.owner(first), c1 = line.owner(first + nblk - 1);
+          const int c0 = whole ? cta : (int)line.owner(first), c1 = whole ? cta : (int)line.owner(first + wt * (nblk - 1));
           PgSeg* s = segs + (seg & 3);
           s->row0 = r.row0 + t0;
           s->ntok = ntok;
@@ -1127,58 +1163,51 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
         if (joined) mbar_arrive(ofree(1));
       }
       bool out_rows = g.whole;
-      if (!g.whole && is_last(g)) {  // join the pieces in the order of their keys: thread = row
+      if (!g.whole && is_last(g)) {  // join the pieces in the order of their keys
         out_rows = true;
-        float M = -INFINITY, L = 0.f;
-        const int row = min(r, rows - 1);
-        auto slot_of = [&](int q) { return 2 * (g.c0 + q) + (q == 0 ? 1 : 0); };
 #pragma unroll 1
-        for (int q = 0; q < g.nc; ++q) M = fmaxf(M, __ldcg(part_m(slot_of(q), row)).x);
-        const float base = M == -INFINITY ? 0.f : M;
+        for (int e = r; e < rows * (D / 8); e += 128) {  // 8 dims of a row, four pieces' loads in flight
+          const int c8 = e / rows, row = e - c8 * rows;
+          float M = -INFINITY, L = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
-        for (int q = 0; q < g.nc; ++q) {
-          const float2 ml = __ldcg(part_m(slot_of(q), row));
-          L += ml.y * exp2f(ml.x - base);
-        }
-        const float inv = L > 0.f ? 1.0f / L : 0.f;
-#pragma unroll 1
-        for (int c8 = 0; c8 < D / 8; c8 += 2) {  // 16 dims at a time
-          float acc[16];
+          for (int q0 = 0; q0 < g.nc; q0 += 4) {
+            float2 p[4];
+            float4 v[4][2];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) acc[e] = 0.f;
-#pragma unroll 1
-          for (int q = 0; q < g.nc; q += 2) {
-            const int q1 = min(q + 1, g.nc - 1);
-            float4 v[2][4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              v[0][c] = __ldcg(part_c(slot_of(q), 2 * c8 + c) + row);
-              v[1][c] = __ldcg(part_c(slot_of(q1), 2 * c8 + c) + row);
+            for (int q = 0; q < 4; ++q) {
+              const int qq = min(q0 + q, g.nc - 1), slot_q = 2 * (g.c0 + qq) + (qq == 0 ? 1 : 0);
+              p[q] = __ldcg(part_m(slot_q, row));
+              v[q][0] = __ldcg(part_c(slot_q, 2 * c8) + row);
+              v[q][1] = __ldcg(part_c(slot_q, 2 * c8 + 1) + row);
             }
-            const float w0 = exp2f(__ldcg(part_m(slot_of(q), row)).x - base) * inv;
-            const float w1 = q + 1 < g.nc ? exp2f(__ldcg(part_m(slot_of(q1), row)).x - base) * inv : 0.f;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              acc[4 * c] = fmaf(v[1][c].x, w1, fmaf(v[0][c].x, w0, acc[4 * c]));
-              acc[4 * c + 1] = fmaf(v[1][c].y, w1, fmaf(v[0][c].y, w0, acc[4 * c + 1]));
-              acc[4 * c + 2] = fmaf(v[1][c].z, w1, fmaf(v[0][c].z, w0, acc[4 * c + 2]));
-              acc[4 * c + 3] = fmaf(v[1][c].w, w1, fmaf(v[0][c].w, w0, acc[4 * c + 3]));
-            }
+            for (int q = 0; q < 4; ++q)
+              if (q0 + q < g.nc && p[q].y > 0.f) {  // a piece in which the row saw no key counts for nothing
+                const float mn = fmaxf(M, p[q].x), wa = exp2f(M - mn), wb = exp2f(p[q].x - mn);
+                M = mn;
+                L = L * wa + p[q].y * wb;
+                const float u[8] = {v[q][0].x, v[q][0].y, v[q][0].z, v[q][0].w, v[q][1].x, v[q][1].y, v[q][1].z, v[q][1].w};
+#pragma unroll
+                for (int d = 0; d < 8; ++d) acc[d] = acc[d] * wa + u[d] * wb;
+              }
           }
-          uint32_t w[8];
+          const float inv = L > 0.f ? 1.0f / L : 0.f;
+          uint32_t w[4];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) w[e] = Elem<T>::pack(acc[2 * e], acc[2 * e + 1]);
-          lay_down(c8, w);
-          lay_down(c8 + 1, w + 4);
+          for (int d = 0; d < 4; ++d) w[d] = Elem<T>::pack(acc[2 * d] * inv, acc[2 * d + 1] * inv);
+          *reinterpret_cast<uint4*>(stage + row * (2 * D) + ((c8 ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+          if (c8 == 0 && a.lse) {
+            const int rt = (row * a.inv_group) >> 16;
+            a.lse[(g.row0 + t0 + rt) * a.ld_lse + g.head * a.group + row - rt * a.group] =
+                L > 0.f ? (M + __log2f(L)) * 0.69314718055994531f : -INFINITY;
+          }
         }
-        m_used = M;
-        l = L;
       }
       if (!ok) break;
       if (out_rows) {
         store_rows();
         if (!ok) break;
-        if (r < rows && a.lse)
+        if (g.whole && r < rows && a.lse)
           a.lse[tok * a.ld_lse + head] = l > 0.f ? (m_used + __log2f(l)) * 0.69314718055994531f : -INFINITY;
       }
       fence_proxy_async_smem();  // the slot's next contents come by TMA
