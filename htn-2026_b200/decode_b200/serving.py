@@ -1,0 +1,175 @@
+"""Serving many requests at once: prompts of any lengths come in while others decode, with sampled answers.
+
+`PagedServer` runs an Engine's packed weights over a paged K/V cache (`paged`) and draws tokens with
+`sample`. Every step is one ragged forward: one token of each request that is decoding and, within a budget
+of tokens, chunks of the prompts that are coming in (no counterpart in the reference, whose batch is fixed
+for the whole answer).
+
+    srv = PagedServer(Engine(path), pages=4096)
+    a = srv.add([151644, 872, 198], max_new_tokens=64, temperature=0.7, top_p=0.8, top_k=20, seed=1)
+    b = srv.add(another_prompt, max_new_tokens=200)            # greedy
+    for finished_step in srv.run():                            # {request: token} of every step
+        ...
+"""
+
+from __future__ import annotations
+
+import random
+from dataclasses import dataclass, field
+
+import torch
+
+from . import lib as L
+from . import ops, paged
+from .sample import sample
+
+BF16 = torch.bfloat16
+
+
+@dataclass
+class Request:
+    prompt: list[int]
+    max_new_tokens: int
+    temperature: float
+    top_k: int
+    top_p: float
+    min_p: float
+    rng: random.Random
+    cached: int = 0                    # positions in the cache
+    pages: list[int] = field(default_factory=list)
+    out: list[int] = field(default_factory=list)
+    logprobs: list[float] = field(default_factory=list)
+
+    def pending(self) -> list[int]:
+        """Tokens that are not in the cache yet."""
+        return (self.prompt + self.out)[self.cached:]
+
+
+class PagedServer:
+    """`pages` pages of `page_size` positions for every layer; at most max_tokens tokens a step and
+    max_requests requests at a time (others wait)."""
+
+    def __init__(self, eng, pages: int, page_size: int = 64, max_tokens: int = 2048, max_requests: int = 64):
+        self.eng, self.page_size, self.max_tokens, self.max_requests = eng, page_size, max_tokens, max_requests
+        dev, D, nq, nkv, H = eng.device, eng.head_dim, eng.nq, eng.nkv, eng.hidden
+        shape = (eng.n_layers, pages, nkv, page_size, D)
+        self.k_pages = torch.zeros(shape, dtype=BF16, device=dev)
+        self.v_pages = torch.zeros(shape, dtype=BF16, device=dev)
+        self.cos, self.sin = paged.rope_table(pages * page_size, D, eng.theta, dev)
+        self.attn = paged.PagedAttention(nq, nkv, D, dev)
+        self.free = list(range(pages - 1, -1, -1))
+        self.waiting: list[int] = []
+        self.active: list[int] = []
+        self.requests: dict[int, Request] = {}
+        self.err = torch.zeros((1,), dtype=torch.int32, device=dev)
+        new = lambda *s: torch.empty(s, dtype=BF16, device=dev)  # noqa: E731
+        self.x, self.h, self.qkv = new(max_tokens, H), new(max_tokens, H), new(max_tokens, (nq + 2 * nkv) * D)
+        self.q, self.att, self.act = new(max_tokens, nq * D), new(max_tokens, nq * D), new(max_tokens, eng.inter)
+        self.vrows = ops.packed_rows(eng.vocab)
+        self.logits = new(max_requests, self.vrows)
+        self.tok = torch.empty((max_requests,), dtype=torch.int64, device=dev)
+        self.logprob = torch.empty((max_requests,), dtype=torch.float32, device=dev)
+        self.next_id = 0
+
+    # ------------------------------------------------------------------ requests
+    def add(self, prompt, max_new_tokens: int, temperature: float = 0.0, top_k: int = 0, top_p: float = 1.0,
+            min_p: float = 0.0, seed: int = 0) -> int:
+        """Queues a request; its number. temperature 0 takes the most likely token."""
+        if not prompt or max_new_tokens < 1:
+            raise ValueError("a request needs a prompt and at least one new token")
+        need = -(-(len(prompt) + max_new_tokens) // self.page_size)
+        if need > self.k_pages.shape[1]:
+            raise ValueError(f"request of {len(prompt) + max_new_tokens} positions needs {need} pages, "
+                             f"there are {self.k_pages.shape[1]}")
+        i, self.next_id = self.next_id, self.next_id + 1
+        self.requests[i] = Request(list(prompt), max_new_tokens, temperature, top_k, top_p, min_p, random.Random(seed))
+        self.waiting.append(i)
+        return i
+
+    def _admit(self) -> None:
+        """A waiting request joins when the pages of its whole answer are free, so no step runs out of them."""
+        while self.waiting and len(self.active) < self.max_requests:
+            r = self.requests[self.waiting[0]]
+            need = -(-(len(r.prompt) + r.max_new_tokens) // self.page_size)
+            if need > len(self.free):
+                return
+            r.pages = [self.free.pop() for _ in range(need)]
+            self.active.append(self.waiting.pop(0))
+
+    def _plan(self) -> list[tuple[int, list[int]]]:
+        """(request, tokens of this step): the decoding requests' tokens, then chunks of prompts."""
+        left, batch = self.max_tokens, []
+        for i in sorted(self.active, key=lambda i: len(self.requests[i].pending()) > 1):
+            tokens = self.requests[i].pending()[:left]
+            if tokens:
+                batch.append((i, tokens))
+                left -= len(tokens)
+        return batch
+
+    # ------------------------------------------------------------------ a step
+    def step(self) -> dict[int, int]:
+        """One forward; {request: drawn token} for those whose last pending token was in it."""
+        self._admit()
+        batch = self._plan()
+        if not batch:
+            return {}
+        dev, reqs = self.eng.device, [self.requests[i] for i, _ in batch]
+        cu, width = [0], max(len(r.pages) for r in reqs)
+        for _, tokens in batch:
+            cu.append(cu[-1] + len(tokens))
+        ids = torch.tensor([t for _, tokens in batch for t in tokens], dtype=torch.int64).to(dev)
+        kv = [r.cached + len(t) for r, (_, t) in zip(reqs, batch)]
+        ints = torch.tensor(cu + kv + [p for r in reqs for p in r.pages + [0] * (width - len(r.pages))],
+                            dtype=torch.int32).to(dev)
+        n = len(batch)
+        logits = self.forward(ids, ints[:n + 1], ints[n + 1:2 * n + 1], ints[2 * n + 1:].view(n, width))
+        draw = torch.tensor([[r.temperature, r.top_p, r.min_p, r.rng.random()] for r in reqs], dtype=torch.float32)
+        t, top_p, min_p, u = draw.t().contiguous().to(dev).unbind(0)
+        top_k = torch.tensor([r.top_k for r in reqs], dtype=torch.int32).to(dev)
+        sample(logits, u, self.tok[:n], temperature=t, top_k=top_k, top_p=top_p, min_p=min_p,
+               logprob=self.logprob[:n], vocab=self.eng.vocab)
+        tok, logprob, err = self.tok[:n].tolist(), self.logprob[:n].tolist(), int(self.err.item())
+        if err:
+            raise RuntimeError(f"serving step reported a device error: {L.describe_device_error(err)}")
+        drawn = {}
+        for (i, _), r, length, token, lp in zip(batch, reqs, kv, tok, logprob):
+            r.cached = length
+            if not r.pending():  # the whole prompt (or the last token) is in: this row's draw is its next token
+                r.out.append(token)
+                r.logprobs.append(lp)
+                drawn[i] = token
+                if len(r.out) == r.max_new_tokens:
+                    self.free += r.pages
+                    r.pages = []
+                    self.active.remove(i)
+        return drawn
+
+    def run(self):
+        """Steps until every request is done; yields each step's {request: token}."""
+        while self.waiting or self.active:
+            yield self.step()
+
+    def forward(self, ids, cu_tokens, kv_len, page_table):
+        """Logits [requests, vocab rows] after each request's last token of the ragged batch."""
+        eng, T = self.eng, ids.shape[0]
+        H, I, eps, nq, nkv, D = eng.hidden, eng.inter, eng.eps, eng.nq, eng.nkv, eng.head_dim
+        x, h, qkv, q, att, act = (b[:T] for b in (self.x, self.h, self.qkv, self.q, self.att, self.act))
+        batch = dict(cu_tokens=cu_tokens, kv_len=kv_len, page_table=page_table, err=self.err)
+        RES, SWIGLU = ops.Gemv.RES, ops.Gemv.SWIGLU
+        ops.embed(ids, eng.e_packed, eng.vocab, x, self.err, pdl=False)
+        for i in range(eng.n_layers):
+            kp, vp = self.k_pages[i], self.v_pages[i]
+            ops.rmsnorm_rows(x, eng.ln1[i], eps, h)
+            ops.tc_gemm(h, eng.w_qkv[i], (nq + 2 * nkv) * D, qkv, err=self.err)
+            paged.rope_append(qkv, nq=nq, nkv=nkv, cos=self.cos, sin=self.sin, q_out=q, k_pages=kp, v_pages=vp,
+                              q_norm=eng.qn[i], k_norm=eng.kn[i], eps=eps, **batch)
+            self.attn(q, kp, vp, out=att, **batch)
+            ops.tc_gemm(att, eng.w_o[i], H, x, res=x, epilogue=RES, err=self.err)
+            ops.rmsnorm_rows(x, eng.ln2[i], eps, h)
+            ops.tc_gemm(h, eng.w_gu[i], 2 * I, act, epilogue=SWIGLU, err=self.err)
+            ops.tc_gemm(act, eng.w_down[i], H, x, res=x, epilogue=RES, err=self.err)
+        last = x.index_select(0, cu_tokens[1:].long() - 1)
+        n = last.shape[0]
+        ops.rmsnorm_rows(last, eng.final_norm, eps, h[:n])  # (no more requests than tokens)
+        ops.tc_gemm(h[:n], eng.e_packed, self.vrows, self.logits[:n], err=self.err)
+        return self.logits[:n]
