@@ -19,8 +19,8 @@
 // are reduced over the warpgroup, P goes to shared memory as the K-major operand of O^T += V^T P^T (M =
 // head_dim, N = 16 rows). Even and odd blocks alternate between the warpgroups as above.
 //
-// Keys and values come page by page: a box of a page's rows x 64 dims per copy (TMA, 128-byte swizzle), the
-// lanes of the producer warp issuing one each, into a ring of slots that K and V blocks take in turn. Rows
+// Keys and values come page by page: a copy (TMA, 128-byte swizzle) per page of a KV head, issued by a lane of
+// the producer warp each, into a ring of slots that K and V blocks take in turn. Rows
 // past the request's last key hold anything, NaN included: their scores are replaced by -inf before any
 // arithmetic, and the MMA warp zeroes their V rows in shared memory (0 x NaN would be NaN).
 //
@@ -57,6 +57,7 @@ struct alignas(64) PagedAttnArgs {
   float* lse;
   int64_t ldo, ld_lse;
   int group, tpt, tpf;        // heads per KV head, tokens per tile and per 16 rows (0: a group is larger)
+  int head_groups;            // groups of 8 rows from a KV head of a page to the next
   int inv_group;              // row / group = row * inv_group >> 16 for the rows of a tile
   int period, period_blocks;  // ceil sums over tile pairs repeat every `period` pairs, `period_blocks` blocks on
   float scale_log2;
@@ -69,6 +70,9 @@ struct alignas(64) PagedAttnArgs {
 template <int D>
 struct PgLayout {
   static constexpr int kItem = D / 64 * kPgBox;  // a K or V block, and a Q tile
+  // a K or V block: groups of 8 rows, in each the halves of 64 dims, in each the rows of 128 bytes (a Q tile: the
+  // halves, in each the rows). So a page, all its dims, is one box of a copy and lies in one piece.
+  static constexpr int kGroup = D / 64 * 1024, kHalf = 1024;
   static constexpr int kSlots = D == 128 ? 5 : 10;
   static constexpr int q = 0;
   static constexpr int kv = q + 2 * kItem;
@@ -107,6 +111,14 @@ __device__ __forceinline__ void pg_tma_4d(uint32_t dst, const CUtensorMap* map, 
       "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
       " [%0], [%1, {%2, %3, %4, %5}], [%6], %7;" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar), "l"(policy)
+      : "memory");
+}
+__device__ __forceinline__ void pg_tma_5d(uint32_t dst, const CUtensorMap* map, int w, int v, uint32_t bar,
+                                          uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%2, %2, %2, %3, %4}], [%5], %6;" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(w), "r"(v), "r"(bar), "l"(policy)
       : "memory");
 }
 __device__ __forceinline__ float pg_max3(float a, float b, float c) {
@@ -438,8 +450,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
     // ------------------------------------------------------------ producer: all lanes walk the line
     const uint64_t pol = policy_evict_normal();
     int at = begin, i = misc[2], k = misc[3], h = misc[4], o = misc[5];
-    const int boxes = (kPgKeys >> a.b.page_shift) * kHalves, box_bytes = a.b.page_size * 128;
-    const int my_page = lane / kHalves, my_half = lane % kHalves;
+    const int boxes = kPgKeys >> a.b.page_shift, box_bytes = a.b.page_size * D * 2;  // lane: page of the block
     int seg = 0, items = 0, slot = 0, next_region = 0, qfills[2] = {0, 0};
     uint32_t phase = 1;  // of empty(slot): a ring's first round passes at once
     bool ok = true;
@@ -447,7 +458,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
     __syncwarp();
     // this lane's page of block j of the current request; -2: no box (past the last key)
     auto page_of = [&](int j) {
-      const int key = j * kPgKeys + (my_page << a.b.page_shift);
+      const int key = j * kPgKeys + (lane << a.b.page_shift);
       if (lane >= boxes || key >= r.kv) return -2;
       return max(ld_i32(a.b.table + i * a.b.ld_table + (key >> a.b.page_shift)), -1);
     };
@@ -513,7 +524,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
             flag_error(a.b.err, QD_DEVERR_PAGE);
             page = -1;  // outside the tensor map: the copy fills zeros
           }
-          const uint32_t at_page = sb + Lay::kv + my_half * kPgBox + my_page * box_bytes;
+          const uint32_t at_page = sb + Lay::kv + lane * box_bytes;
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {
             const bool got = mbar_wait_abort(empty(slot), phase, a.b.err, kErrWaitEmpty, abort);
@@ -527,7 +538,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
             }
             __syncwarp();
             if (need)
-              pg_tma_4d(at_page + slot * Lay::kItem, kv ? &a.tv : &a.tk, 64 * my_half, 0, h, page, full(slot), pol);
+              pg_tma_5d(at_page + slot * Lay::kItem, kv ? &a.tv : &a.tk, h * a.head_groups, page, full(slot), pol);
             if (++slot == kSlots) {
               slot = 0;
               phase ^= 1;
@@ -562,9 +573,9 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
     constexpr uint32_t id_of = (umma_idesc_bf16(kFewRows, true, false) & ~kTypes) | kind;
     // low words of the operand descriptors: a start address in units of 16 B, so steps are plain additions
     const uint32_t d_q = umma_desc_lo(sb + Lay::q), d_k = umma_desc_lo(sb + Lay::kv);
-    const uint32_t d_v = umma_desc_lo(sb + Lay::kv, kPgBox);
+    const uint32_t d_v = umma_desc_lo(sb + Lay::kv, Lay::kHalf);
     // few rows, head_dim 64: the 64 upper rows of O^T repeat the lower ones (block stride 0)
-    const uint32_t d_vf = umma_desc_lo(sb + Lay::kv, D == 128 ? kPgBox : 0);
+    const uint32_t d_vf = umma_desc_lo(sb + Lay::kv, D == 128 ? Lay::kHalf : 0);
     constexpr uint32_t kItem16 = Lay::kItem >> 4;
     int slot = 0, pc[2] = {0, 0}, units[2] = {0, 0};
     uint32_t phase = 0, quse = 0;  // of full(slot); bit r: the phase of qfull(r)
@@ -601,8 +612,11 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
         const uint32_t q = d_q + reg * kItem16, kt = d_k + k.slot * kItem16;
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) {  // 16 dims per MMA: +32 B inside a 64-dim half, the next half after 4
-          const uint32_t step = ((d >> 2) * kPgBox + (d & 3) * 32) >> 4;
-          umma_f16(tS(x), (few ? kt : q) + step, (few ? q : kt) + step, few ? id_sf : id_s, d > 0 ? 1u : 0u);
+          const uint32_t q_d = q + (((d >> 2) * kPgBox + (d & 3) * 32) >> 4), k_d = kt + (((d >> 2) * Lay::kHalf + (d & 3) * 32) >> 4);
+          if constexpr (few)
+            umma_f16<Lay::kGroup, 1024>(tS(x), k_d, q_d, id_sf, d > 0 ? 1u : 0u);
+          else
+            umma_f16<1024, Lay::kGroup>(tS(x), q_d, k_d, id_s, d > 0 ? 1u : 0u);
         }
       }
       umma_commit(sfull(x));
@@ -620,10 +634,11 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk) {  // 16 keys per MMA: 8 columns of P pairs; V two 8-key atoms
           const uint32_t acc = kk ? 1u : first ? 0u : 1u;
-          if (few)
-            umma_f16(tO(x), vt + kk * (2048 >> 4), pt + (((kk >> 2) * (kFewP / 2) + (kk & 3) * 32) >> 4), id_of, acc);
+          const uint32_t v_k = vt + kk * (2 * Lay::kGroup >> 4);
+          if constexpr (few)
+            umma_f16<Lay::kGroup, 1024>(tO(x), v_k, pt + (((kk >> 2) * (kFewP / 2) + (kk & 3) * 32) >> 4), id_of, acc);
           else
-            umma_f16_ts(tO(x), tS(pair ? 1 - x : x) + 8 * kk, vt + kk * (2048 >> 4), id_o, acc);
+            umma_f16_ts<Lay::kGroup>(tO(x), tS(pair ? 1 - x : x) + 8 * kk, v_k, id_o, acc);
         }
       }
       ++pc[x];
@@ -637,7 +652,8 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
 #pragma unroll 1
       for (int c = max(rows, 0) * 8 + lane; c < kPgKeys * 8; c += 32)
 #pragma unroll
-        for (int hf = 0; hf < kHalves; ++hf) *reinterpret_cast<uint4*>(vt + hf * kPgBox + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+        for (int hf = 0; hf < kHalves; ++hf)
+          *reinterpret_cast<uint4*>(vt + (c >> 6) * Lay::kGroup + hf * Lay::kHalf + (c & 63) * 16) = make_uint4(0u, 0u, 0u, 0u);
       fence_proxy_async_smem();
       __syncwarp();
     };
@@ -1274,6 +1290,8 @@ extern "C" int qd_paged_attn(const void* q, int64_t ldq, int dtype, int64_t toke
   if (grid < 1 || !scratch || scratch_bytes < plan.bytes || (reinterpret_cast<uintptr_t>(scratch) & 31))
     return set_error(QD_ERR_SCRATCH, "paged attention: grid %d needs %lld B of 32-byte aligned scratch (have %lld)", grid,
                      (long long)plan.bytes, (long long)scratch_bytes);
+  if (ps_head % (8 * head_dim))
+    return set_error(QD_ERR_ARG, "paged attention: head stride %lld (whole groups of 8 rows)", (long long)ps_head);
   if (tokens == 0) return QD_OK;
   const PFN_cuTensorMapEncodeTiled_v12000 encode = tensor_map_encoder();
   if (!encode) return set_error(QD_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
@@ -1297,12 +1315,18 @@ extern "C" int qd_paged_attn(const void* q, int64_t ldq, int dtype, int64_t toke
     if (!map4(&a.tq, q, dims, strides, box) || !map4(&a.tqf, q, dims, strides, boxf) || !map4(&a.tq1, q, dims, strides, box1))
       return set_error(QD_ERR_CUDA, "cuTensorMapEncodeTiled failed for q");
   }
-  {
-    const cuuint64_t dims[4] = {(cuuint64_t)head_dim, (cuuint64_t)page_size, (cuuint64_t)nkv_heads, (cuuint64_t)n_pages};
-    const cuuint64_t strides[3] = {(cuuint64_t)head_dim * 2, (cuuint64_t)ps_head * 2, (cuuint64_t)ps_page * 2};
-    const cuuint32_t box[4] = {64, (cuuint32_t)page_size, 1, 1};
-    if (!map4(&a.tk, k_pages, dims, strides, box) || !map4(&a.tv, v_pages, dims, strides, box))
-      return set_error(QD_ERR_CUDA, "cuTensorMapEncodeTiled failed for the pools");
+  {  // a page of a KV head: 64 dims x 8 rows x halves x groups of 8 rows, in that order; heads are whole groups apart
+    const int64_t group = 8 * (int64_t)head_dim;
+    a.head_groups = (int)(ps_head / group);
+    const cuuint64_t dims[5] = {64, 8, (cuuint64_t)head_dim / 64, (cuuint64_t)((nkv_heads - 1) * (ps_head / group) + page_size / 8),
+                                (cuuint64_t)n_pages};
+    const cuuint64_t strides[4] = {(cuuint64_t)head_dim * 2, 128, (cuuint64_t)group * 2, (cuuint64_t)ps_page * 2};
+    const cuuint32_t box[5] = {64, 8, (cuuint32_t)head_dim / 64, (cuuint32_t)page_size / 8, 1}, one[5] = {1, 1, 1, 1, 1};
+    for (int v = 0; v < 2; ++v)
+      if (encode(v ? &a.tv : &a.tk, type, 5, const_cast<void*>(v ? v_pages : k_pages), dims, strides, box, one,
+                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return set_error(QD_ERR_CUDA, "cuTensorMapEncodeTiled failed for the pools");
   }
   int g = 2 * a.tpt;  // gcd(2 tpt, 128): the power of two in 2 tpt, up to 128
   g = (g & -g) < kPgKeys ? (g & -g) : kPgKeys;

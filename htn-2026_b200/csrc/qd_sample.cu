@@ -570,7 +570,19 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     // halves of up to 2^20 a logit: 32 bits hold the sums of a lane's 512 vectors (2^18 logits over 128 or
     // more warps), and of the warp in 64
     uint32_t hi = 0, lo = 0, eq = 0;
-    each([&](const float* v, int) { add_kept(v, hi, lo, eq); });
+    if (thr == -INFINITY && floor_d == -INFINITY)  // every token that is not masked
+      each([&](const float* v, int) {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) {
+          // the bound turns NaN and -inf into weight 0, as it is for all that deep
+          uint32_t h, l;
+          weight_halves(expf(fmaxf(logit_depth(v[j], m, inv_t), -100.f)), h, l);
+          hi += h - kHalfBits;
+          lo += l - kHalfBits;
+        }
+      });
+    else
+      each([&](const float* v, int) { add_kept(v, hi, lo, eq); });
     const uint64_t w = warp_sum64(((uint64_t)hi << 20) + lo);
     eq = __reduce_add_sync(0xffffffffu, eq);
     if (lane == 0) {

@@ -43,27 +43,29 @@ __device__ __forceinline__ void umma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, u
       "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u));
 }
 // The two products without the (all-zero) lane mask operand, for any kind::f16 types, issued by one elected
-// lane (elect_one), from the low words of descriptors of 1024-byte stride (umma_desc_lo): what an instruction
+// lane (elect_one), from the low words of the descriptors (umma_desc_lo; the strides sbo of A and B are constants): what an instruction
 // takes from ordinary registers is moved to uniform ones first, and those moves bound the issue. Measured with
 // one warp issuing 128 x 128 x 16 products back to back: 137 cycles each with the mask, 65 without (the tensor
 // core itself takes 64).
-constexpr uint32_t kUmmaDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+constexpr uint32_t umma_desc_hi(uint32_t sbo) { return (sbo >> 4) | (1u << 14) | (2u << 29); }
 __device__ __forceinline__ uint32_t umma_desc_lo(uint32_t saddr, uint32_t lbo = 16) {
   return ((saddr >> 4) & 0x3FFFu) | ((lbo >> 4) << 16);
 }
+template <uint32_t kSboA = 1024, uint32_t kSboB = 1024>
 __device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n .reg .pred p;\n .reg .b64 da, db;\n setp.ne.b32 p, %4, 0;\n mov.b64 da, {%1, %5};\n mov.b64 db, {%2, %5};\n"
+      "{\n .reg .pred p;\n .reg .b64 da, db;\n setp.ne.b32 p, %4, 0;\n mov.b64 da, {%1, %5};\n mov.b64 db, {%2, %6};\n"
       " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}\n" ::"r"(d_tmem),
-      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(acc), "n"(kUmmaDescHi)
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(acc), "n"(umma_desc_hi(kSboA)), "n"(umma_desc_hi(kSboB))
       : "memory");
 }
+template <uint32_t kSboB = 1024>
 __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc,
                                             uint32_t acc) {
   asm volatile(
       "{\n .reg .pred p;\n .reg .b64 db;\n setp.ne.b32 p, %4, 0;\n mov.b64 db, {%2, %5};\n"
       " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n}\n" ::"r"(d_tmem),
-      "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(acc), "n"(kUmmaDescHi)
+      "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(acc), "n"(umma_desc_hi(kSboB))
       : "memory");
 }
 // True in one lane of a converged warp, the same one every time.

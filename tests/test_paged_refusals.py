@@ -58,7 +58,7 @@ def test_append_refuses(lib, change, code):
 
 @pytest.mark.parametrize("change,code", SHARED + [
     ({"q": None}, 1), ({"q": P + 2}, 1), ({"out": None}, 1), ({"out": P + 8}, 1), ({"ldq": 4095}, 1), ({"ldo": 4088}, 1),
-    ({"ld_lse": 31}, 1), ({"scale": 0.0}, 1), ({"scale": float("nan")}, 1), ({"grid": 0}, 2), ({"scratch": None}, 2),
+    ({"ld_lse": 31}, 1), ({"ps_head": 16 * 128 + 8}, 1), ({"scale": 0.0}, 1), ({"scale": float("nan")}, 1), ({"grid": 0}, 2), ({"scratch": None}, 2),
     ({"bytes": 8}, 2)])
 def test_attention_refuses(lib, change, code):
     assert lib.qd_paged_attn(*_attn_args(**change)) == code, change
