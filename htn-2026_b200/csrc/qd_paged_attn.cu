@@ -19,8 +19,8 @@
 // are reduced over the warpgroup, P goes to shared memory as the K-major operand of O^T += V^T P^T (M =
 // head_dim, N = 16 rows). Even and odd blocks alternate between the warpgroups as above.
 //
-// Keys and values come page by page: a copy (TMA, 128-byte swizzle) per page of a KV head, issued by a lane of
-// the producer warp each, into a ring of slots that K and V blocks take in turn. Rows
+// Keys and values come page by page: a copy (TMA, 128-byte swizzle) per page and half of 64 dims (or per page),
+// issued by a lane of the producer warp each, into a ring of slots that K and V blocks take in turn. Rows
 // past the request's last key hold anything, NaN included: their scores are replaced by -inf before any
 // arithmetic, and the MMA warp zeroes their V rows in shared memory (0 x NaN would be NaN).
 //
@@ -70,9 +70,6 @@ struct alignas(64) PagedAttnArgs {
 template <int D>
 struct PgLayout {
   static constexpr int kItem = D / 64 * kPgBox;  // a K or V block, and a Q tile
-  // a K or V block: groups of 8 rows, in each the halves of 64 dims, in each the rows of 128 bytes (a Q tile: the
-  // halves, in each the rows). So a page, all its dims, is one box of a copy and lies in one piece.
-  static constexpr int kGroup = D / 64 * 1024, kHalf = 1024;
   static constexpr int kSlots = D == 128 ? 5 : 10;
   static constexpr int q = 0;
   static constexpr int kv = q + 2 * kItem;
@@ -113,12 +110,12 @@ __device__ __forceinline__ void pg_tma_4d(uint32_t dst, const CUtensorMap* map, 
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar), "l"(policy)
       : "memory");
 }
-__device__ __forceinline__ void pg_tma_5d(uint32_t dst, const CUtensorMap* map, int w, int v, uint32_t bar,
+__device__ __forceinline__ void pg_tma_5d(uint32_t dst, const CUtensorMap* map, int z, int w, int v, uint32_t bar,
                                           uint64_t policy) {
   asm volatile(
       "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
-      " [%0], [%1, {%2, %2, %2, %3, %4}], [%5], %6;" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(w), "r"(v), "r"(bar), "l"(policy)
+      " [%0], [%1, {%2, %2, %3, %4, %5}], [%6], %7;" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(z), "r"(w), "r"(v), "r"(bar), "l"(policy)
       : "memory");
 }
 __device__ __forceinline__ float pg_max3(float a, float b, float c) {
@@ -297,10 +294,13 @@ __device__ __forceinline__ void pg_join_few(const PagedAttnArgs& a, const PgSeg&
   }
 }
 
-template <typename T, int D>
+// A K or V block in shared memory: the halves of 64 dims, in each the rows of 128 bytes, 8 to a group; or, merged,
+// the groups and in each the halves, so that a page's whole rows are one box of a copy.
+template <typename T, int D, bool kMerged>
 __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {
   using Lay = PgLayout<D>;
   constexpr int kHalves = D / 64, kSlots = Lay::kSlots;
+  constexpr uint32_t kGroup = kMerged ? 2048 : 1024, kHalf = kMerged ? 1024 : kPgBox;  // bytes from one to the next
   grid_dep_wait();
   extern __shared__ __align__(1024) char smem[];
   if (smem_u32(smem) & 1023u) {  // the swizzled tiles need 1 KiB alignment, and there is no room to realign
@@ -450,7 +450,10 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
     // ------------------------------------------------------------ producer: all lanes walk the line
     const uint64_t pol = policy_evict_normal();
     int at = begin, i = misc[2], k = misc[3], h = misc[4], o = misc[5];
-    const int boxes = kPgKeys >> a.b.page_shift, box_bytes = a.b.page_size * D * 2;  // lane: page of the block
+    // a lane's copy: a page of the block, and a half of its dims unless they are merged
+    constexpr int copies = kMerged ? 1 : kHalves;
+    const int boxes = (kPgKeys >> a.b.page_shift) * copies;
+    const int box_bytes = a.b.page_size * (D * 2) / copies, my_page = lane / copies, my_half = lane % copies;
     int seg = 0, items = 0, slot = 0, next_region = 0, qfills[2] = {0, 0};
     uint32_t phase = 1;  // of empty(slot): a ring's first round passes at once
     bool ok = true;
@@ -458,7 +461,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
     __syncwarp();
     // this lane's page of block j of the current request; -2: no box (past the last key)
     auto page_of = [&](int j) {
-      const int key = j * kPgKeys + (lane << a.b.page_shift);
+      const int key = j * kPgKeys + (my_page << a.b.page_shift);
       if (lane >= boxes || key >= r.kv) return -2;
       return max(ld_i32(a.b.table + i * a.b.ld_table + (key >> a.b.page_shift)), -1);
     };
@@ -524,7 +527,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
             flag_error(a.b.err, QD_DEVERR_PAGE);
             page = -1;  // outside the tensor map: the copy fills zeros
           }
-          const uint32_t at_page = sb + Lay::kv + lane * box_bytes;
+          const uint32_t at_page = sb + Lay::kv + my_half * kPgBox + my_page * box_bytes;
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {
             const bool got = mbar_wait_abort(empty(slot), phase, a.b.err, kErrWaitEmpty, abort);
@@ -538,7 +541,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
             }
             __syncwarp();
             if (need)
-              pg_tma_5d(at_page + slot * Lay::kItem, kv ? &a.tv : &a.tk, h * a.head_groups, page, full(slot), pol);
+              pg_tma_5d(at_page + slot * Lay::kItem, kv ? &a.tv : &a.tk, my_half, h * a.head_groups, page, full(slot), pol);
             if (++slot == kSlots) {
               slot = 0;
               phase ^= 1;
@@ -573,9 +576,9 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
     constexpr uint32_t id_of = (umma_idesc_bf16(kFewRows, true, false) & ~kTypes) | kind;
     // low words of the operand descriptors: a start address in units of 16 B, so steps are plain additions
     const uint32_t d_q = umma_desc_lo(sb + Lay::q), d_k = umma_desc_lo(sb + Lay::kv);
-    const uint32_t d_v = umma_desc_lo(sb + Lay::kv, Lay::kHalf);
+    const uint32_t d_v = umma_desc_lo(sb + Lay::kv, kHalf);
     // few rows, head_dim 64: the 64 upper rows of O^T repeat the lower ones (block stride 0)
-    const uint32_t d_vf = umma_desc_lo(sb + Lay::kv, D == 128 ? Lay::kHalf : 0);
+    const uint32_t d_vf = umma_desc_lo(sb + Lay::kv, D == 128 ? kHalf : 0);
     constexpr uint32_t kItem16 = Lay::kItem >> 4;
     int slot = 0, pc[2] = {0, 0}, units[2] = {0, 0};
     uint32_t phase = 0, quse = 0;  // of full(slot); bit r: the phase of qfull(r)
@@ -612,11 +615,11 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
         const uint32_t q = d_q + reg * kItem16, kt = d_k + k.slot * kItem16;
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) {  // 16 dims per MMA: +32 B inside a 64-dim half, the next half after 4
-          const uint32_t q_d = q + (((d >> 2) * kPgBox + (d & 3) * 32) >> 4), k_d = kt + (((d >> 2) * Lay::kHalf + (d & 3) * 32) >> 4);
+          const uint32_t q_d = q + (((d >> 2) * kPgBox + (d & 3) * 32) >> 4), k_d = kt + (((d >> 2) * kHalf + (d & 3) * 32) >> 4);
           if constexpr (few)
-            umma_f16<Lay::kGroup, 1024>(tS(x), k_d, q_d, id_sf, d > 0 ? 1u : 0u);
+            umma_f16<kGroup, 1024>(tS(x), k_d, q_d, id_sf, d > 0 ? 1u : 0u);
           else
-            umma_f16<1024, Lay::kGroup>(tS(x), q_d, k_d, id_s, d > 0 ? 1u : 0u);
+            umma_f16<1024, kGroup>(tS(x), q_d, k_d, id_s, d > 0 ? 1u : 0u);
         }
       }
       umma_commit(sfull(x));
@@ -634,11 +637,11 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk) {  // 16 keys per MMA: 8 columns of P pairs; V two 8-key atoms
           const uint32_t acc = kk ? 1u : first ? 0u : 1u;
-          const uint32_t v_k = vt + kk * (2 * Lay::kGroup >> 4);
+          const uint32_t v_k = vt + kk * (2 * kGroup >> 4);
           if constexpr (few)
-            umma_f16<Lay::kGroup, 1024>(tO(x), v_k, pt + (((kk >> 2) * (kFewP / 2) + (kk & 3) * 32) >> 4), id_of, acc);
+            umma_f16<kGroup, 1024>(tO(x), v_k, pt + (((kk >> 2) * (kFewP / 2) + (kk & 3) * 32) >> 4), id_of, acc);
           else
-            umma_f16_ts<Lay::kGroup>(tO(x), tS(pair ? 1 - x : x) + 8 * kk, v_k, id_o, acc);
+            umma_f16_ts<kGroup>(tO(x), tS(pair ? 1 - x : x) + 8 * kk, v_k, id_o, acc);
         }
       }
       ++pc[x];
@@ -653,7 +656,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
       for (int c = max(rows, 0) * 8 + lane; c < kPgKeys * 8; c += 32)
 #pragma unroll
         for (int hf = 0; hf < kHalves; ++hf)
-          *reinterpret_cast<uint4*>(vt + (c >> 6) * Lay::kGroup + hf * Lay::kHalf + (c & 63) * 16) = make_uint4(0u, 0u, 0u, 0u);
+          *reinterpret_cast<uint4*>(vt + (c >> 6) * kGroup + hf * kHalf + (c & 63) * 16) = make_uint4(0u, 0u, 0u, 0u);
       fence_proxy_async_smem();
       __syncwarp();
     };
@@ -1245,6 +1248,13 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
   }
 }
 
+template <typename T>
+static const void* attn_kernel(int head_dim, bool merged) {
+  return head_dim == 64 ? (const void*)paged_attn_kernel<T, 64, false>
+         : merged       ? (const void*)paged_attn_kernel<T, 128, true>
+                        : (const void*)paged_attn_kernel<T, 128, false>;
+}
+
 struct PagedAttnPlan {
   int64_t off_partials, bytes;
 };
@@ -1315,13 +1325,16 @@ extern "C" int qd_paged_attn(const void* q, int64_t ldq, int dtype, int64_t toke
     if (!map4(&a.tq, q, dims, strides, box) || !map4(&a.tqf, q, dims, strides, boxf) || !map4(&a.tq1, q, dims, strides, box1))
       return set_error(QD_ERR_CUDA, "cuTensorMapEncodeTiled failed for q");
   }
+  // Pages of 16 rows are merged: half the copies (64 decoding requests 71 us, 84 apart). Larger pages are not: the
+  // products read the interleaved rows slower (a chunk of 2048 after 8192 keys 349 us, 341 apart).
+  const bool merged = page_size == 16 && head_dim == 128;
   {  // a page of a KV head: 64 dims x 8 rows x halves x groups of 8 rows, in that order; heads are whole groups apart
     const int64_t group = 8 * (int64_t)head_dim;
     a.head_groups = (int)(ps_head / group);
     const cuuint64_t dims[5] = {64, 8, (cuuint64_t)head_dim / 64, (cuuint64_t)((nkv_heads - 1) * (ps_head / group) + page_size / 8),
                                 (cuuint64_t)n_pages};
     const cuuint64_t strides[4] = {(cuuint64_t)head_dim * 2, 128, (cuuint64_t)group * 2, (cuuint64_t)ps_page * 2};
-    const cuuint32_t box[5] = {64, 8, (cuuint32_t)head_dim / 64, (cuuint32_t)page_size / 8, 1}, one[5] = {1, 1, 1, 1, 1};
+    const cuuint32_t box[5] = {64, 8, merged ? (cuuint32_t)head_dim / 64 : 1, (cuuint32_t)page_size / 8, 1}, one[5] = {1, 1, 1, 1, 1};
     for (int v = 0; v < 2; ++v)
       if (encode(v ? &a.tv : &a.tk, type, 5, const_cast<void*>(v ? v_pages : k_pages), dims, strides, box, one,
                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -1339,10 +1352,7 @@ extern "C" int qd_paged_attn(const void* q, int64_t ldq, int dtype, int64_t toke
   a.scale_log2 = scale * 1.4426950408889634f;
   a.tickets = static_cast<int*>(scratch);
   a.partials = reinterpret_cast<float*>(static_cast<char*>(scratch) + plan.off_partials);
-  const void* fn = dtype == QD_BF16 ? (head_dim == 128 ? (const void*)paged_attn_kernel<__nv_bfloat16, 128>
-                                                       : (const void*)paged_attn_kernel<__nv_bfloat16, 64>)
-                                    : (head_dim == 128 ? (const void*)paged_attn_kernel<__half, 128>
-                                                       : (const void*)paged_attn_kernel<__half, 64>);
+  const void* fn = dtype == QD_BF16 ? attn_kernel<__nv_bfloat16>(head_dim, merged) : attn_kernel<__half>(head_dim, merged);
   const int smem = head_dim == 128 ? PgLayout<128>::total : PgLayout<64>::total;
   const int rs = set_max_dynamic_smem(fn, smem);
   if (rs != QD_OK) return rs;
