@@ -119,7 +119,11 @@ __device__ __forceinline__ uint64_t depth_weight(float d) {
   weight_halves(expf(d), hi, lo);
   return ((uint64_t)(hi - kHalfBits) << 20) + (lo - kHalfBits);
 }
-__device__ __forceinline__ int depth_bin(float d, float per_d, int bins) { return min((int)(-d * per_d), bins - 1); }
+// the step of d in which a d of -kSampleDeep to 0 lies (by an addition of 2^23 too: a conversion to int would
+// take the exponentials' pipe)
+__device__ __forceinline__ int depth_bin(float d, float per_d, int bins) {
+  return min((int)(__float_as_uint(__fmaf_rd(-d, per_d, 8388608.0f)) - kHalfBits), bins - 1);
+}
 
 // 64-bit sum over the warp by 16-bit pieces: four reduction instructions in place of ten dependent shuffles
 __device__ __forceinline__ uint64_t warp_sum64(uint64_t v) {
@@ -153,13 +157,13 @@ struct BinSums {
 };
 
 struct SampleShared {
-  uint32_t cnt[kSampleBins], lo[kSampleBins], hi[kSampleBins];  // this CTA's histogram
-  uint64_t list[kSampleList];                                   // gathered tokens (key, ~index)
+  uint64_t weight[kSampleBins];  // this CTA's histogram; then the lists of the bin that is cut
+  uint32_t cnt[kSampleBins];
   Pair64 xch[2][kSampleMaxCluster];                             // a value of every CTA, two exchanges in turn
   uint64_t warp_a[kSampleWarps], warp_b[kSampleWarps];
   Bracket found;
-  Pair64 cut;  // weight of the prefix, (threshold key, ties taken)
-  int list_n;
+  Pair64 cut;  // weight of the prefix, its last token
+  int list_n[2];  // tokens of this CTA in that bin, for the cut by top-k and by top-p
   uint32_t key_min, key_max;
 };
 constexpr int kSampleShared = (sizeof(SampleShared) + 15) / 16 * 16;
@@ -182,10 +186,15 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   const int first = (rank * kSampleWarps + warp) * a.per_warp;  // index of this warp's first logit
   uint4* const mine = part + warp * vecs;
   const T* const x = static_cast<const T*>(a.logits) + row * a.ld + first;
+  // the row's parameters come with the logits
+  const float temp = a.temperature ? a.temperature[row] : 1.f, p = a.top_p ? a.top_p[row] : 1.f;
+  const float mp = a.min_p ? a.min_p[row] : 0.f, u = a.u[row];
+  const int k = a.top_k ? a.top_k[row] : 0;
   uint64_t best = 0;  // (key, ~index): the lowest index among equals
   {
     constexpr int kAhead = 4;  // vectors in flight per lane
     float top = -INFINITY;
+    int top_i = 0;  // the first vector that has it
     for (int v0 = lane; v0 < vecs; v0 += 32 * kAhead) {
       uint4 v[kAhead];
 #pragma unroll
@@ -209,13 +218,22 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
         mine[i] = v[k];
         float f[kVec];
         Vec<T>::get(v[k], f);
+        float most = f[0];
 #pragma unroll
-        for (int j = 0; j < kVec; ++j)
-          if (f[j] > top) {  // this lane's indices ascend, so the first of equals stays
-            top = f[j];
-            best = ((uint64_t)logit_key(f[j]) << 32) | (uint32_t)~(first + i * kVec + j);
-          }
+        for (int j = 1; j < kVec; ++j) most = fmaxf(most, f[j]);
+        if (most > top) {  // this lane's indices ascend, so the first of equals stays
+          top = most;
+          top_i = i;
+        }
       }
+    }
+    if (top > -INFINITY) {
+      float f[kVec];
+      Vec<T>::get(mine[top_i], f);
+      int at = 0;
+#pragma unroll
+      for (int j = kVec - 1; j >= 0; --j) at = f[j] == top ? j : at;
+      best = ((uint64_t)logit_key(top) << 32) | (uint32_t)~(first + top_i * kVec + at);
     }
   }
 #pragma unroll
@@ -225,7 +243,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   }
   if (lane == 0) sh.warp_a[warp] = best;
   if (tid == 0) {
-    sh.list_n = 0;
+    sh.list_n[0] = sh.list_n[1] = 0;
     sh.key_min = 0xffffffffu;
     sh.key_max = 0;
   }
@@ -252,7 +270,6 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     best = 0;
     for (int c = 0; c < C; ++c) best = r[c].a > best ? r[c].a : best;
   }
-  const float temp = a.temperature ? a.temperature[row] : 1.f;
   const float m = best ? key_logit((uint32_t)(best >> 32)) : -INFINITY;
   if (m == -INFINITY || !(temp >= 1e-5f)) {
     if (rank == 0 && tid == 0) {
@@ -276,8 +293,6 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     }
   };
 
-  const int k = a.top_k ? a.top_k[row] : 0;
-  const float p = a.top_p ? a.top_p[row] : 1.f;
   const bool cut_k = k > 0 && k < n, cut_p = p < 1.f;
   float thr = top_inf ? INFINITY : -INFINITY;  // kept: logits above it ...
   uint64_t take = 0;                           // ... and this many of those equal to it
@@ -285,29 +300,55 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   if ((cut_k || cut_p) && !top_inf) {
     const int bins = min(kSampleBins, kSampleThreads * C), share = bins / C;  // a CTA's share: a bin a thread
     const float per_d = bins / kSampleDeep;
-    auto clear = [&]() {
-      for (int i = tid; i < bins; i += kSampleThreads) sh.cnt[i] = sh.lo[i] = sh.hi[i] = 0;
-      __syncthreads();
-    };
-    // four tokens into the bins (-1: none), their weights with the carry from the low words' old values; the
-    // additions of all four are under way together
-    auto count_in = [&](const int* bin, const float* d) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (bin[j] >= 0) atomicAdd(&sh.cnt[bin[j]], 1u);
-      if (!cut_p) return;  // numbers are enough
-      uint64_t w[4];
-      uint32_t old[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = depth_weight(d[j]);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (bin[j] >= 0) old[j] = atomicAdd(&sh.lo[bin[j]], (uint32_t)w[j]);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t hi = (uint32_t)(w[j] >> 32) + (old[j] + (uint32_t)w[j] < old[j] ? 1u : 0u);
-        if (bin[j] >= 0 && hi) atomicAdd(&sh.hi[bin[j]], hi);
+    // The tokens (number and weight) by bins: bin_of(logit, d), -1 for none, over the vectors that `in_part` is
+    // true of. The weights' halves, with the bits above them, are added up apart: additions that return nothing,
+    // and up to 4095 tokens of a bin leave 32 bits enough. Where a bin has more, 64-bit sums with a carry.
+    auto histogram = [&](auto in_part, auto bin_of) {
+      uint32_t* const words = reinterpret_cast<uint32_t*>(sh.weight);
+      for (int i = tid; i < bins; i += kSampleThreads) {
+        sh.cnt[i] = 0;
+        sh.weight[i] = 0;
       }
+      __syncthreads();
+      each([&](const float* v, int) {
+        if (!in_part(v)) return;
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) {
+          const float d = logit_depth(v[j], m, inv_t);
+          const int bin = bin_of(v[j], d);
+          if (bin >= 0) atomicAdd(&sh.cnt[bin], 1u);
+          if (cut_p && bin >= 0) {  // (without top-p numbers are enough)
+            uint32_t hi, lo;
+            weight_halves(expf(d), hi, lo);
+            atomicAdd(&words[2 * bin], lo);
+            atomicAdd(&words[2 * bin + 1], hi);
+          }
+        }
+      });
+      __syncthreads();
+      if (!cut_p) return;
+      bool many = false;
+      for (int i = tid; i < bins; i += kSampleThreads) {
+        const uint32_t c = sh.cnt[i], off = c * kHalfBits;
+        many |= c > 4095;
+        sh.weight[i] = ((uint64_t)(words[2 * i + 1] - off) << 20) + (words[2 * i] - off);
+      }
+      if (!__syncthreads_or(many)) return;
+      for (int i = tid; i < bins; i += kSampleThreads) sh.weight[i] = 0;
+      __syncthreads();
+      each([&](const float* v, int) {
+        if (!in_part(v)) return;
+#pragma unroll 1
+        for (int j = 0; j < kVec; ++j) {
+          const float d = logit_depth(v[j], m, inv_t);
+          const int bin = bin_of(v[j], d);
+          if (bin < 0) continue;
+          const uint64_t w = depth_weight(d);
+          const uint32_t old = atomicAdd(&words[2 * bin], (uint32_t)w);
+          const uint32_t hi = (uint32_t)(w >> 32) + (old + (uint32_t)w < old ? 1u : 0u);
+          if (hi) atomicAdd(&words[2 * bin + 1], hi);
+        }
+      });
     };
     // the cluster's histograms added up, each CTA a share of the bins, and the sums before this thread's
     auto sum_bins = [&]() {
@@ -322,8 +363,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
         if (cut_p) {
 #pragma unroll
           for (int q = 0; q < kSampleMaxCluster; ++q)
-            if (q < C)
-              w += *cluster.map_shared_rank(&sh.lo[b], q) + ((uint64_t)*cluster.map_shared_rank(&sh.hi[b], q) << 32);
+            if (q < C) w += *cluster.map_shared_rank(&sh.weight[b], q);
         }
       }
       s.n = (uint32_t)c;
@@ -420,23 +460,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
         if (k_lo == k_hi) break;  // equal logits: arithmetic
         int shift = 0;
         while (((k_hi - k_lo) >> shift) >= (uint32_t)bins) ++shift;
-        clear();
-        each([&](const float* v, int) {
-          if (!may_be(v)) return;
-#pragma unroll
-          for (int h = 0; h < kVec; h += 4) {
-            int bin[4];
-            float d[4];
-            bool any = false;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              d[j] = logit_depth(v[h + j], m, inv_t);
-              bin[j] = inside(v[h + j]) ? (int)((k_hi - logit_key(v[h + j])) >> shift) : -1;
-              any |= bin[j] >= 0;
-            }
-            if (any) count_in(bin, d);
-          }
-        });
+        histogram(may_be, [&](float l, float) { return inside(l) ? (int)((k_hi - logit_key(l)) >> shift) : -1; });
         const BinSums s = sum_bins();
         br = find(s, want, by_weight, br.count, br.weight);
         k_hi -= (uint32_t)br.bin << shift;
@@ -449,9 +473,11 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
         take = by_weight ? (want - br.weight + w1 - 1) / w1 : want - br.count;
         weight = br.weight + take * w1;
       } else {
-        // the bracket's tokens into the first CTA, in any order
-        uint64_t* const list = cluster.map_shared_rank(sh.list, 0);
-        int* const list_n = cluster.map_shared_rank(&sh.list_n, 0);
+        uint64_t* const list = sh.weight;  // in place of the histogram, which all have read
+        uint64_t* const sorted = list + kSampleList;
+        uint64_t* const sums = sorted + kSampleList;
+        int* const list_n = &sh.list_n[by_weight];
+        // the bracket's tokens into this CTA's list, in any order; then every CTA takes all of them, one a thread
         each([&](const float* v, int i) {
           if (!may_be(v)) return;
           unsigned in = 0;
@@ -465,65 +491,60 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
           }
         });
         cluster.sync();
-        if (rank == 0) {
-          // sorted by (key, ~index) downwards, a token a thread: bitonic, by shuffles within a warp
-          uint64_t me = tid < br.n ? sh.list[tid] : 0;
-          for (int size = 2; size < 2 * br.n; size *= 2) {  // (a sorted block holds what the others pad with 0)
-            for (int step = size / 2; step > 0; step /= 2) {
-              uint64_t o;
-              if (step >= 32) {
-                __syncthreads();
-                sh.list[tid] = me;
-                __syncthreads();
-                o = sh.list[tid ^ step];
-              } else {
-                o = __shfl_xor_sync(0xffffffffu, me, step);
-              }
-              const bool keep_max = ((tid & step) == 0) == ((tid & size) == 0);
-              me = (me > o) == keep_max ? me : o;
+        uint64_t me = 0;
+        {
+          const int share = lane < C ? *cluster.map_shared_rank(list_n, lane) : 0;
+          int q = -1, at = 0;
+          for (int c = 0, before = 0; c < C; ++c) {
+            const int in_c = __shfl_sync(0xffffffffu, share, c);
+            if (tid >= before && tid < before + in_c) {
+              q = c;
+              at = tid - before;
             }
+            before += in_c;
           }
-          const uint64_t w = me ? depth_weight(logit_depth(key_logit((uint32_t)(me >> 32)), m, inv_t)) : 0;
-          uint64_t upto = warp_scan64(w, lane);
-          if (lane == 31) sh.warp_a[warp] = upto;
-          __syncthreads();
-          const uint64_t others = lane < kSampleWarps ? sh.warp_a[lane] : 0;
-          upto += br.weight + warp_sum64(lane < warp ? others : 0);
-          if (tid < br.n && (by_weight ? upto - w < want && want <= upto : br.count + tid + 1 == want)) {
-            sh.cut = Pair64{upto, me};
-            sh.list_n = tid;  // the place of the last one kept
-          }
-          __syncthreads();
-          const Pair64 last = sh.cut;
-          const int place = sh.list_n;
-          const int ties = __syncthreads_count(tid <= place && (me >> 32) == (last.b >> 32));
-          if (tid < C)
-            *cluster.map_shared_rank(&sh.cut, tid) = Pair64{last.a, (last.b & 0xffffffff00000000ull) | (unsigned)ties};
-          if (tid == 0) sh.list_n = 0;
+          if (q >= 0) me = *cluster.map_shared_rank(&list[at], q);
         }
-        cluster.sync();
+        // sorted downwards within the warp; a token's place and the weight up to it are then sums over the warps
+        // of what is above it in each, found by halving
+#pragma unroll
+        for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+          for (int step = size / 2; step > 0; step /= 2) {
+            const uint64_t o = __shfl_xor_sync(0xffffffffu, me, step);
+            const bool keep_max = ((lane & step) == 0) == ((lane & size) == 0);
+            me = (me > o) == keep_max ? me : o;
+          }
+        const uint64_t w = me ? depth_weight(logit_depth(key_logit((uint32_t)(me >> 32)), m, inv_t)) : 0;
+        sorted[tid] = me;
+        sums[tid] = warp_scan64(w, lane);
+        __syncthreads();
+        int place = 0;
+        uint64_t upto = br.weight;
+#pragma unroll 4
+        for (int at = 0; at < br.n; at += 32) {
+          int above = 0;  // of this warp's tokens, those not below this one
+#pragma unroll
+          for (int half = 16; half > 0; half /= 2) above += sorted[at + above + half - 1] >= me ? half : 0;
+          above += sorted[at + above] >= me;
+          place += above;
+          upto += above ? sums[at + above - 1] : 0;
+        }
+        if (me && (by_weight ? upto - w < want && want <= upto : br.count + place == want)) sh.cut = Pair64{upto, me};
+        __syncthreads();
+        const uint64_t last = sh.cut.b;
+        const int ties = __syncthreads_count(me >= last && (me >> 32) == (last >> 32));
         weight = sh.cut.a;
-        thr = key_logit((uint32_t)(sh.cut.b >> 32));
-        take = (uint32_t)sh.cut.b;
+        thr = key_logit((uint32_t)(last >> 32));
+        take = ties;
       }
       return weight;
     };
 
     // ---- 2, 3: the histogram over steps of d, and the cuts
-    clear();
-    each([&](const float* v, int) {
-#pragma unroll
-      for (int h = 0; h < kVec; h += 4) {
-        int bin[4];
-        float d[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          d[j] = logit_depth(v[h + j], m, inv_t);
-          bin[j] = v[h + j] > -INFINITY && d[j] >= -kSampleDeep ? depth_bin(d[j], per_d, bins) : -1;
-        }
-        count_in(bin, d);
-      }
-    });
+    // (-inf and NaN are below every step)
+    histogram([](const float*) { return true; },
+              [&](float, float d) { return d >= -kSampleDeep ? depth_bin(d, per_d, bins) : -1; });
     const BinSums s = sum_bins();
     uint64_t weight = s.total_weight;
     // tokens too deep to be counted weigh nothing: a prefix that would reach them needs no cut
@@ -535,35 +556,30 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   }
 
   // ---- 4: the kept weights, ties counted apart (they all weigh the same)
-  const float mp = a.min_p ? a.min_p[row] : 0.f;
   const float floor_d = mp > 0.f ? logf(fminf(mp, 1.f)) : -INFINITY;
   const bool tied = top_inf || (thr > -INFINITY && logit_depth(thr, m, inv_t) >= floor_d);
   const uint64_t w1 = top_inf ? (uint64_t)1 << 40 : tied ? depth_weight(logit_depth(thr, m, inv_t)) : 0;
   auto taken = [&](uint64_t before, uint64_t here) {  // the weight of `here` ties that come after `before` others
     return before >= take ? (uint64_t)0 : min(here, take - before) * w1;
   };
-  // expf(d) of a logit above the threshold, 0 of others
+  // d of a kept logit above the threshold; of others one whose weight is 0 (of NaN too)
   auto kept = [&](float l) {
     const float d = logit_depth(l, m, inv_t);
-    return l > thr && d >= floor_d ? expf(d) : 0.f;
+    return l > thr && d >= floor_d ? d : -100.f;
   };
   // adds a vector's kept weights in halves, and its ties
   auto add_kept = [&](const float* v, uint32_t& hi, uint32_t& lo, uint32_t& eq) {
-    bool any = false;
+    float most = v[0];
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) any |= v[j] >= thr;
-    if (any) {
-      uint32_t h[kVec], l[kVec];
+    for (int j = 1; j < kVec; ++j) most = fmaxf(most, v[j]);
+    if (!(most >= thr)) return;
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) weight_halves(kept(v[j]), h[j], l[j]);
-      if (tied)
-#pragma unroll
-        for (int j = 0; j < kVec; ++j) eq += v[j] == thr;
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) {
-        hi += h[j] - kHalfBits;
-        lo += l[j] - kHalfBits;
-      }
+    for (int j = 0; j < kVec; ++j) {
+      uint32_t h, l;
+      weight_halves(expf(kept(v[j])), h, l);
+      hi += h - kHalfBits;
+      lo += l - kHalfBits;
+      eq += v[j] == thr;
     }
   };
   {
@@ -584,7 +600,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     else
       each([&](const float* v, int) { add_kept(v, hi, lo, eq); });
     const uint64_t w = warp_sum64(((uint64_t)hi << 20) + lo);
-    eq = __reduce_add_sync(0xffffffffu, eq);
+    eq = tied ? __reduce_add_sync(0xffffffffu, eq) : 0;
     if (lane == 0) {
       sh.warp_a[warp] = w;
       sh.warp_b[warp] = eq;
@@ -616,10 +632,10 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     total += w;
     seen += r[c].b;
   }
-  const double at_d = floor((double)a.u[row] * (double)(int64_t)total);
+  const double at_d = floor((double)u * (double)(int64_t)total);
   uint64_t at = at_d >= 1. ? (uint64_t)at_d : 0;  // NaN and negative numbers count as 0
   if (at >= total) at = total - 1;
-  if (warp == 0 && run <= at && at < run + here) {
+  if (run <= at && at < run + here) {  // this CTA has it
     // the warp's part in which the running sum passes `at`: lane q looks at part q
     uint64_t eq = lane < kSampleWarps ? sh.warp_b[lane] : 0, w = lane < kSampleWarps ? sh.warp_a[lane] : 0;
     uint64_t eq_before = seen0 + warp_scan64(eq, lane) - eq;
@@ -630,35 +646,47 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     seen = __shfl_sync(0xffffffffu, eq_before, q);
     const uint4* const from = part + q * vecs;
     const int base = (rank * kSampleWarps + q) * a.per_warp;
-    // 32 vectors at a time up to the one in which the sum passes, then its lane, then that lane's logits
-    for (int i0 = 0; i0 < vecs; i0 += 32) {
-      const int i = i0 + lane;
-      uint32_t hi = 0, lo = 0, el = 0;
-      if (i < vecs) {
-        float v[kVec];
-        Vec<T>::get(from[i], v);
-        add_kept(v, hi, lo, el);
+    // its vectors, 32 to a warp (vecs <= 512), then the warp in whose vectors the sum passes, its lane, and that
+    // lane's logits
+    const int i = warp * 32 + lane;
+    uint32_t hi = 0, lo = 0, el = 0;
+    if (i < vecs) {
+      float v[kVec];
+      Vec<T>::get(from[i], v);
+      add_kept(v, hi, lo, el);
+    }
+    if (!tied) el = 0;
+    const uint64_t wl = ((uint64_t)hi << 20) + lo;
+    const uint32_t el_all = __reduce_add_sync(0xffffffffu, el);
+    {
+      const uint64_t sum = warp_sum64(wl);
+      __syncthreads();  // all have read the sums of the parts
+      if (lane == 0) {
+        sh.warp_a[warp] = sum;
+        sh.warp_b[warp] = el_all;
       }
-      const uint64_t wl = ((uint64_t)hi << 20) + lo;
-      const uint32_t el_all = __reduce_add_sync(0xffffffffu, el);
-      const uint64_t w_all = warp_sum64(wl) + (el_all ? taken(seen, el_all) : 0);
-      if (run + w_all <= at) {
-        run += w_all;
-        seen += el_all;
-        continue;
-      }
+      __syncthreads();
+      eq = lane < kSampleWarps ? sh.warp_b[lane] : 0;
+      w = lane < kSampleWarps ? sh.warp_a[lane] : 0;
+      eq_before = seen + warp_scan64(eq, lane) - eq;
+      if (tied) w += taken(eq_before, eq);
+      incl = run + warp_scan64(w, lane);
+    }
+    if (warp == __ffs(__ballot_sync(0xffffffffu, incl > at)) - 1) {
+      run = __shfl_sync(0xffffffffu, incl - w, warp);
+      seen = __shfl_sync(0xffffffffu, eq_before, warp);
       uint64_t e_before = seen;
       if (el_all) e_before += warp_scan64(el, lane) - el;
       const uint64_t wt = wl + (el_all ? taken(e_before, el) : 0), upto = run + warp_scan64(wt, lane);
       const int at_lane = __ffs(__ballot_sync(0xffffffffu, upto > at)) - 1;
       run = __shfl_sync(0xffffffffu, upto - wt, at_lane);
       seen = __shfl_sync(0xffffffffu, e_before, at_lane);
-      const int iv = i0 + at_lane;  // the vector; lane j takes its logit j
+      const int iv = warp * 32 + at_lane;  // the vector; lane j takes its logit j
       const float l = lane < kVec ? Vec<T>::one(reinterpret_cast<const T*>(from + iv)[lane]) : -INFINITY;
       const bool tie = tied && l == thr;
       const unsigned ties = __ballot_sync(0xffffffffu, tie);
       uint32_t wh, wo;
-      weight_halves(kept(l), wh, wo);
+      weight_halves(expf(kept(l)), wh, wo);
       const uint64_t wj = tie ? taken(seen + __popc(ties & ((1u << lane) - 1u)), 1)
                               : ((uint64_t)(wh - kHalfBits) << 20) + (wo - kHalfBits);
       const unsigned past = __ballot_sync(0xffffffffu, run + warp_scan64(wj, lane) > at);
@@ -666,7 +694,6 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
         a.tok[row] = base + iv * kVec + lane;
         if (a.logprob) a.logprob[row] = (top_inf ? 0.f : logit_depth(l, m, inv_t)) - logf((float)(int64_t)total * (1.f / kSampleOne));
       }
-      break;
     }
   }
 }
