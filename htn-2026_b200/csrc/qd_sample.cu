@@ -30,7 +30,8 @@ namespace cg = cooperative_groups;
 
 constexpr int kSampleThreads = 512, kSampleWarps = kSampleThreads / 32;
 constexpr int kSampleBins = 2048;
-constexpr int kSampleList = kSampleThreads;     // tokens that one CTA sorts, one a thread
+constexpr int kSampleList = 1024;               // tokens that are sorted, kSampleOwn a thread
+constexpr int kSampleOwn = kSampleList / kSampleThreads;
 constexpr float kSampleOne = 1099511627776.0f;  // 2^40
 constexpr float kSampleDeep = 28.5f;            // e^-28.42 = 2^-41: beyond, weights round to 0
 constexpr int64_t kSampleMaxVocab = 1 << 18;    // 2^18 weights of 2^40 stay below 2^63
@@ -119,10 +120,10 @@ __device__ __forceinline__ uint64_t depth_weight(float d) {
   weight_halves(expf(d), hi, lo);
   return ((uint64_t)(hi - kHalfBits) << 20) + (lo - kHalfBits);
 }
-// the step of d in which a d of -kSampleDeep to 0 lies (by an addition of 2^23 too: a conversion to int would
-// take the exponentials' pipe)
-__device__ __forceinline__ int depth_bin(float d, float per_d, int bins) {
-  return min((int)(__float_as_uint(__fmaf_rd(-d, per_d, 8388608.0f)) - kHalfBits), bins - 1);
+// d in 256ths of the steps into which 0 to -kSampleDeep is cut, rounded down (a larger number for what is deeper,
+// -inf or NaN). An addition of 2^23 here too: a conversion to int would take the exponentials' pipe.
+__device__ __forceinline__ uint32_t depth_place(float d, float per_d256) {
+  return __float_as_uint(__fmaf_rd(-d, per_d256, 8388608.0f)) - kHalfBits;
 }
 
 // 64-bit sum over the warp by 16-bit pieces: four reduction instructions in place of ten dependent shuffles
@@ -142,29 +143,42 @@ __device__ __forceinline__ uint64_t warp_scan64(uint64_t v, int lane) {  // incl
   return v;
 }
 
-struct Pair64 {
-  uint64_t a, b;
+struct Trio64 {
+  uint64_t a, b, c;
 };
-// Where a prefix ends: in one of the bins, `n` tokens, after `count` tokens of `weight` in the bins before it.
+// Where a prefix ends: in the bins `bin` to `last`, which hold `n` tokens, after `count` tokens of `weight`.
 struct Bracket {
   uint64_t count, weight;
-  int bin, n;
+  int bin, last, n;
 };
 // The bin of which this thread has the cluster's sums (none: 0), and the sums before it.
 struct BinSums {
   uint32_t n;
   uint64_t w, count, weight, total_count, total_weight;
+  bool complete;  // the words' numbers add up to the tokens counted (they are never more)
 };
 
 struct SampleShared {
-  uint64_t weight[kSampleBins];  // this CTA's histogram; then the lists of the bin that is cut
-  uint32_t cnt[kSampleBins];
-  Pair64 xch[2][kSampleMaxCluster];                             // a value of every CTA, two exchanges in turn
+  union {
+    struct {
+      uint64_t weight[kSampleBins];  // of the bins by key
+      uint32_t cnt[kSampleBins];     // this CTA's histogram
+    };
+    struct {  // once all have read that, the bracket's tokens: this CTA's, all, and the weights up to each
+      uint64_t list[kSampleList], sorted[kSampleList], sums[kSampleList];
+    };
+  };
+  Trio64 xch[2][kSampleMaxCluster];  // values of every CTA, two exchanges in turn
   uint64_t warp_a[kSampleWarps], warp_b[kSampleWarps];
   Bracket found;
-  Pair64 cut;  // weight of the prefix, its last token
-  int list_n[2];  // tokens of this CTA in that bin, for the cut by top-k and by top-p
-  uint32_t key_min, key_max;
+  int found_last;
+  uint64_t found_after;       // tokens up to the bracket's end
+  uint64_t cut_weight, cut;   // weight of the prefix, its last token
+  unsigned long long part_w[kSampleWarps];  // per warp: weight of all, then of the tokens above the bracket or kept
+  uint32_t part_eq[kSampleWarps];           // and its ties
+  unsigned long long above[2];  // weight of this CTA's tokens above the bracket, by top-k and by top-p
+  int list_n[2];              // this CTA's tokens in the bracket, by top-k and by top-p
+  uint32_t key_min, key_max, counted;
 };
 constexpr int kSampleShared = (sizeof(SampleShared) + 15) / 16 * 16;
 
@@ -244,16 +258,16 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   if (lane == 0) sh.warp_a[warp] = best;
   if (tid == 0) {
     sh.list_n[0] = sh.list_n[1] = 0;
-    sh.key_min = 0xffffffffu;
-    sh.key_max = 0;
+    sh.above[0] = sh.above[1] = 0;
+    sh.counted = 0;
   }
   __syncthreads();
   int turn = 0;
-  // (va, vb), known to warp 0, to every CTA of the cluster; all threads pass the barrier
-  auto exchange = [&](uint64_t va, uint64_t vb) {
-    if (tid < C) *cluster.map_shared_rank(&sh.xch[turn][rank], tid) = Pair64{va, vb};
+  // (va, vb, vc), known to warp 0, to every CTA of the cluster; all threads pass the barrier
+  auto exchange = [&](uint64_t va, uint64_t vb, uint64_t vc) {
+    if (tid < C) *cluster.map_shared_rank(&sh.xch[turn][rank], tid) = Trio64{va, vb, vc};
     cluster.sync();
-    const Pair64* r = sh.xch[turn];
+    const Trio64* r = sh.xch[turn];
     turn ^= 1;
     return r;
   };
@@ -266,7 +280,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     }
   }
   {
-    const Pair64* r = exchange(best, 0);
+    const Trio64* r = exchange(best, 0, 0);
     best = 0;
     for (int c = 0; c < C; ++c) best = r[c].a > best ? r[c].a : best;
   }
@@ -296,258 +310,358 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   const bool cut_k = k > 0 && k < n, cut_p = p < 1.f;
   float thr = top_inf ? INFINITY : -INFINITY;  // kept: logits above it ...
   uint64_t take = 0;                           // ... and this many of those equal to it
+  bool summed = false;                         // the kept weights are already in part_w, part_eq
 
   if ((cut_k || cut_p) && !top_inf) {
     const int bins = min(kSampleBins, kSampleThreads * C), share = bins / C;  // a CTA's share: a bin a thread
-    const float per_d = bins / kSampleDeep;
-    // The tokens (number and weight) by bins: bin_of(logit, d), -1 for none, over the vectors that `in_part` is
-    // true of. The weights' halves, with the bits above them, are added up apart: additions that return nothing,
-    // and up to 4095 tokens of a bin leave 32 bits enough. Where a bin has more, 64-bit sums with a carry.
-    auto histogram = [&](auto in_part, auto bin_of) {
-      uint32_t* const words = reinterpret_cast<uint32_t*>(sh.weight);
-      for (int i = tid; i < bins; i += kSampleThreads) {
-        sh.cnt[i] = 0;
-        sh.weight[i] = 0;
-      }
-      __syncthreads();
-      each([&](const float* v, int) {
-        if (!in_part(v)) return;
-#pragma unroll
-        for (int j = 0; j < kVec; ++j) {
-          const float d = logit_depth(v[j], m, inv_t);
-          const int bin = bin_of(v[j], d);
-          if (bin >= 0) atomicAdd(&sh.cnt[bin], 1u);
-          if (cut_p && bin >= 0) {  // (without top-p numbers are enough)
-            uint32_t hi, lo;
-            weight_halves(expf(d), hi, lo);
-            atomicAdd(&words[2 * bin], lo);
-            atomicAdd(&words[2 * bin + 1], hi);
-          }
-        }
-      });
-      __syncthreads();
-      if (!cut_p) return;
-      bool many = false;
-      for (int i = tid; i < bins; i += kSampleThreads) {
-        const uint32_t c = sh.cnt[i], off = c * kHalfBits;
-        many |= c > 4095;
-        sh.weight[i] = ((uint64_t)(words[2 * i + 1] - off) << 20) + (words[2 * i] - off);
-      }
-      if (!__syncthreads_or(many)) return;
-      for (int i = tid; i < bins; i += kSampleThreads) sh.weight[i] = 0;
-      __syncthreads();
-      each([&](const float* v, int) {
-        if (!in_part(v)) return;
-#pragma unroll 1
-        for (int j = 0; j < kVec; ++j) {
-          const float d = logit_depth(v[j], m, inv_t);
-          const int bin = bin_of(v[j], d);
-          if (bin < 0) continue;
-          const uint64_t w = depth_weight(d);
-          const uint32_t old = atomicAdd(&words[2 * bin], (uint32_t)w);
-          const uint32_t hi = (uint32_t)(w >> 32) + (old + (uint32_t)w < old ? 1u : 0u);
-          if (hi) atomicAdd(&words[2 * bin + 1], hi);
-        }
-      });
-    };
-    // the cluster's histograms added up, each CTA a share of the bins, and the sums before this thread's
-    auto sum_bins = [&]() {
-      cluster.sync();
+    const float width = kSampleDeep / bins, per_d256 = 256.f / width;
+    bool packed = cut_p;  // a bin's word: tokens << 20 | their 256ths; or, where that may not fit, tokens
+    uint64_t weight = 0;  // of all tokens, then of the prefix
+    // the cluster's histograms added up, each CTA a share of the bins, and the sums before this thread's; `vc`
+    // (known to warp 0) is added up over the CTAs as the total weight
+    auto sum_bins = [&](auto bin_sums, uint64_t vc) {
       BinSums s;
-      uint64_t c = 0, w = 0;
-      if (tid < share) {
-        const int b = rank * share + tid;
-#pragma unroll
-        for (int q = 0; q < kSampleMaxCluster; ++q)
-          if (q < C) c += *cluster.map_shared_rank(&sh.cnt[b], q);
-        if (cut_p) {
-#pragma unroll
-          for (int q = 0; q < kSampleMaxCluster; ++q)
-            if (q < C) w += *cluster.map_shared_rank(&sh.weight[b], q);
-        }
-      }
-      s.n = (uint32_t)c;
-      s.w = w;
-      const uint64_t ci = warp_scan64(c, lane), wi = warp_scan64(w, lane);
+      s.n = 0;
+      s.w = 0;
+      if (tid < share) bin_sums(rank * share + tid, s.n, s.w);
+      const uint64_t ci = warp_scan64(s.n, lane), wi = warp_scan64(s.w, lane);
       if (lane == 31) {
         sh.warp_a[warp] = ci;
         sh.warp_b[warp] = wi;
       }
       __syncthreads();
-      s.count = ci - c;
-      s.weight = wi - w;
+      s.count = ci - s.n;
+      s.weight = wi - s.w;
       uint64_t ct = lane < kSampleWarps ? sh.warp_a[lane] : 0, wt = lane < kSampleWarps ? sh.warp_b[lane] : 0;
       s.count += warp_sum64(lane < warp ? ct : 0);
       s.weight += warp_sum64(lane < warp ? wt : 0);
       ct = warp_sum64(ct);
       wt = warp_sum64(wt);
-      const Pair64* r = exchange(ct, wt);
+      const Trio64* r = exchange(ct | (uint64_t)sh.counted << 32, wt, vc);
       s.total_count = s.total_weight = 0;
+      uint64_t counted = 0;
       for (int q = 0; q < C; ++q) {
         if (q < rank) {
-          s.count += r[q].a;
+          s.count += (uint32_t)r[q].a;
           s.weight += r[q].b;
         }
-        s.total_count += r[q].a;
-        s.total_weight += r[q].b;
+        s.total_count += (uint32_t)r[q].a;
+        s.total_weight += r[q].c;
+        counted += r[q].a >> 32;
       }
+      s.complete = s.total_count == counted;
       return s;
     };
-    // the bin in which the prefix of `want` tokens (of weight `want`) ends, given what lies above all bins
-    auto find = [&](const BinSums& s, uint64_t want, bool by_weight, uint64_t count0, uint64_t weight0) {
+    // the bins in which the prefix of `want` tokens (of weight `want`) ends, given what lies above all bins. The
+    // weights may be lower bounds: what they are of is then at most w (1 + eps) + 3 per token.
+    auto find = [&](const BinSums& s, uint64_t want, bool by_weight, uint64_t count0, uint64_t weight0, float eps) {
       const uint64_t c = count0 + s.count, w = weight0 + s.weight;
-      const uint64_t before = by_weight ? w : c, here = by_weight ? s.w : s.n;
-      if (before < want && want <= before + here)
-        for (int q = 0; q < C; ++q)
-          *cluster.map_shared_rank(&sh.found, q) = Bracket{c, w, rank * share + tid, (int)s.n};
-      cluster.sync();
-      return sh.found;
-    };
-    // cuts the prefix within a step of d: thr, take; returns the prefix's weight
-    auto cut = [&](const BinSums& s0, uint64_t want, bool by_weight) {
-      Bracket br = find(s0, want, by_weight, 0, 0);
-      const int step = br.bin;
-      uint32_t k_lo = 0, k_hi = 0;  // by key, once the bracket is narrower than the step
-      // logits of the step lie in between these, by more than the roundings of d (2^-20 of it and of l, m)
-      // (a temperature that has no such bounds in fp32 gets none)
-      const bool bounded = temp < 1e30f;
-      const float slop = 1e-5f * (fabsf(m) + kSampleDeep * temp), width = kSampleDeep / bins;
-      const float l_top = bounded ? m - step * width * temp + slop : INFINITY;
-      const float l_low = bounded && step < bins - 1 ? m - (step + 1) * width * temp - slop : -INFINITY;
-      auto may_be = [&](const float* v) {
-        bool any = false;
-#pragma unroll
-        for (int j = 0; j < kVec; ++j) any |= v[j] >= l_low && v[j] <= l_top;
-        return any;
+      auto most = [&](uint64_t x, uint64_t n) {
+        return eps > 0.f ? x + (uint64_t)((double)(int64_t)x * eps) + 3 * n : x;
       };
-      auto inside = [&](float l) {
-        const float d = logit_depth(l, m, inv_t);
-        const uint32_t key = logit_key(l);
-        return l > -INFINITY && (k_hi ? key >= k_lo && key <= k_hi : d >= -kSampleDeep && depth_bin(d, per_d, bins) == step);
-      };
-      // a round leaves a 512th or less of the keys' range: 32 bits take four
-      for (int round = 0; round < 4 && br.n > kSampleList; ++round) {
-        if (!k_hi) {  // the keys in this step
-          if (tid == 0) {
-            sh.key_min = 0xffffffffu;
-            sh.key_max = 0;
-          }
-          __syncthreads();
-          uint32_t lo = 0xffffffffu, hi = 0;
-          each([&](const float* v, int) {
-            if (!may_be(v)) return;
-#pragma unroll
-            for (int j = 0; j < kVec; ++j) {
-              const bool in = inside(v[j]);
-              lo = min(lo, in ? logit_key(v[j]) : 0xffffffffu);
-              hi = max(hi, in ? logit_key(v[j]) : 0u);
-            }
-          });
-          lo = __reduce_min_sync(0xffffffffu, lo);
-          hi = __reduce_max_sync(0xffffffffu, hi);
-          if (lane == 0) {
-            atomicMin(&sh.key_min, lo);
-            atomicMax(&sh.key_max, hi);
-          }
-          __syncthreads();
-          const Pair64* r = exchange(sh.key_min, sh.key_max);
-          k_lo = 0xffffffffu;
-          for (int q = 0; q < C; ++q) {
-            k_lo = min(k_lo, (uint32_t)r[q].a);
-            k_hi = max(k_hi, (uint32_t)r[q].b);
-          }
+      const uint64_t low = by_weight ? w : c, low_end = by_weight ? w + s.w : c + s.n;
+      const uint64_t top = by_weight ? most(w, c) : c, top_end = by_weight ? most(w + s.w, c + s.n) : c + s.n;
+      const int bin = rank * share + tid;
+      if (top < want && want <= top_end)
+        for (int q = 0; q < C; ++q) {
+          Bracket* const to = cluster.map_shared_rank(&sh.found, q);
+          to->count = c;
+          to->weight = w;
+          to->bin = bin;
         }
-        if (k_lo == k_hi) break;  // equal logits: arithmetic
+      if ((low < want && want <= low_end) || (bin == bins - 1 && tid < share && low_end < want))
+        for (int q = 0; q < C; ++q) {
+          *cluster.map_shared_rank(&sh.found_last, q) = bin;
+          *cluster.map_shared_rank(&sh.found_after, q) = c + s.n;
+        }
+      cluster.sync();
+      Bracket br = sh.found;
+      br.last = sh.found_last;
+      br.n = (int)(sh.found_after - br.count);
+      return br;
+    };
+    // cuts the prefix: thr, take; returns the prefix's weight (if there is top-p)
+    auto cut = [&](const BinSums& s0, uint64_t want, bool by_weight) {
+      // what bin_sums below leaves open, relative to a weight of at least 1 - width
+      const float eps = packed ? 1.1f * (width * width / 8 + width / 256) + 4e-5f : 1.05f * width + 4e-5f;
+      Bracket br = find(s0, want, by_weight, 0, 0, eps);
+      const uint32_t from_q = (uint32_t)br.bin << 8, end_q = (uint32_t)(br.last + 1) << 8;
+      // logits below this are below the bracket, by more than the roundings of d (2^-20 of it and of l, m); a
+      // temperature that has no such bound in fp32 gets none
+      const float l_low = temp < 1e30f && br.last < bins - 1
+                              ? m - (br.last + 1) * width * temp - 1e-5f * (fabsf(m) + kSampleDeep * temp)
+                              : -INFINITY;
+      // the weight of this CTA's tokens above the bracket, and f(logits, index, mask) of the bracket's
+      auto pass = [&](auto f) {
+        uint32_t hi = 0, lo = 0;
+        each([&](const float* v, int i) {
+          float most = v[0];
+#pragma unroll
+          for (int j = 1; j < kVec; ++j) most = fmaxf(most, v[j]);
+          if (!(most >= l_low)) return;
+          unsigned in = 0;
+#pragma unroll
+          for (int j = 0; j < kVec; ++j) {
+            const float d = logit_depth(v[j], m, inv_t);
+            const uint32_t at = depth_place(d, per_d256);
+            in |= (unsigned)(at >= from_q && at < end_q) << j;
+            uint32_t h, l;
+            weight_halves(expf(at < from_q ? d : -100.f), h, l);
+            hi += h - kHalfBits;
+            lo += l - kHalfBits;
+          }
+          if (in) f(v, i, in);
+        });
+        const uint64_t w = warp_sum64(((uint64_t)hi << 20) + lo);
+        if (lane == 0) {
+          atomicAdd(&sh.above[by_weight], (unsigned long long)w);
+          sh.part_w[warp] = w;
+          sh.part_eq[warp] = 0;
+        }
+      };
+      uint32_t k_lo = 0, k_hi = 0;
+      const bool by_key = br.n > kSampleList;  // too many to sort: cut by key first
+      if (by_key) {
+        if (tid == 0) {
+          sh.key_min = 0xffffffffu;
+          sh.key_max = 0;
+        }
+        __syncthreads();
+        uint32_t lo = 0xffffffffu, hi = 0;
+        pass([&](const float* v, int, unsigned in) {
+#pragma unroll
+          for (int j = 0; j < kVec; ++j)
+            if (in >> j & 1u) {
+              lo = min(lo, logit_key(v[j]));
+              hi = max(hi, logit_key(v[j]));
+            }
+        });
+        lo = __reduce_min_sync(0xffffffffu, lo);
+        hi = __reduce_max_sync(0xffffffffu, hi);
+        if (lane == 0) {
+          atomicMin(&sh.key_min, lo);
+          atomicMax(&sh.key_max, hi);
+        }
+        __syncthreads();
+        const Trio64* r = exchange(sh.key_min, sh.key_max, sh.above[by_weight]);
+        k_lo = 0xffffffffu;
+        br.weight = 0;
+        for (int q = 0; q < C; ++q) {
+          k_lo = min(k_lo, (uint32_t)r[q].a);
+          k_hi = max(k_hi, (uint32_t)r[q].b);
+          br.weight += r[q].c;
+        }
+      }
+      // f(logit, its key, index) of the tokens from k_lo to k_hi
+      auto each_key = [&](auto f) {
+        each([&](const float* v, int i) {
+#pragma unroll
+          for (int j = 0; j < kVec; ++j) {
+            const uint32_t key = logit_key(v[j]);
+            if (key >= k_lo && key <= k_hi) f(v[j], key, i + j);
+          }
+        });
+      };
+      // a round leaves a 512th or less of the keys' range: 32 bits take four; equal logits are arithmetic
+      for (int round = 0; round < 4 && br.n > kSampleList && k_lo != k_hi; ++round) {
         int shift = 0;
         while (((k_hi - k_lo) >> shift) >= (uint32_t)bins) ++shift;
-        histogram(may_be, [&](float l, float) { return inside(l) ? (int)((k_hi - logit_key(l)) >> shift) : -1; });
-        const BinSums s = sum_bins();
-        br = find(s, want, by_weight, br.count, br.weight);
+        for (int i = tid; i < bins; i += kSampleThreads) {
+          sh.cnt[i] = 0;
+          sh.weight[i] = 0;
+        }
+        __syncthreads();
+        each_key([&](float l, uint32_t key, int) {
+          const uint32_t bin = (k_hi - key) >> shift;
+          atomicAdd(&sh.cnt[bin], 1u);
+          if (cut_p) {  // 64 bits by two words, with the carry of the lower one
+            uint32_t* const words = reinterpret_cast<uint32_t*>(&sh.weight[bin]);
+            const uint64_t w = depth_weight(logit_depth(l, m, inv_t));
+            const uint32_t old = atomicAdd(words, (uint32_t)w);
+            const uint32_t hi = (uint32_t)(w >> 32) + (old + (uint32_t)w < old ? 1u : 0u);
+            if (hi) atomicAdd(words + 1, hi);
+          }
+        });
+        cluster.sync();
+        const BinSums s = sum_bins(
+            [&](int bin, uint32_t& n, uint64_t& w) {
+              for (int q = 0; q < C; ++q) {
+                n += *cluster.map_shared_rank(&sh.cnt[bin], q);
+                w += *cluster.map_shared_rank(&sh.weight[bin], q);
+              }
+            },
+            0);
+        br = find(s, want, by_weight, br.count, br.weight, 0.f);
         k_hi -= (uint32_t)br.bin << shift;
         k_lo = max(k_lo, k_hi - ((1u << shift) - 1u));
       }
-      uint64_t weight;
       if (br.n > kSampleList) {
         thr = key_logit(k_lo);
         const uint64_t w1 = depth_weight(logit_depth(thr, m, inv_t));
         take = by_weight ? (want - br.weight + w1 - 1) / w1 : want - br.count;
-        weight = br.weight + take * w1;
-      } else {
-        uint64_t* const list = sh.weight;  // in place of the histogram, which all have read
-        uint64_t* const sorted = list + kSampleList;
-        uint64_t* const sums = sorted + kSampleList;
-        int* const list_n = &sh.list_n[by_weight];
-        // the bracket's tokens into this CTA's list, in any order; then every CTA takes all of them, one a thread
-        each([&](const float* v, int i) {
-          if (!may_be(v)) return;
-          unsigned in = 0;
+        summed = false;
+        return br.weight + take * w1;
+      }
+      // the bracket's tokens into this CTA's list, in any order; then every CTA takes all of them
+      int* const list_n = &sh.list_n[by_weight];
+      if (by_key)
+        each_key([&](float, uint32_t key, int i) { sh.list[atomicAdd(list_n, 1)] = ((uint64_t)key << 32) | (uint32_t)~i; });
+      else
+        pass([&](const float* v, int i, unsigned in) {
+          int to = atomicAdd(list_n, __popc(in));
 #pragma unroll
-          for (int j = 0; j < kVec; ++j) in |= (unsigned)inside(v[j]) << j;
-          if (in) {
-            int to = atomicAdd(list_n, __popc(in));
-#pragma unroll
-            for (int j = 0; j < kVec; ++j)
-              if (in >> j & 1u) list[to++] = ((uint64_t)logit_key(v[j]) << 32) | (uint32_t)~(i + j);
-          }
+          for (int j = 0; j < kVec; ++j)
+            if (in >> j & 1u) sh.list[to++] = ((uint64_t)logit_key(v[j]) << 32) | (uint32_t)~(i + j);
         });
-        cluster.sync();
-        uint64_t me = 0;
-        {
-          const int share = lane < C ? *cluster.map_shared_rank(list_n, lane) : 0;
+      cluster.sync();
+      uint64_t me[kSampleOwn], w[kSampleOwn] = {};
+      auto own = [](const uint64_t* v, int o) {
+        uint64_t x = v[0];
+#pragma unroll
+        for (int i = 1; i < kSampleOwn; ++i) x = i == o ? v[i] : x;
+        return x;
+      };
+      {
+        const int in_q = lane < C ? *cluster.map_shared_rank(list_n, lane) : 0;
+        if (!by_key) br.weight = warp_sum64(lane < C ? *cluster.map_shared_rank(&sh.above[by_weight], lane) : 0);
+#pragma unroll
+        for (int o = 0; o < kSampleOwn; ++o) {
+          const int t = tid + o * kSampleThreads;
           int q = -1, at = 0;
           for (int c = 0, before = 0; c < C; ++c) {
-            const int in_c = __shfl_sync(0xffffffffu, share, c);
-            if (tid >= before && tid < before + in_c) {
+            const int in_c = __shfl_sync(0xffffffffu, in_q, c);
+            if (t >= before && t < before + in_c) {
               q = c;
-              at = tid - before;
+              at = t - before;
             }
             before += in_c;
           }
-          if (q >= 0) me = *cluster.map_shared_rank(&list[at], q);
+          me[o] = q >= 0 ? *cluster.map_shared_rank(&sh.list[at], q) : 0;
         }
-        // sorted downwards within the warp; a token's place and the weight up to it are then sums over the warps
-        // of what is above it in each, found by halving
+      }
+      // sorted downwards within the warp; a token's place and the weight up to it are then sums over the lots of
+      // 32 of what is above it in each, found by halving
+#pragma unroll 1
+      for (int o = 0; o < kSampleOwn && o * kSampleThreads < br.n; ++o) {
+        uint64_t x = own(me, o);
 #pragma unroll
         for (int size = 2; size <= 32; size *= 2)
 #pragma unroll
           for (int step = size / 2; step > 0; step /= 2) {
-            const uint64_t o = __shfl_xor_sync(0xffffffffu, me, step);
+            const uint64_t other = __shfl_xor_sync(0xffffffffu, x, step);
             const bool keep_max = ((lane & step) == 0) == ((lane & size) == 0);
-            me = (me > o) == keep_max ? me : o;
+            x = (x > other) == keep_max ? x : other;
           }
-        const uint64_t w = me ? depth_weight(logit_depth(key_logit((uint32_t)(me >> 32)), m, inv_t)) : 0;
-        sorted[tid] = me;
-        sums[tid] = warp_scan64(w, lane);
-        __syncthreads();
+        const uint64_t wx = x ? depth_weight(logit_depth(key_logit((uint32_t)(x >> 32)), m, inv_t)) : 0;
+        sh.sorted[tid + o * kSampleThreads] = x;
+        sh.sums[tid + o * kSampleThreads] = warp_scan64(wx, lane);
+#pragma unroll
+        for (int i = 0; i < kSampleOwn; ++i)
+          if (i == o) {
+            me[i] = x;
+            w[i] = wx;
+          }
+      }
+      __syncthreads();
+#pragma unroll 1
+      for (int o = 0; o < kSampleOwn && o * kSampleThreads < br.n; ++o) {
+        const uint64_t x = own(me, o), wx = own(w, o);
+        if (!x) continue;
         int place = 0;
         uint64_t upto = br.weight;
-#pragma unroll 4
+#pragma unroll 2
         for (int at = 0; at < br.n; at += 32) {
-          int above = 0;  // of this warp's tokens, those not below this one
+          int above = 0;  // of these 32 tokens, those not below this one
 #pragma unroll
-          for (int half = 16; half > 0; half /= 2) above += sorted[at + above + half - 1] >= me ? half : 0;
-          above += sorted[at + above] >= me;
+          for (int half = 16; half > 0; half /= 2) above += sh.sorted[at + above + half - 1] >= x ? half : 0;
+          above += sh.sorted[at + above] >= x;
           place += above;
-          upto += above ? sums[at + above - 1] : 0;
+          upto += above ? sh.sums[at + above - 1] : 0;
         }
-        if (me && (by_weight ? upto - w < want && want <= upto : br.count + place == want)) sh.cut = Pair64{upto, me};
-        __syncthreads();
-        const uint64_t last = sh.cut.b;
-        const int ties = __syncthreads_count(me >= last && (me >> 32) == (last >> 32));
-        weight = sh.cut.a;
-        thr = key_logit((uint32_t)(last >> 32));
-        take = ties;
+        if (by_weight ? upto - wx < want && want <= upto : br.count + place == want) {
+          sh.cut_weight = upto;
+          sh.cut = x;
+        }
       }
-      return weight;
+      __syncthreads();
+      const uint64_t last = sh.cut;
+      thr = key_logit((uint32_t)(last >> 32));
+      take = 0;
+#pragma unroll
+      for (int o = 0; o < kSampleOwn; ++o) {
+        const bool tie = (me[o] >> 32) == (last >> 32);
+        take += __syncthreads_count(tie && me[o] >= last);
+        // what is kept of these, and the ties, to the sums of the warps whose tokens they are
+        const int of_warp = (int)((~(uint32_t)me[o] - rank * kSampleWarps * a.per_warp) / (uint32_t)a.per_warp);
+        if (!by_key && me[o] && of_warp >= 0 && of_warp < kSampleWarps) {
+          if (tie)
+            atomicAdd(&sh.part_eq[of_warp], 1u);
+          else if (me[o] > last)
+            atomicAdd(&sh.part_w[of_warp], (unsigned long long)w[o]);
+        }
+      }
+      summed = !by_key;
+      return sh.cut_weight;
     };
 
-    // ---- 2, 3: the histogram over steps of d, and the cuts
-    // (-inf and NaN are below every step)
-    histogram([](const float*) { return true; },
-              [&](float, float d) { return d >= -kSampleDeep ? depth_bin(d, per_d, bins) : -1; });
-    const BinSums s = sum_bins();
-    uint64_t weight = s.total_weight;
-    // tokens too deep to be counted weigh nothing: a prefix that would reach them needs no cut
+    // ---- 2: the histogram over steps of d, and the exact weight of all. One addition to shared memory per logit
+    // (they fall into banks at random, 3.5 to one at the worst of 32): the number of a bin's tokens and the sum of
+    // their 256ths of a step bound its weight to 2^-13. What is too deep to weigh anything is not counted.
+    auto count = [&](bool weigh) {
+      for (int i = tid; i < bins; i += kSampleThreads) sh.cnt[i] = 0;
+      __syncthreads();
+      uint32_t hi = 0, lo = 0, n_in = 0;
+      const uint32_t end_q = (uint32_t)bins << 8;
+      each([&](const float* v, int) {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) {
+          const float d = logit_depth(v[j], m, inv_t);
+          const uint32_t at = depth_place(d, per_d256);
+          if (at < end_q) atomicAdd(&sh.cnt[at >> 8], packed ? (1u << 20) + (at & 255u) : 1u);
+          n_in += at < end_q;
+          if (weigh) {
+            uint32_t h, l;
+            weight_halves(expf(fmaxf(d, -100.f)), h, l);
+            hi += h - kHalfBits;
+            lo += l - kHalfBits;
+          }
+        }
+      });
+      const uint64_t w = warp_sum64(((uint64_t)hi << 20) + lo);
+      n_in = __reduce_add_sync(0xffffffffu, n_in);
+      if (lane == 0) {
+        sh.part_w[warp] = w;
+        atomicAdd(&sh.counted, n_in);
+      }
+      cluster.sync();
+    };
+    auto bin_sums = [&](int bin, uint32_t& n, uint64_t& w) {
+      uint32_t f = 0;
+      for (int q = 0; q < C; ++q) {
+        const uint32_t word = *cluster.map_shared_rank(&sh.cnt[bin], q);
+        n += packed ? word >> 20 : word;
+        f += packed ? word & 0xfffffu : 0u;
+      }
+      // Lower bound of the weight: e^-x lies under its chord over the step, by width^2 / 8 at most, and a
+      // place is a 256th deeper at most; 1e-5 for the roundings, and a weight is rounded by 1/2 itself.
+      const float top = expf(-bin * width) * (kSampleOne * (1.f - 1e-5f)), slope = 1.f - expf(-width);
+      const float part = packed ? n - (f + n) * (slope / 256) - n * (width * width / 8) : n * (1.f - slope);
+      w = cut_p && n ? (uint64_t)fmaxf(top * part - n, 0.f) : 0;
+    };
+    auto all_weights = [&]() { return warp_sum64(warp == 0 && lane < kSampleWarps ? sh.part_w[lane] : 0); };
+    count(cut_p && !cut_k);  // (top-k gives the prefix's weight itself)
+    BinSums s = sum_bins(bin_sums, all_weights());
+    // more than 4095 tokens of a bin in a CTA leave the word's upper 12 bits; and a top-k that reaches the tokens
+    // that are not counted cuts nothing
+    const bool whole = cut_p && cut_k && (uint64_t)k >= s.total_count;
+    if ((packed && !s.complete) || whole) {
+      packed = packed && s.complete;
+      if (tid == 0) sh.counted = 0;  // (count() has a barrier before it adds to it)
+      count(cut_p);
+      s = sum_bins(bin_sums, all_weights());
+    }
+    // ---- 3: the cuts. A prefix that would reach the tokens that are not counted needs none.
+    weight = s.total_weight;
     if (cut_k && (uint64_t)k < s.total_count) weight = cut(s, (uint64_t)k, false);
     if (cut_p) {
       const double want = ceil((double)p * (double)(int64_t)weight);
@@ -562,6 +676,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   auto taken = [&](uint64_t before, uint64_t here) {  // the weight of `here` ties that come after `before` others
     return before >= take ? (uint64_t)0 : min(here, take - before) * w1;
   };
+  // logits below it are not kept: of the floor, by more than the roundings of d (a NaN bound leaves the threshold)
+  const float low = temp < 1e30f ? fmaxf(thr, m + floor_d * temp - 1e-5f * (fabsf(m) - floor_d * temp)) : thr;
   // d of a kept logit above the threshold; of others one whose weight is 0 (of NaN too)
   auto kept = [&](float l) {
     const float d = logit_depth(l, m, inv_t);
@@ -572,7 +688,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     float most = v[0];
 #pragma unroll
     for (int j = 1; j < kVec; ++j) most = fmaxf(most, v[j]);
-    if (!(most >= thr)) return;
+    if (!(most >= low)) return;
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
       uint32_t h, l;
@@ -582,7 +698,13 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
       eq += v[j] == thr;
     }
   };
-  {
+  if (summed && tied) {  // (a floor below the threshold cuts nothing)
+    __syncthreads();
+    if (tid < kSampleWarps) {
+      sh.warp_a[tid] = sh.part_w[tid];
+      sh.warp_b[tid] = tied ? sh.part_eq[tid] : 0;
+    }
+  } else {
     // halves of up to 2^20 a logit: 32 bits hold the sums of a lane's 512 vectors (2^18 logits over 128 or
     // more warps), and of the warp in 64
     uint32_t hi = 0, lo = 0, eq = 0;
@@ -612,7 +734,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     sum_w = warp_sum64(lane < kSampleWarps ? sh.warp_a[lane] : 0);
     sum_eq = __reduce_add_sync(0xffffffffu, lane < kSampleWarps ? (uint32_t)sh.warp_b[lane] : 0u);
   }
-  const Pair64* r = exchange(sum_w, sum_eq);
+  const Trio64* r = exchange(sum_w, sum_eq, 0);
   if (top_inf) {
     for (int c = 0; c < C; ++c) take += r[c].b;
     if (cut_k) take = min(take, (uint64_t)k);
