@@ -10,14 +10,21 @@
 // sums by warp are sums in index order. Values that all CTAs need go to every CTA's memory (distributed
 // shared memory) behind a cluster barrier.
 //   1  load, largest logit
-//   2  (top-k or top-p) a histogram of number and weight over up to 2048 equal steps of d down to the weights
-//      that round to 0, summed over the cluster by shares of bins: the bin in which the prefix ends is exact
-//   3  the tokens of that bin, a few hundred, are gathered into one CTA, which sorts them and finds the last
-//      one kept; a bin of more than 512 (many ties, a high temperature) is cut again, by key, first
-//   4  the kept weight of every warp, the warp in which u falls, and a walk through its tokens
-// Without top-k and top-p only 1 and 4 are left, and the weights are computed once. What bounds it: the
-// instructions per logit (exponential, conversion, 64-bit sums; shared-memory atomics in 2) for many rows,
-// the cluster barriers for few.
+//   2  (top-k or top-p) a histogram over up to 2048 equal steps of d down to the weights that round to 0, summed
+//      over the cluster by shares of bins: the bin in which the prefix ends, by weight sometimes two. A bin holds
+//      its number of tokens and bounds of its weight; the exact weight of all is added up beside it
+//   3  one pass for the exact weight above that bracket, and its tokens, a few hundred, gathered by CTA. Every
+//      CTA takes all of them, ranks them and finds the last one kept. A bracket of more than 1024 (many ties, a
+//      high temperature) is cut again, by key, first
+//   4  the kept weight of every warp (known from 3, unless min-p cuts off more), the warp in which u falls, and
+//      the walk through its tokens by all warps of its CTA
+// Without top-k and top-p only 1 and 4 are left, and the weights are computed once.
+//
+// Measured with 151,936 BF16 logits a row: one row 8 us unfiltered, 17 us with top-k, 21 us with top-p; 64 rows
+// 18, 31 and 50 us; 256 rows 65 us (1.2 TB/s), 113 and 160 us; 256 unfiltered FP32 rows 101 us. A row's chain
+// bounds it: some 20 barriers of the CTA or the cluster (1000 to 1500 cycles each for the cluster's) with two CTAs
+// an SM to fill them, and for many filtered rows the instructions and shared-memory additions of 2 and 3 (20,000
+// and 11,000 of 58,000 cycles of a row with top-p).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -840,8 +847,8 @@ extern "C" int qd_sample(const void* logits, int dtype, int64_t ld, int64_t rows
     return set_error(QD_ERR_ARG, "sample: misaligned logits");
   if (rows == 0) return QD_OK;
   // The cluster: the fewest CTAs of which two fit an SM (so that one's loads and barriers hide behind the
-  // other's arithmetic) and which fill the SMs, but at most one for 4096 logits. Measured on 64 / 256 rows of
-  // 151,936 BF16 logits: see the kernel.
+  // other's arithmetic) and which fill the SMs, but at most one for 4096 logits. Measured on rows of 151,936 BF16
+  // logits, with clusters of 4 / 8: 8 rows with top-p 29 / 22 us, 64 rows 50 / 65 us, 256 unfiltered 65 / 88 us.
   const int size = dtype == QD_FP32 ? 4 : 2;
   int cluster = 1;
   while (cluster < kSampleMaxCluster && vocab >= (int64_t)8192 * cluster &&

@@ -236,3 +236,16 @@ def test_repeats_bit_for_bit_and_in_a_graph():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(tok.cpu(), a[0])
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("n", [3000, 100003])
+@pytest.mark.parametrize("spread", [1e-4, 0.02, 0.5])
+@pytest.mark.parametrize("kept", [{"top_k": 2000}, {"top_p": 0.6}, {"top_k": 2500, "top_p": 0.5}, {"top_k": 10 ** 6, "top_p": 0.999}])
+def test_many_tokens_of_nearly_the_same_weight(kept, spread, n, dtype):
+    # thousands within a step of d, so that the cut is refined by value, and more than a short count of them holds
+    g = torch.Generator().manual_seed(n)
+    x = (spread * torch.randn((4, n), generator=g)).to(dtype)
+    x[1, ::3] = -math.inf
+    x[2, n // 2:] = x[2, 0]
+    _check(x, torch.rand((4,), generator=g), temperature=1.0, **kept)
