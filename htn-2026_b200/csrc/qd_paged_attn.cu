@@ -44,9 +44,11 @@ constexpr int kPgKeys = 128;     // keys per block
 constexpr int kPgBox = 128 * 128;  // [128 rows][64 dims] of 16 bits
 constexpr int kFewRows = 16;       // rows of a few-row unit (MMA N)
 constexpr int kFewP = 2 * kFewRows * 128;  // its P: 2 halves of 64 keys x 16 rows of 128 B
-// The line of work, in places: a key block of a pair of tiles takes 3, one of a single tile (or few rows) 2, and
-// a unit's fixed cost (Q, its rows' way out) 7; measured, 2.1 us, 1.4 us and some 5 us. A CTA takes whole blocks.
-constexpr int kPgPairCost = 3, kPgBlockCost = 2, kPgUnitCost = 7;
+// The line of work, in places: a key block of a pair of tiles takes 5, one of a single tile 4, one of few rows 2
+// (measured 2.5, 1.8 and 1.3 us; the tiles a little more, since their pieces take longer to join), and a unit of tiles
+// 8 more for Q and its rows' way out (some 5 us), which few rows' units do not show. 30 single tokens and 2 chunks
+// of 251 after up to 2 k keys take 98 us; with 3, 2, 2 and 7 for every unit 128. A CTA takes whole blocks.
+constexpr int kPgPairCost = 5, kPgTileCost = 4, kPgBlockCost = 2, kPgUnitCost = 8;
 constexpr int kPgPiece = 12;  // places that a CTA takes at least, where units are whole tiles
 constexpr int kPgWhole = 8;   // key blocks up to which units of tiles are left whole, when there are CTAs for all
 
@@ -200,10 +202,15 @@ __device__ __forceinline__ int pg_blocks(const PagedAttnArgs& a, const PgReq& r,
 }
 // places of a key block of tile pair k
 __device__ __forceinline__ int pg_weight(const PagedAttnArgs& a, const PgReq& r, int k) {
-  return r.n - k * 2 * a.tpt > a.tpt ? kPgPairCost : kPgBlockCost;
+  const int tok = r.n - k * 2 * a.tpt;
+  return tok > a.tpt ? kPgPairCost : tok > a.tpf ? kPgTileCost : kPgBlockCost;
+}
+// and of its fixed cost
+__device__ __forceinline__ int pg_fixed(const PagedAttnArgs& a, const PgReq& r, int k) {
+  return r.n - k * 2 * a.tpt > a.tpf ? kPgUnitCost : 0;
 }
 __device__ __forceinline__ int pg_cost(const PagedAttnArgs& a, const PgReq& r, int k) {
-  return kPgUnitCost + pg_weight(a, r, k) * pg_blocks(a, r, k);
+  return pg_fixed(a, r, k) + pg_weight(a, r, k) * pg_blocks(a, r, k);
 }
 // sum of pg_cost over the request's pairs. Where nothing is cut the terms are ceil((pos0 + 2 tpt k) / 128),
 // which grow by period_blocks every `period` pairs: one pass over a period suffices (all but the last are pairs).
@@ -466,14 +473,15 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
       return max(ld_i32(a.b.table + i * a.b.ld_table + (key >> a.b.page_shift)), -1);
     };
     while (at < end && ok) {
-      const int nblk = pg_blocks(a, r, k), wt = pg_weight(a, r, k), len = whole ? 1 : kPgUnitCost + wt * nblk;
+      const int nblk = pg_blocks(a, r, k), wt = pg_weight(a, r, k), fixed = pg_fixed(a, r, k);
+      const int len = whole ? 1 : fixed + wt * nblk;
       const int take = min(end - at, len - o);
       // the blocks whose first places are among these
-      const int j0 = whole ? 0 : (max(o - kPgUnitCost, 0) + wt - 1) / wt;
-      const int j1 = whole ? nblk : (max(o + take - kPgUnitCost, 0) + wt - 1) / wt;
+      const int j0 = whole ? 0 : (max(o - fixed, 0) + wt - 1) / wt;
+      const int j1 = whole ? nblk : (max(o + take - fixed, 0) + wt - 1) / wt;
       if (j1 > j0) {
         int page = page_of(j0);
-        const int first = at - o + kPgUnitCost;  // place of the unit's first block
+        const int first = at - o + fixed;  // place of the unit's first block
         const int t0 = k * 2 * a.tpt, ntok = min(2 * a.tpt, r.n - t0);
         const bool two = ntok > a.tpt, few = ntok <= a.tpf;
         const int ra = two ? 0 : next_region;
@@ -1184,43 +1192,73 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
       bool out_rows = g.whole;
       if (!g.whole && is_last(g)) {  // join the pieces in the order of their keys
         out_rows = true;
+        // kP pieces of 4 / kP times 8 dims of a row at a time: 8 loads in flight, none twice where a unit is cut once
+        // (16 in flight spill)
+        auto join_pieces = [&](auto pieces) __attribute__((always_inline)) {
+          constexpr int kP = decltype(pieces)::value, kI = 4 / kP;
+          const int items = rows * (D / 8);
 #pragma unroll 1
-        for (int e = r; e < rows * (D / 8); e += 128) {  // 8 dims of a row, four pieces' loads in flight
-          const int c8 = e / rows, row = e - c8 * rows;
-          float M = -INFINITY, L = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-          for (int q0 = 0; q0 < g.nc; q0 += 4) {
-            float2 p[4];
-            float4 v[4][2];
+          for (int e0 = r; e0 < items; e0 += 128 * kI) {
+            float M[kI], L[kI], acc[kI][8];
+            int c8[kI], row[kI];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const int qq = min(q0 + q, g.nc - 1), slot_q = 2 * (g.c0 + qq) + (qq == 0 ? 1 : 0);
-              p[q] = __ldcg(part_m(slot_q, row));
-              v[q][0] = __ldcg(part_c(slot_q, 2 * c8) + row);
-              v[q][1] = __ldcg(part_c(slot_q, 2 * c8 + 1) + row);
+            for (int i = 0; i < kI; ++i) {
+              const int e = min(e0 + 128 * i, items - 1);
+              c8[i] = e / rows;
+              row[i] = e - c8[i] * rows;
+              M[i] = -INFINITY;
+              L[i] = 0.f;
+#pragma unroll
+              for (int d = 0; d < 8; ++d) acc[i][d] = 0.f;
+            }
+#pragma unroll 1
+            for (int q0 = 0; q0 < g.nc; q0 += kP) {
+              float2 p[kI][kP];
+              float4 v[kI][kP][2];
+#pragma unroll
+              for (int i = 0; i < kI; ++i)
+#pragma unroll
+                for (int q = 0; q < kP; ++q) {
+                  const int qq = min(q0 + q, g.nc - 1), slot_q = 2 * (g.c0 + qq) + (qq == 0 ? 1 : 0);
+                  p[i][q] = __ldcg(part_m(slot_q, row[i]));
+                  v[i][q][0] = __ldcg(part_c(slot_q, 2 * c8[i]) + row[i]);
+                  v[i][q][1] = __ldcg(part_c(slot_q, 2 * c8[i] + 1) + row[i]);
+                }
+#pragma unroll
+              for (int i = 0; i < kI; ++i)
+#pragma unroll
+                for (int q = 0; q < kP; ++q)
+                  if (q0 + q < g.nc && p[i][q].y > 0.f) {  // a piece in which the row saw no key counts for nothing
+                    const float mn = fmaxf(M[i], p[i][q].x), wa = exp2f(M[i] - mn), wb = exp2f(p[i][q].x - mn);
+                    M[i] = mn;
+                    L[i] = L[i] * wa + p[i][q].y * wb;
+                    const float4 lo = v[i][q][0], hi = v[i][q][1];
+                    const float u[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+                    for (int d = 0; d < 8; ++d) acc[i][d] = acc[i][d] * wa + u[d] * wb;
+                  }
             }
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-              if (q0 + q < g.nc && p[q].y > 0.f) {  // a piece in which the row saw no key counts for nothing
-                const float mn = fmaxf(M, p[q].x), wa = exp2f(M - mn), wb = exp2f(p[q].x - mn);
-                M = mn;
-                L = L * wa + p[q].y * wb;
-                const float u[8] = {v[q][0].x, v[q][0].y, v[q][0].z, v[q][0].w, v[q][1].x, v[q][1].y, v[q][1].z, v[q][1].w};
+            for (int i = 0; i < kI; ++i) {
+              if (e0 + 128 * i >= items) break;
+              const float inv = L[i] > 0.f ? 1.0f / L[i] : 0.f;
+              uint32_t w[4];
 #pragma unroll
-                for (int d = 0; d < 8; ++d) acc[d] = acc[d] * wa + u[d] * wb;
+              for (int d = 0; d < 4; ++d) w[d] = Elem<T>::pack(acc[i][2 * d] * inv, acc[i][2 * d + 1] * inv);
+              *reinterpret_cast<uint4*>(stage + row[i] * (2 * D) + ((c8[i] ^ (row[i] & 7)) << 4)) =
+                  make_uint4(w[0], w[1], w[2], w[3]);
+              if (c8[i] == 0 && a.lse) {
+                const int rt = (row[i] * a.inv_group) >> 16;
+                a.lse[(g.row0 + t0 + rt) * a.ld_lse + g.head * a.group + row[i] - rt * a.group] =
+                    L[i] > 0.f ? (M[i] + __log2f(L[i])) * 0.69314718055994531f : -INFINITY;
               }
+            }
           }
-          const float inv = L > 0.f ? 1.0f / L : 0.f;
-          uint32_t w[4];
-#pragma unroll
-          for (int d = 0; d < 4; ++d) w[d] = Elem<T>::pack(acc[2 * d] * inv, acc[2 * d + 1] * inv);
-          *reinterpret_cast<uint4*>(stage + row * (2 * D) + ((c8 ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-          if (c8 == 0 && a.lse) {
-            const int rt = (row * a.inv_group) >> 16;
-            a.lse[(g.row0 + t0 + rt) * a.ld_lse + g.head * a.group + row - rt * a.group] =
-                L > 0.f ? (M + __log2f(L)) * 0.69314718055994531f : -INFINITY;
-          }
-        }
+        };
+        if (g.nc == 2)
+          join_pieces(Const<2>());
+        else
+          join_pieces(Const<4>());
       }
       if (!ok) break;
       if (out_rows) {
