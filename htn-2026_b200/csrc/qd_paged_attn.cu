@@ -29,6 +29,11 @@
 // leaves fp32 partials (O, m, l) in the scratch, and the CTA that finishes last (a ticket per cut unit)
 // joins them in the order of the keys, so results repeat bit for bit. Every CTA finds its place on the line
 // from cu_tokens and kv_len itself: no planning launch, and no length is needed on the host.
+//
+// Measured, 32 query and 8 KV heads of 128 in BF16: 8 single tokens over up to 41 k keys 184 us (HBM: 6.3 TB/s); 64
+// single tokens over 1 to 1.5 k keys 72 us (4.7 TB/s: each CTA's start and end); one token over 1 k keys 12.6 us
+// (latency); 2048 tokens after 8192 keys 342 to 368 us (0.50 to 0.54 of the BF16 peak: a pair's block of 128 keys takes
+// some 4000 cycles, 2048 of them products, since each tile's softmax and products wait for one another).
 #include <climits>
 
 #include "qd_host.h"
