@@ -249,3 +249,11 @@ def test_many_tokens_of_nearly_the_same_weight(kept, spread, n, dtype):
     x[1, ::3] = -math.inf
     x[2, n // 2:] = x[2, 0]
     _check(x, torch.rand((4,), generator=g), temperature=1.0, **kept)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("kept", ["none", "top_p", "all"])
+def test_largest_vocabulary(kept, dtype):
+    x, u = _logits(3, 1 << 18, dtype, seed=5)
+    u[0] = 0.9999999  # ends in the last part of the row
+    _check(x, u, temperature=1.1, **FILTERS[kept])
