@@ -199,6 +199,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t row = blockIdx.x / C;
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;");  // waited for before the first store to another CTA
   grid_dep_wait();
   grid_dep_launch();
 
@@ -269,6 +270,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     sh.counted = 0;
   }
   __syncthreads();
+  // a CTA's shared memory may be written to from outside only once the CTA runs: all have, long before this
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
   int turn = 0;
   // (va, vb, vc), known to warp 0, to every CTA of the cluster; all threads pass the barrier
   auto exchange = [&](uint64_t va, uint64_t vb, uint64_t vc) {

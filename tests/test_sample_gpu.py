@@ -257,3 +257,20 @@ def test_largest_vocabulary(kept, dtype):
     x, u = _logits(3, 1 << 18, dtype, seed=5)
     u[0] = 0.9999999  # ends in the last part of the row
     _check(x, u, temperature=1.1, **FILTERS[kept])
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("kept", ["none", "all"])
+def test_many_more_clusters_than_fit_the_gpu(kept, dtype):
+    """CTAs come and go while others of the same call run; a row's draw does not depend on the rows beside it,
+    nor on how many CTAs share it (fewer where there are more rows)."""
+    rows = 1200
+    x, u = _logits(rows, 30011, dtype, seed=11)
+    kw = {k: torch.as_tensor(v).expand(rows) for k, v in FILTERS[kept].items()}
+    tok, lp = _draw(x, u, **kw)
+    for at in range(0, rows, 100):
+        some = slice(at, at + (at // 100) % 3 + 1)
+        part, part_lp = _draw(x[some].contiguous(), u[some], **{k: v[some] for k, v in kw.items()})
+        assert torch.equal(tok[some], part) and torch.equal(lp[some], part_lp)
+    for i in range(0, rows, 97):
+        _row_ok(x[i].double(), float(u[i]), int(tok[i]), float(lp[i]), **FILTERS[kept])
