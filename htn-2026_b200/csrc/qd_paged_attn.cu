@@ -34,10 +34,12 @@
 // single tokens over 1 to 1.5 k keys 72 us (4.7 TB/s: each CTA's start and end); one token over 1 k keys 12.6 us
 // (latency); 2048 tokens after 8192 keys 342 to 368 us (0.50 to 0.54 of the BF16 peak: a pair's block of 128 keys takes
 // some 4000 cycles, 2048 of them products, since each tile's softmax and products wait for one another).
+#include <algorithm>
 #include <climits>
 
 #include "qd_host.h"
 #include "qd_paged_dev.cuh"
+#include "qd_paged_line.h"
 #include "qd_umma.cuh"
 
 namespace qd {
@@ -45,16 +47,9 @@ namespace qd {
 constexpr int kPgThreads = 384;  // warps 0-3 softmax A, 4-7 softmax B, 8 producer, 9 MMA, 10-11 only start up
 // registers per thread after the start: 2 * 224 + 56 = 3 * 168, what the launch gave the three warpgroups
 constexpr int kPgSoftmaxRegs = 224, kPgOtherRegs = 56;
-constexpr int kPgKeys = 128;     // keys per block
 constexpr int kPgBox = 128 * 128;  // [128 rows][64 dims] of 16 bits
-constexpr int kFewRows = 16;       // rows of a few-row unit (MMA N)
 constexpr int kFewP = 2 * kFewRows * 128;  // its P: 2 halves of 64 keys x 16 rows of 128 B
-// The line of work, in places: a key block of a pair of tiles takes 5, one of a single tile 4, one of few rows 2
-// (measured 2.5, 1.8 and 1.3 us; the tiles a little more, since their pieces take longer to join), and a unit of tiles
-// 8 more for Q and its rows' way out (some 5 us), which few rows' units do not show. 30 single tokens and 2 chunks
-// of 251 after up to 2 k keys take 98 us; with 3, 2, 2 and 7 for every unit 128. A CTA takes whole blocks.
-constexpr int kPgPairCost = 5, kPgTileCost = 4, kPgBlockCost = 2, kPgUnitCost = 8;
-constexpr int kPgPiece = 12;  // places that a CTA takes at least, where units are whole tiles
+constexpr int kPgManyUnits = 1 << 20;  // above any grid (whose scratch would be 280 GB); 384 of them fit 32 bits
 constexpr int kPgWhole = 8;   // key blocks up to which units of tiles are left whole, when there are CTAs for all
 
 struct alignas(64) PagedAttnArgs {
@@ -63,10 +58,10 @@ struct alignas(64) PagedAttnArgs {
   char* out;
   float* lse;
   int64_t ldo, ld_lse;
-  int group, tpt, tpf;        // heads per KV head, tokens per tile and per 16 rows (0: a group is larger)
-  int head_groups;            // groups of 8 rows from a KV head of a page to the next
-  int inv_group;              // row / group = row * inv_group >> 16 for the rows of a tile
-  int period, period_blocks;  // ceil sums over tile pairs repeat every `period` pairs, `period_blocks` blocks on
+  PgShape s;
+  int room;         // positions in a row of the page table, kPgMaxKeys at most
+  int head_groups;  // groups of 8 rows from a KV head of a page to the next
+  int inv_group;    // row / group = row * inv_group >> 16 for the rows of a tile
   float scale_log2;
   // [2 * grid slots][2 tiles] of 128 x D floats ([D / 4][128 rows][4], few-row units [rows][D]), then the rows'
   // (m, l) [slots][2][128]
@@ -182,68 +177,9 @@ __device__ __forceinline__ void tmem_wait_ld64(uint32_t* r) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]), "+r"(r[32]), "+r"(r[33]), "+r"(r[34]), "+r"(r[35]), "+r"(r[36]), "+r"(r[37]), "+r"(r[38]), "+r"(r[39]), "+r"(r[40]), "+r"(r[41]), "+r"(r[42]), "+r"(r[43]), "+r"(r[44]), "+r"(r[45]), "+r"(r[46]), "+r"(r[47]), "+r"(r[48]), "+r"(r[49]), "+r"(r[50]), "+r"(r[51]), "+r"(r[52]), "+r"(r[53]), "+r"(r[54]), "+r"(r[55]), "+r"(r[56]), "+r"(r[57]), "+r"(r[58]), "+r"(r[59]), "+r"(r[60]), "+r"(r[61]), "+r"(r[62]), "+r"(r[63])::"memory");
 }
-// One request on the line of key blocks.
-struct PgReq {
-  int row0, n, pos0, kv;  // token rows, the first one's position, keys (cut to the table row)
-  int pairs;              // tile pairs
-};
 __device__ __forceinline__ PgReq pg_request(const PagedAttnArgs& a, int i) {
-  PgReq r;
-  const int tok = (int)a.b.tokens;
-  const int end = min(max(ld_i32(a.b.cu + i + 1), 0), tok);
-  r.row0 = min(max(ld_i32(a.b.cu + i), 0), end);
-  r.n = end - r.row0;
-  const int kv = max(ld_i32(a.b.kv_len + i), 0);
-  r.pos0 = kv - r.n;
-  r.kv = (int)min((int64_t)kv, (int64_t)a.b.max_pages * a.b.page_size);
-  r.pairs = (r.n + 2 * a.tpt - 1) / (2 * a.tpt);
-  return r;
+  return pg_make_request(a.s, ld_i32(a.b.cu + i), ld_i32(a.b.cu + i + 1), ld_i32(a.b.kv_len + i), (int)a.b.tokens, a.room);
 }
-// key blocks of tile pair k: up to its last token's position (at least one, so that rows without keys are
-// written too)
-__device__ __forceinline__ int pg_blocks(const PagedAttnArgs& a, const PgReq& r, int k) {
-  const int keys = min(r.kv, r.pos0 + min(r.n, (k + 1) * 2 * a.tpt));
-  return max((keys + kPgKeys - 1) / kPgKeys, 1);
-}
-// places of a key block of tile pair k
-__device__ __forceinline__ int pg_weight(const PagedAttnArgs& a, const PgReq& r, int k) {
-  const int tok = r.n - k * 2 * a.tpt;
-  return tok > a.tpt ? kPgPairCost : tok > a.tpf ? kPgTileCost : kPgBlockCost;
-}
-// and of its fixed cost
-__device__ __forceinline__ int pg_fixed(const PagedAttnArgs& a, const PgReq& r, int k) {
-  return r.n - k * 2 * a.tpt > a.tpf ? kPgUnitCost : 0;
-}
-__device__ __forceinline__ int pg_cost(const PagedAttnArgs& a, const PgReq& r, int k) {
-  return pg_fixed(a, r, k) + pg_weight(a, r, k) * pg_blocks(a, r, k);
-}
-// sum of pg_cost over the request's pairs. Where nothing is cut the terms are ceil((pos0 + 2 tpt k) / 128),
-// which grow by period_blocks every `period` pairs: one pass over a period suffices (all but the last are pairs).
-__device__ __forceinline__ int pg_sum_cost(const PagedAttnArgs& a, const PgReq& r) {
-  if (r.pairs <= 1) return r.pairs ? pg_cost(a, r, 0) : 0;
-  int sum = 0;
-  if (r.pos0 >= 0 && r.kv == r.pos0 + r.n) {
-    const int m = r.pairs - 1, q = m / a.period, rest = m - q * a.period;
-#pragma unroll 1
-    for (int j = 1; j <= min(a.period, m); ++j) {
-      const int cnt = q + (j <= rest);
-      sum += cnt * ((r.pos0 + 2 * a.tpt * j + kPgKeys - 1) / kPgKeys) + a.period_blocks * (cnt * (cnt - 1) / 2);
-    }
-    return kPgUnitCost * m + kPgPairCost * sum + pg_cost(a, r, m);
-  }
-#pragma unroll 1
-  for (int k = 0; k < r.pairs; ++k) sum += pg_cost(a, r, k);
-  return sum;
-}
-// The line of `total` places over `ctas` CTAs: the first total % ctas take one more than the others.
-struct PgLine {
-  unsigned total, ctas, each, more;
-  __device__ __forceinline__ unsigned begin(unsigned c) const { return c * each + min(c, more); }
-  __device__ __forceinline__ unsigned owner(unsigned at) const {
-    const unsigned big = more * (each + 1);
-    return at < big ? at / (each + 1) : more + (at - big) / each;
-  }
-};
 
 // Joins a cut few-row unit's pieces (rows of D floats) in the order of their keys: four warps, a row per D / 4
 // lanes, kRows such rows at a time with kPieces pieces' loads in flight for each.
@@ -296,7 +232,7 @@ __device__ __forceinline__ void pg_join_few(const PagedAttnArgs& a, const PgSeg&
       const int row = r0 + kAt * i;
       if (row < rows) {
         const float inv = L[i] > 0.f ? 1.0f / L[i] : 0.f;
-        const int tok = (row * a.inv_group) >> 16, t2 = g.row0 + tok, h2 = g.head * a.group + row - tok * a.group;
+        const int tok = (row * a.inv_group) >> 16, t2 = g.row0 + tok, h2 = g.head * a.s.group + row - tok * a.s.group;
         *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + t2 * a.ldo + (int64_t)h2 * D + 4 * c4) =
             make_uint2(Elem<T>::pack(acc[i].x * inv, acc[i].y * inv), Elem<T>::pack(acc[i].z * inv, acc[i].w * inv));
         if (c4 == 0 && a.lse)
@@ -339,7 +275,8 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
   PgSeg* segs = reinterpret_cast<PgSeg*>(smem + Lay::seg);
   int* misc = reinterpret_cast<int*>(smem + Lay::misc);
   int* abort = misc + 1;
-  int* scan = misc + 16;  // warp totals [2][12]
+  int64_t* scan = reinterpret_cast<int64_t*>(misc + 12);  // the warps' totals: places, and units
+  int* scan_u = misc + 36;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int x = 0; x < 2; ++x) {
@@ -363,30 +300,32 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
       mbar_init(empty(s), 1);
     }
     fence_mbar_init();
-    for (int m = 1; m < 16; ++m) misc[m] = 0;
+    for (int m = 1; m < 12; ++m) misc[m] = 0;  // (the scan comes after them)
   }
   if (warp == 9) tmem_alloc(smem_u32(misc), 512);
 
   // ---- this CTA's place on the line: a prefix sum over the requests, and a walk from the one it starts in
-  // (in 32 bits: 2^31 key blocks would be hours of work)
-  int mine = 0, mine_u = 0;  // places, and units
+  int64_t mine = 0;  // places
+  int mine_u = 0;    // and units, of which no more are counted than make the sum larger than any grid
   const int per = (a.b.batch + kPgThreads - 1) / kPgThreads;
   const int i0 = min(tid * per, a.b.batch), i1 = min(i0 + per, a.b.batch);
   PgReq r = {};
   bool cut = false, tiles = false, longer = false;
   for (int i = i0; i < i1; ++i) {
     r = pg_request(a, i);
-    tiles |= r.n > a.tpf;
+    tiles |= r.n > a.s.tpf;
     cut |= r.kv != r.pos0 + r.n && r.n > 0;
-    mine += a.b.nkv * pg_sum_cost(a, r);
-    mine_u += a.b.nkv * r.pairs;
-    longer |= r.pairs && pg_blocks(a, r, r.pairs - 1) > kPgWhole;
+    mine += a.b.nkv * pg_sum_cost(a.s, r);
+    mine_u = (int)min(mine_u + (int64_t)a.b.nkv * r.pairs, (int64_t)kPgManyUnits);
+    longer |= r.pairs && pg_blocks(a.s, r, r.pairs - 1) > kPgWhole;
   }
   if (cut && blockIdx.x == 0) flag_error(a.b.err, QD_DEVERR_PAGE);
-  int incl = mine, incl_u = mine_u;
+  int64_t incl = mine;
+  int incl_u = mine_u;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, incl, o), u = __shfl_up_sync(0xffffffffu, incl_u, o);
+    const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+    const int u = __shfl_up_sync(0xffffffffu, incl_u, o);
     if (lane >= o) {
       incl += v;
       incl_u += u;
@@ -394,7 +333,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
   }
   if (lane == 31) {
     scan[warp] = incl;
-    scan[12 + warp] = incl_u;
+    scan_u[warp] = incl_u;
   }
   tc_fence_before();
   tiles = __syncthreads_or(tiles);
@@ -403,52 +342,41 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
   grid_dep_launch();
   int units = 0;
 #pragma unroll
-  for (int w = 0; w < kPgThreads / 32; ++w) units += scan[12 + w];
+  for (int w = 0; w < kPgThreads / 32; ++w) units += scan_u[w];
   // Units of tiles that are few and short are not cut: a place each, and a CTA each
   const bool whole = tiles && !longer && units <= (int)gridDim.x;
   if (whole) {
     mine = mine_u;
     incl = incl_u;
-    scan += 12;
   }
-  int before = incl - mine;
-  PgLine line;
-  line.total = 0;
+  int64_t before = incl - mine, total = 0;
 #pragma unroll
   for (int w = 0; w < kPgThreads / 32; ++w) {
-    const int v = scan[w];
+    const int64_t v = whole ? scan_u[w] : scan[w];
     if (w < warp) before += v;
-    line.total += v;
+    total += v;
   }
   // With little work the first CTAs take kPgPiece places each (a block, if all units have few rows), the rest
   // nothing: joining the pieces of a tile of 128 rows costs about as much as some blocks of keys. No CTA takes
   // less than a block, so that every one between the first and the last of a cut unit has some of it.
-  const unsigned least = whole ? 1 : tiles ? kPgPiece : kPgBlockCost;
-  line.ctas = min((unsigned)gridDim.x, max(line.total / least, min(line.total, 1u)));
-  line.each = line.ctas ? line.total / line.ctas : 0;
-  line.more = line.total - line.each * line.ctas;
+  const PgLine line = pg_line(total, (int)gridDim.x, whole ? 1 : tiles ? kPgPiece : kPgBlockCost);
   const int cta = blockIdx.x;
-  const int begin = cta < (int)line.ctas ? (int)line.begin(cta) : 0;
-  const int end = cta < (int)line.ctas ? (int)line.begin(cta + 1) : 0;
+  const int64_t begin = cta < line.ctas ? line.begin(cta) : 0, end = cta < line.ctas ? line.begin(cta + 1) : 0;
   if (begin < end && begin >= before && begin < before + mine) {
-    int w = begin - before, i = i0;
+    int64_t w = begin - before;
+    int i = i0;
     if (per > 1) {
       for (r = pg_request(a, i);; r = pg_request(a, ++i)) {
-        const int c = a.b.nkv * (whole ? r.pairs : pg_sum_cost(a, r));
+        const int64_t c = a.b.nkv * (whole ? r.pairs : pg_sum_cost(a.s, r));
         if (w < c) break;
         w -= c;
       }
     }
-    int k = 0, len = whole ? 1 : pg_cost(a, r, 0);
-    while (w >= a.b.nkv * len) {
-      w -= a.b.nkv * len;
-      ++k;
-      len = whole ? 1 : pg_cost(a, r, k);
-    }
+    const PgPlace at = pg_place(a.s, r, w, whole);
     misc[2] = i;
-    misc[3] = k;
-    misc[4] = w / len;  // KV head
-    misc[5] = w % len;  // place in the unit
+    misc[3] = at.k;
+    misc[4] = at.h;
+    misc[5] = at.o;
     *reinterpret_cast<PgReq*>(smem + Lay::mx) = r;
   }
   __syncthreads();
@@ -461,7 +389,8 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
   if (warp == 8) {
     // ------------------------------------------------------------ producer: all lanes walk the line
     const uint64_t pol = policy_evict_normal();
-    int at = begin, i = misc[2], k = misc[3], h = misc[4], o = misc[5];
+    int64_t at = begin;
+    int i = misc[2], k = misc[3], h = misc[4], o = misc[5];
     // a lane's copy: a page of the block, and a half of its dims unless they are merged
     constexpr int copies = kMerged ? 1 : kHalves;
     const int boxes = (kPgKeys >> a.b.page_shift) * copies;
@@ -478,17 +407,17 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
       return max(ld_i32(a.b.table + i * a.b.ld_table + (key >> a.b.page_shift)), -1);
     };
     while (at < end && ok) {
-      const int nblk = pg_blocks(a, r, k), wt = pg_weight(a, r, k), fixed = pg_fixed(a, r, k);
+      const int nblk = pg_blocks(a.s, r, k), wt = pg_weight(a.s, r, k), fixed = pg_fixed(a.s, r, k);
       const int len = whole ? 1 : fixed + wt * nblk;
-      const int take = min(end - at, len - o);
+      const int take = (int)min(end - at, (int64_t)(len - o));
       // the blocks whose first places are among these
       const int j0 = whole ? 0 : (max(o - fixed, 0) + wt - 1) / wt;
       const int j1 = whole ? nblk : (max(o + take - fixed, 0) + wt - 1) / wt;
       if (j1 > j0) {
         int page = page_of(j0);
-        const int first = at - o + fixed;  // place of the unit's first block
-        const int t0 = k * 2 * a.tpt, ntok = min(2 * a.tpt, r.n - t0);
-        const bool two = ntok > a.tpt, few = ntok <= a.tpf;
+        const int64_t first = at - o + fixed;  // place of the unit's first block
+        const int t0 = k * 2 * a.s.tpt, ntok = min(2 * a.s.tpt, r.n - t0);
+        const bool two = ntok > a.s.tpt, few = ntok <= a.s.tpf;
         const int ra = two ? 0 : next_region;
         // Q: the regions this unit takes, once their last users are done
         for (int x = 0; x <= (two ? 1 : 0) && ok; ++x) {
@@ -502,16 +431,16 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
         if (lane == 0) {
           for (int x = 0; x <= (two ? 1 : 0); ++x) {
             const int reg = two ? x : ra;
-            const bool one = ntok - x * a.tpt == 1;
+            const bool one = ntok - x * a.s.tpt == 1;
             const CUtensorMap* map = one ? &a.tq1 : few ? &a.tqf : &a.tq;
-            mbar_arrive_expect_tx(qfull(reg), kHalves * a.group * (one ? 1 : few ? a.tpf : a.tpt) * 128);
+            mbar_arrive_expect_tx(qfull(reg), kHalves * a.s.group * (one ? 1 : few ? a.s.tpf : a.s.tpt) * 128);
 #pragma unroll
             for (int hf = 0; hf < kHalves; ++hf)
-              pg_tma_4d(sb + Lay::q + reg * Lay::kItem + hf * kPgBox, map, 64 * hf, 0, h, r.row0 + t0 + x * a.tpt,
+              pg_tma_4d(sb + Lay::q + reg * Lay::kItem + hf * kPgBox, map, 64 * hf, 0, h, r.row0 + t0 + x * a.s.tpt,
                         qfull(reg), pol);
             misc[6 + reg] = qfills[reg] + 1;
           }
-          const int c0 = whole ? cta : (int)line.owner(first), c1 = whole ? cta : (int)line.owner(first + wt * (nblk - 1));
+          const int c0 = whole ? cta : line.owner(first), c1 = whole ? cta : line.owner(first + wt * (nblk - 1));
           PgSeg* s = segs + (seg & 3);
           s->row0 = r.row0 + t0;
           s->ntok = ntok;
@@ -859,12 +788,12 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
         const int key0 = (g.j0 + j) * kPgKeys;
         if (key0 + kPgKeys > min(g.kv, g.pos0 + 1)) {  // some row sees only a part of this block
           const int key = key0 + r;
-          int lim = g.pos0 + 1, next = a.group;  // of the row's token
+          int lim = g.pos0 + 1, next = a.s.group;  // of the row's token
 #pragma unroll
           for (int c = 0; c < kC; ++c) {
             if (c == next) {
               ++lim;
-              next += a.group;
+              next += a.s.group;
             }
             if (key >= min(lim, g.kv)) sv[c] = __float_as_uint(-INFINITY);
           }
@@ -954,7 +883,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
           L = L * fa + ((s2.x + s2.y) + (s2.z + s2.w)) * fb;
           M = mn;
         }
-        const int tok = (lane * a.inv_group) >> 16, hq = g.head * a.group + lane - tok * a.group;
+        const int tok = (lane * a.inv_group) >> 16, hq = g.head * a.s.group + lane - tok * a.s.group;
         row_at = (g.row0 + tok) * a.ldo + (int64_t)hq * D;
         if (g.whole) {
           const float inv = L > 0.f ? 1.0f / L : 0.f;
@@ -996,10 +925,10 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
       blocks += g.nb;
       const bool two = g.region < 0, joined = !two && g.nb > 1;
       if (x == 1 && !two && !joined) continue;  // one tile, one block
-      const int t0 = two ? x * a.tpt : 0;       // this tile's first token
-      const int ntok = min(a.tpt, g.ntok - t0), rows = ntok * a.group;
+      const int t0 = two ? x * a.s.tpt : 0;       // this tile's first token
+      const int ntok = min(a.s.tpt, g.ntok - t0), rows = ntok * a.s.group;
       const int my_tok = (r * a.inv_group) >> 16, tok = g.row0 + t0 + my_tok;
-      const int head = g.head * a.group + r - my_tok * a.group;
+      const int head = g.head * a.s.group + r - my_tok * a.s.group;
       // keys this row sees: up to its own position (MMA rows past the last token hold anything)
       const int lim = r < rows ? min(g.kv, g.pos0 + t0 + my_tok + 1) : INT_MAX;
       const bool idle = (r & ~31) >= rows;  // no row of this warp is a token's
@@ -1153,7 +1082,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
           const int row = i / (D / 8), c = i % (D / 8), rt = (row * a.inv_group) >> 16;
           const uint4 v = *reinterpret_cast<const uint4*>(stage + row * (2 * D) + ((c ^ (row & 7)) << 4));
           T* const to = reinterpret_cast<T*>(a.out) + (g.row0 + t0 + rt) * a.ldo +
-                        (int64_t)(g.head * a.group + row - rt * a.group) * D + 8 * c;
+                        (int64_t)(g.head * a.s.group + row - rt * a.s.group) * D + 8 * c;
           *reinterpret_cast<uint4*>(to) = v;
         }
       };
@@ -1254,7 +1183,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
                   make_uint4(w[0], w[1], w[2], w[3]);
               if (c8[i] == 0 && a.lse) {
                 const int rt = (row[i] * a.inv_group) >> 16;
-                a.lse[(g.row0 + t0 + rt) * a.ld_lse + g.head * a.group + row[i] - rt * a.group] =
+                a.lse[(g.row0 + t0 + rt) * a.ld_lse + g.head * a.s.group + row[i] - rt * a.s.group] =
                     L[i] > 0.f ? (M[i] + __log2f(L[i])) * 0.69314718055994531f : -INFINITY;
               }
             }
@@ -1348,10 +1277,9 @@ extern "C" int qd_paged_attn(const void* q, int64_t ldq, int dtype, int64_t toke
   if (tokens == 0) return QD_OK;
   const PFN_cuTensorMapEncodeTiled_v12000 encode = tensor_map_encoder();
   if (!encode) return set_error(QD_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
-  a.group = nq_heads / nkv_heads;
-  a.tpt = 128 / a.group;
-  a.tpf = kFewRows / a.group;
-  a.inv_group = 65536 / a.group + 1;  // exact: the excess is below 128 / 65536, a fraction's distance to 1 at least 1 / 128
+  a.s = pg_shape(nq_heads, nkv_heads);
+  a.room = (int)std::min((int64_t)max_pages * page_size, (int64_t)kPgMaxKeys);
+  a.inv_group = 65536 / a.s.group + 1;  // exact: the excess is below 128 / 65536, a fraction's distance to 1 at least 1 / 128
   const CUtensorMapDataType type = dtype == QD_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const cuuint32_t estr[4] = {1, 1, 1, 1};
   auto map4 = [&](CUtensorMap* m, const void* base, const cuuint64_t* dims, const cuuint64_t* strides,
@@ -1361,10 +1289,10 @@ extern "C" int qd_paged_attn(const void* q, int64_t ldq, int dtype, int64_t toke
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
   };
   {  // a tile's rows are token-major, its KV head's query heads inner
-    const cuuint64_t dims[4] = {(cuuint64_t)head_dim, (cuuint64_t)a.group, (cuuint64_t)nkv_heads, (cuuint64_t)tokens};
-    const cuuint64_t strides[3] = {(cuuint64_t)head_dim * 2, (cuuint64_t)a.group * head_dim * 2, (cuuint64_t)ldq * 2};
-    const cuuint32_t box[4] = {64, (cuuint32_t)a.group, 1, (cuuint32_t)a.tpt}, box1[4] = {64, (cuuint32_t)a.group, 1, 1};
-    const cuuint32_t boxf[4] = {64, (cuuint32_t)a.group, 1, (cuuint32_t)(a.tpf > 0 ? a.tpf : 1)};
+    const cuuint64_t dims[4] = {(cuuint64_t)head_dim, (cuuint64_t)a.s.group, (cuuint64_t)nkv_heads, (cuuint64_t)tokens};
+    const cuuint64_t strides[3] = {(cuuint64_t)head_dim * 2, (cuuint64_t)a.s.group * head_dim * 2, (cuuint64_t)ldq * 2};
+    const cuuint32_t box[4] = {64, (cuuint32_t)a.s.group, 1, (cuuint32_t)a.s.tpt}, box1[4] = {64, (cuuint32_t)a.s.group, 1, 1};
+    const cuuint32_t boxf[4] = {64, (cuuint32_t)a.s.group, 1, (cuuint32_t)(a.s.tpf > 0 ? a.s.tpf : 1)};
     if (!map4(&a.tq, q, dims, strides, box) || !map4(&a.tqf, q, dims, strides, boxf) || !map4(&a.tq1, q, dims, strides, box1))
       return set_error(QD_ERR_CUDA, "cuTensorMapEncodeTiled failed for q");
   }
@@ -1384,10 +1312,6 @@ extern "C" int qd_paged_attn(const void* q, int64_t ldq, int dtype, int64_t toke
                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return set_error(QD_ERR_CUDA, "cuTensorMapEncodeTiled failed for the pools");
   }
-  int g = 2 * a.tpt;  // gcd(2 tpt, 128): the power of two in 2 tpt, up to 128
-  g = (g & -g) < kPgKeys ? (g & -g) : kPgKeys;
-  a.period = kPgKeys / g;
-  a.period_blocks = 2 * a.tpt / g;
   a.out = static_cast<char*>(out);
   a.lse = lse;
   a.ldo = ldo;
