@@ -173,7 +173,7 @@ def call(name: str, *args) -> None:
     if _RECORDING is not None:
         _RECORDING.append((name, list(args)))
         return
-    lib = load()
+    lib = _LIB or load()
     rc = getattr(lib, name)(*args)
     if rc != QD_OK:
         raise QDError(name, rc, lib.qd_last_error().decode(errors="replace"))

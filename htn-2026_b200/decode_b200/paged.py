@@ -9,9 +9,10 @@ ragged batch (all int32 on the device, so a captured graph follows what a later 
   page_table  [batch, max_pages]   position p is row p % page_size of page page_table[i, p // page_size]
 
 and pools [pages, KV heads, page_size, head_dim] of BF16 or FP16 (`new_pools`). One call serves single
-tokens, chunks of prompts and whole prompts together. Calls launch on the current torch CUDA stream and
-allocate nothing, so they are graph-capturable; device-side faults (a page outside the pool, a position
-past the tables) are flagged in the optional `err` word (lib.describe_device_error).
+tokens, chunks of prompts and whole prompts together. Calls launch on the current torch CUDA stream of the
+current device, on which every tensor has to be, and allocate nothing, so they are graph-capturable; device-side
+faults (a page outside the pool, a position past the tables) are flagged in the optional `err` word, int32
+(lib.describe_device_error).
 """
 
 from __future__ import annotations
@@ -25,6 +26,7 @@ from . import lib as L
 
 # the current stream's handle of a device, without the Stream object that torch.cuda.current_stream() makes
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
 I32, F32 = torch.int32, torch.float32
 TYPES = {torch.bfloat16: L.QD_BF16, torch.float16: L.QD_FP16}
 
@@ -42,15 +44,20 @@ def rope_table(positions: int, head_dim: int, theta: float, device):
     return angle.cos().float().to(device), angle.sin().float().to(device)
 
 
-def _check_batch(dtype, k_pages, v_pages, cu_tokens, kv_len, page_table):
-    """(pool shape, pool strides, batch, table row stride, table columns); each property is read once, since a
-    call for a few tokens takes the GPU less time than reading it twice takes the host."""
+def _check_batch(dev, dtype, k_pages, v_pages, cu_tokens, kv_len, page_table, err):
+    """(pool shape, pool strides, batch, table row stride, table columns), everything on the current device `dev`;
+    each property is read once, since a call for a few tokens takes the GPU less time than reading it twice takes
+    the host."""
     shape, strides, table = k_pages.shape, k_pages.stride(), page_table.shape
-    assert k_pages.dtype is dtype and v_pages.dtype is dtype and k_pages.is_cuda and v_pages.is_cuda
+    assert dev >= 0 and dev == _current_device(), f"tensors on device {dev} (-1: the host), which is not the current one"
+    assert k_pages.dtype is dtype and v_pages.dtype is dtype
+    assert k_pages.get_device() == dev and v_pages.get_device() == dev
     assert v_pages.shape == shape and v_pages.stride() == strides and len(shape) == 4
     assert strides[3] == 1 and strides[2] == shape[3], "rows of a page must be contiguous"
     assert cu_tokens.dtype is I32 and kv_len.dtype is I32 and page_table.dtype is I32
-    assert cu_tokens.is_cuda and kv_len.is_cuda and page_table.is_cuda
+    assert cu_tokens.get_device() == dev and kv_len.get_device() == dev and page_table.get_device() == dev
+    if err is not None:
+        assert err.dtype is I32 and err.get_device() == dev and err.numel() > 0
     ld_table, step = page_table.stride()
     assert cu_tokens.is_contiguous() and kv_len.is_contiguous() and (step == 1 or table[1] == 1)
     assert kv_len.shape == table[:1] and cu_tokens.shape == (table[0] + 1,)
@@ -74,20 +81,24 @@ def rope_append(qkv, cu_tokens, kv_len, page_table, nq: int, nkv: int, cos, sin,
     [tokens, nq * head_dim]; cos / sin fp32 [positions, pairs turned] (`rope_table`)."""
     dtype = qkv.dtype
     assert dtype in TYPES, f"expected BF16 or FP16 tensors, got {dtype}"
-    pool, ps, batch, ld_table, max_pages = _check_batch(dtype, k_pages, v_pages, cu_tokens, kv_len, page_table)
+    dev = qkv.get_device()
+    pool, ps, batch, ld_table, max_pages = _check_batch(dev, dtype, k_pages, v_pages, cu_tokens, kv_len, page_table, err)
     D, tokens = pool[3], qkv.shape[0]
-    assert qkv.is_cuda and q_out.is_cuda and q_out.dtype is dtype and pool[1] == nkv
+    assert q_out.get_device() == dev and q_out.dtype is dtype and pool[1] == nkv
     ldqkv, ldq = _rows(qkv, tokens, nq + 2 * nkv, D), _rows(q_out, tokens, nq, D)
     angles, ld = cos.shape, cos.stride()
     assert cos.dtype is F32 and sin.dtype is F32 and sin.shape == angles and sin.stride() == ld and ld[1] == 1
+    assert cos.get_device() == dev and sin.get_device() == dev
+    qn = kn = None
     if q_norm is not None or k_norm is not None:
-        for w in (q_norm, k_norm):
-            assert w is not None and w.dtype is dtype and w.shape == (D,) and w.is_contiguous()
-    L.call("qd_paged_rope_append", qkv.data_ptr(), ldqkv, TYPES[dtype], tokens, nq, nkv, D,
-           q_norm.data_ptr() if q_norm is not None else None, k_norm.data_ptr() if k_norm is not None else None, eps,
+        assert q_norm is not None and k_norm is not None and q_norm.shape == k_norm.shape == (D,)
+        assert q_norm.dtype is dtype and q_norm.get_device() == dev and q_norm.is_contiguous()
+        assert k_norm.dtype is dtype and k_norm.get_device() == dev and k_norm.is_contiguous()
+        qn, kn = q_norm.data_ptr(), k_norm.data_ptr()
+    L.call("qd_paged_rope_append", qkv.data_ptr(), ldqkv, TYPES[dtype], tokens, nq, nkv, D, qn, kn, eps,
            cos.data_ptr(), sin.data_ptr(), ld[0], angles[0], angles[1], cu_tokens.data_ptr(), kv_len.data_ptr(), batch,
            page_table.data_ptr(), ld_table, max_pages, q_out.data_ptr(), ldq, k_pages.data_ptr(), v_pages.data_ptr(),
-           pool[0], pool[2], ps[0], ps[1], None if err is None else err.data_ptr(), pdl, _raw_stream(qkv.get_device()))
+           pool[0], pool[2], ps[0], ps[1], None if err is None else err.data_ptr(), pdl, _raw_stream(dev))
     return q_out
 
 
@@ -110,15 +121,15 @@ class PagedAttention:
     def __call__(self, q, k_pages, v_pages, cu_tokens, kv_len, page_table, out, lse=None, scale: float | None = None,
                  err=None, pdl: bool = True):
         """q, out [tokens, nq, head_dim] or [tokens, nq * head_dim]; lse (optional) fp32 [tokens, nq]."""
-        nq, D, dtype = self.nq, self.head_dim, self.dtype
-        pool, ps, batch, ld_table, max_pages = _check_batch(dtype, k_pages, v_pages, cu_tokens, kv_len, page_table)
+        nq, D, dtype, dev = self.nq, self.head_dim, self.dtype, q.get_device()
+        pool, ps, batch, ld_table, max_pages = _check_batch(dev, dtype, k_pages, v_pages, cu_tokens, kv_len, page_table, err)
         tokens = q.shape[0]
-        assert q.dtype is dtype and out.dtype is dtype and q.is_cuda and out.is_cuda
+        assert q.dtype is dtype and out.dtype is dtype and out.get_device() == dev and self.scratch.get_device() == dev
         assert pool[1] == self.nkv and pool[3] == D
         ldq, ldo = _rows(q, tokens, nq, D), _rows(out, tokens, nq, D)
         lse_ptr, ld_lse = None, 0
         if lse is not None:
-            assert lse.dtype is F32 and lse.is_cuda and lse.shape == (tokens, nq)
+            assert lse.dtype is F32 and lse.get_device() == dev and lse.shape == (tokens, nq)
             ld_lse, step = lse.stride()
             assert step == 1 or nq == 1
             lse_ptr, ld_lse = lse.data_ptr(), max(ld_lse, nq) if tokens <= 1 else ld_lse
@@ -126,5 +137,5 @@ class PagedAttention:
                v_pages.data_ptr(), pool[0], pool[2], ps[0], ps[1], cu_tokens.data_ptr(), kv_len.data_ptr(), batch,
                page_table.data_ptr(), ld_table, max_pages, self.scale if scale is None else scale, out.data_ptr(), ldo,
                lse_ptr, ld_lse, self.grid, self.scratch.data_ptr(), self.scratch_bytes,
-               None if err is None else err.data_ptr(), pdl, _raw_stream(q.get_device()))
+               None if err is None else err.data_ptr(), pdl, _raw_stream(dev))
         return out

@@ -115,3 +115,91 @@ def test_rope_table_is_the_angles_in_64_bits():
     import math
 
     assert abs(float(cos[p, r]) - math.cos(angle)) < 1e-7 and abs(float(sin[p, r]) - math.sin(angle)) < 1e-7
+
+
+# ------------------------------------------------------------------------------------ devices
+class Stand:
+    """Stands for a tensor on GPU `dev` (-1: the host): what the wrappers ask one for, without a GPU."""
+
+    def __init__(self, shape, dtype, dev=0):
+        self.shape, self.dtype, self.dev = torch.Size(shape), dtype, dev
+
+    is_cuda = property(lambda self: self.dev >= 0)
+    device = property(lambda self: torch.device("cuda", self.dev) if self.dev >= 0 else torch.device("cpu"))
+
+    def get_device(self):
+        return self.dev
+
+    def stride(self):
+        out = [1]
+        for n in reversed(self.shape[1:]):
+            out.append(out[-1] * n)
+        return tuple(reversed(out))
+
+    def is_contiguous(self):
+        return True
+
+    def numel(self):
+        return self.shape.numel()
+
+    def data_ptr(self):
+        return P
+
+
+def _stands():
+    B, I, F = torch.bfloat16, torch.int32, torch.float32
+    batch = dict(cu_tokens=Stand((3,), I), kv_len=Stand((2,), I), page_table=Stand((2, 4), I), k_pages=Stand((9, 2, 16, 128), B),
+                 v_pages=Stand((9, 2, 16, 128), B), err=Stand((1,), I))
+    return {"append": dict(batch, qkv=Stand((5, 8 * 128), B), cos=Stand((50, 64), F), sin=Stand((50, 64), F), q_out=Stand((5, 4, 128), B),
+                           q_norm=Stand((128,), B), k_norm=Stand((128,), B)),
+            "attn": dict(batch, q=Stand((5, 4, 128), B), out=Stand((5, 4, 128), B), lse=Stand((5, 4), F), scratch=Stand((1 << 20,), torch.uint8)),
+            "sample": dict(logits=Stand((3, 100), B), u=Stand((3,), F), tok=Stand((3,), torch.int64), temperature=Stand((3,), F),
+                           top_k=Stand((3,), I), top_p=Stand((3,), F), min_p=Stand((3,), F), logprob=Stand((3,), F))}
+
+
+@pytest.mark.parametrize("op", ["append", "attn", "sample"])
+def test_wrappers_refuse_tensors_on_other_devices(op, monkeypatch):
+    """Every tensor of a call is on the current GPU: a host pointer, or one of another GPU, never reaches a kernel."""
+    from decode_b200 import paged
+    from decode_b200 import sample as S
+
+    handle = paged.PagedAttention(4, 2, 128, "cpu")
+    calls = []
+    current = [0]
+    for m in (paged, S):
+        monkeypatch.setattr(m, "_raw_stream", lambda dev: 0)
+        monkeypatch.setattr(m, "_current_device", lambda: current[0], raising=False)
+    monkeypatch.setattr(paged.L, "call", lambda name, *a: calls.append(name))
+
+    def run(t):
+        if op == "append":
+            return paged.rope_append(nq=4, nkv=2, **t)
+        if op == "attn":
+            handle.scratch = t.pop("scratch")
+            return handle(**t)
+        return S.sample(**t)
+
+    run(_stands()[op])
+    assert len(calls) == 1
+    for name in _stands()[op]:
+        for dev in (-1, 1):
+            t = _stands()[op]
+            t[name].dev = dev
+            with pytest.raises(AssertionError):
+                run(t)
+            assert len(calls) == 1, f"{name} on device {dev} reached the kernel"
+    current[0] = 1
+    with pytest.raises(AssertionError):
+        run(_stands()[op])
+    assert len(calls) == 1, "a launch goes to the current device"
+
+
+def test_wrappers_refuse_a_wrong_error_word(monkeypatch):
+    from decode_b200 import paged
+
+    monkeypatch.setattr(paged, "_raw_stream", lambda dev: 0)
+    monkeypatch.setattr(paged, "_current_device", lambda: 0, raising=False)
+    monkeypatch.setattr(paged.L, "call", lambda name, *a: pytest.fail("reached the kernel"))
+    for bad in (Stand((0,), torch.int32), Stand((1,), torch.uint8)):
+        with pytest.raises(AssertionError):
+            paged.rope_append(nq=4, nkv=2, **dict(_stands()["append"], err=bad))
