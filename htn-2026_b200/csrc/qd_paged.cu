@@ -166,11 +166,12 @@ int paged_batch_check(const char* what, int dtype, int64_t tokens, int nq, int n
     return set_error(QD_ERR_UNSUPPORTED, "%s: page_size %d (16, 32, 64 or 128)", what, page_size);
   if (nkv < 1 || nq < nkv || nq % nkv || nq / nkv > 128 || nq > 65536)
     return set_error(QD_ERR_ARG, "%s: %d query heads over %d KV heads", what, nq, nkv);
-  if (batch < 1 || max_pages < 1 || ld_table < max_pages || n_pages < 1 || n_pages > INT32_MAX || tokens < 0 ||
+  const int some = tokens > 0;  // without tokens nothing is read: no requests, and null arrays, are allowed
+  if (batch < some || max_pages < some || ld_table < max_pages || n_pages < 1 || n_pages > INT32_MAX || tokens < 0 ||
       tokens > INT32_MAX)
     return set_error(QD_ERR_ARG, "%s: batch %d, %d pages a row (stride %lld), %lld pages, %lld tokens", what, batch,
                      max_pages, (long long)ld_table, (long long)n_pages, (long long)tokens);
-  if (!k_pages || !v_pages || !aligned16(k_pages) || !aligned16(v_pages) || !cu || !kv_len || !table)
+  if (!aligned16(k_pages) || !aligned16(v_pages) || (some && (!k_pages || !v_pages || !cu || !kv_len || !table)))
     return set_error(QD_ERR_ARG, "%s: null or misaligned pool, or null batch array", what);
   // rows, heads and pages must not overlap: heads inside a page, or pages inside a head
   if (ps_head % 8 || ps_page % 8 || ps_head < (int64_t)page_size * head_dim || ps_page < (int64_t)page_size * head_dim)
@@ -198,7 +199,7 @@ extern "C" int qd_paged_rope_append(const void* qkv, int64_t ldqkv, int dtype, i
                                    ld_table, max_pages, err, &a.b);
   if (rc != QD_OK) return rc;
   const int heads = nq_heads + 2 * nkv_heads;
-  if (!qkv || !q_out || !aligned16(qkv) || !aligned16(q_out) || ldqkv % 8 || ldq % 8 ||
+  if ((tokens > 0 && (!qkv || !q_out)) || !aligned16(qkv) || !aligned16(q_out) || ldqkv % 8 || ldq % 8 ||
       ldqkv < (int64_t)heads * head_dim || ldq < (int64_t)nq_heads * head_dim)
     return set_error(QD_ERR_ARG, "paged append: qkv / q_out null, misaligned or with a bad stride (%lld, %lld)",
                      (long long)ldqkv, (long long)ldq);

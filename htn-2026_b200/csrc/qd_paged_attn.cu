@@ -1264,7 +1264,7 @@ extern "C" int qd_paged_attn(const void* q, int64_t ldq, int dtype, int64_t toke
                                    n_pages, page_size, ps_page, ps_head, cu_tokens, kv_len, batch, page_table,
                                    ld_table, max_pages, err, &a.b);
   if (rc != QD_OK) return rc;
-  if (!q || !out || !aligned16(q) || !aligned16(out) || ldq % 8 || ldo % 8 || ldq < (int64_t)nq_heads * head_dim ||
+  if ((tokens > 0 && (!q || !out)) || !aligned16(q) || !aligned16(out) || ldq % 8 || ldo % 8 || ldq < (int64_t)nq_heads * head_dim ||
       ldo < (int64_t)nq_heads * head_dim || (lse && ld_lse < nq_heads) || !(scale > 0.f))
     return set_error(QD_ERR_ARG, "paged attention: q / out / lse null, misaligned or with a bad stride (%lld, %lld, %lld), or scale %g",
                      (long long)ldq, (long long)ldo, (long long)ld_lse, (double)scale);

@@ -839,7 +839,7 @@ extern "C" int qd_sample(const void* logits, int dtype, int64_t ld, int64_t rows
                          const float* u, int64_t* tok, float* logprob, int pdl, cudaStream_t stream) {
   if (dtype != QD_BF16 && dtype != QD_FP16 && dtype != QD_FP32)
     return set_error(QD_ERR_UNSUPPORTED, "sample: element type %d", dtype);
-  if (!logits || !u || !tok) return set_error(QD_ERR_ARG, "sample: null logits, u or tok");
+  if (rows > 0 && (!logits || !u || !tok)) return set_error(QD_ERR_ARG, "sample: null logits, u or tok");
   if (rows < 0 || rows > INT32_MAX || vocab < 1 || ld < vocab)
     return set_error(QD_ERR_ARG, "sample: %lld rows of %lld logits, stride %lld", (long long)rows, (long long)vocab,
                      (long long)ld);

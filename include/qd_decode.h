@@ -426,7 +426,8 @@ int qd_prefill_attn_rows(const void* q, int64_t ldq, int batch, int64_t S, int64
  * needed one are never read). The pools k_pages / v_pages hold [n_pages][nkv_heads][page_size][head_dim]
  * elements of `dtype` (QD_BF16 or QD_FP16) at page stride ps_page and head stride ps_head (elements; for the
  * attention, whole groups of 8 rows apart), rows contiguous. head_dim is 64 or 128; page_size 16, 32, 64 or 128; nq_heads a multiple of nkv_heads; every
- * pointer 16-byte aligned and every stride of 16-bit elements a multiple of 8.
+ * pointer 16-byte aligned and every stride of 16-bit elements a multiple of 8. A call without tokens (batch may
+ * be 0 then, and arrays null) does nothing.
  *
  * qd_paged_rope_append: for every new token, from its row of qkv [tokens][(nq + 2 nkv) * head_dim] (row
  * stride ldqkv):  q_out[t][h] = rope(norm(q_h)) (row stride ldq),  K row = rope(norm(k_h)),  V row = v_h

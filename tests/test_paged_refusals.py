@@ -203,3 +203,42 @@ def test_wrappers_refuse_a_wrong_error_word(monkeypatch):
     for bad in (Stand((0,), torch.int32), Stand((1,), torch.uint8)):
         with pytest.raises(AssertionError):
             paged.rope_append(nq=4, nkv=2, **dict(_stands()["append"], err=bad))
+
+
+# ------------------------------------------------------------------------------------ nothing to do
+def test_empty_calls_may_have_null_arrays(lib):
+    """An empty tensor's pointer is null: a step in which no request has a token is not an error."""
+    assert lib.qd_paged_rope_append(*_append_args(tokens=0, qkv=None, q_out=None)) == 0
+    assert lib.qd_paged_rope_append(*_append_args(tokens=0, qkv=None, q_out=None, batch=0, kv=None, table=None, max_pages=0)) == 0
+    assert lib.qd_paged_attn(*_attn_args(tokens=0, q=None, out=None, lse=None)) == 0
+    assert lib.qd_paged_attn(*_attn_args(tokens=0, q=None, out=None, lse=None, batch=0, kv=None, table=None, max_pages=0)) == 0
+    assert lib.qd_sample(*_sample_args(rows=0, logits=None, u=None, tok=None)) == 0
+    # what does not depend on the number of tokens is refused all the same
+    for change in ({"dim": 96}, {"page": 24}, {"nkv": 7}, {"batch": -1}, {"max_pages": -1}):
+        assert lib.qd_paged_rope_append(*_append_args(tokens=0, **change)) != 0
+        assert lib.qd_paged_attn(*_attn_args(tokens=0, **change)) != 0
+    assert lib.qd_sample(*_sample_args(rows=0, vocab=0)) == 1
+
+
+def test_wrappers_take_empty_batches(lib, monkeypatch):
+    """No tokens (with and without requests) and no rows, through the wrappers: nothing is launched, so no GPU is
+    needed."""
+    from decode_b200 import paged
+    from decode_b200 import sample as S
+
+    class Empty(Stand):
+        def data_ptr(self):
+            return P if self.numel() else 0
+
+    for m in (paged, S):
+        monkeypatch.setattr(m, "_raw_stream", lambda dev: 0)
+        monkeypatch.setattr(m, "_current_device", lambda: 0)
+    handle = paged.PagedAttention(4, 2, 128, "cpu")
+    handle.scratch = Stand((handle.scratch_bytes,), torch.uint8)
+    B, I, F = torch.bfloat16, torch.int32, torch.float32
+    for n in (0, 2):
+        batch = dict(cu_tokens=Empty((n + 1,), I), kv_len=Empty((n,), I), page_table=Empty((n, 3), I),
+                     k_pages=Empty((9, 2, 16, 128), B), v_pages=Empty((9, 2, 16, 128), B))
+        paged.rope_append(Empty((0, 1024), B), nq=4, nkv=2, cos=Empty((50, 64), F), sin=Empty((50, 64), F), q_out=Empty((0, 4, 128), B), **batch)
+        handle(Empty((0, 512), B), out=Empty((0, 512), B), lse=Empty((0, 4), F), **batch)
+    S.sample(Empty((0, 100), B), Empty((0,), F), Empty((0,), torch.int64), top_k=Empty((0,), I))
