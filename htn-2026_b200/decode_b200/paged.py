@@ -71,7 +71,7 @@ def _rows(t, tokens: int, heads: int, D: int) -> int:
         assert t.shape == (tokens, heads, D) and strides[2] == 1 and (strides[1] == D or heads == 1)
     else:
         assert t.shape == (tokens, heads * D) and strides[1] == 1
-    return max(strides[0], heads * D) if tokens <= 1 else strides[0]
+    return heads * D if tokens <= 1 else strides[0]
 
 
 def rope_append(qkv, cu_tokens, kv_len, page_table, nq: int, nkv: int, cos, sin, q_out, k_pages, v_pages, q_norm=None,

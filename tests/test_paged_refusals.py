@@ -242,3 +242,26 @@ def test_wrappers_take_empty_batches(lib, monkeypatch):
         paged.rope_append(Empty((0, 1024), B), nq=4, nkv=2, cos=Empty((50, 64), F), sin=Empty((50, 64), F), q_out=Empty((0, 4, 128), B), **batch)
         handle(Empty((0, 512), B), out=Empty((0, 512), B), lse=Empty((0, 4), F), **batch)
     S.sample(Empty((0, 100), B), Empty((0,), F), Empty((0,), torch.int64), top_k=Empty((0,), I))
+
+
+def test_a_single_row_has_no_row_stride(lib, monkeypatch):
+    """One token's row may be a view of any buffer: the stride to a next row, which there is not, is not checked."""
+    from decode_b200 import paged
+
+    class View(Stand):
+        def stride(self):
+            return (self.shape[-1] * self.shape[-2] + 3 if len(self.shape) == 3 else self.shape[-1] + 3,) + super().stride()[1:]
+
+    monkeypatch.setattr(paged, "_raw_stream", lambda dev: 0)
+    monkeypatch.setattr(paged, "_current_device", lambda: 0)
+    seen = []
+    monkeypatch.setattr(paged.L, "call", lambda name, *a: seen.append(a))
+    handle = paged.PagedAttention.__new__(paged.PagedAttention)
+    handle.nq, handle.nkv, handle.head_dim, handle.dtype, handle.grid, handle.scratch_bytes, handle.scale = 4, 2, 128, torch.bfloat16, 1, 0, 0.1
+    handle.scratch = Stand((1,), torch.uint8)
+    t = _stands()
+    handle(**{**{k: v for k, v in t["attn"].items() if k != "scratch"}, "q": View((1, 4, 128), torch.bfloat16),
+              "out": View((1, 512), torch.bfloat16), "lse": Stand((1, 4), torch.float32)})
+    assert seen[-1][1] == 512 and seen[-1][21] == 512
+    paged.rope_append(nq=4, nkv=2, **{**t["append"], "qkv": View((1, 1024), torch.bfloat16), "q_out": View((1, 4, 128), torch.bfloat16)})
+    assert seen[-1][1] == 1024
