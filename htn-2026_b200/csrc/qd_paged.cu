@@ -174,7 +174,9 @@ int paged_batch_check(const char* what, int dtype, int64_t tokens, int nq, int n
   if (!aligned16(k_pages) || !aligned16(v_pages) || (some && (!k_pages || !v_pages || !cu || !kv_len || !table)))
     return set_error(QD_ERR_ARG, "%s: null or misaligned pool, or null batch array", what);
   // rows, heads and pages must not overlap: heads inside a page, or pages inside a head
-  if (ps_head % 8 || ps_page % 8 || ps_head < (int64_t)page_size * head_dim || ps_page < (int64_t)page_size * head_dim)
+  const int64_t rows = (int64_t)page_size * head_dim;
+  if (ps_head % 8 || ps_page % 8 || ps_head < rows || ps_page < rows ||
+      ((ps_page - rows) / ps_head < nkv - 1 && (ps_head - rows) / ps_page < n_pages - 1))
     return set_error(QD_ERR_ARG, "%s: page stride %lld, head stride %lld", what, (long long)ps_page,
                      (long long)ps_head);
   *b = PagedBatch{cu, kv_len, table, ld_table, tokens, n_pages, ps_page, ps_head, batch, max_pages, page_size,

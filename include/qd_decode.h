@@ -425,7 +425,8 @@ int qd_prefill_attn_rows(const void* q, int64_t ldq, int batch, int64_t S, int64
  * page_table[i * ld_table + p / page_size] (device int32, max_pages entries a row; entries past the last
  * needed one are never read). The pools k_pages / v_pages hold [n_pages][nkv_heads][page_size][head_dim]
  * elements of `dtype` (QD_BF16 or QD_FP16) at page stride ps_page and head stride ps_head (elements; for the
- * attention, whole groups of 8 rows apart), rows contiguous. head_dim is 64 or 128; page_size 16, 32, 64 or 128; nq_heads a multiple of nkv_heads; every
+ * attention, whole groups of 8 rows apart), rows contiguous, heads inside a page or pages inside a head without
+ * overlap. head_dim is 64 or 128; page_size 16, 32, 64 or 128; nq_heads a multiple of nkv_heads; every
  * pointer 16-byte aligned and every stride of 16-bit elements a multiple of 8. A call without tokens (batch may
  * be 0 then, and arrays null) does nothing.
  *

@@ -265,3 +265,15 @@ def test_a_single_row_has_no_row_stride(lib, monkeypatch):
     assert seen[-1][1] == 512 and seen[-1][21] == 512
     paged.rope_append(nq=4, nkv=2, **{**t["append"], "qkv": View((1, 1024), torch.bfloat16), "q_out": View((1, 4, 128), torch.bfloat16)})
     assert seen[-1][1] == 1024
+
+
+@pytest.mark.parametrize("change,code", [
+    ({"ps_page": 16 * 128}, 1), ({"ps_page": 8 * 16 * 128 - 8}, 1), ({"ps_head": 9 * 16 * 128}, 1),
+    ({"ps_page": 16 * 128, "ps_head": 9 * 16 * 128 - 1024}, 1), ({"ps_page": 16 * 128, "ps_head": 1 << 62, "pages": (1 << 31) - 1}, 0),
+    ({"ps_page": 16 * 128, "ps_head": 9 * 16 * 128}, 0), ({"ps_page": 2 * 8 * 16 * 128}, 0), ({"ps_page": 8 * 16 * 128, "pages": 1}, 0),
+    ({"ps_page": 16 * 128, "nkv": 1, "nq": 4}, 0), ({"ps_page": 1 << 62}, 0)])
+def test_pools_whose_rows_overlap_are_refused(lib, change, code):
+    """Heads lie inside a page, or pages inside a head; two rows in one place would be written by two tokens at once."""
+    for call, args in ((lib.qd_paged_rope_append, _append_args), (lib.qd_paged_attn, _attn_args)):
+        for tokens in ((4,) if code else (0,)):  # (an accepted call must not launch here)
+            assert call(*args(**{**change, "tokens": tokens})) == code, change
