@@ -131,6 +131,13 @@ __device__ __forceinline__ float pg_ex2(float x) {
   return r;
 }
 
+// A row's end: 1 / sum of its exponentials, and its log-sum-exp. A sum of 0 is a row that saw no key; a sum that is
+// not a number stays one.
+__device__ __forceinline__ float pg_inverse(float l) { return l == 0.f ? 0.f : 1.0f / l; }
+__device__ __forceinline__ float pg_lse(float m, float l) {
+  return l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.69314718055994531f;
+}
+
 template <int N>
 struct Const {
   static constexpr int value = N;
@@ -217,7 +224,7 @@ __device__ __forceinline__ void pg_join_few(const PagedAttnArgs& a, const PgSeg&
       for (int q = 0; q < kPieces; ++q)
 #pragma unroll
         for (int i = 0; i < kRows; ++i)
-          if (q0 + q < g.nc && ml[q][i].y > 0.f) {  // a piece in which the row saw no key counts for nothing
+          if (q0 + q < g.nc && ml[q][i].y != 0.f) {  // a piece in which the row saw no key counts for nothing
             const float mn = fmaxf(M[i], ml[q][i].x), fa = exp2f(M[i] - mn), fb = exp2f(ml[q][i].x - mn);
             M[i] = mn;
             L[i] = L[i] * fa + ml[q][i].y * fb;
@@ -231,12 +238,12 @@ __device__ __forceinline__ void pg_join_few(const PagedAttnArgs& a, const PgSeg&
     for (int i = 0; i < kRows; ++i) {
       const int row = r0 + kAt * i;
       if (row < rows) {
-        const float inv = L[i] > 0.f ? 1.0f / L[i] : 0.f;
+        const float inv = pg_inverse(L[i]);
         const int tok = (row * a.inv_group) >> 16, t2 = g.row0 + tok, h2 = g.head * a.s.group + row - tok * a.s.group;
         *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + t2 * a.ldo + (int64_t)h2 * D + 4 * c4) =
             make_uint2(Elem<T>::pack(acc[i].x * inv, acc[i].y * inv), Elem<T>::pack(acc[i].z * inv, acc[i].w * inv));
         if (c4 == 0 && a.lse)
-          a.lse[t2 * a.ld_lse + h2] = L[i] > 0.f ? (M[i] + __log2f(L[i])) * 0.69314718055994531f : -INFINITY;
+          a.lse[t2 * a.ld_lse + h2] = pg_lse(M[i], L[i]);
       }
     }
   }
@@ -886,11 +893,11 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
         const int tok = (lane * a.inv_group) >> 16, hq = g.head * a.s.group + lane - tok * a.s.group;
         row_at = (g.row0 + tok) * a.ldo + (int64_t)hq * D;
         if (g.whole) {
-          const float inv = L > 0.f ? 1.0f / L : 0.f;
+          const float inv = pg_inverse(L);
           fa *= inv;
           fb *= inv;
           if (wg == 0 && a.lse)
-            a.lse[(g.row0 + tok) * a.ld_lse + hq] = L > 0.f ? (M + __log2f(L)) * 0.69314718055994531f : -INFINITY;
+            a.lse[(g.row0 + tok) * a.ld_lse + hq] = pg_lse(M, L);
         } else if (wg == 0) {
           __stcg(part_m(g.slot, lane), make_float2(M, L));
         }
@@ -1086,7 +1093,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
           *reinterpret_cast<uint4*>(to) = v;
         }
       };
-      const float norm = !g.whole ? 1.f : l > 0.f ? 1.0f / l : 0.f;  // a piece's rows stay as they are
+      const float norm = !g.whole ? 1.f : pg_inverse(l);  // a piece's rows stay as they are
       fa *= norm;
       fb *= norm;
       if (!idle) {
@@ -1162,7 +1169,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
               for (int i = 0; i < kI; ++i)
 #pragma unroll
                 for (int q = 0; q < kP; ++q)
-                  if (q0 + q < g.nc && p[i][q].y > 0.f) {  // a piece in which the row saw no key counts for nothing
+                  if (q0 + q < g.nc && p[i][q].y != 0.f) {  // a piece in which the row saw no key counts for nothing
                     const float mn = fmaxf(M[i], p[i][q].x), wa = exp2f(M[i] - mn), wb = exp2f(p[i][q].x - mn);
                     M[i] = mn;
                     L[i] = L[i] * wa + p[i][q].y * wb;
@@ -1175,7 +1182,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
 #pragma unroll
             for (int i = 0; i < kI; ++i) {
               if (e0 + 128 * i >= items) break;
-              const float inv = L[i] > 0.f ? 1.0f / L[i] : 0.f;
+              const float inv = pg_inverse(L[i]);
               uint32_t w[4];
 #pragma unroll
               for (int d = 0; d < 4; ++d) w[d] = Elem<T>::pack(acc[i][2 * d] * inv, acc[i][2 * d + 1] * inv);
@@ -1184,7 +1191,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
               if (c8[i] == 0 && a.lse) {
                 const int rt = (row[i] * a.inv_group) >> 16;
                 a.lse[(g.row0 + t0 + rt) * a.ld_lse + g.head * a.s.group + row[i] - rt * a.s.group] =
-                    L[i] > 0.f ? (M[i] + __log2f(L[i])) * 0.69314718055994531f : -INFINITY;
+                    pg_lse(M[i], L[i]);
               }
             }
           }
@@ -1199,7 +1206,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
         store_rows();
         if (!ok) break;
         if (g.whole && r < rows && a.lse)
-          a.lse[tok * a.ld_lse + head] = l > 0.f ? (m_used + __log2f(l)) * 0.69314718055994531f : -INFINITY;
+          a.lse[tok * a.ld_lse + head] = pg_lse(m_used, l);
       }
       fence_proxy_async_smem();  // the slot's next contents come by TMA
       meet();

@@ -453,7 +453,9 @@ int qd_paged_rope_append(const void* qkv, int64_t ldqkv, int dtype, int64_t toke
  * (lse fp32, row stride ld_lse, may be null). A token that sees no key (kv_len smaller than the number of
  * new tokens) gets zeros and lse = -inf. One call serves single tokens, chunks of a prompt and whole
  * prompts side by side. Scores, softmax statistics and sums are fp32; probabilities are rounded to `dtype`
- * before the product with V. Cache rows at and past kv_len are never used, whatever they hold. A request
+ * before the product with V. Cache rows at and past kv_len are never used, whatever they hold. A row that sees a
+ * score that is not a number is NaN, and so is its lse; a key that it does not see does not reach it, but a V row
+ * of its own request that is not finite may reach the rows before it in the same chunk (0 x inf). A request
  * that outgrows its table row (kv_len > max_pages * page_size) is cut to it and flags QD_DEVERR_PAGE, as
  * does a page outside the pool (its keys then read as zeros). qd_paged_attn_plan gives the grid
  * (grid_hint <= 0: one CTA per SM) and the size of the scratch (32-byte aligned), which depend on neither

@@ -331,3 +331,48 @@ def test_append_then_attention_on_another_stream():
         b.k[i], b.v[i] = torch.stack([kc[a, :, r] for a, r in at]), torch.stack([vc[a, :, r] for a, r in at])
     ref, _, tol, _ = R.attention(b)
     assert bool(((out.double().cpu() - ref).abs() <= tol).all())
+
+
+def _with_nan_key(spec, at, dim, dtype, what):
+    """Requests whose key (or value) at position `at` is not a number, in one KV head."""
+    b = R.Batch(spec, 8, 2, dim, 32, dtype, seed=31, device=DEV)
+    for i, (_, kv) in enumerate(spec):
+        if at < kv:
+            (b.k if what == "key" else b.v)[i][at, 1] = math.nan
+            (b.k_pages if what == "key" else b.v_pages)[int(b.table[i, at // 32]), 1, at % 32] = math.nan
+    return b
+
+
+@pytest.mark.parametrize("dim,dtype", [(128, BF16), (64, FP16)])
+@pytest.mark.parametrize("spec", [[(1, 9000)], [(3, 9000)], [(1, 700), (4, 300), (70, 4000)], [(200, 5000), (1, 60)], [(8, 70)]])
+def test_attention_shows_a_key_that_is_not_a_number(spec, dim, dtype):
+    """A row that sees a NaN score is NaN, its log-sum-exp too, wherever its request is cut into pieces; the rows of
+    other heads, and those that do not see the key, are as they are without it."""
+    at = 50
+    b = _with_nan_key(spec, at, dim, dtype, "key")
+    out, lse = _attend(b)
+    out, lse = out.cpu(), lse.cpu()
+    clean = R.Batch(spec, 8, 2, dim, 32, dtype, seed=31)
+    ref, ref_lse, tol, lse_tol = R.attention(clean)
+    for i, t, pos in b.rows():
+        sees = at <= pos and at < b.spec[i][1]
+        for h in range(8):
+            if sees and h >= 4:
+                assert bool(out[t, h].isnan().all()) and bool(lse[t, h].isnan()), (i, t, h, float(lse[t, h]))
+            else:
+                assert bool(((out[t, h].double() - ref[t, h]).abs() <= tol[t, h]).all()), (i, t, h)
+                assert float((lse[t, h].double() - ref_lse[t, h]).abs()) <= float(lse_tol[t, h])
+
+
+@pytest.mark.parametrize("spec", [[(1, 9000)], [(3, 9000)], [(60, 5000)]])
+def test_attention_of_queries_that_are_not_numbers(spec):
+    """A NaN query: all its scores are NaN, in every piece."""
+    b = R.Batch(spec, 8, 2, 128, 64, seed=5, device=DEV)
+    b.q[0, 3] = math.nan
+    out, lse = _attend(b)
+    assert bool(out[0, 3].isnan().all()) and bool(lse[0, 3].isnan())
+    other = torch.ones((b.tokens, 8), dtype=torch.bool)
+    other[0, 3] = False
+    ref, ref_lse, tol, lse_tol = R.attention(b)
+    assert bool(((out.cpu().double() - ref).abs() <= tol)[other].all())
+    assert bool(((lse.cpu().double() - ref_lse).abs() <= lse_tol)[other].all())
