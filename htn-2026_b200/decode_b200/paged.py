@@ -106,7 +106,8 @@ class PagedAttention:
     """Causal attention of every new token over its request's pages (qd_paged_attn), for one head layout.
 
     Holds the scratch, whose size depends on neither the batch nor the lengths; two calls that share an
-    object must not overlap on the GPU."""
+    object must not overlap on the GPU. After a device error other than a page outside the pool (`err`),
+    `reset` makes it ready again."""
 
     def __init__(self, nq: int, nkv: int, head_dim: int, device, dtype=torch.bfloat16, grid: int = 0):
         assert dtype in TYPES, f"expected BF16 or FP16, got {dtype}"
@@ -117,6 +118,11 @@ class PagedAttention:
         self.scratch = torch.zeros((nbytes.value,), dtype=torch.uint8, device=device)
         self.scratch_bytes = nbytes.value
         self.scale = 1.0 / math.sqrt(head_dim)
+
+    def reset(self) -> None:
+        """Zeroes the counts of finished pieces, which a call that ended early leaves behind: later calls would
+        join pieces too early, or never."""
+        self.scratch[:8 * self.grid].zero_()
 
     def __call__(self, q, k_pages, v_pages, cu_tokens, kv_len, page_table, out, lse=None, scale: float | None = None,
                  err=None, pdl: bool = True):

@@ -459,7 +459,8 @@ int qd_paged_rope_append(const void* qkv, int64_t ldqkv, int dtype, int64_t toke
  * that outgrows its table row (kv_len > max_pages * page_size) is cut to it and flags QD_DEVERR_PAGE, as
  * does a page outside the pool (its keys then read as zeros). qd_paged_attn_plan gives the grid
  * (grid_hint <= 0: one CTA per SM) and the size of the scratch (32-byte aligned), which depend on neither
- * batch nor lengths. */
+ * batch nor lengths. The scratch is zero before its first call; each call leaves it ready for the next, unless a
+ * bounded wait ran out (a bit of *err other than QD_DEVERR_PAGE): its first 8 * grid bytes are zeroed again then. */
 int qd_paged_attn_plan(int nq_heads, int nkv_heads, int head_dim, int grid_hint, int* grid, int64_t* scratch_bytes);
 int qd_paged_attn(const void* q, int64_t ldq, int dtype, int64_t tokens, int nq_heads, int nkv_heads, int head_dim,
                   const void* k_pages, const void* v_pages, int64_t n_pages, int page_size, int64_t ps_page,

@@ -376,3 +376,17 @@ def test_attention_of_queries_that_are_not_numbers(spec):
     ref, ref_lse, tol, lse_tol = R.attention(b)
     assert bool(((out.cpu().double() - ref).abs() <= tol)[other].all())
     assert bool(((lse.cpu().double() - ref_lse).abs() <= lse_tol)[other].all())
+
+
+def test_attention_scratch_is_made_ready_again():
+    """A call that ends early (a bounded wait that runs out, flagged in `err`) leaves counts in the scratch, as
+    they are set here; after reset() the object answers as a new one does."""
+    P = _paged()
+    b = R.Batch([(1, 2900), (70, 1333), (1, 5)], 8, 2, 128, 32, seed=1, device=DEV)
+    handle = P.PagedAttention(8, 2, 128, DEV)
+    first, _ = _attend(b, handle)
+    handle.scratch[:8 * handle.grid] = 1
+    handle.reset()
+    out, lse = _attend(b, handle)
+    _check(b, out, lse)
+    assert torch.equal(out, first)
