@@ -35,6 +35,7 @@ class Request:
     top_p: float
     min_p: float
     rng: random.Random
+    u: float = 0.0                     # the number that its next token is drawn with
     cached: int = 0                    # positions in the cache
     pages: list[int] = field(default_factory=list)
     out: list[int] = field(default_factory=list)
@@ -82,7 +83,8 @@ class PagedServer:
             raise ValueError(f"request of {len(prompt) + max_new_tokens} positions needs {need} pages, "
                              f"there are {self.k_pages.shape[1]}")
         i, self.next_id = self.next_id, self.next_id + 1
-        self.requests[i] = Request(list(prompt), max_new_tokens, temperature, top_k, top_p, min_p, random.Random(seed))
+        rng = random.Random(seed)
+        self.requests[i] = Request(list(prompt), max_new_tokens, temperature, top_k, top_p, min_p, rng, rng.random())
         self.waiting.append(i)
         return i
 
@@ -123,7 +125,7 @@ class PagedServer:
                             dtype=torch.int32).to(dev)
         n = len(batch)
         logits = self.forward(ids, ints[:n + 1], ints[n + 1:2 * n + 1], ints[2 * n + 1:].view(n, width))
-        draw = torch.tensor([[r.temperature, r.top_p, r.min_p, r.rng.random()] for r in reqs], dtype=torch.float32)
+        draw = torch.tensor([[r.temperature, r.top_p, r.min_p, r.u] for r in reqs], dtype=torch.float32)
         t, top_p, min_p, u = draw.t().contiguous().to(dev).unbind(0)
         top_k = torch.tensor([r.top_k for r in reqs], dtype=torch.int32).to(dev)
         sample(logits, u, self.tok[:n], temperature=t, top_k=top_k, top_p=top_p, min_p=min_p,
@@ -135,6 +137,7 @@ class PagedServer:
         for (i, _), r, length, token, lp in zip(batch, reqs, kv, tok, logprob):
             r.cached = length
             if not r.pending():  # the whole prompt (or the last token) is in: this row's draw is its next token
+                r.u = r.rng.random()  # (rows in the middle of a prompt draw too, but use up no number)
                 r.out.append(token)
                 r.logprobs.append(lp)
                 drawn[i] = token

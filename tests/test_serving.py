@@ -1,0 +1,62 @@
+"""PagedServer's planning on the CPU: which tokens, numbers and pages each step takes. The forward and the draw are
+replaced (a draw here is the row's number), so no GPU is needed."""
+
+import types
+
+import pytest
+import torch
+
+VOCAB = 1000
+
+
+@pytest.fixture()
+def server(monkeypatch):
+    from decode_b200 import serving
+
+    seen = []  # (u of the rows) of every step
+
+    def draw(logits, u, tok, temperature, top_k, top_p, min_p, logprob, vocab):
+        assert vocab == VOCAB and logits.shape[0] == u.shape[0] == tok.shape[0]
+        seen.append([round(float(x), 6) for x in u])
+        tok.copy_((u * VOCAB).long())
+        logprob.zero_()
+
+    monkeypatch.setattr(serving, "sample", draw)
+
+    def make(**kw):
+        eng = types.SimpleNamespace(device=torch.device("cpu"), head_dim=64, nq=2, nkv=1, hidden=8, inter=8, n_layers=1, theta=1e4,
+                                    vocab=VOCAB, eps=1e-6)
+        srv = serving.PagedServer(eng, **{**dict(pages=64, page_size=16, max_tokens=32, max_requests=4), **kw})
+        srv.seen, srv.fed = seen, {}
+
+        def forward(ids, cu, kv_len, table):
+            srv.fed[len(srv.fed)] = ids.tolist()
+            return torch.zeros((cu.shape[0] - 1, VOCAB))
+
+        srv.forward = forward
+        return srv
+
+    return make
+
+
+def _answers(srv):
+    list(srv.run())
+    return {i: r.out for i, r in srv.requests.items()}
+
+
+def test_a_seed_gives_one_answer_whatever_the_load(server):
+    """The numbers of an answer do not depend on how its prompt was cut into steps, nor on the requests beside it."""
+    kw = dict(temperature=1.0, seed=7)
+    alone = server(max_tokens=64)
+    i = alone.add(range(60), 5, **kw)
+    ref = _answers(alone)[i]
+    assert len(set(ref)) == 5
+    for max_tokens in (7, 16, 59, 60):
+        srv = server(max_tokens=max_tokens)
+        i = srv.add(range(60), 5, **kw)
+        assert _answers(srv)[i] == ref, max_tokens
+    srv = server(max_tokens=20)
+    others = [srv.add(range(n), 9, temperature=1.0, seed=n) for n in (30, 2)]
+    i = srv.add(range(60), 5, **kw)
+    got = _answers(srv)
+    assert got[i] == ref and got[others[0]] != got[others[1]]
