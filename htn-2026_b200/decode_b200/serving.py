@@ -74,8 +74,9 @@ class PagedServer:
 
     # ------------------------------------------------------------------ requests
     def add(self, prompt, max_new_tokens: int, temperature: float = 0.0, top_k: int = 0, top_p: float = 1.0,
-            min_p: float = 0.0, seed: int = 0) -> int:
-        """Queues a request; its number. temperature 0 takes the most likely token."""
+            min_p: float = 0.0, seed: int | None = None) -> int:
+        """Queues a request; its number. temperature 0 takes the most likely token. The seed fixes the answer's
+        random numbers; without one they are the request number's."""
         if not prompt or max_new_tokens < 1:
             raise ValueError("a request needs a prompt and at least one new token")
         need = -(-(len(prompt) + max_new_tokens) // self.page_size)
@@ -83,7 +84,7 @@ class PagedServer:
             raise ValueError(f"request of {len(prompt) + max_new_tokens} positions needs {need} pages, "
                              f"there are {self.k_pages.shape[1]}")
         i, self.next_id = self.next_id, self.next_id + 1
-        rng = random.Random(seed)
+        rng = random.Random(i if seed is None else seed)
         self.requests[i] = Request(list(prompt), max_new_tokens, temperature, top_k, top_p, min_p, rng, rng.random())
         self.waiting.append(i)
         return i

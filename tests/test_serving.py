@@ -60,3 +60,17 @@ def test_a_seed_gives_one_answer_whatever_the_load(server):
     i = srv.add(range(60), 5, **kw)
     got = _answers(srv)
     assert got[i] == ref and got[others[0]] != got[others[1]]
+
+
+def test_requests_without_a_seed_draw_numbers_of_their_own(server):
+    srv = server()
+    ids = [srv.add([1, 2, 3], 6, temperature=1.0) for _ in range(4)]
+    got = _answers(srv)
+    assert len({tuple(got[i]) for i in ids}) == 4
+    again = server()
+    ids2 = [again.add([1, 2, 3], 6, temperature=1.0) for _ in range(4)]
+    assert [_answers(again)[i] for i in ids2] == [got[i] for i in ids], "a server's answers repeat"
+    seeded = server()
+    zero = [seeded.add([1, 2, 3], 6, temperature=1.0, seed=0) for _ in range(2)]
+    got = _answers(seeded)
+    assert got[zero[0]] == got[zero[1]]
