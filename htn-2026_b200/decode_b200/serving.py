@@ -52,6 +52,8 @@ class PagedServer:
 
     def __init__(self, eng, pages: int, page_size: int = 64, max_tokens: int = 2048, max_requests: int = 64):
         self.eng, self.page_size, self.max_tokens, self.max_requests = eng, page_size, max_tokens, max_requests
+        if min(pages, max_tokens, max_requests) < 1:
+            raise ValueError(f"a server of {pages} pages, {max_tokens} tokens a step and {max_requests} requests")
         dev, D, nq, nkv, H = eng.device, eng.head_dim, eng.nq, eng.nkv, eng.hidden
         shape = (eng.n_layers, pages, nkv, page_size, D)
         self.k_pages = torch.zeros(shape, dtype=BF16, device=dev)
@@ -77,15 +79,20 @@ class PagedServer:
             min_p: float = 0.0, seed: int | None = None) -> int:
         """Queues a request; its number. temperature 0 takes the most likely token. The seed fixes the answer's
         random numbers; without one they are the request number's."""
+        prompt = [int(t) for t in prompt]
         if not prompt or max_new_tokens < 1:
             raise ValueError("a request needs a prompt and at least one new token")
+        if min(prompt) < 0 or max(prompt) >= self.eng.vocab:
+            raise ValueError(f"token ids from {min(prompt)} to {max(prompt)}, the vocabulary has {self.eng.vocab}")
+        if not -2 ** 31 <= top_k < 2 ** 31:
+            raise ValueError(f"top_k {top_k} does not fit 32 bits")
         need = -(-(len(prompt) + max_new_tokens) // self.page_size)
         if need > self.k_pages.shape[1]:
             raise ValueError(f"request of {len(prompt) + max_new_tokens} positions needs {need} pages, "
                              f"there are {self.k_pages.shape[1]}")
         i, self.next_id = self.next_id, self.next_id + 1
         rng = random.Random(i if seed is None else seed)
-        self.requests[i] = Request(list(prompt), max_new_tokens, temperature, top_k, top_p, min_p, rng, rng.random())
+        self.requests[i] = Request(prompt, max_new_tokens, temperature, top_k, top_p, min_p, rng, rng.random())
         self.waiting.append(i)
         return i
 

@@ -74,3 +74,26 @@ def test_requests_without_a_seed_draw_numbers_of_their_own(server):
     zero = [seeded.add([1, 2, 3], 6, temperature=1.0, seed=0) for _ in range(2)]
     got = _answers(seeded)
     assert got[zero[0]] == got[zero[1]]
+
+
+@pytest.mark.parametrize("bad", [dict(prompt=[1, VOCAB]), dict(prompt=[-1]), dict(prompt=[3, 2 ** 70]), dict(prompt=[]),
+                                 dict(max_new_tokens=0), dict(top_k=2 ** 31), dict(top_k=-2 ** 31 - 1)])
+def test_add_refuses_what_would_stop_a_step(server, bad):
+    srv = server()
+    good = srv.add([1, 2], 3)
+    with pytest.raises(ValueError):
+        srv.add(**{**dict(prompt=[1], max_new_tokens=2), **bad})
+    assert len(_answers(srv)[good]) == 3 and sorted(srv.free) == list(range(64)) and list(srv.requests) == [good]
+
+
+def test_add_takes_any_sequence_of_ids(server):
+    srv = server()
+    a, b = srv.add(torch.arange(5), 2), srv.add((3, 4), 2, top_k=2 ** 31 - 1)
+    assert srv.requests[a].prompt == [0, 1, 2, 3, 4]
+    assert {i: len(o) for i, o in _answers(srv).items()} == {a: 2, b: 2}
+
+
+@pytest.mark.parametrize("bad", [dict(max_tokens=0), dict(max_requests=0), dict(pages=0)])
+def test_a_server_that_could_never_step_is_refused(server, bad):
+    with pytest.raises(ValueError):
+        server(**bad)
