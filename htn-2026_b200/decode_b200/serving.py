@@ -139,7 +139,9 @@ class PagedServer:
         sample(logits, u, self.tok[:n], temperature=t, top_k=top_k, top_p=top_p, min_p=min_p,
                logprob=self.logprob[:n], vocab=self.eng.vocab)
         tok, logprob, err = self.tok[:n].tolist(), self.logprob[:n].tolist(), int(self.err.item())
-        if err:
+        if err:  # nothing of this step counts: it can be taken again
+            self.err.zero_()
+            self.attn.reset()
             raise RuntimeError(f"serving step reported a device error: {L.describe_device_error(err)}")
         drawn = {}
         for (i, _), r, length, token, lp in zip(batch, reqs, kv, tok, logprob):

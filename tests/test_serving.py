@@ -97,3 +97,30 @@ def test_add_takes_any_sequence_of_ids(server):
 def test_a_server_that_could_never_step_is_refused(server, bad):
     with pytest.raises(ValueError):
         server(**bad)
+
+
+def test_a_device_error_stops_one_step_only(server):
+    """A flagged step raises; the word is cleared, the attention's scratch made ready, and the step can be taken again."""
+    ref = server()
+    ids = [ref.add(range(40), 4, temperature=1.0), ref.add([5], 6, temperature=1.0)]
+    want = _answers(ref)
+    srv = server()
+    assert [srv.add(range(40), 4, temperature=1.0), srv.add([5], 6, temperature=1.0)] == ids
+    forward, fail = srv.forward, [False, True, False, False, True, False]
+
+    def flagged(*a):
+        if fail and fail.pop(0):
+            srv.err.fill_(16)
+            srv.attn.scratch[:8 * srv.attn.grid] = 1
+        return forward(*a)
+
+    srv.forward = flagged
+    raised = 0
+    while srv.waiting or srv.active:
+        try:
+            srv.step()
+        except RuntimeError as e:
+            assert "position" in str(e)
+            raised += 1
+            assert raised <= 2 and int(srv.err) == 0 and int(srv.attn.scratch.max()) == 0
+    assert raised == 2 and {i: r.out for i, r in srv.requests.items()} == want
