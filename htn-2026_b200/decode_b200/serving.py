@@ -40,6 +40,7 @@ class Request:
     pages: list[int] = field(default_factory=list)
     out: list[int] = field(default_factory=list)
     logprobs: list[float] = field(default_factory=list)
+    failed: bool = False               # ended because a row of logits had nothing to draw
 
     def pending(self) -> list[int]:
         """Tokens that are not in the cache yet."""
@@ -118,7 +119,8 @@ class PagedServer:
 
     # ------------------------------------------------------------------ a step
     def step(self) -> dict[int, int]:
-        """One forward; {request: drawn token} for those whose last pending token was in it."""
+        """One forward; {request: drawn token} for those whose last pending token was in it. Token -1: its logits
+        had nothing above -inf, and the request has ended (`failed`)."""
         self._admit()
         batch = self._plan()
         if not batch:
@@ -147,15 +149,21 @@ class PagedServer:
         for (i, _), r, length, token, lp in zip(batch, reqs, kv, tok, logprob):
             r.cached = length
             if not r.pending():  # the whole prompt (or the last token) is in: this row's draw is its next token
-                r.u = r.rng.random()  # (rows in the middle of a prompt draw too, but use up no number)
-                r.out.append(token)
-                r.logprobs.append(lp)
                 drawn[i] = token
-                if len(r.out) == r.max_new_tokens:
-                    self.free += r.pages
-                    r.pages = []
-                    self.active.remove(i)
+                r.failed = token < 0
+                if not r.failed:
+                    r.u = r.rng.random()  # (rows in the middle of a prompt draw too, but use up no number)
+                    r.out.append(token)
+                    r.logprobs.append(lp)
+                if r.failed or len(r.out) == r.max_new_tokens:
+                    self._end(i)
         return drawn
+
+    def _end(self, i: int) -> None:
+        r = self.requests[i]
+        self.free += r.pages
+        r.pages = []
+        self.active.remove(i)
 
     def run(self):
         """Steps until every request is done; yields each step's {request: token}."""

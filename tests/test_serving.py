@@ -124,3 +124,28 @@ def test_a_device_error_stops_one_step_only(server):
             raised += 1
             assert raised <= 2 and int(srv.err) == 0 and int(srv.attn.scratch.max()) == 0
     assert raised == 2 and {i: r.out for i, r in srv.requests.items()} == want
+
+
+def test_a_row_with_nothing_to_draw_ends_its_request_only(server, monkeypatch):
+    """qd_sample's token -1 (no logit above -inf): that request ends, its pages are free, the others go on."""
+    from decode_b200 import serving
+
+    ref = server()
+    keep, kw = ref.add([5] * 20, 6, temperature=1.0, seed=3), dict(temperature=1.0, seed=4)
+    want = _answers(ref)[keep]
+    srv = server()
+    assert srv.add([5] * 20, 6, temperature=1.0, seed=3) == keep
+    bad = srv.add([9] * 30, 8, **kw)
+    inner = serving.sample
+
+    def draw(logits, u, tok, **k):
+        inner(logits, u, tok, **k)
+        if len(srv.requests[bad].out) == 2 and bad in srv.active:
+            tok[[i for i, _ in srv._plan()].index(bad)] = -1
+
+    monkeypatch.setattr(serving, "sample", draw)
+    steps = list(srv.run())
+    assert srv.requests[keep].out == want and not srv.requests[keep].failed
+    assert srv.requests[bad].failed and len(srv.requests[bad].out) == 2 and min(srv.requests[bad].out) >= 0
+    assert [s[bad] for s in steps if bad in s][-1] == -1
+    assert sorted(srv.free) == list(range(64)) and not srv.active
