@@ -97,6 +97,17 @@ class PagedServer:
         self.waiting.append(i)
         return i
 
+    def cancel(self, i: int) -> Request:
+        """Ends request i wherever it is (waiting, in its prompt, answering, done) and hands it back; its pages are
+        free and the server forgets it. For answers that end before max_new_tokens, and for done ones, which are
+        kept in `requests` until then."""
+        r = self.requests[i]
+        if i in self.waiting:
+            self.waiting.remove(i)
+        elif i in self.active:
+            self._end(i)
+        return self.requests.pop(i)
+
     def _admit(self) -> None:
         """A waiting request joins when the pages of its whole answer are free, so no step runs out of them."""
         while self.waiting and len(self.active) < self.max_requests:

@@ -149,3 +149,25 @@ def test_a_row_with_nothing_to_draw_ends_its_request_only(server, monkeypatch):
     assert srv.requests[bad].failed and len(srv.requests[bad].out) == 2 and min(srv.requests[bad].out) >= 0
     assert [s[bad] for s in steps if bad in s][-1] == -1
     assert sorted(srv.free) == list(range(64)) and not srv.active
+
+
+def test_cancel_frees_and_forgets(server):
+    """Waiting, in the middle of its prompt, answering or done: the request is handed back and nothing of it stays."""
+    ref = server()
+    keep = ref.add([5] * 20, 9, temperature=1.0, seed=3)
+    want = _answers(ref)[keep]
+    srv = server(max_requests=3, max_tokens=24)
+    assert srv.add([5] * 20, 9, temperature=1.0, seed=3) == keep
+    done, answering, middle, waiting = srv.add([1], 1), srv.add([2], 9), srv.add([3] * 200, 2), srv.add([4], 2)
+    for _ in range(3):
+        srv.step()
+    assert waiting in srv.waiting and {answering, middle} <= set(srv.active) and done not in srv.active
+    assert 0 < srv.requests[middle].cached < 200
+    for i, tokens in ((done, 1), (answering, 3), (middle, 0), (waiting, 0)):
+        assert len(srv.cancel(i).out) == tokens and i not in srv.requests
+        with pytest.raises(KeyError):
+            srv.cancel(i)
+    list(srv.run())
+    assert srv.requests[keep].out == want and sorted(srv.free) == list(range(64))
+    srv.cancel(keep)
+    assert not srv.requests and not srv.active and not srv.waiting
