@@ -42,9 +42,14 @@ class Request:
     logprobs: list[float] = field(default_factory=list)
     failed: bool = False               # ended because a row of logits had nothing to draw
 
-    def pending(self) -> list[int]:
+    def left(self) -> int:
         """Tokens that are not in the cache yet."""
-        return (self.prompt + self.out)[self.cached:]
+        return len(self.prompt) + len(self.out) - self.cached
+
+    def take(self, n: int) -> list[int]:
+        """The first n of them: of the prompt, then of the answer."""
+        at, end, p = self.cached, self.cached + n, len(self.prompt)
+        return self.prompt[at:end] + self.out[max(at - p, 0):max(end - p, 0)]
 
 
 class PagedServer:
@@ -121,11 +126,11 @@ class PagedServer:
     def _plan(self) -> list[tuple[int, list[int]]]:
         """(request, tokens of this step): the decoding requests' tokens, then chunks of prompts."""
         left, batch = self.max_tokens, []
-        for i in sorted(self.active, key=lambda i: len(self.requests[i].pending()) > 1):
-            tokens = self.requests[i].pending()[:left]
-            if tokens:
-                batch.append((i, tokens))
-                left -= len(tokens)
+        for i in sorted(self.active, key=lambda i: self.requests[i].left() > 1):
+            n = min(self.requests[i].left(), left)
+            if n:
+                batch.append((i, self.requests[i].take(n)))
+                left -= n
         return batch
 
     # ------------------------------------------------------------------ a step
@@ -159,7 +164,7 @@ class PagedServer:
         drawn = {}
         for (i, _), r, length, token, lp in zip(batch, reqs, kv, tok, logprob):
             r.cached = length
-            if not r.pending():  # the whole prompt (or the last token) is in: this row's draw is its next token
+            if not r.left():  # the whole prompt (or the last token) is in: this row's draw is its next token
                 drawn[i] = token
                 r.failed = token < 0
                 if not r.failed:

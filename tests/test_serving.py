@@ -171,3 +171,34 @@ def test_cancel_frees_and_forgets(server):
     assert srv.requests[keep].out == want and sorted(srv.free) == list(range(64))
     srv.cancel(keep)
     assert not srv.requests and not srv.active and not srv.waiting
+
+
+def test_a_step_copies_the_tokens_it_takes(server):
+    """A decode step after a long prompt does not copy the prompt; a chunk copies the chunk."""
+    class Watched(list):
+        copied = 0
+
+        def __getitem__(self, at):
+            got = list.__getitem__(self, at)
+            Watched.copied += len(got) if isinstance(at, slice) else 1
+            return got
+
+        def __iter__(self):
+            Watched.copied += len(self)
+            return list.__iter__(self)
+
+        def __add__(self, other):
+            Watched.copied += len(self) + len(other)
+            return list.__add__(self, other)
+
+    n = 500
+    srv = server(max_tokens=100)
+    i = srv.add(range(n), 20)
+    r = srv.requests[i]
+    r.prompt, r.out = Watched(r.prompt), Watched()
+    for step in range(25):
+        Watched.copied = 0
+        srv.step()
+        assert Watched.copied <= (100 if step < 5 else 1), (step, Watched.copied)
+    assert sum(srv.fed.values(), [])[:n] == list(range(n)) and len(r.out) == 20
+    assert sum(srv.fed.values(), [])[n:] == r.out[:19]
