@@ -715,8 +715,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
       sh.warp_b[tid] = tied ? sh.part_eq[tid] : 0;
     }
   } else {
-    // halves of up to 2^20 a logit: 32 bits hold the sums of a lane's 512 vectors (2^18 logits over 128 or
-    // more warps), and of the warp in 64
+    // halves of up to 2^20 a logit: 32 bits hold the sums of a lane's 16 vectors (at most 512 a warp, see the
+    // cluster's choice), 2^27, and 64 the warp's
     uint32_t hi = 0, lo = 0, eq = 0;
     if (thr == -INFINITY && floor_d == -INFINITY)  // every token that is not masked
       each([&](const float* v, int) {
@@ -778,7 +778,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     seen = __shfl_sync(0xffffffffu, eq_before, q);
     const uint4* const from = part + q * vecs;
     const int base = (rank * kSampleWarps + q) * a.per_warp;
-    // its vectors, 32 to a warp (vecs <= 512), then the warp in whose vectors the sum passes, its lane, and that
+    // its vectors, 32 to a warp (at most 512), then the warp in whose vectors the sum passes, its lane, and that
     // lane's logits
     const int i = warp * 32 + lane;
     uint32_t hi = 0, lo = 0, el = 0;
@@ -852,10 +852,16 @@ extern "C" int qd_sample(const void* logits, int dtype, int64_t ld, int64_t rows
   // The cluster: the fewest CTAs of which two fit an SM (so that one's loads and barriers hide behind the
   // other's arithmetic) and which fill the SMs, but at most one for 4096 logits. Measured on rows of 151,936 BF16
   // logits, with clusters of 4 / 8: 8 rows with top-p 29 / 22 us, 64 rows 50 / 65 us, 256 unfiltered 65 / 88 us.
+  // However the choice ends, a warp has at most 512 vectors of 16 bytes, one per thread of its CTA, which the last
+  // walk and the sums of halves rely on.
+  constexpr int kFit = 110 * 1024, kFew = 8192, kMost = 16 * kSampleThreads;  // kMost: bytes of a warp's logits
+  static_assert(kSampleMaxVocab / (kSampleMaxCluster * kSampleWarps) * 4 <= kMost, "the largest cluster");
+  static_assert(kFew / kSampleWarps * 4 <= kMost, "few logits a CTA");
+  static_assert((kFit - kSampleShared) / kSampleWarps + 8 * 4 <= kMost, "two CTAs an SM");
   const int size = dtype == QD_FP32 ? 4 : 2;
   int cluster = 1;
-  while (cluster < kSampleMaxCluster && vocab >= (int64_t)8192 * cluster &&
-         (rows * cluster < host_sm_count() || kSampleShared + vocab * size / cluster > 110 * 1024))
+  while (cluster < kSampleMaxCluster && vocab >= (int64_t)kFew * cluster &&
+         (rows * cluster < host_sm_count() || kSampleShared + vocab * size / cluster > kFit))
     cluster *= 2;
   SampleArgs a = {logits, ld, vocab, temperature, top_k, top_p, min_p, u, tok, logprob, 0, 0};
   const int parts = cluster * kSampleWarps;
