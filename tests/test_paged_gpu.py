@@ -390,3 +390,16 @@ def test_attention_scratch_is_made_ready_again():
     out, lse = _attend(b, handle)
     _check(b, out, lse)
     assert torch.equal(out, first)
+
+
+@pytest.mark.parametrize("n", [385, 1000])
+def test_attention_more_requests_than_threads(n):
+    """Each thread of the start sums the work of several requests, some of them empty."""
+    g = torch.Generator().manual_seed(n)
+    r = lambda lo, hi: int(torch.randint(lo, hi, (1,), generator=g))  # noqa: E731
+    spec = [(r(0, 3) if i % 50 else r(30, 90), r(90, 200)) for i in range(n)]
+    b = R.Batch(spec, 4, 2, 64, 16, FP16, seed=n, device=DEV)
+    err = _err()
+    out, lse = _attend(b, err=err)
+    _check(b, out, lse)
+    assert int(err.item()) == 0
