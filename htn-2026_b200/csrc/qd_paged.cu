@@ -29,8 +29,9 @@ struct AppendArgs {
 constexpr int kAppendThreads = 128;
 
 // kUnits: groups of heads of one token that a warp takes, all their loads in flight before the first is used.
-// 13,808 prompt tokens of 48 heads of 128 take 70 us, 5.2 TB/s over the 364 MB that have to move (a copy
-// reaches 6.5); 64 single tokens 3.2 us and one 2.4 us, of which the launch is most.
+// 13,808 prompt tokens of 48 heads of 128 take 71 us, 5.1 TB/s over the 364 MB that have to move (a copy
+// reaches 6.5); 64 single tokens 3.0 us and one 2.2 us in a graph, of which the launch is most (a call takes the
+// host 11.8).
 template <typename T, int D, int kUnits>
 __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __grid_constant__ AppendArgs a) {
   constexpr int kLanes = D / 16, kHeads = 32 / kLanes;  // lanes per head, heads per unit
@@ -227,7 +228,7 @@ extern "C" int qd_paged_rope_append(const void* qkv, int64_t ldqkv, int dtype, i
   a.rot_half = rot_half;
   a.eps = eps;
   // Two groups of heads a warp once there are warps enough to fill the SMs without: 64 tokens of 48 heads (768
-  // groups of 4) take 2.7 us one by one and 3.1 in twos, 256 tokens 4.5 and 3.6, 13,808 tokens 85 and 70.
+  // groups of 4) take 3.0 us one by one and 3.3 in twos, 256 tokens 6.7 and 4.2, 13,808 tokens 85 and 71.
   const int group = 512 / head_dim;
   const bool two = tokens * ((heads + group - 1) / group) > 2048;
   const int per = (heads + group * (two ? 2 : 1) - 1) / (group * (two ? 2 : 1));

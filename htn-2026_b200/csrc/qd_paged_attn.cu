@@ -11,7 +11,9 @@
 // keeps both busy too: A takes its even blocks, B its odd ones, and A's warps add O_B to O_A at the end, each
 // with its own maximum. The maximum only moves when a row's grows by more than 2^8 (then the warp rescales
 // O_x in tensor memory): O / l does not depend on which maximum is used, and 2^8 leaves the fp32 sums and the
-// 16-bit P far from overflow.
+// 16-bit P far from overflow. P is rounded to the 16-bit element type because a 16-bit product of the tensor cores
+// takes both operands in it; l sums the unrounded P. Against 64 bits the results are off by 0.0017 to 0.0024 of
+// their size in BF16 and 0.00028 in FP16, where their own last rounding alone gives 0.0017 and 0.00021.
 //
 // Few rows. With at most 16 rows (a single token of up to 16 heads a group, or a few tokens) most of a
 // 128-row tile would be exponentials of nothing, so the products are turned round: S^T = K Q^T (M = 128
@@ -30,10 +32,13 @@
 // joins them in the order of the keys, so results repeat bit for bit. Every CTA finds its place on the line
 // from cu_tokens and kv_len itself: no planning launch, and no length is needed on the host.
 //
-// Measured, 32 query and 8 KV heads of 128 in BF16: 8 single tokens over up to 41 k keys 184 us (HBM: 6.3 TB/s); 64
-// single tokens over 1 to 1.5 k keys 72 us (4.7 TB/s: each CTA's start and end); one token over 1 k keys 12.6 us
-// (latency); 2048 tokens after 8192 keys 342 to 368 us (0.50 to 0.54 of the BF16 peak: a pair's block of 128 keys takes
-// some 4000 cycles, 2048 of them products, since each tile's softmax and products wait for one another).
+// Measured, 32 query and 8 KV heads of 128 in BF16: 8 single tokens over up to 41 k keys 183 us (HBM: 6.3 TB/s); 64
+// single tokens over 1 to 1.5 k keys 72 us (4.7 TB/s: each CTA's start and end); one token over 1 k keys 12.3 us in a
+// graph, 14.5 with the keys not in L2 (latency; a call takes the host 11.9); 2048 tokens after 8192 keys 340 to 368 us
+// (0.50 to 0.54 of the BF16 peak: a pair's block of 128 keys takes some 4000 cycles, 2048 of them products, since each
+// tile's softmax and products wait for one another). Heads of 64 in FP16, 14 over 2: the 64 single tokens 33 us, the 8
+// long ones 51. At 168 registers a thread the instances spill: 168 bytes stored and 456 loaded in the code of a
+// thread with heads of 128 (156 and 428 with pages of 16 rows), 120 and 356 with heads of 64.
 #include <algorithm>
 #include <climits>
 
@@ -842,7 +847,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
         for (int c = 0; c < kC; ++c) {
           const float p = pg_ex2(fmaf(__uint_as_float(sv[c]), a.scale_log2, __shfl_sync(0xffffffffu, nm, c)));
           l[c] += p;
-          const uint32_t w = Elem<T>::pack(p, 0.f);
+          const uint32_t w = Elem<T>::pack(p, 0.f);  // rounded: the operand's type
           *reinterpret_cast<uint16_t*>(p_row + c * 128 + ((chunk ^ (c & 7)) << 4)) = (uint16_t)w;
         }
         tc_fence_before();
@@ -1020,7 +1025,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
           const float nm = m_used == -INFINITY ? 0.f : -m_used;  // a row that has seen no key yet: P = 0
           float ls[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int c = 0; c < 64; ++c) {  // P pair c = keys 2c, 2c + 1, packed in place over the scores
+          for (int c = 0; c < 64; ++c) {  // P pair c = keys 2c, 2c + 1, rounded (the operand's type), over the scores
             const float p0 = pg_ex2(fmaf(__uint_as_float(sv[2 * c]), a.scale_log2, nm));
             const float p1 = pg_ex2(fmaf(__uint_as_float(sv[2 * c + 1]), a.scale_log2, nm));
             ls[(2 * c) & 3] += p0;

@@ -43,10 +43,9 @@ __device__ __forceinline__ void umma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, u
       "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u));
 }
 // The two products without the (all-zero) lane mask operand, for any kind::f16 types, issued by one elected
-// lane (elect_one), from the low words of the descriptors (umma_desc_lo; the strides sbo of A and B are constants): what an instruction
-// takes from ordinary registers is moved to uniform ones first, and those moves bound the issue. Measured with
-// one warp issuing 128 x 128 x 16 products back to back: 137 cycles each with the mask, 65 without (the tensor
-// core itself takes 64).
+// lane (elect_one), from the low words of the descriptors (umma_desc_lo; the strides sbo of A and B are
+// constants), so that few operands are in registers. Measured with one warp issuing 128 x 128 x 16 products back
+// to back: 137 cycles each with the mask, 65 without (the tensor core itself takes 64); the cause is not known.
 constexpr uint32_t umma_desc_hi(uint32_t sbo) { return (sbo >> 4) | (1u << 14) | (2u << 29); }
 __device__ __forceinline__ uint32_t umma_desc_lo(uint32_t saddr, uint32_t lbo = 16) {
   return ((saddr >> 4) & 0x3FFFu) | ((lbo >> 4) << 16);
