@@ -8,6 +8,15 @@
 // exchange), and of the rest past 2 * rot_half two neighbouring chunks. The mean of squares is a butterfly
 // over the group. A warp takes 4 heads (8 of head_dim 64) of one token, or twice as many, so the request
 // lookup, the page and the cos / sin rows are the warp's.
+//
+// Into 8-bit pages the rotated K row and the V row go as E4M3 values and one power of two for the row: the least
+// 2^e with |x| <= 448 * 2^e, from the exponent and the mantissa of the row's largest finite |x| (a butterfly over
+// the head's lanes). A power of two because E4M3 has an exponent of its own: a scale between two powers would save
+// less than a bit of its range and none of its precision, and with a power of two what is read back is exact in
+// BF16 and in FP16 (e from -15 to 7 keeps the least and the largest code in FP16's range).
+#include <cuda_fp8.h>
+
+#include <cfloat>
 #include <climits>
 
 #include "qd_host.h"
@@ -24,7 +33,23 @@ struct AppendArgs {
   int64_t ldqkv, ldq, ld_cs, n_pos;
   int rot_half;
   float eps;
+  uint8_t *k_scale, *v_scale;  // 8-bit pages: the rows' exponents + 127, [page][KV head][row of the page]
+  int64_t ss_page, ss_head;
 };
+
+// The exponent of a row whose largest finite |x| is `most`: the least e with most <= 448 * 2^e (448 = 1.75 * 2^8),
+// within what FP16 can hold all codes of. A row of zeros has the least one.
+__device__ __forceinline__ int row_exponent(float most) {
+  const uint32_t u = __float_as_uint(most);
+  const int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return min(max(e, kHeldLeastExp), kHeldMostExp);
+}
+// Two values over the row's power of two as E4M3: beyond +-448 (where the exponent was cut) +-448, infinities as NaN.
+__device__ __forceinline__ uint32_t held_pair(float a, float b, float inv) {
+  const float nan = __uint_as_float(0x7fffffffu);
+  return __nv_cvt_float2_to_fp8x2(make_float2(fabsf(a) <= FLT_MAX ? a * inv : nan, fabsf(b) <= FLT_MAX ? b * inv : nan),
+                                  __NV_SATFINITE, __NV_E4M3);
+}
 
 constexpr int kAppendThreads = 128;
 
@@ -32,7 +57,7 @@ constexpr int kAppendThreads = 128;
 // 13,808 prompt tokens of 48 heads of 128 take 71 us, 5.1 TB/s over the 364 MB that have to move (a copy
 // reaches 6.5); 64 single tokens 3.0 us and one 2.2 us in a graph, of which the launch is most (a call takes the
 // host 11.8).
-template <typename T, int D, int kUnits>
+template <typename T, int D, int kUnits, bool kHeld>
 __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __grid_constant__ AppendArgs a) {
   constexpr int kLanes = D / 16, kHeads = 32 / kLanes;  // lanes per head, heads per unit
   grid_dep_wait();
@@ -72,14 +97,16 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __gr
     if (lane == 0) flag_error(a.b.err, QD_DEVERR_POS);
     return;
   }
-  int64_t page_at = -1;  // of this position's row of KV head 0
+  int64_t page_at = -1, scale_at = 0;  // of this position's row of KV head 0
   if (h0 + (kUnits - 1) * kHeads >= a.b.nq) {
     const int entry = pos >> a.b.page_shift;
     const int page = entry < a.b.max_pages ? ld_i32(a.b.table + i * a.b.ld_table + entry) : -1;
-    if (page >= 0 && page < a.b.n_pages)
+    if (page >= 0 && page < a.b.n_pages) {
       page_at = page * a.b.ps_page + (int64_t)(pos & (a.b.page_size - 1)) * D;
-    else if (c == 0)
+      if constexpr (kHeld) scale_at = page * a.ss_page + (pos & (a.b.page_size - 1));
+    } else if (c == 0) {
       flag_error(a.b.err, QD_DEVERR_PAGE);
+    }
   }
   float cs[8], sn[8];
   if (turned) {
@@ -96,20 +123,24 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __gr
   for (int unit = 0; unit < kUnits; ++unit) {
     const int h = h0 + unit * kHeads;
     const bool is_v = h >= a.b.nq + a.b.nkv;
+    const int kv_head = h - a.b.nq - (is_v ? a.b.nkv : 0);
     char* dst = nullptr;
     if (h < a.b.nq)
       dst = a.q_out + (t * a.ldq + (int64_t)h * D) * 2;
     else if (page_at >= 0)
-      dst = (is_v ? a.v_pages : a.k_pages) + (page_at + (h - a.b.nq - (is_v ? a.b.nkv : 0)) * a.b.ps_head) * 2;
+      dst = (is_v ? a.v_pages : a.k_pages) + (page_at + kv_head * a.b.ps_head) * (kHeld ? 1 : 2);
     float x[16];
+    auto unpack = [&]() {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float2 p = Elem<T>::unpack((&u0[unit].x)[k]), q = Elem<T>::unpack((&u1[unit].x)[k]);
-      x[2 * k] = p.x;
-      x[2 * k + 1] = p.y;
-      x[8 + 2 * k] = q.x;
-      x[8 + 2 * k + 1] = q.y;
-    }
+      for (int k = 0; k < 4; ++k) {
+        const float2 p = Elem<T>::unpack((&u0[unit].x)[k]), q = Elem<T>::unpack((&u1[unit].x)[k]);
+        x[2 * k] = p.x;
+        x[2 * k + 1] = p.y;
+        x[8 + 2 * k] = q.x;
+        x[8 + 2 * k + 1] = q.y;
+      }
+    };
+    unpack();
     if (a.q_norm) {  // every lane takes part in the sum; V heads do not use it
       float sq = 0.f;
 #pragma unroll
@@ -136,6 +167,27 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __gr
         x[8 + k] = q * cs[k] + p * sn[k];
       }
     }
+    if constexpr (kHeld) {
+      if (is_v) unpack();  // V goes in as it was
+      float most = 0.f;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) most = fmaxf(most, fabsf(x[k]) <= FLT_MAX ? fabsf(x[k]) : 0.f);
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      if (h >= heads || !dst) continue;
+      if (h >= a.b.nq) {
+        const int e = row_exponent(most);
+        const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          w[k] = held_pair(x[4 * k], x[4 * k + 1], inv) | held_pair(x[4 * k + 2], x[4 * k + 3], inv) << 16;
+        *reinterpret_cast<uint2*>(dst + e0) = make_uint2(w[0], w[1]);
+        *reinterpret_cast<uint2*>(dst + e1) = make_uint2(w[2], w[3]);
+        if (c == 0) (is_v ? a.v_scale : a.k_scale)[scale_at + kv_head * a.ss_head] = (uint8_t)(e + 127);
+        continue;
+      }
+    }
     if (h >= heads || !dst) continue;
     uint4 o0 = u0[unit], o1 = u1[unit];  // V goes into the page as it is
     if (!is_v) {
@@ -151,8 +203,16 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __gr
 }
 
 template <typename T, int D>
-static const void* append_kernel(bool two) {
-  return two ? (const void*)paged_append_kernel<T, D, 2> : (const void*)paged_append_kernel<T, D, 1>;
+static const void* append_kernel(bool two, bool held) {
+  return held  ? (two ? (const void*)paged_append_kernel<T, D, 2, true> : (const void*)paged_append_kernel<T, D, 1, true>)
+         : two ? (const void*)paged_append_kernel<T, D, 2, false>
+               : (const void*)paged_append_kernel<T, D, 1, false>;
+}
+
+// Pages of `rows` elements of a head must not overlap: heads lie inside a page, or pages inside a head.
+static bool pools_overlap(int64_t rows, int64_t ps_page, int64_t ps_head, int64_t n_pages, int nkv) {
+  return ps_head < rows || ps_page < rows ||
+         ((ps_page - rows) / ps_head < nkv - 1 && (ps_head - rows) / ps_page < n_pages - 1);
 }
 
 int paged_batch_check(const char* what, int dtype, int64_t tokens, int nq, int nkv, int head_dim, const void* k_pages,
@@ -174,10 +234,7 @@ int paged_batch_check(const char* what, int dtype, int64_t tokens, int nq, int n
                      max_pages, (long long)ld_table, (long long)n_pages, (long long)tokens);
   if (!aligned16(k_pages) || !aligned16(v_pages) || (some && (!k_pages || !v_pages || !cu || !kv_len || !table)))
     return set_error(QD_ERR_ARG, "%s: null or misaligned pool, or null batch array", what);
-  // rows, heads and pages must not overlap: heads inside a page, or pages inside a head
-  const int64_t rows = (int64_t)page_size * head_dim;
-  if (ps_head % 8 || ps_page % 8 || ps_head < rows || ps_page < rows ||
-      ((ps_page - rows) / ps_head < nkv - 1 && (ps_head - rows) / ps_page < n_pages - 1))
+  if (ps_head % 8 || ps_page % 8 || pools_overlap((int64_t)page_size * head_dim, ps_page, ps_head, n_pages, nkv))
     return set_error(QD_ERR_ARG, "%s: page stride %lld, head stride %lld", what, (long long)ps_page,
                      (long long)ps_head);
   *b = PagedBatch{cu, kv_len, table, ld_table, tokens, n_pages, ps_page, ps_head, batch, max_pages, page_size,
@@ -185,32 +242,43 @@ int paged_batch_check(const char* what, int dtype, int64_t tokens, int nq, int n
   return QD_OK;
 }
 
+int paged_batch_check8(const char* what, int dtype, int64_t tokens, int nq, int nkv, int head_dim, const void* k_pages,
+                       const void* v_pages, const void* k_scale, const void* v_scale, int64_t n_pages, int page_size,
+                       int64_t ps_page, int64_t ps_head, int64_t ss_page, int64_t ss_head, const int32_t* cu,
+                       const int32_t* kv_len, int batch, const int32_t* table, int64_t ld_table, int max_pages, int* err,
+                       PagedBatch* b) {
+  const int rc = paged_batch_check(what, dtype, tokens, nq, nkv, head_dim, k_pages, v_pages, n_pages, page_size, ps_page,
+                                   ps_head, cu, kv_len, batch, table, ld_table, max_pages, err, b);
+  if (rc != QD_OK) return rc;
+  if (!aligned16(k_scale) || !aligned16(v_scale) || (tokens > 0 && (!k_scale || !v_scale)))
+    return set_error(QD_ERR_ARG, "%s: null or misaligned scales", what);
+  // whole 16-byte pieces: what a copy of a page takes
+  if (ps_head % 16 || ps_page % 16 || ss_head % 16 || ss_page % 16 || pools_overlap(page_size, ss_page, ss_head, n_pages, nkv))
+    return set_error(QD_ERR_ARG, "%s: page strides %lld, %lld, head strides %lld, %lld (values, scales)", what,
+                     (long long)ps_page, (long long)ss_page, (long long)ps_head, (long long)ss_head);
+  return QD_OK;
+}
+
 }  // namespace qd
 
 using namespace qd;
 
-extern "C" int qd_paged_rope_append(const void* qkv, int64_t ldqkv, int dtype, int64_t tokens, int nq_heads,
-                                    int nkv_heads, int head_dim, const void* q_norm, const void* k_norm, float eps,
-                                    const float* cos, const float* sin, int64_t ld_cs, int64_t n_pos, int rot_half,
-                                    const int32_t* cu_tokens, const int32_t* kv_len, int batch,
-                                    const int32_t* page_table, int64_t ld_table, int max_pages, void* q_out,
-                                    int64_t ldq, void* k_pages, void* v_pages, int64_t n_pages, int page_size,
-                                    int64_t ps_page, int64_t ps_head, int* err, int pdl, cudaStream_t stream) {
-  AppendArgs a = {};
-  const int rc = paged_batch_check("paged append", dtype, tokens, nq_heads, nkv_heads, head_dim, k_pages, v_pages,
-                                   n_pages, page_size, ps_page, ps_head, cu_tokens, kv_len, batch, page_table,
-                                   ld_table, max_pages, err, &a.b);
-  if (rc != QD_OK) return rc;
+// What both entry points check and launch: 16-bit pages without scales, 8-bit pages with.
+static int launch_append(const char* what, const void* qkv, int64_t ldqkv, int dtype, int64_t tokens, int nq_heads,
+                         int nkv_heads, int head_dim, const void* q_norm, const void* k_norm, float eps,
+                         const float* cos, const float* sin, int64_t ld_cs, int64_t n_pos, int rot_half, void* q_out,
+                         int64_t ldq, void* k_pages, void* v_pages, int pdl, cudaStream_t stream, bool held,
+                         AppendArgs& a) {
   const int heads = nq_heads + 2 * nkv_heads;
   if ((tokens > 0 && (!qkv || !q_out)) || !aligned16(qkv) || !aligned16(q_out) || ldqkv % 8 || ldq % 8 ||
       ldqkv < (int64_t)heads * head_dim || ldq < (int64_t)nq_heads * head_dim)
-    return set_error(QD_ERR_ARG, "paged append: qkv / q_out null, misaligned or with a bad stride (%lld, %lld)",
+    return set_error(QD_ERR_ARG, "%s: qkv / q_out null, misaligned or with a bad stride (%lld, %lld)", what,
                      (long long)ldqkv, (long long)ldq);
   if ((q_norm == nullptr) != (k_norm == nullptr) || !aligned16(q_norm) || !aligned16(k_norm))
-    return set_error(QD_ERR_ARG, "paged append: q_norm and k_norm go together, 16-byte aligned");
+    return set_error(QD_ERR_ARG, "%s: q_norm and k_norm go together, 16-byte aligned", what);
   if (!cos || !sin || !aligned16(cos) || !aligned16(sin) || rot_half < 8 || rot_half % 8 || 2 * rot_half > head_dim ||
       ld_cs < rot_half || ld_cs % 4 || n_pos < 1)
-    return set_error(QD_ERR_ARG, "paged append: tables of %lld positions, %d angles, stride %lld", (long long)n_pos,
+    return set_error(QD_ERR_ARG, "%s: tables of %lld positions, %d angles, stride %lld", what, (long long)n_pos,
                      rot_half, (long long)ld_cs);
   if (tokens == 0) return QD_OK;
   a.qkv = static_cast<const char*>(qkv);
@@ -233,9 +301,46 @@ extern "C" int qd_paged_rope_append(const void* qkv, int64_t ldqkv, int dtype, i
   const bool two = tokens * ((heads + group - 1) / group) > 2048;
   const int per = (heads + group * (two ? 2 : 1) - 1) / (group * (two ? 2 : 1));
   const int64_t blocks = (tokens * per + kAppendThreads / 32 - 1) / (kAppendThreads / 32);
-  if (blocks > INT32_MAX) return set_error(QD_ERR_UNSUPPORTED, "paged append: %lld tokens", (long long)tokens);
+  if (blocks > INT32_MAX) return set_error(QD_ERR_UNSUPPORTED, "%s: %lld tokens", what, (long long)tokens);
   const void* fn = dtype == QD_BF16
-                       ? (head_dim == 128 ? append_kernel<__nv_bfloat16, 128>(two) : append_kernel<__nv_bfloat16, 64>(two))
-                       : (head_dim == 128 ? append_kernel<__half, 128>(two) : append_kernel<__half, 64>(two));
+                       ? (head_dim == 128 ? append_kernel<__nv_bfloat16, 128>(two, held) : append_kernel<__nv_bfloat16, 64>(two, held))
+                       : (head_dim == 128 ? append_kernel<__half, 128>(two, held) : append_kernel<__half, 64>(two, held));
   return launch_kernel(fn, dim3((unsigned)blocks), dim3(kAppendThreads), 0, pdl, stream, &a);
+}
+
+extern "C" int qd_paged_rope_append(const void* qkv, int64_t ldqkv, int dtype, int64_t tokens, int nq_heads,
+                                    int nkv_heads, int head_dim, const void* q_norm, const void* k_norm, float eps,
+                                    const float* cos, const float* sin, int64_t ld_cs, int64_t n_pos, int rot_half,
+                                    const int32_t* cu_tokens, const int32_t* kv_len, int batch,
+                                    const int32_t* page_table, int64_t ld_table, int max_pages, void* q_out,
+                                    int64_t ldq, void* k_pages, void* v_pages, int64_t n_pages, int page_size,
+                                    int64_t ps_page, int64_t ps_head, int* err, int pdl, cudaStream_t stream) {
+  AppendArgs a = {};
+  const int rc = paged_batch_check("paged append", dtype, tokens, nq_heads, nkv_heads, head_dim, k_pages, v_pages,
+                                   n_pages, page_size, ps_page, ps_head, cu_tokens, kv_len, batch, page_table,
+                                   ld_table, max_pages, err, &a.b);
+  if (rc != QD_OK) return rc;
+  return launch_append("paged append", qkv, ldqkv, dtype, tokens, nq_heads, nkv_heads, head_dim, q_norm, k_norm, eps, cos,
+                       sin, ld_cs, n_pos, rot_half, q_out, ldq, k_pages, v_pages, pdl, stream, false, a);
+}
+
+extern "C" int qd_paged_rope_append8(const void* qkv, int64_t ldqkv, int dtype, int64_t tokens, int nq_heads,
+                                     int nkv_heads, int head_dim, const void* q_norm, const void* k_norm, float eps,
+                                     const float* cos, const float* sin, int64_t ld_cs, int64_t n_pos, int rot_half,
+                                     const int32_t* cu_tokens, const int32_t* kv_len, int batch,
+                                     const int32_t* page_table, int64_t ld_table, int max_pages, void* q_out,
+                                     int64_t ldq, void* k_pages, void* v_pages, void* k_scale, void* v_scale,
+                                     int64_t n_pages, int page_size, int64_t ps_page, int64_t ps_head, int64_t ss_page,
+                                     int64_t ss_head, int* err, int pdl, cudaStream_t stream) {
+  AppendArgs a = {};
+  const int rc = paged_batch_check8("paged append (8 bits)", dtype, tokens, nq_heads, nkv_heads, head_dim, k_pages,
+                                    v_pages, k_scale, v_scale, n_pages, page_size, ps_page, ps_head, ss_page, ss_head,
+                                    cu_tokens, kv_len, batch, page_table, ld_table, max_pages, err, &a.b);
+  if (rc != QD_OK) return rc;
+  a.k_scale = static_cast<uint8_t*>(k_scale);
+  a.v_scale = static_cast<uint8_t*>(v_scale);
+  a.ss_page = ss_page;
+  a.ss_head = ss_head;
+  return launch_append("paged append (8 bits)", qkv, ldqkv, dtype, tokens, nq_heads, nkv_heads, head_dim, q_norm, k_norm, eps, cos,
+                       sin, ld_cs, n_pos, rot_half, q_out, ldq, k_pages, v_pages, pdl, stream, true, a);
 }

@@ -23,6 +23,16 @@ int paged_batch_check(const char* what, int dtype, int64_t tokens, int nq, int n
                       const int32_t* cu, const int32_t* kv_len, int batch, const int32_t* table, int64_t ld_table,
                       int max_pages, int* err, PagedBatch* b);
 
+// The same for pages of 8 bits: values of E4M3 and, per row, the exponent of the power of two that they are multiples of
+// (+ 127) in pools [page][KV head][row of the page]; strides in bytes, the scales' ss_page and ss_head.
+int paged_batch_check8(const char* what, int dtype, int64_t tokens, int nq, int nkv, int head_dim, const void* k_pages,
+                       const void* v_pages, const void* k_scale, const void* v_scale, int64_t n_pages, int page_size,
+                       int64_t ps_page, int64_t ps_head, int64_t ss_page, int64_t ss_head, const int32_t* cu,
+                       const int32_t* kv_len, int batch, const int32_t* table, int64_t ld_table, int max_pages, int* err,
+                       PagedBatch* b);
+// The exponents that an 8-bit row can have: 2^-9 (the least code) and 448 times these are in FP16's range.
+constexpr int kHeldLeastExp = -15, kHeldMostExp = 7;
+
 template <typename T>
 struct Elem;
 template <>

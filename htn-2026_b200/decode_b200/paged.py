@@ -29,12 +29,26 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _current_device = getattr(torch._C, "_cuda_getDevice", None)
 I32, F32 = torch.int32, torch.float32
 TYPES = {torch.bfloat16: L.QD_BF16, torch.float16: L.QD_FP16}
+E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
 
 
 def new_pools(pages: int, nkv: int, page_size: int, head_dim: int, device, dtype=torch.bfloat16):
     """Zeroed (k_pages, v_pages) of `pages` pages."""
     shape = (pages, nkv, page_size, head_dim)
     return torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device)
+
+
+def new_pools8(pages: int, nkv: int, page_size: int, head_dim: int, device):
+    """Zeroed (k_pages, v_pages, k_scale, v_scale) of `pages` pages of 8 bits: E4M3 values [pages, KV heads, page_size,
+    head_dim], and the powers of two that a position's values count [pages, KV heads, page_size] (1)."""
+    shape = (pages, nkv, page_size, head_dim)
+    byte = lambda s, v: torch.full(s, v, dtype=torch.uint8, device=device)  # noqa: E731
+    return (*(byte(shape, 0).view(E4M3) for _ in range(2)), *(byte(shape[:3], 127).view(E8M0) for _ in range(2)))
+
+
+def held_values(pages, scale, dtype=torch.float32):
+    """What an 8-bit pool's rows stand for: values times their row's power of two (exact in every `dtype`)."""
+    return (pages.float() * scale.float()[..., None]).to(dtype)
 
 
 def rope_table(positions: int, head_dim: int, theta: float, device):
@@ -74,15 +88,30 @@ def _rows(t, tokens: int, heads: int, D: int) -> int:
     return heads * D if tokens <= 1 else strides[0]
 
 
+def _check_scales(dev, shape, k_scale, v_scale):
+    """(page stride, head stride) of the scales of 8-bit pools."""
+    strides = k_scale.stride()
+    assert k_scale.dtype is E8M0 and v_scale.dtype is E8M0
+    assert k_scale.get_device() == dev and v_scale.get_device() == dev
+    assert k_scale.shape == shape[:3] and v_scale.shape == shape[:3] and v_scale.stride() == strides and strides[2] == 1
+    return strides
+
+
 def rope_append(qkv, cu_tokens, kv_len, page_table, nq: int, nkv: int, cos, sin, q_out, k_pages, v_pages, q_norm=None,
-                k_norm=None, eps: float = 1e-6, err=None, pdl: bool = True):
+                k_norm=None, eps: float = 1e-6, err=None, pdl: bool = True, k_scale=None, v_scale=None):
     """q_out[t] = rope(norm(q)) and K = rope(norm(k)), V into the pages, for every new token t
     (qd_paged_rope_append). qkv [tokens, (nq + 2 nkv) * head_dim]; q_out [tokens, nq, head_dim] or
-    [tokens, nq * head_dim]; cos / sin fp32 [positions, pairs turned] (`rope_table`)."""
+    [tokens, nq * head_dim]; cos / sin fp32 [positions, pairs turned] (`rope_table`).
+    With k_scale, v_scale the pages are of 8 bits: `rope_append8`."""
     dtype = qkv.dtype
     assert dtype in TYPES, f"expected BF16 or FP16 tensors, got {dtype}"
-    dev = qkv.get_device()
-    pool, ps, batch, ld_table, max_pages = _check_batch(dev, dtype, k_pages, v_pages, cu_tokens, kv_len, page_table, err)
+    dev, held = qkv.get_device(), k_scale is not None
+    pool, ps, batch, ld_table, max_pages = _check_batch(dev, E4M3 if held else dtype, k_pages, v_pages, cu_tokens, kv_len,
+                                                        page_table, err)
+    name, scales, scale_strides = "qd_paged_rope_append", (), ()
+    if held:
+        name, scale_strides = "qd_paged_rope_append8", _check_scales(dev, pool, k_scale, v_scale)[:2]
+        scales = k_scale.data_ptr(), v_scale.data_ptr()
     D, tokens = pool[3], qkv.shape[0]
     assert q_out.get_device() == dev and q_out.dtype is dtype and pool[1] == nkv
     ldqkv, ldq = _rows(qkv, tokens, nq + 2 * nkv, D), _rows(q_out, tokens, nq, D)
@@ -95,11 +124,18 @@ def rope_append(qkv, cu_tokens, kv_len, page_table, nq: int, nkv: int, cos, sin,
         assert q_norm.dtype is dtype and q_norm.get_device() == dev and q_norm.is_contiguous()
         assert k_norm.dtype is dtype and k_norm.get_device() == dev and k_norm.is_contiguous()
         qn, kn = q_norm.data_ptr(), k_norm.data_ptr()
-    L.call("qd_paged_rope_append", qkv.data_ptr(), ldqkv, TYPES[dtype], tokens, nq, nkv, D, qn, kn, eps,
+    L.call(name, qkv.data_ptr(), ldqkv, TYPES[dtype], tokens, nq, nkv, D, qn, kn, eps,
            cos.data_ptr(), sin.data_ptr(), ld[0], angles[0], angles[1], cu_tokens.data_ptr(), kv_len.data_ptr(), batch,
            page_table.data_ptr(), ld_table, max_pages, q_out.data_ptr(), ldq, k_pages.data_ptr(), v_pages.data_ptr(),
-           pool[0], pool[2], ps[0], ps[1], None if err is None else err.data_ptr(), pdl, _raw_stream(dev))
+           *scales, pool[0], pool[2], ps[0], ps[1], *scale_strides, None if err is None else err.data_ptr(), pdl, _raw_stream(dev))
     return q_out
+
+
+def rope_append8(qkv, cu_tokens, kv_len, page_table, nq: int, nkv: int, cos, sin, q_out, k_pages, v_pages, k_scale, v_scale,
+                 q_norm=None, k_norm=None, eps: float = 1e-6, err=None, pdl: bool = True):
+    """`rope_append` into pages of 8 bits (`new_pools8`; qd_paged_rope_append8, which defines how a row is held)."""
+    return rope_append(qkv, cu_tokens, kv_len, page_table, nq, nkv, cos, sin, q_out, k_pages, v_pages, q_norm, k_norm, eps,
+                       err, pdl, k_scale, v_scale)
 
 
 class PagedAttention:
@@ -109,11 +145,13 @@ class PagedAttention:
     object must not overlap on the GPU. After a device error other than a page outside the pool (`err`),
     `reset` makes it ready again."""
 
+    PLAN = "qd_paged_attn_plan"
+
     def __init__(self, nq: int, nkv: int, head_dim: int, device, dtype=torch.bfloat16, grid: int = 0):
         assert dtype in TYPES, f"expected BF16 or FP16, got {dtype}"
         self.nq, self.nkv, self.head_dim, self.dtype = nq, nkv, head_dim, dtype
         g, nbytes = ctypes.c_int(0), ctypes.c_int64(0)
-        L.call("qd_paged_attn_plan", nq, nkv, head_dim, grid, ctypes.byref(g), ctypes.byref(nbytes))
+        L.call(self.PLAN, nq, nkv, head_dim, grid, ctypes.byref(g), ctypes.byref(nbytes))
         self.grid = g.value
         self.scratch = torch.zeros((nbytes.value,), dtype=torch.uint8, device=device)
         self.scratch_bytes = nbytes.value
@@ -144,4 +182,33 @@ class PagedAttention:
                page_table.data_ptr(), ld_table, max_pages, self.scale if scale is None else scale, out.data_ptr(), ldo,
                lse_ptr, ld_lse, self.grid, self.scratch.data_ptr(), self.scratch_bytes,
                None if err is None else err.data_ptr(), pdl, _raw_stream(dev))
+        return out
+
+
+class PagedAttention8(PagedAttention):
+    """`PagedAttention` over pages of 8 bits (`new_pools8`; qd_paged_attn8)."""
+
+    PLAN = "qd_paged_attn8_plan"
+
+    def __call__(self, q, k_pages, v_pages, k_scale, v_scale, cu_tokens, kv_len, page_table, out, lse=None,
+                 scale: float | None = None, max_new: int | None = None, err=None, pdl: bool = True):
+        """As PagedAttention's. max_new: no request of this call has more new tokens (1 for a step of single tokens)."""
+        nq, D, dtype, dev = self.nq, self.head_dim, self.dtype, q.get_device()
+        pool, ps, batch, ld_table, max_pages = _check_batch(dev, E4M3, k_pages, v_pages, cu_tokens, kv_len, page_table, err)
+        ss_page, ss_head, _ = _check_scales(dev, pool, k_scale, v_scale)
+        tokens = q.shape[0]
+        assert q.dtype is dtype and out.dtype is dtype and out.get_device() == dev and self.scratch.get_device() == dev
+        assert pool[1] == self.nkv and pool[3] == D
+        ldq, ldo = _rows(q, tokens, nq, D), _rows(out, tokens, nq, D)
+        lse_ptr, ld_lse = None, 0
+        if lse is not None:
+            assert lse.dtype is F32 and lse.get_device() == dev and lse.shape == (tokens, nq)
+            ld_lse, step = lse.stride()
+            assert step == 1 or nq == 1
+            lse_ptr, ld_lse = lse.data_ptr(), max(ld_lse, nq) if tokens <= 1 else ld_lse
+        L.call("qd_paged_attn8", q.data_ptr(), ldq, TYPES[dtype], tokens, nq, self.nkv, D, k_pages.data_ptr(),
+               v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pool[0], pool[2], ps[0], ps[1], ss_page, ss_head,
+               cu_tokens.data_ptr(), kv_len.data_ptr(), batch, page_table.data_ptr(), ld_table, max_pages, max_new or 0,
+               self.scale if scale is None else scale, out.data_ptr(), ldo, lse_ptr, ld_lse, self.grid,
+               self.scratch.data_ptr(), self.scratch_bytes, None if err is None else err.data_ptr(), pdl, _raw_stream(dev))
         return out

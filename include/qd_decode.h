@@ -469,6 +469,40 @@ int qd_paged_attn(const void* q, int64_t ldq, int dtype, int64_t tokens, int nq_
                   float* lse, int64_t ld_lse, int grid, void* scratch, int64_t scratch_bytes, int* err, int pdl,
                   cudaStream_t stream);
 
+/* ---------------------------------------------------------------- paged K/V cache of 8 bits
+ * Pages that hold a position of a KV head in head_dim + 1 bytes: head_dim values of E4M3 (4 bits of exponent, 3 of
+ * mantissa, largest 448) in pools [n_pages][nkv_heads][page_size][head_dim], and one byte e + 127 in pools
+ * [n_pages][nkv_heads][page_size]: the values count 2^e. Strides are in bytes and multiples of 16 (ps_page, ps_head of
+ * the values, ss_page, ss_head of the scales), pointers 16-byte aligned; the rest is as for 16-bit pages.
+ *
+ * qd_paged_rope_append8 is qd_paged_rope_append into such pages. For each K row (rotated, in fp32) and V row,
+ *   e = the least whole number from -15 to 7 with |x| <= 448 * 2^e for the row's largest finite x,  code = E4M3(x / 2^e)
+ * rounded once, to nearest even. Where e would have to be above 7, larger values are held as +-448 * 2^7; infinities and
+ * NaN are held as NaN. q_out is of `dtype`, as qkv is.
+ *
+ * A row read back is exact in BF16 and in FP16. Other exponents than these may not be written into a pool. */
+int qd_paged_rope_append8(const void* qkv, int64_t ldqkv, int dtype, int64_t tokens, int nq_heads, int nkv_heads,
+                          int head_dim, const void* q_norm, const void* k_norm, float eps, const float* cos,
+                          const float* sin, int64_t ld_cs, int64_t n_pos, int rot_half, const int32_t* cu_tokens,
+                          const int32_t* kv_len, int batch, const int32_t* page_table, int64_t ld_table, int max_pages,
+                          void* q_out, int64_t ldq, void* k_pages, void* v_pages, void* k_scale, void* v_scale,
+                          int64_t n_pages, int page_size, int64_t ps_page, int64_t ps_head, int64_t ss_page,
+                          int64_t ss_head, int* err, int pdl, cudaStream_t stream);
+
+/* qd_paged_attn8 is qd_paged_attn over such pages: q and out are of `dtype`, scores, softmax statistics and sums fp32.
+ * max_new > 0 says that no request has more new tokens than this (a step of single tokens: 1), which saves a launch
+ * for requests of more; the rows of one that has more all the same may be left as they were, with QD_DEVERR_POS
+ * flagged. A row that sees a code of NaN in a K row, or whose request has one in a V row that it sees, has NaN there.
+ * Grid and scratch as for qd_paged_attn (qd_paged_attn8_plan). */
+int qd_paged_attn8_plan(int nq_heads, int nkv_heads, int head_dim, int grid_hint, int* grid, int64_t* scratch_bytes);
+int qd_paged_attn8(const void* q, int64_t ldq, int dtype, int64_t tokens, int nq_heads, int nkv_heads, int head_dim,
+                   const void* k_pages, const void* v_pages, const void* k_scale, const void* v_scale, int64_t n_pages,
+                   int page_size, int64_t ps_page, int64_t ps_head, int64_t ss_page, int64_t ss_head,
+                   const int32_t* cu_tokens, const int32_t* kv_len, int batch, const int32_t* page_table,
+                   int64_t ld_table, int max_pages, int max_new, float scale, void* out, int64_t ldo, float* lse,
+                   int64_t ld_lse, int grid, void* scratch, int64_t scratch_bytes, int* err, int pdl,
+                   cudaStream_t stream);
+
 /* ---------------------------------------------------------------- sampling
  * One token per row of logits [rows][vocab] (QD_BF16, QD_FP16 or QD_FP32; row stride ld), drawn with the
  * row's uniform number u in [0, 1). The tokens are ordered by logit, the largest first and equal logits by
