@@ -43,6 +43,8 @@
 #include <climits>
 
 #include "qd_host.h"
+#include "qd_paged_attn8.h"
+#include "qd_paged_attn_dev.cuh"
 #include "qd_paged_dev.cuh"
 #include "qd_paged_line.h"
 #include "qd_umma.cuh"
@@ -109,14 +111,6 @@ struct PgSeg {
 };
 static_assert(sizeof(PgSeg) <= 64, "segment ring entry");
 
-__device__ __forceinline__ void pg_tma_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w,
-                                          uint32_t bar, uint64_t policy) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
-      " [%0], [%1, {%2, %3, %4, %5}], [%6], %7;" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar), "l"(policy)
-      : "memory");
-}
 __device__ __forceinline__ void pg_tma_5d(uint32_t dst, const CUtensorMap* map, int z, int w, int v, uint32_t bar,
                                           uint64_t policy) {
   asm volatile(
@@ -128,30 +122,6 @@ __device__ __forceinline__ void pg_tma_5d(uint32_t dst, const CUtensorMap* map, 
 __device__ __forceinline__ float pg_max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-__device__ __forceinline__ float pg_ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
-// A row's end: 1 / sum of its exponentials, and its log-sum-exp. A sum of 0 is a row that saw no key; a sum that is
-// not a number stays one.
-__device__ __forceinline__ float pg_inverse(float l) { return l == 0.f ? 0.f : 1.0f / l; }
-__device__ __forceinline__ float pg_lse(float m, float l) {
-  return l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.69314718055994531f;
-}
-
-template <int N>
-struct Const {
-  static constexpr int value = N;
-};
-
-// maximum over the warp (NaN where a lane has one only if all have)
-__device__ __forceinline__ float redux_max(float v) {
-  float r;
-  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
   return r;
 }
 __device__ __forceinline__ void tmem_ld4_wait(uint32_t taddr, uint32_t* r) {
@@ -169,16 +139,6 @@ __device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint32_t* r) {
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
       : "memory");
 }
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-      "%15, %16};\n"
-      "tcgen05.wait::st.sync.aligned;" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
-}
-
 // 64 consecutive columns of this thread's lane, not waited for; and the wait, which ties the registers
 __device__ __forceinline__ void tmem_ld64_raw(uint32_t taddr, uint32_t* r) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];"
@@ -1237,16 +1197,6 @@ static const void* attn_kernel(int head_dim, bool merged) {
   return head_dim == 64 ? (const void*)paged_attn_kernel<T, 64, false>
          : merged       ? (const void*)paged_attn_kernel<T, 128, true>
                         : (const void*)paged_attn_kernel<T, 128, false>;
-}
-
-struct PagedAttnPlan {
-  int64_t off_partials, bytes;
-};
-static PagedAttnPlan paged_attn_plan(int grid, int head_dim) {
-  PagedAttnPlan p;
-  p.off_partials = ((int64_t)grid * 2 * 4 + 255) / 256 * 256;  // the tickets first
-  p.bytes = p.off_partials + (int64_t)2 * grid * 2 * 128 * (head_dim * 4 + 8);
-  return p;
 }
 
 }  // namespace qd

@@ -7,7 +7,7 @@
 #include <climits>
 
 #include "qd_host.h"
-#include "qd_paged_dev.cuh"
+#include "qd_paged_attn8.h"
 
 namespace qd {
 
@@ -19,6 +19,7 @@ struct Attn8Args {
   float* lse;
   int64_t ldq, ldo, ld_lse, ss_page, ss_head;
   float scale;
+  int least;  // requests of fewer tokens are another kernel's
 };
 
 __device__ __forceinline__ float held_value(uint8_t code) {
@@ -38,6 +39,7 @@ __global__ void __launch_bounds__(128) paged_attn8_kernel(const __grid_constant_
   const int h = (int)(w - t * a.b.nq), kvh = h / (a.b.nq / a.b.nkv);
   const int i = warp_find_request(a.b.cu, a.b.batch, (int)t, lane);
   if (i >= a.b.batch) return;
+  if (ld_i32(a.b.cu + i + 1) - ld_i32(a.b.cu + i) < a.least) return;
   const int kv_len = max(ld_i32(a.b.kv_len + i), 0), pos = kv_len - ld_i32(a.b.cu + i + 1) + (int)t;
   const int64_t room = (int64_t)a.b.max_pages << a.b.page_shift;
   if (kv_len > room && lane == 0) flag_error(a.b.err, QD_DEVERR_PAGE);
@@ -103,8 +105,17 @@ extern "C" int qd_paged_attn8(const void* q, int64_t ldq, int dtype, int64_t tok
   if (grid < 1 || !scratch || scratch_bytes < need || (reinterpret_cast<uintptr_t>(scratch) & 31))
     return set_error(QD_ERR_SCRATCH, "%s: grid %d needs %lld B of 32-byte aligned scratch (have %lld)", what, grid,
                      (long long)need, (long long)scratch_bytes);
-  (void)max_new;
   if (tokens == 0) return QD_OK;
+  // Requests of at most `few` tokens have a kernel of their own, and the others one.
+  const int few = kFewRows / (nq_heads / nkv_heads);
+  const bool only_few = (max_new > 0 && max_new <= few) || tokens <= few;
+  if (few > 0) {
+    Paged8Call c = {a.b, q, k_pages, v_pages, k_scale, v_scale, out, lse, ldq, ldo, ld_lse, ss_page, ss_head, dtype, head_dim,
+                    grid, pdl, scale, scratch, stream};
+    const int rf = launch_few8(c, only_few);
+    if (rf != QD_OK || only_few) return rf;
+  }
+  a.least = few + 1;
   a.q = static_cast<const char*>(q);
   a.k_pages = static_cast<const uint8_t*>(k_pages);
   a.v_pages = static_cast<const uint8_t*>(v_pages);

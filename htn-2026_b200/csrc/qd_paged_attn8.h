@@ -1,0 +1,36 @@
+// The two kernels of the attention over pages of 8 bits, for requests of few rows and of tiles of them.
+#pragma once
+
+#include "qd_paged_dev.cuh"
+#include "qd_paged_line.h"
+
+namespace qd {
+
+// Scratch of the paged attentions: tickets [grid][2], then the pieces of cut units, as large as two tiles' at most.
+struct PagedAttnPlan {
+  int64_t off_partials, bytes;
+};
+inline PagedAttnPlan paged_attn_plan(int grid, int head_dim) {
+  PagedAttnPlan p;
+  p.off_partials = ((int64_t)grid * 2 * 4 + 255) / 256 * 256;  // the tickets first
+  p.bytes = p.off_partials + (int64_t)2 * grid * 2 * 128 * (head_dim * 4 + 8);
+  return p;
+}
+
+// A checked call.
+struct Paged8Call {
+  PagedBatch b;
+  const void *q, *k_pages, *v_pages, *k_scale, *v_scale;
+  void* out;
+  float* lse;
+  int64_t ldq, ldo, ld_lse, ss_page, ss_head;
+  int dtype, head_dim, grid, pdl;
+  float scale;
+  void* scratch;
+  cudaStream_t stream;
+};
+// The requests of at most 16 query rows a KV head (of none, where a group of heads is larger). `alone`: there is no
+// other launch for the rest, whose rows are left as they are and flagged.
+int launch_few8(const Paged8Call& c, bool alone);
+
+}  // namespace qd
