@@ -18,9 +18,10 @@
 // to the exponent of the weight, P' = exp2(s log2 e + e_v - m), whose running maximum m is that of the weights of the
 // codes. l sums P' / 2^e_v.
 //
-// The key blocks of all units form one line that is cut evenly over the CTAs; blocks alternate between two warpgroups,
-// across the units too, and the scores of the next two blocks are always under way. Pieces of a cut unit are left in the
-// scratch and joined in the order of their keys by the CTA that ends last.
+// The key blocks of all units form one line that is cut evenly over the CTAs, two to an SM: a warpgroup that turns scores
+// into weights each, so that one CTA's start, unit ends and last block hide behind the other's stream of blocks. The
+// scores of the next two blocks are always under way, across the units too. Pieces of a cut unit are left in the scratch
+// and joined in the order of their keys by the CTA that ends last.
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -32,7 +33,8 @@
 
 namespace qd {
 
-constexpr int kF8Threads = 384;  // warps 0-3 softmax A, 4-7 softmax B, 8 producer, 9 MMA, 10-11 the queries' terms
+constexpr int kF8Threads = 256;  // warps 0-3 softmax, 4 producer, 5 MMA, 6 the line and the queries, 7 the scales
+constexpr int kF8Resident = 2;   // CTAs an SM
 constexpr int kF8Scales = 8;     // blocks whose scales are in shared memory
 constexpr int kF8Bias = 7;       // P' is up to 2^(8 + 7): the upper end of E5M2's range
 
@@ -42,24 +44,22 @@ struct F8Lay {
   static constexpr int kItem = kPgKeys * D;         // a K or V block
   static constexpr int kQ = kFewRows * kTQ * D;     // a unit's queries
   static constexpr int kP = kFewRows * kTP * kPgKeys;
-  static constexpr int kSlots = D == 128 ? 11 : 20;
+  static constexpr int kSlots = D == 128 ? 5 : 10;
   static constexpr int q = 0;                       // two units'
-  static constexpr int p = q + 2 * kQ;              // the two warpgroups'
+  static constexpr int p = q + 2 * kQ;              // two blocks'
   static constexpr int kv = p + 2 * kP;
   static constexpr int sc = kv + kSlots * kItem;    // [block][K, V][128 keys]
   static constexpr int bars = sc + kF8Scales * 2 * kPgKeys;
-  // q8full[2], qempty[2], sfull[2], pfull[2], odone[2], ofree[2], group[2], segfull[4], segempty[4], join, then
-  // scfull[], scempty[], full[], empty[]
-  static constexpr int nbars = 23 + 2 * kF8Scales + 2 * kSlots;
+  // q8full[2], qempty[2], sfull[2], pfull[2], odone[2], group, segfull[4], segempty[4], then scfull[], scempty[], full[], empty[]
+  static constexpr int nbars = 19 + 2 * kF8Scales + 2 * kSlots;
   static constexpr int seg = bars + (nbars * 8 + 63) / 64 * 64;
   static constexpr int qs = seg + 4 * 64;     // the queries' powers of two [2 units][16]
-  static constexpr int misc = qs + 128;       // tmem, abort, line start, last flags, drain counts; then the scan's totals
-  static constexpr int sums = misc + 256;     // the warps' sums [2 groups][16 rows][4 warps]
-  static constexpr int mx = sums + 512;       // and maxima
-  static constexpr int mb = mx + 512;         // warpgroup B's maxima [16]
-  static constexpr int total = mb + 64;
+  static constexpr int misc = qs + 128;       // tmem, abort, line start, drain count, last flag; then the scan's totals
+  static constexpr int sums = misc + 256;     // the warps' sums [16 rows][4 warps]
+  static constexpr int mx = sums + 256;       // and maxima, of two blocks
+  static constexpr int total = mx + 512;
   static_assert(kQ % 1024 == 0 && kP % 1024 == 0 && kItem % 1024 == 0, "operands start on 1 KiB");
-  static_assert(total <= 227 * 1024, "shared memory of an SM");
+  static_assert(kF8Resident * (total + 1024) <= 228 * 1024, "shared memory of an SM");
 };
 
 struct alignas(64) Few8Args {
@@ -76,13 +76,14 @@ struct alignas(64) Few8Args {
   int alone;      // no other kernel takes the requests of more tokens
   float scale_log2;
   float* partials;  // [2 * grid slots][16 rows][D], then the rows' (m, l)
-  int* tickets;     // [grid][2], of which the first
+  int* tickets;     // [grid]
 };
 
 struct F8Seg {
   int row0, ntok, pos0, kv;  // first token row, tokens, the first's position, keys of the request
   int head, j0, nb, whole;   // KV head, first key block, blocks (0 ends the list), all of the unit's
   int slot, c0, nc;          // partial slot, first CTA and number of CTAs of the unit
+  int request;
 };
 static_assert(sizeof(F8Seg) <= 64, "segment ring entry");
 
@@ -112,6 +113,28 @@ __device__ __forceinline__ void f8_load(uint32_t taddr, uint32_t* r) {
   for (int i = 0; i < N; i += 16) tmem_wait_ld16(r + i);
 }
 constexpr int f8_cols(int n) { return (n + 15) / 16 * 16; }
+// The sums of kC rows' terms, each `step` of the one before it: column c + t kC is row c's term t.
+template <int kC, int kTerms>
+__device__ __forceinline__ void f8_terms(uint32_t taddr, float step, float* v) {
+  if constexpr (kC < 16) {  // all in one load
+    uint32_t u[16];
+    f8_load<16>(taddr, u);
+#pragma unroll
+    for (int c = 0; c < kC; ++c) {
+      v[c] = __uint_as_float(u[c + (kTerms - 1) * kC]);
+#pragma unroll
+      for (int t = kTerms - 2; t >= 0; --t) v[c] = fmaf(v[c], step, __uint_as_float(u[c + t * kC]));
+    }
+  } else {
+#pragma unroll
+    for (int t = kTerms - 1; t >= 0; --t) {
+      uint32_t u[16];
+      f8_load<16>(taddr + t * kC, u);
+#pragma unroll
+      for (int c = 0; c < kC; ++c) v[c] = t == kTerms - 1 ? __uint_as_float(u[c]) : fmaf(v[c], step, __uint_as_float(u[c]));
+    }
+  }
+}
 
 // one request's blocks in this kernel (0: not its)
 __device__ __forceinline__ int f8_blocks(const PgShape& s, const PgReq& r) {
@@ -160,7 +183,7 @@ __device__ __forceinline__ void f8_join(const Few8Args& a, const F8Seg& g, int r
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kF8Threads, 1) paged_few8_kernel(const __grid_constant__ Few8Args a) {
+__global__ void __launch_bounds__(kF8Threads, kF8Resident) paged_few8_kernel(const __grid_constant__ Few8Args a) {
   using Lay = F8Lay<T, D>;
   constexpr int kSlots = Lay::kSlots, kTQ = Lay::kTQ, kTP = Lay::kTP;
   extern __shared__ __align__(1024) char smem[];
@@ -168,17 +191,17 @@ __global__ void __launch_bounds__(kF8Threads, 1) paged_few8_kernel(const __grid_
   auto q8full = [&](int s) { return bars + 8u * (s & 1); };
   auto qempty = [&](int s) { return bars + 16 + 8u * (s & 1); };
   auto sfull = [&](int x) { return bars + 32 + 8u * x; };
+  // A barrier for each of two blocks: the softmax may be done with two before the first product, and two products may be
+  // under way at a unit's end. A parity wait two phases behind a barrier never ends, and two ahead of it does not wait.
   auto pfull = [&](int x) { return bars + 48 + 8u * x; };
   auto odone = [&](int x) { return bars + 64 + 8u * x; };
-  auto ofree = [&](int x) { return bars + 80 + 8u * x; };
-  auto group = [&](int x) { return bars + 96 + 8u * x; };
-  auto segfull = [&](int s) { return bars + 112 + 8u * (s & 3); };
-  auto segempty = [&](int s) { return bars + 144 + 8u * (s & 3); };
-  const uint32_t join = bars + 176;
-  auto scfull = [&](int b) { return bars + 184 + 8u * (b & (kF8Scales - 1)); };
-  auto scempty = [&](int b) { return bars + 184 + 8u * (kF8Scales + (b & (kF8Scales - 1))); };
-  auto full = [&](int s) { return bars + 184 + 8u * (2 * kF8Scales + s); };
-  auto empty = [&](int s) { return bars + 184 + 8u * (2 * kF8Scales + kSlots + s); };
+  const uint32_t group = bars + 80;
+  auto segfull = [&](int s) { return bars + 88 + 8u * (s & 3); };
+  auto segempty = [&](int s) { return bars + 120 + 8u * (s & 3); };
+  auto scfull = [&](int b) { return bars + 152 + 8u * (b & (kF8Scales - 1)); };
+  auto scempty = [&](int b) { return bars + 152 + 8u * (kF8Scales + (b & (kF8Scales - 1))); };
+  auto full = [&](int s) { return bars + 152 + 8u * (2 * kF8Scales + s); };
+  auto empty = [&](int s) { return bars + 152 + 8u * (2 * kF8Scales + kSlots + s); };
   F8Seg* segs = reinterpret_cast<F8Seg*>(smem + Lay::seg);
   int* misc = reinterpret_cast<int*>(smem + Lay::misc);
   int* abort = misc + 1;
@@ -191,19 +214,17 @@ __global__ void __launch_bounds__(kF8Threads, 1) paged_few8_kernel(const __grid_
   }
   if (tid == 0) {
     for (int x = 0; x < 2; ++x) {
-      mbar_init(q8full(x), 2);
-      mbar_init(qempty(x), 9);  // the MMA's products and eight softmax warps
+      mbar_init(q8full(x), 1);
+      mbar_init(qempty(x), 5);  // the MMA's products and four softmax warps
       mbar_init(sfull(x), 1);
       mbar_init(pfull(x), 4);
       mbar_init(odone(x), 1);
-      mbar_init(ofree(x), 4);
-      mbar_init(group(x), 4);
     }
+    mbar_init(group, 4);
     for (int k = 0; k < 4; ++k) {
       mbar_init(segfull(k), 1);
-      mbar_init(segempty(k), 11);  // the MMA warp, eight softmax warps, two for the queries
+      mbar_init(segempty(k), 7);  // all warps but the one that walks the line
     }
-    mbar_init(join, 4);
     for (int k = 0; k < kF8Scales; ++k) {
       mbar_init(scfull(k), 1);
       mbar_init(scempty(k), 4);
@@ -215,8 +236,13 @@ __global__ void __launch_bounds__(kF8Threads, 1) paged_few8_kernel(const __grid_
     fence_mbar_init();
     for (int m = 1; m < 16; ++m) misc[m] = 0;
   }
-  if (warp == 9) tmem_alloc(smem_u32(misc), 256);
+  if (warp == 5) tmem_alloc(smem_u32(misc), 256);
   grid_dep_wait();
+  {  // the page table on its way to L2 while the lengths are read: a line per thread of the grid
+    const int lines = (a.b.max_pages + 31) / 32;
+    const int64_t at = (int64_t)blockIdx.x * kF8Threads + tid, row = at / lines;
+    if (row < a.b.batch) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.b.table + row * a.b.ld_table + (at - row * lines) * 32));
+  }
 
   // ---- this CTA's place on the line: a prefix sum over the requests, and a walk from the one it starts in
   const int per = (a.b.batch + kF8Threads - 1) / kF8Threads;
@@ -274,128 +300,75 @@ __global__ void __launch_bounds__(kF8Threads, 1) paged_few8_kernel(const __grid_
   __syncthreads();
   const uint32_t tmem = (uint32_t)misc[0];
   auto tS = [&](int x) { return tmem + 64u * x; };
-  auto tO = [&](int x) { return tmem + 128u + 64u * x; };
+  const uint32_t tO = tmem + 128u;
 
-  if (warp == 8) {
-    // ------------------------------------------------------------ producer: all lanes walk the line
+  if (warp == 4) {
+    // ------------------------------------------------------------ producer: a lane per page of a block
     const uint64_t pol = policy_evict_normal();
-    int64_t at = begin;
-    int i = misc[2], h = misc[3], o = misc[4];
     const int boxes = kPgKeys >> a.b.page_shift, box_bytes = a.b.page_size * D;
-    int seg = 0, blk = 0, slot = 0;
+    const int per_lot = 32 / boxes;  // blocks
+    int items = 0, slot = 0, of_request = -1, first_lot = -2;
     uint32_t phase = 1;  // of empty(slot): a ring's first round passes at once
     bool ok = true;
-    r = *reinterpret_cast<const PgReq*>(smem + Lay::mx);
-    __syncwarp();
-    // this lane's page of block j of the current request; -2: none (past the last key)
-    auto page_of = [&](int j) {
-      const int key = j * kPgKeys + (lane << a.b.page_shift);
-      if (lane >= boxes || key >= r.kv) return -2;
-      return max(ld_i32(a.b.table + i * a.b.ld_table + (key >> a.b.page_shift)), -1);
-    };
-    while (at < end && ok) {
-      const int nblk = f8_blocks(a.s, r), take = (int)min(end - at, (int64_t)(nblk - o));
-      const int j0 = o, j1 = o + take;
-      int page = page_of(j0);
-      if (seg >= 4) ok = mbar_wait_abort(segempty(seg), ((seg >> 2) - 1) & 1, a.b.err, kErrWaitEmpty, abort);
+    auto wait = [&](uint32_t bar, int parity, int code) {
+      if (ok) ok = mbar_wait_abort(bar, parity & 1, a.b.err, code, abort);
       ok = __all_sync(0xffffffffu, ok);
+    };
+#pragma unroll 1
+    for (int seg = 0;; ++seg) {
+      wait(segfull(seg), seg >> 2, kErrWaitFull);
       if (!ok) break;
-      if (lane == 0) {
-        const int64_t first = at - o;
-        const int c0 = line.owner(first), c1 = line.owner(first + nblk - 1);
-        F8Seg* s = segs + (seg & 3);
-        s->row0 = r.row0;
-        s->ntok = r.n;
-        s->pos0 = r.pos0;
-        s->kv = r.kv;
-        s->head = h;
-        s->j0 = j0;
-        s->nb = take;
-        s->whole = take == nblk;
-        s->slot = 2 * cta + (j0 > 0 ? 0 : 1);
-        s->c0 = c0;
-        s->nc = c1 - c0 + 1;
-        mbar_arrive(segfull(seg));
-      }
-      ++seg;
-      for (int j = j0; j < j1 && ok; ++j, ++blk) {
-        const int next = j + 1 < j1 ? page_of(j + 1) : -2;
-        const bool need = page != -2;
-        bool in = need;
+      const F8Seg g = segs[seg & 3];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(segempty(seg));
+      if (g.nb == 0) break;
+      // The request's page entries, 32 at a time (aligned, so that a block's lie in one lot), a lot ahead: a block's
+      // copies take less time than a load of their entries. The first lot stays for the request's other heads.
+      auto lot = [&](int n) {
+        const int entry = 32 * n + lane;
+        return (int64_t)entry << a.b.page_shift < g.kv ? ld_i32(a.b.table + g.request * a.b.ld_table + entry) : -2;
+      };
+      if (g.request != of_request) first_lot = lot(0);
+      of_request = g.request;
+      int n_lot = g.j0 / per_lot, entries = n_lot ? lot(n_lot) : first_lot, ahead = lot(n_lot + 1);
+      for (int j = g.j0; j < g.j0 + g.nb && ok; ++j) {
+        if (j / per_lot != n_lot) {
+          entries = ahead;
+          ahead = lot(++n_lot + 1);
+        }
+        int page = __shfl_sync(0xffffffffu, entries, (j % per_lot) * boxes + (lane & (boxes - 1)));
+        const bool need = lane < boxes && ((int64_t)j * kPgKeys + (lane << a.b.page_shift)) < g.kv;
         if (need && (page < 0 || page >= a.b.n_pages)) {
           flag_error(a.b.err, QD_DEVERR_PAGE);
           page = -1;  // outside the tensor map: the copy fills zeros
-          in = false;
         }
-        const int n_need = __popc(__ballot_sync(0xffffffffu, need)), n_in = __popc(__ballot_sync(0xffffffffu, in));
-        {  // the rows' powers of two
-          const bool got = mbar_wait_abort(scempty(blk), ((blk / kF8Scales) & 1) ^ 1, a.b.err, kErrWaitEmpty, abort);
-          if (!__all_sync(0xffffffffu, got)) {
-            ok = false;
-            break;
-          }
-          const int at_scale = Lay::sc + (blk & (kF8Scales - 1)) * 2 * kPgKeys + (lane << a.b.page_shift);
-          if (need && !in) {
-            for (int c = 0; c < a.b.page_size; c += 16) {
-              *reinterpret_cast<uint4*>(smem + at_scale + c) = make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu);
-              *reinterpret_cast<uint4*>(smem + at_scale + kPgKeys + c) = make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu);
-            }
-            fence_proxy_async_smem();  // a later block's come by copies
-          }
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive_expect_tx(scfull(blk), n_in * a.b.page_size * 2);
-            misc[9] = blk + 1;
-          }
-          __syncwarp();
-          if (in) {
-            const int64_t from = page * a.ss_page + h * a.ss_head;
-            bulk_g2s(sb + at_scale, a.k_scale + from, a.b.page_size, scfull(blk), pol);
-            bulk_g2s(sb + at_scale + kPgKeys, a.v_scale + from, a.b.page_size, scfull(blk), pol);
-          }
-        }
+        const int n_need = __popc(__ballot_sync(0xffffffffu, need));
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
-          const bool got = mbar_wait_abort(empty(slot), phase, a.b.err, kErrWaitEmpty, abort);
-          if (!__all_sync(0xffffffffu, got)) {
-            ok = false;
-            break;
-          }
+          wait(empty(slot), phase, kErrWaitEmpty);
+          if (!ok) break;
           if (lane == 0) {
             mbar_arrive_expect_tx(full(slot), n_need * box_bytes);
-            misc[8] = 2 * blk + kv + 1;
+            misc[8] = ++items;
           }
           __syncwarp();
           if (need)
-            pg_tma_4d(sb + Lay::kv + slot * Lay::kItem + lane * box_bytes, kv ? &a.tv : &a.tk, 0, 0, h, page, full(slot), pol);
+            pg_tma_4d(sb + Lay::kv + slot * Lay::kItem + lane * box_bytes, kv ? &a.tv : &a.tk, 0, 0, g.head, page, full(slot), pol);
           if (++slot == kSlots) {
             slot = 0;
             phase ^= 1;
           }
         }
-        page = next;
       }
-      at += take;
-      o = 0;
-      if (at < end && ++h == a.b.nkv) {
-        h = 0;
-        do r = request(++i);
-        while (f8_blocks(a.s, r) == 0);
-      }
+      if (!ok) break;
     }
-    // the end of the list: a segment without blocks
-    if (ok && seg >= 4) ok = mbar_wait_abort(segempty(seg), ((seg >> 2) - 1) & 1, a.b.err, kErrWaitEmpty, abort);
-    if (ok && lane == 0) {
-      segs[seg & 3].nb = 0;
-      mbar_arrive(segfull(seg));
-    }
-  } else if (warp == 9) {
+  } else if (warp == 5) {
     // ------------------------------------------------------------ MMA: one elected lane waits and issues
     constexpr uint32_t hi = f8_desc_hi<D>(), hi_p = f8_desc_hi<128>(), kItem16 = Lay::kItem >> 4;
     const uint32_t d_q = umma_desc_lo(sb + Lay::q), d_k = umma_desc_lo(sb + Lay::kv), d_p = umma_desc_lo(sb + Lay::p);
     // heads of 64: the 64 upper rows of O^T repeat the lower ones (block stride 0)
     const uint32_t d_v = umma_desc_lo(sb + Lay::kv, 0);
-    int slot = 0, pc[2] = {0, 0}, units[2] = {0, 0};  // slot: of the next V product's K block
+    int slot = 0;  // of the next V product's K block
     uint32_t phase = 0;
     int s_seg = 0, s_left = 0, s_blk = 0, s_slot = 0;  // of the next scores
     uint32_t s_phase = 0, s_id = 0;
@@ -471,21 +444,18 @@ __global__ void __launch_bounds__(kF8Threads, 1) paged_few8_kernel(const __grid_
         if (rows < kPgKeys) zero_v(rows, v, v_phase);
         if (leader) {
           wait(full(v), v_phase);
-          if (j < 2 && units[x] > 0) wait(ofree(x), units[x] - 1);
-          wait(pfull(x), pc[x]);
+          wait(pfull(x), b >> 1);  // (a unit's first: its rows have taken the last unit's sums by then)
           tc_fence_after();
           if (ok) {
             const uint32_t vt = d_v + v * kItem16, pt = d_p + x * (Lay::kP >> 4);
 #pragma unroll
             for (int k = 0; k < 4; ++k)  // 32 keys per MMA: four groups of 8 rows of V
-              umma_f8<hi, hi_p>(tO(x), vt + k * (32 * D >> 4), pt + 2 * k, id, k ? 1u : j < 2 ? 0u : 1u);
+              umma_f8<hi, hi_p>(tO, vt + k * (32 * D >> 4), pt + 2 * k, id, k || j ? 1u : 0u);
           }
-          ++pc[x];
           umma_commit(odone(x));
           umma_commit(empty(v));
           next_scores();
         }
-        if (j < 2) ++units[x];
         slot += 2;
         if (slot >= kSlots) {
           slot -= kSlots;
@@ -495,14 +465,13 @@ __global__ void __launch_bounds__(kF8Threads, 1) paged_few8_kernel(const __grid_
       }
       if (lane == 0) mbar_arrive(segempty(seg));  // (the scores are at most two blocks ahead, in a ring of four)
     }
-    if (leader)  // no MMA may still run when its memory is given back
-      for (int x = 0; x < 2; ++x)
-        if (pc[x] > 0) mbar_wait(odone(x), (pc[x] - 1) & 1, a.b.err, kErrDrain);
-  } else if (warp >= 10) {
-    // ------------------------------------------------------------ the queries' terms, a unit ahead
-    constexpr int kLanes = D / 8, kAt = 32 / kLanes;  // lanes of a row, rows at a time
-    const int sub = lane % kLanes;
+    if (leader && s_blk > 0) mbar_wait(sfull((s_blk - 1) & 1), ((s_blk - 1) >> 1) & 1, a.b.err, kErrDrain);
+    if (leader && b > 0) mbar_wait(odone((b - 1) & 1), ((b - 1) >> 1) & 1, a.b.err, kErrDrain);  // no MMA may still run when its memory is given back
+  } else if (warp == 7) {
+    // ------------------------------------------------------------ the rows' powers of two, four keys a lane
+    constexpr int kAhead = 4;  // blocks whose loads are in flight (entries, then scales: two waits for memory)
     bool ok = true;
+    int blk = 0;
     auto wait = [&](uint32_t bar, int parity) {
       if (ok) ok = mbar_wait_abort(bar, parity & 1, a.b.err, kErrWaitFull, abort);
       ok = __all_sync(0xffffffffu, ok);
@@ -515,110 +484,191 @@ __global__ void __launch_bounds__(kF8Threads, 1) paged_few8_kernel(const __grid_
       __syncwarp();
       if (lane == 0) mbar_arrive(segempty(seg));
       if (g.nb == 0) break;
-      if (seg >= 2) wait(qempty(seg), (seg >> 1) - 1);
+      const int32_t* const table = a.b.table + g.request * a.b.ld_table;
+#pragma unroll 1
+      for (int j0 = 0; j0 < g.nb && ok; j0 += kAhead) {
+        int page[kAhead];
+        uint32_t ks[kAhead], vs[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+          const int key = (g.j0 + j0 + j) * kPgKeys + 4 * lane;
+          page[j] = j0 + j < g.nb && key < g.kv ? ld_i32(table + (key >> a.b.page_shift)) : -1;
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {  // keys of no page: 1
+          const int64_t at = page[j] * a.ss_page + g.head * a.ss_head + (((g.j0 + j0 + j) * kPgKeys + 4 * lane) & (a.b.page_size - 1));
+          const bool in = page[j] >= 0 && page[j] < a.b.n_pages;
+          ks[j] = in ? __ldcg(reinterpret_cast<const uint32_t*>(a.k_scale + at)) : 0x7f7f7f7fu;
+          vs[j] = in ? __ldcg(reinterpret_cast<const uint32_t*>(a.v_scale + at)) : 0x7f7f7f7fu;
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+          if (j0 + j >= g.nb) break;
+          wait(scempty(blk), (blk / kF8Scales) + 1);  // (a ring's first round passes at once)
+          if (!ok) break;
+          uint32_t* const to = reinterpret_cast<uint32_t*>(smem + Lay::sc + (blk & (kF8Scales - 1)) * 2 * kPgKeys);
+          to[lane] = ks[j];
+          to[lane + 32] = vs[j];
+          __syncwarp();
+          if (lane == 0) mbar_arrive(scfull(blk));
+          ++blk;
+        }
+      }
+      if (!ok) break;
+    }
+  } else if (warp == 6) {
+    // ------------------------------------------------------------ walks the line, and makes the queries' terms
+    constexpr int kLanes = D / 8, kAt = 32 / kLanes, kAhead = 2;  // lanes of a row, rows at a time, loads in flight
+    const int sub = lane % kLanes;
+    bool ok = true;
+    auto wait = [&](uint32_t bar, int parity, int code) {
+      if (ok) ok = mbar_wait_abort(bar, parity & 1, a.b.err, code, abort);
+      ok = __all_sync(0xffffffffu, ok);
+    };
+    int64_t at = begin;
+    int i = misc[2], h = misc[3], o = misc[4];
+    r = *reinterpret_cast<const PgReq*>(smem + Lay::mx);
+    __syncwarp();
+    // Names the next piece of the line, or its end (0 blocks). The others then know of it while the one before is under
+    // way, and have its page entries, scales and queries at hand when they come to it.
+    auto publish = [&](int seg) {
+      if (seg >= 4) wait(segempty(seg), (seg >> 2) - 1, kErrWaitEmpty);
+      if (!ok) return;
+      F8Seg g = {};
+      if (at < end) {
+        const int nblk = f8_blocks(a.s, r), take = (int)min(end - at, (int64_t)(nblk - o));
+        const int64_t first = at - o;
+        g.row0 = r.row0;
+        g.ntok = r.n;
+        g.pos0 = r.pos0;
+        g.kv = r.kv;
+        g.head = h;
+        g.j0 = o;
+        g.nb = take;
+        g.whole = take == nblk;
+        g.slot = 2 * cta + (o > 0 ? 0 : 1);
+        g.c0 = line.owner(first);
+        g.nc = line.owner(first + nblk - 1) - g.c0 + 1;
+        g.request = i;
+        at += take;
+        o = 0;
+        if (at < end && ++h == a.b.nkv) {
+          h = 0;
+          do r = request(++i);
+          while (f8_blocks(a.s, r) == 0);
+        }
+      }
+      if (lane == 0) {
+        segs[seg & 3] = g;
+        mbar_arrive(segfull(seg));
+      }
+      __syncwarp();
+    };
+    publish(0);
+#pragma unroll 1
+    for (int seg = 0; ok; ++seg) {
+      const F8Seg g = segs[seg & 3];
+      if (g.nb == 0) break;
+      publish(seg + 1);
+      if (seg >= 2) wait(qempty(seg), (seg >> 1) - 1, kErrWaitEmpty);
       if (!ok) break;
       const int rows = g.ntok * a.s.group, step = rows <= 4 ? 4 : kFewRows;
       char* const to = smem + Lay::q + (seg & 1) * Lay::kQ;
 #pragma unroll 1
-      for (int c0 = (warp - 10) * kAt; c0 < rows; c0 += 2 * kAt) {
-        const int c = min(c0 + lane / kLanes, rows - 1);  // (past the last row: that one again)
-        const int tok = (c * a.inv_group) >> 16, hq = g.head * a.s.group + c - tok * a.s.group;
-        const uint4 u = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + (g.row0 + tok) * a.ldq +
-                                                        (int64_t)hq * D + 8 * sub);
-        float x[8], most = 0.f;
+      for (int c0 = 0; c0 < rows; c0 += kAhead * kAt) {
+        uint4 u[kAhead];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float2 f = Elem<T>::unpack((&u.x)[k]);
-          x[2 * k] = f.x;
-          x[2 * k + 1] = f.y;
+        for (int y = 0; y < kAhead; ++y) {
+          const int c = min(c0 + y * kAt + lane / kLanes, rows - 1);  // (past the last row: that one again)
+          const int tok = (c * a.inv_group) >> 16, hq = g.head * a.s.group + c - tok * a.s.group;
+          u[y] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + (g.row0 + tok) * a.ldq + (int64_t)hq * D + 8 * sub);
         }
 #pragma unroll
-        for (int k = 0; k < 8; ++k) most = fmaxf(most, fabsf(x[k]) <= FLT_MAX ? fabsf(x[k]) : 0.f);
-#pragma unroll
-        for (int o = kLanes / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-        // the row's largest comes to (224, 448] (or less, where it is below 2^-100); what is not finite is NaN
-        const int e = max((int)(__float_as_uint(most) >> 23) - 127 - 8 + ((__float_as_uint(most) & 0x7fffffu) > 0x600000u ? 1 : 0), -110);
-        const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] = fabsf(x[k]) <= FLT_MAX ? x[k] * inv : __uint_as_float(0x7fffffffu);
-#pragma unroll
-        for (int t = 0; t < kTQ; ++t) {
-          uint32_t w[4];
+        for (int y = 0; y < kAhead; ++y) {
+          const int c = min(c0 + y * kAt + lane / kLanes, rows - 1);
+          float x[8], most = 0.f;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            w[k] = __nv_cvt_float2_to_fp8x2(make_float2(x[2 * k], x[2 * k + 1]), __NV_SATFINITE, __NV_E4M3);
-            const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)w[k], __NV_E4M3);
-            const float2 f = __half22float2(__half2(h));
-            x[2 * k] = (x[2 * k] - f.x) * 16.f;
-            x[2 * k + 1] = (x[2 * k + 1] - f.y) * 16.f;
+            const float2 f = Elem<T>::unpack((&u[y].x)[k]);
+            x[2 * k] = f.x;
+            x[2 * k + 1] = f.y;
           }
-          const int n = t * step + c, sw = D == 128 ? n & 7 : (n >> 1) & 3;
-          *reinterpret_cast<uint2*>(to + n * D + (((sub >> 1) ^ sw) << 4) + (sub & 1) * 8) =
-              make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) most = fmaxf(most, fabsf(x[k]) <= FLT_MAX ? fabsf(x[k]) : 0.f);
+#pragma unroll
+          for (int n = kLanes / 2; n > 0; n >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, n));
+          // the row's largest comes to (224, 448] (or less, where it is below 2^-100); what is not finite is NaN
+          const int e = max((int)(__float_as_uint(most) >> 23) - 127 - 8 + ((__float_as_uint(most) & 0x7fffffu) > 0x600000u ? 1 : 0), -110);
+          const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) x[k] = fabsf(x[k]) <= FLT_MAX ? x[k] * inv : __uint_as_float(0x7fffffffu);
+#pragma unroll
+          for (int t = 0; t < kTQ; ++t) {
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              w[k] = __nv_cvt_float2_to_fp8x2(make_float2(x[2 * k], x[2 * k + 1]), __NV_SATFINITE, __NV_E4M3);
+              const __half2_raw f2 = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)w[k], __NV_E4M3);
+              const float2 f = __half22float2(__half2(f2));
+              x[2 * k] = (x[2 * k] - f.x) * 16.f;
+              x[2 * k + 1] = (x[2 * k + 1] - f.y) * 16.f;
+            }
+            const int n = t * step + c, sw = D == 128 ? n & 7 : (n >> 1) & 3;
+            *reinterpret_cast<uint2*>(to + n * D + (((sub >> 1) ^ sw) << 4) + (sub & 1) * 8) =
+                make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+          }
+          if (sub == 0) reinterpret_cast<float*>(smem + Lay::qs)[(seg & 1) * kFewRows + c] = __uint_as_float((uint32_t)(127 + e) << 23);
         }
-        if (sub == 0) reinterpret_cast<float*>(smem + Lay::qs)[(seg & 1) * kFewRows + c] = __uint_as_float((uint32_t)(127 + e) << 23);
       }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(q8full(seg));
     }
   } else {
-    // ------------------------------------------------------------ softmax and epilogue: every second block
-    const int x = warp >> 2, r = 32 * (warp & 3) + lane, wg = warp & 3;  // (r: the key, or the dim of O^T)
+    // ------------------------------------------------------------ softmax and epilogue
+    const int r = tid, wg = warp;  // r: the key, or the dim of O^T
     const uint32_t lane_off = (uint32_t)(32 * wg) << 16;
-    int cnt = 0, b0 = 0, meets = 0, joins = 0;  // blocks of this group, of all units so far
+    int b = 0, meets = 0;  // blocks of all units so far
     bool ok = true;
     auto wait = [&](uint32_t bar, int parity) {
       if (ok) ok = mbar_wait_abort(bar, parity & 1, a.b.err, kErrWaitFull, abort);
       ok = __all_sync(0xffffffffu, ok);
     };
-    auto meet = [&]() {  // the four warps of this group; bounded, unlike a named barrier
+    auto meet = [&]() {  // the four warps; bounded, unlike a named barrier
       __syncwarp();
-      if (lane == 0) mbar_arrive(group(x));
-      wait(group(x), meets++);
+      if (lane == 0) mbar_arrive(group);
+      wait(group, meets++);
     };
     float2* const pm = reinterpret_cast<float2*>(a.partials + (int64_t)2 * gridDim.x * kFewRows * D);
-    float4* const mx = reinterpret_cast<float4*>(smem + Lay::mx) + x * kFewRows;
     float4* const sums = reinterpret_cast<float4*>(smem + Lay::sums);
-    float* const mb = reinterpret_cast<float*>(smem + Lay::mb);
-    char* const p_to = smem + Lay::p + x * Lay::kP + (r & 15);
     auto unit = [&](auto cols, const F8Seg& g, int seg) __attribute__((always_inline)) {
-      constexpr int kC = decltype(cols)::value, kSc = f8_cols(kC * kTQ), kOc = f8_cols(kC * kTP);
-      const int rows = g.ntok * a.s.group, jf = (b0 ^ x) & 1;  // this group's first block
-      const bool joined = g.nb > 1;
+      constexpr int kC = decltype(cols)::value;
+      const int rows = g.ntok * a.s.group;
       wait(q8full(seg), seg >> 1);
       if (!ok) return;
       const float sc = lane < rows ? reinterpret_cast<const float*>(smem + Lay::qs)[(seg & 1) * kFewRows + lane] * a.scale_log2 : 0.f;
       __syncwarp();
       if (lane == 0) mbar_arrive(qempty(seg));
-      if (jf >= g.nb) return;
-      float m = -INFINITY;  // of row `lane`
+      float m = -INFINITY;  // of row `lane`, the same in all four warps
       float l[kC];          // of every row, this thread's keys
 #pragma unroll
       for (int c = 0; c < kC; ++c) l[c] = 0.f;
 #pragma unroll 1
-      for (int j = jf; j < g.nb; j += 2, ++cnt) {
-        const int b = b0 + j;
+      for (int j = 0; j < g.nb; ++j, ++b) {
         wait(scfull(b), b / kF8Scales);
         if (!ok) return;
         const uint8_t* const two = reinterpret_cast<const uint8_t*>(smem) + Lay::sc + (b & (kF8Scales - 1)) * 2 * kPgKeys;
         const float ks = __uint_as_float((uint32_t)two[r] << 23), ev = (float)two[kPgKeys + r] - 127.f;
         __syncwarp();
         if (lane == 0) mbar_arrive(scempty(b));
-        wait(sfull(x), cnt);
+        wait(sfull(b & 1), b >> 1);
         if (!ok) return;
         tc_fence_after();
         float t[kC];  // the weights' exponents, in twos
         {
-          uint32_t sv[kSc];
-          f8_load<kSc>(tS(x) + lane_off, sv);
+          f8_terms<kC, kTQ>(tS(b & 1) + lane_off, 0.0625f, t);
 #pragma unroll
-          for (int c = 0; c < kC; ++c) {
-            float s = __uint_as_float(sv[c + (kTQ - 1) * kC]);
-#pragma unroll
-            for (int q = kTQ - 2; q >= 0; --q) s = fmaf(s, 0.0625f, __uint_as_float(sv[c + q * kC]));
-            t[c] = fmaf(s * ks, __shfl_sync(0xffffffffu, sc, c), ev);
-          }
+          for (int c = 0; c < kC; ++c) t[c] = fmaf(t[c] * ks, __shfl_sync(0xffffffffu, sc, c), ev);
         }
         const int key0 = (g.j0 + j) * kPgKeys;
         if (key0 + kPgKeys > min(g.kv, g.pos0 + 1)) {  // some row sees only a part of this block
@@ -639,6 +689,8 @@ __global__ void __launch_bounds__(kF8Threads, 1) paged_few8_kernel(const __grid_
           const float v = redux_max(t[c]);
           top = lane == c ? v : top;
         }
+        // (a warp may write the next block's before the others have read this one's)
+        float4* const mx = reinterpret_cast<float4*>(smem + Lay::mx) + (b & 1) * kFewRows;
         if (lane < rows) reinterpret_cast<float*>(mx + lane)[wg] = top;
         meet();
         if (!ok) return;
@@ -647,24 +699,28 @@ __global__ void __launch_bounds__(kF8Threads, 1) paged_few8_kernel(const __grid_
           const float4 v = mx[lane];
           mn = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
         }
-        if (__any_sync(0xffffffffu, mn > m + 8.f)) {  // the same in every warp of the group
+        if (__any_sync(0xffffffffu, mn > m + 8.f)) {  // the same in every warp
           const float m_to = fmaxf(m, mn), alpha = m_to == -INFINITY ? 1.f : exp2f(m - m_to);
           m = m_to;
-          if (j > jf) {
-            uint32_t o[kOc];
-            f8_load<kOc>(tO(x) + lane_off, o);
+          if (j > 0) {
+            wait(odone((b - 1) & 1), (b - 1) >> 1);  // the sums with every block before this one
+            if (!ok) return;
+            tc_fence_after();
 #pragma unroll
-            for (int c = 0; c < kC; ++c) {
-              const float f = __shfl_sync(0xffffffffu, alpha, c);
+            for (int c = 0; c < kC; ++c) l[c] *= __shfl_sync(0xffffffffu, alpha, c);
+#pragma unroll 1
+            for (int i = 0; i < f8_cols(kC * kTP); i += 16) {
+              uint32_t o[16];
+              f8_load<16>(tO + lane_off + i, o);
 #pragma unroll
-              for (int q = 0; q < kTP; ++q) o[c + q * kC] = __float_as_uint(__uint_as_float(o[c + q * kC]) * f);
-              l[c] *= f;
+              for (int c = 0; c < 16; ++c)
+                o[c] = __float_as_uint(__uint_as_float(o[c]) * __shfl_sync(0xffffffffu, alpha, c & (kC - 1)));
+              tmem_st16(tO + lane_off + i, o);
             }
-#pragma unroll
-            for (int i = 0; i < kOc; i += 16) tmem_st16(tO(x) + lane_off + i, o + i);
           }
         }
         const float nm = m == -INFINITY ? (float)kF8Bias : kF8Bias - m, per_code = exp2f(-ev);
+        char* const p_to = smem + Lay::p + (b & 1) * Lay::kP + (r & 15);  // (the product of two blocks ago has been done)
 #pragma unroll
         for (int c = 0; c < kC; c += 2) {
           float2 p;
@@ -689,11 +745,8 @@ __global__ void __launch_bounds__(kF8Threads, 1) paged_few8_kernel(const __grid_
         tc_fence_before();
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(pfull(x));
+        if (lane == 0) mbar_arrive(pfull(b & 1));
       }
-      wait(odone(x), cnt - 1);
-      if (!ok) return;
-      tc_fence_after();
       {  // the warps' sums of every row, side by side
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1)
@@ -702,62 +755,33 @@ __global__ void __launch_bounds__(kF8Threads, 1) paged_few8_kernel(const __grid_
         float mine = 0.f;
 #pragma unroll
         for (int c = 0; c < kC; ++c) mine = lane == c ? l[c] : mine;
-        if (lane < rows) reinterpret_cast<float*>(sums + x * kFewRows + lane)[wg] = mine;
-      }
-      if (x == 1 && joined) {  // A's warps (same lanes of tensor memory) take O_B from here
-        if (wg == 0 && lane < rows) mb[lane] = m;
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(join);
-        return;
+        if (lane < rows) reinterpret_cast<float*>(sums + lane)[wg] = mine;
       }
       meet();
-      if (ok && joined) wait(join, joins++);
+      wait(odone((b - 1) & 1), (b - 1) >> 1);
       if (!ok) return;
       tc_fence_after();
-      float ov[kC], ob[kC];
-      auto load_o = [&](int y, float* v) {
-        uint32_t o[kOc];
-        f8_load<kOc>(tO(y) + lane_off, o);
-#pragma unroll
-        for (int c = 0; c < kC; ++c) {
-          v[c] = __uint_as_float(o[c + (kTP - 1) * kC]);
-#pragma unroll
-          for (int q = kTP - 2; q >= 0; --q) v[c] = fmaf(v[c], 0.125f, __uint_as_float(o[c + q * kC]));
-        }
-      };
-      load_o(x, ov);
-      if (joined) load_o(1, ob);
-      float fa = 1.f, fb = 0.f;
+      float ov[kC];
+      f8_terms<kC, kTP>(tO + lane_off, 0.125f, ov);
+      tc_fence_before();
+      float inv = 1.f;
       int64_t row_at = 0;  // of row `lane`, in elements
       if (lane < rows) {
-        const float4 s = sums[x * kFewRows + lane];
-        float L = (s.x + s.y) + (s.z + s.w), M = m;
-        if (joined) {
-          const float4 s2 = sums[kFewRows + lane];
-          const float m2 = mb[lane], mn = fmaxf(M, m2);
-          fa = mn == -INFINITY ? 1.f : exp2f(M - mn);
-          fb = mn == -INFINITY ? 0.f : exp2f(m2 - mn);
-          L = L * fa + ((s2.x + s2.y) + (s2.z + s2.w)) * fb;
-          M = mn;
-        }
+        const float4 s = sums[lane];
+        const float L = (s.x + s.y) + (s.z + s.w);
         const int tok = (lane * a.inv_group) >> 16, hq = g.head * a.s.group + lane - tok * a.s.group;
         row_at = (g.row0 + tok) * a.ldo + (int64_t)hq * D;
         if (g.whole) {
-          const float inv = pg_inverse(L);
-          fa *= inv;
-          fb *= inv;
-          if (wg == 0 && a.lse) a.lse[(g.row0 + tok) * a.ld_lse + hq] = pg_lse(M - kF8Bias, L);
+          inv = pg_inverse(L);
+          if (wg == 0 && a.lse) a.lse[(g.row0 + tok) * a.ld_lse + hq] = pg_lse(m - kF8Bias, L);
         } else if (wg == 0) {
-          __stcg(pm + (int64_t)g.slot * kFewRows + lane, make_float2(M, L));
+          __stcg(pm + (int64_t)g.slot * kFewRows + lane, make_float2(m, L));
         }
       }
 #pragma unroll
       for (int c = 0; c < kC; ++c) {
-        float v = ov[c] * __shfl_sync(0xffffffffu, fa, c);
-        const float f = __shfl_sync(0xffffffffu, fb, c);
+        const float v = ov[c] * __shfl_sync(0xffffffffu, inv, c);
         const int64_t to = __shfl_sync(0xffffffffu, row_at, c);
-        if (joined) v = fmaf(ob[c], f, v);
         if (c < rows && r < D) {
           if (g.whole)
             reinterpret_cast<uint16_t*>(a.out)[to + r] = (uint16_t)Elem<T>::pack(v, 0.f);
@@ -765,24 +789,18 @@ __global__ void __launch_bounds__(kF8Threads, 1) paged_few8_kernel(const __grid_
             __stcg(a.partials + ((int64_t)g.slot * kFewRows + c) * D + r, v);
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(ofree(x));
-        if (joined) mbar_arrive(ofree(1));
-      }
       if (g.whole) return;
       // a cut unit: whoever finishes last joins the pieces. Their stores are made visible by the barrier and the
       // ticket (release is cumulative)
       meet();
       if (!ok) return;
       if (r == 0) {
-        const bool last = atom_add_acq_rel(a.tickets + 2 * g.c0, 1) == g.nc - 1;
-        if (last) a.tickets[2 * g.c0] = 0;
-        misc[10 + x] = last;
+        const bool last = atom_add_acq_rel(a.tickets + g.c0, 1) == g.nc - 1;
+        if (last) a.tickets[g.c0] = 0;
+        misc[10] = last;
       }
       meet();
-      if (ok && misc[10 + x]) f8_join<T, D>(a, g, r, rows);
+      if (ok && misc[10]) f8_join<T, D>(a, g, r, rows);
     };
 #pragma unroll 1
     for (int seg = 0;; ++seg) {
@@ -797,19 +815,16 @@ __global__ void __launch_bounds__(kF8Threads, 1) paged_few8_kernel(const __grid_
       else
         unit(Const<kFewRows>(), g, seg);
       if (!ok) break;
-      b0 += g.nb;
     }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 9) tmem_dealloc(tmem, 256);
+  if (warp == 5) tmem_dealloc(tmem, 256);
   if (tid == 0) {  // no copy may still be writing shared memory when the CTA exits
-    const int n = misc[8], k = misc[9];
+    const int n = misc[8];
     for (int it = max(n - kSlots, 0); it < n; ++it)
       if (!mbar_wait(full(it % kSlots), (it / kSlots) & 1, a.b.err, kErrDrain)) break;
-    for (int it = max(k - kF8Scales, 0); it < k; ++it)
-      if (!mbar_wait(scfull(it), (it / kF8Scales) & 1, a.b.err, kErrDrain)) break;
   }
 }
 
@@ -852,7 +867,7 @@ int launch_few8(const Paged8Call& c, bool alone) {
                       : (D == 128 ? F8Lay<__half, 128>::total : F8Lay<__half, 64>::total);
   const int rc = set_max_dynamic_smem(fn, smem);
   if (rc != QD_OK) return rc;
-  return launch_kernel(fn, dim3((unsigned)c.grid), dim3(kF8Threads), smem, c.pdl, c.stream, &a);
+  return launch_kernel(fn, dim3((unsigned)(kF8Resident * c.grid)), dim3(kF8Threads), smem, c.pdl, c.stream, &a);
 }
 
 }  // namespace qd
