@@ -36,6 +36,7 @@ namespace qd {
 constexpr int kF8Threads = 256;  // warps 0-3 softmax, 4 producer, 5 MMA, 6 the line and the queries, 7 the scales
 constexpr int kF8Resident = 2;   // CTAs an SM
 constexpr int kF8Scales = 8;     // blocks whose scales are in shared memory
+constexpr int kF8Unit = 2;       // blocks' time that a unit's start and end take
 constexpr int kF8Bias = 7;       // P' is up to 2^(8 + 7): the upper end of E5M2's range
 
 template <typename T, int D>
@@ -136,10 +137,24 @@ __device__ __forceinline__ void f8_terms(uint32_t taddr, float step, float* v) {
   }
 }
 
+// whether the phase with `parity` has completed, without waiting
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
 // one request's blocks in this kernel (0: not its)
 __device__ __forceinline__ int f8_blocks(const PgShape& s, const PgReq& r) {
   return r.n > 0 && r.n <= s.tpf ? pg_max((pg_min(r.kv, r.pos0 + r.n) + kPgKeys - 1) / kPgKeys, 1) : 0;
 }
+
+// and places on the line for each KV head: the unit's own, then a block each
+__device__ __forceinline__ int f8_places(int blocks) { return blocks ? blocks + kF8Unit : 0; }
 
 // Joins a cut unit's pieces in the order of their keys: a row per D / 4 lanes of four warps, eight pieces in flight.
 template <typename T, int D>
@@ -256,7 +271,7 @@ __global__ void __launch_bounds__(kF8Threads, kF8Resident) paged_few8_kernel(con
   for (int i = i0; i < i1; ++i) {
     r = request(i);
     const int nb = f8_blocks(a.s, r);
-    mine += (int64_t)a.b.nkv * nb;
+    mine += (int64_t)a.b.nkv * f8_places(nb);
     if (nb && r.kv != r.pos0 + r.n) flags |= QD_DEVERR_PAGE;
     if (a.alone && r.n > a.s.tpf) flags |= QD_DEVERR_POS;
   }
@@ -286,12 +301,12 @@ __global__ void __launch_bounds__(kF8Threads, kF8Resident) paged_few8_kernel(con
     int i = i0;
     if (per > 1) {
       for (r = request(i);; r = request(++i)) {
-        const int64_t c = (int64_t)a.b.nkv * f8_blocks(a.s, r);
+        const int64_t c = (int64_t)a.b.nkv * f8_places(f8_blocks(a.s, r));
         if (w < c) break;
         w -= c;
       }
     }
-    const int nb = f8_blocks(a.s, r);
+    const int nb = f8_places(f8_blocks(a.s, r));
     misc[2] = i;
     misc[3] = (int)(w / nb);
     misc[4] = (int)(w % nb);
@@ -363,110 +378,80 @@ __global__ void __launch_bounds__(kF8Threads, kF8Resident) paged_few8_kernel(con
       if (!ok) break;
     }
   } else if (warp == 5) {
-    // ------------------------------------------------------------ MMA: one elected lane waits and issues
+    // ------------------------------------------------------------ MMA: one elected lane, whatever is ready first
     constexpr uint32_t hi = f8_desc_hi<D>(), hi_p = f8_desc_hi<128>(), kItem16 = Lay::kItem >> 4;
-    const uint32_t d_q = umma_desc_lo(sb + Lay::q), d_k = umma_desc_lo(sb + Lay::kv), d_p = umma_desc_lo(sb + Lay::p);
-    // heads of 64: the 64 upper rows of O^T repeat the lower ones (block stride 0)
-    const uint32_t d_v = umma_desc_lo(sb + Lay::kv, 0);
-    int slot = 0;  // of the next V product's K block
-    uint32_t phase = 0;
-    int s_seg = 0, s_left = 0, s_blk = 0, s_slot = 0;  // of the next scores
-    uint32_t s_phase = 0, s_id = 0;
-    bool s_end = false, ok = true;
-    const bool leader = elect_one();
-    auto wait = [&](uint32_t bar, int parity) {
-      if (ok) ok = mbar_wait_abort(bar, parity & 1, a.b.err, kErrWaitFull, abort);
-    };
-    // the scores of the next block on the line, whichever unit's it is
-    auto next_scores = [&]() {
-      if (s_end || !ok) return;
-      if (s_left == 0) {
-        wait(segfull(s_seg), s_seg >> 2);
-        if (!ok) return;
-        const F8Seg& g = segs[s_seg & 3];
-        s_left = g.nb;
-        if (s_left == 0) {
-          s_end = true;
-          return;
+    if (elect_one()) {
+      const uint32_t d_q = umma_desc_lo(sb + Lay::q), d_k = umma_desc_lo(sb + Lay::kv), d_p = umma_desc_lo(sb + Lay::p);
+      // heads of 64: the 64 upper rows of O^T repeat the lower ones (block stride 0)
+      const uint32_t d_v = umma_desc_lo(sb + Lay::kv, 0);
+      struct Side {  // of the next scores, and of the next product with V: segment, blocks left of it, block, its slot
+        int seg, left, blk, slot;
+        uint32_t phase, id;
+      };
+      Side s = {0, 0, 0, 0, 0, 0}, v = {0, 0, 0, 1, 0, 0};
+      auto step = [&](Side& x) {
+        ++x.blk;
+        x.slot += 2;
+        if (x.slot >= kSlots) {
+          x.slot -= kSlots;
+          x.phase ^= 1;
         }
-        s_id = g.ntok * a.s.group <= 4 ? f8_idesc(f8_cols(4 * kTQ), false, false) : f8_idesc(kFewRows * kTQ, false, false);
-        wait(q8full(s_seg), s_seg >> 1);
-      }
-      const int x = s_blk & 1;
-      wait(full(s_slot), s_phase);
-      tc_fence_after();
-      if (ok) {
-        const uint32_t qt = d_q + (s_seg & 1) * (Lay::kQ >> 4), kt = d_k + s_slot * kItem16;
+      };
+      bool s_end = false, first = false, ok = true;
+      uint64_t t0 = globaltimer();
+      for (uint32_t idle = 0; ok; ++idle) {
+        if (v.left == 0 && (v.blk < s.blk || s_end)) {  // (its segment is known: the scores are ahead)
+          const F8Seg& g = segs[v.seg & 3];
+          v.left = g.nb;
+          if (v.left == 0) break;
+          v.id = g.ntok * a.s.group <= 4 ? f8_idesc(f8_cols(4 * kTP), true, true) : f8_idesc(kFewRows * kTP, true, true);
+          first = true;
+        }
+        if (v.blk < s.blk && mbar_test(pfull(v.blk & 1), (v.blk >> 1) & 1) && mbar_test(full(v.slot), v.phase)) {
+          tc_fence_after();
+          const uint32_t vt = d_v + v.slot * kItem16, pt = d_p + (v.blk & 1) * (Lay::kP >> 4);
 #pragma unroll
-        for (int d = 0; d < D / 32; ++d) umma_f8<hi, hi>(tS(x), kt + 2 * d, qt + 2 * d, s_id, d > 0 ? 1u : 0u);
+          for (int k = 0; k < 4; ++k)  // 32 keys per MMA: four groups of 8 rows of V
+            umma_f8<hi, hi_p>(tO, vt + k * (32 * D >> 4), pt + 2 * k, v.id, k || !first ? 1u : 0u);
+          first = false;
+          umma_commit(odone(v.blk & 1));
+          umma_commit(empty(v.slot));
+          step(v);
+          if (--v.left == 0) mbar_arrive(segempty(v.seg++));
+          idle = 0;
+        }
+        if (s.left == 0 && !s_end && mbar_test(segfull(s.seg), (s.seg >> 2) & 1)) {
+          const F8Seg& g = segs[s.seg & 3];
+          s.left = g.nb;
+          s_end = s.left == 0;
+          s.id = g.ntok * a.s.group <= 4 ? f8_idesc(f8_cols(4 * kTQ), false, false) : f8_idesc(kFewRows * kTQ, false, false);
+        }
+        if (s.left > 0 && s.blk < v.blk + 2 && mbar_test(q8full(s.seg), (s.seg >> 1) & 1) && mbar_test(full(s.slot), s.phase)) {
+          tc_fence_after();
+          const uint32_t qt = d_q + (s.seg & 1) * (Lay::kQ >> 4), kt = d_k + s.slot * kItem16;
+#pragma unroll
+          for (int d = 0; d < D / 32; ++d) umma_f8<hi, hi>(tS(s.blk & 1), kt + 2 * d, qt + 2 * d, s.id, d > 0 ? 1u : 0u);
+          umma_commit(sfull(s.blk & 1));
+          umma_commit(empty(s.slot));
+          step(s);
+          if (--s.left == 0) umma_commit(qempty(s.seg++));
+          idle = 0;
+        }
+        if (idle == 0) t0 = globaltimer();
+        if ((idle & 63u) == 63u) {  // bounded, as every wait
+          if (*reinterpret_cast<volatile int*>(abort)) ok = false;
+          if (globaltimer() - t0 > kWaitLimitNs) {
+            if (a.b.err) atomicOr(a.b.err, kErrWaitFull);
+            atomicExch(abort, 1);
+            ok = false;
+          }
+        }
       }
-      umma_commit(sfull(x));
-      umma_commit(empty(s_slot));
-      ++s_blk;
-      s_slot += 2;
-      if (s_slot >= kSlots) {
-        s_slot -= kSlots;
-        s_phase ^= 1;
-      }
-      if (--s_left == 0) umma_commit(qempty(s_seg++));
-    };
-    // `rows` of V are keys; the ones past them hold anything and are zeroed (the whole warp comes here)
-    auto zero_v = [&](int rows, int s, uint32_t ph) {
-      if (leader) wait(full(s), ph);
-      __syncwarp();
-      char* const vt = smem + Lay::kv + s * Lay::kItem;
-#pragma unroll 1
-      for (int c = max(rows, 0) * (D / 16) + lane; c < kPgKeys * (D / 16); c += 32)
-        *reinterpret_cast<uint4*>(vt + 16 * c) = make_uint4(0u, 0u, 0u, 0u);
-      fence_proxy_async_smem();
-      __syncwarp();
-    };
-    if (leader) {
-      next_scores();
-      next_scores();
+      // no MMA may still run when its memory is given back
+      if (s.blk > 0) mbar_wait(sfull((s.blk - 1) & 1), ((s.blk - 1) >> 1) & 1, a.b.err, kErrDrain);
+      if (v.blk > 0) mbar_wait(odone((v.blk - 1) & 1), ((v.blk - 1) >> 1) & 1, a.b.err, kErrDrain);
     }
     __syncwarp();
-    int b = 0;
-#pragma unroll 1
-    for (int seg = 0;; ++seg) {
-      wait(segfull(seg), seg >> 2);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      const int nb = segs[seg & 3].nb, keys = segs[seg & 3].kv - segs[seg & 3].j0 * kPgKeys;
-      const bool four = segs[seg & 3].ntok * a.s.group <= 4;
-      __syncwarp();
-      if (nb == 0) break;
-      const uint32_t id = four ? f8_idesc(f8_cols(4 * kTP), true, true) : f8_idesc(kFewRows * kTP, true, true);
-#pragma unroll 1
-      for (int j = 0; j < nb; ++j, ++b) {
-        const int x = b & 1, v = slot + 1 == kSlots ? 0 : slot + 1;
-        const uint32_t v_phase = slot + 1 == kSlots ? phase ^ 1u : phase;
-        const int rows = keys - j * kPgKeys;
-        if (rows < kPgKeys) zero_v(rows, v, v_phase);
-        if (leader) {
-          wait(full(v), v_phase);
-          wait(pfull(x), b >> 1);  // (a unit's first: its rows have taken the last unit's sums by then)
-          tc_fence_after();
-          if (ok) {
-            const uint32_t vt = d_v + v * kItem16, pt = d_p + x * (Lay::kP >> 4);
-#pragma unroll
-            for (int k = 0; k < 4; ++k)  // 32 keys per MMA: four groups of 8 rows of V
-              umma_f8<hi, hi_p>(tO, vt + k * (32 * D >> 4), pt + 2 * k, id, k || j ? 1u : 0u);
-          }
-          umma_commit(odone(x));
-          umma_commit(empty(v));
-          next_scores();
-        }
-        slot += 2;
-        if (slot >= kSlots) {
-          slot -= kSlots;
-          phase ^= 1;
-        }
-        __syncwarp();
-      }
-      if (lane == 0) mbar_arrive(segempty(seg));  // (the scores are at most two blocks ahead, in a ring of four)
-    }
-    if (leader && s_blk > 0) mbar_wait(sfull((s_blk - 1) & 1), ((s_blk - 1) >> 1) & 1, a.b.err, kErrDrain);
-    if (leader && b > 0) mbar_wait(odone((b - 1) & 1), ((b - 1) >> 1) & 1, a.b.err, kErrDrain);  // no MMA may still run when its memory is given back
   } else if (warp == 7) {
     // ------------------------------------------------------------ the rows' powers of two, four keys a lane
     constexpr int kAhead = 4;  // blocks whose loads are in flight (entries, then scales: two waits for memory)
@@ -535,18 +520,18 @@ __global__ void __launch_bounds__(kF8Threads, kF8Resident) paged_few8_kernel(con
       if (seg >= 4) wait(segempty(seg), (seg >> 2) - 1, kErrWaitEmpty);
       if (!ok) return;
       F8Seg g = {};
-      if (at < end) {
-        const int nblk = f8_blocks(a.s, r), take = (int)min(end - at, (int64_t)(nblk - o));
-        const int64_t first = at - o;
+      while (at < end && g.nb == 0) {  // (a CTA whose share ends in a unit's own places has no block of it)
+        const int nblk = f8_blocks(a.s, r), take = (int)min(end - at, (int64_t)(f8_places(nblk) - o));
+        const int64_t first = at - o + kF8Unit;  // place of the unit's first block
         g.row0 = r.row0;
         g.ntok = r.n;
         g.pos0 = r.pos0;
         g.kv = r.kv;
         g.head = h;
-        g.j0 = o;
-        g.nb = take;
-        g.whole = take == nblk;
-        g.slot = 2 * cta + (o > 0 ? 0 : 1);
+        g.j0 = max(o - kF8Unit, 0);
+        g.nb = max(o + take - kF8Unit, 0) - g.j0;
+        g.whole = g.nb == nblk;
+        g.slot = 2 * cta + (g.j0 > 0 ? 0 : 1);
         g.c0 = line.owner(first);
         g.nc = line.owner(first + nblk - 1) - g.c0 + 1;
         g.request = i;
@@ -681,6 +666,16 @@ __global__ void __launch_bounds__(kF8Threads, kF8Resident) paged_few8_kernel(con
               next += a.s.group;
             }
             if (key >= min(lim, g.kv)) t[c] = -INFINITY;
+          }
+          if (key0 + kPgKeys > g.kv) {  // V rows past the last key hold anything: zeroed, since 0 x NaN is NaN
+            const int item = 2 * b + 1, slot = item % kSlots;
+            wait(full(slot), item / kSlots);
+            if (!ok) return;
+            if (key >= g.kv) {
+              char* const row = smem + Lay::kv + slot * Lay::kItem + r * D;
+#pragma unroll
+              for (int i = 0; i < D / 16; ++i) *reinterpret_cast<uint4*>(row + ((i ^ (r & (D / 16 - 1))) << 4)) = make_uint4(0u, 0u, 0u, 0u);
+            }
           }
         }
         float top = -INFINITY;
