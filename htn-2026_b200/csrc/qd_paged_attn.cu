@@ -32,6 +32,12 @@
 // joins them in the order of the keys, so results repeat bit for bit. Every CTA finds its place on the line
 // from cu_tokens and kv_len itself: no planning launch, and no length is needed on the host.
 //
+// Pages of 8 bits (kHeld): requests of few rows have a kernel of their own (qd_paged_few8.cu), which reads the codes as
+// they are. Tiles get 16-bit operands: two warps that have nothing else to do widen each block from a ring of raw blocks
+// into the ring of K and V blocks (a code times a power of two is exact in both 16-bit types), so that the products, the
+// softmax and P are those of 16-bit pages; a block of two tiles takes the tensor cores and the softmax longer than it
+// takes the two warps. Rows past the last key, and of pages that are not there, are written as zeros.
+//
 // Measured, 32 query and 8 KV heads of 128 in BF16: 8 single tokens over up to 41 k keys 183 us (HBM: 6.3 TB/s); 64
 // single tokens over 1 to 1.5 k keys 72 us (4.7 TB/s: each CTA's start and end); one token over 1 k keys 12.3 us in a
 // graph, 14.5 with the keys not in L2 (latency; a call takes the host 11.9); 2048 tokens after 8192 keys 340 to 368 us
@@ -39,6 +45,8 @@
 // tile's softmax and products wait for one another). Heads of 64 in FP16, 14 over 2: the 64 single tokens 33 us, the 8
 // long ones 51. At 168 registers a thread the instances spill: 168 bytes stored and 456 loaded in the code of a
 // thread with heads of 128 (156 and 428 with pages of 16 rows), 120 and 356 with heads of 64.
+#include <cuda_fp8.h>
+
 #include <algorithm>
 #include <climits>
 
@@ -51,7 +59,8 @@
 
 namespace qd {
 
-constexpr int kPgThreads = 384;  // warps 0-3 softmax A, 4-7 softmax B, 8 producer, 9 MMA, 10-11 only start up
+// warps 0-3 softmax A, 4-7 softmax B, 8 producer, 9 MMA, 10-11 only start up, or widen pages of 8 bits
+constexpr int kPgThreads = 384;
 // registers per thread after the start: 2 * 224 + 56 = 3 * 168, what the launch gave the three warpgroups
 constexpr int kPgSoftmaxRegs = 224, kPgOtherRegs = 56;
 constexpr int kPgBox = 128 * 128;  // [128 rows][64 dims] of 16 bits
@@ -74,26 +83,34 @@ struct alignas(64) PagedAttnArgs {
   // (m, l) [slots][2][128]
   float* partials;
   int* tickets;     // [grid][2]
+  // pages of 8 bits: the rows' powers of two, and the fewest tokens of a request that is this kernel's
+  const uint8_t *k_scale, *v_scale;
+  int64_t ss_page, ss_head;
+  int least;
 };
 
-template <int D>
+template <int D, bool kHeld>
 struct PgLayout {
   static constexpr int kItem = D / 64 * kPgBox;  // a K or V block, and a Q tile
-  static constexpr int kSlots = D == 128 ? 5 : 10;
+  static constexpr int kSlots = kHeld ? (D == 128 ? 3 : 6) : D == 128 ? 5 : 10;
+  static_assert(kSlots >= 3, "a pair of tiles holds K and V of a block and the next K");
+  static constexpr int kRawItem = kPgKeys * D, kRaw = kHeld ? (D == 128 ? 4 : 8) : 0;  // blocks of 8 bits
   static constexpr int q = 0;
   static constexpr int kv = q + 2 * kItem;
-  static constexpr int p = kv + kSlots * kItem;  // P of few-row units (head_dim 128: in their Q region)
-  static constexpr int bars = p + (D == 64 ? 2 * kFewP : 0);
+  static constexpr int raw = kv + kSlots * kItem;
+  static constexpr int p = raw + kRaw * kRawItem;  // P of few-row units (head_dim 128: in their Q region)
+  static constexpr int bars = p + (D == 64 && !kHeld ? 2 * kFewP : 0);
   // qfull[2], qempty[2], sfull[2], pfull[2], odone[2], ofree[2], group[2], segfull[4], segempty[4], join,
-  // sload A odd, A even, B, full[slots], empty[slots]
-  static constexpr int nbars = 26 + 2 * kSlots;
+  // sload A odd, A even, B, full[slots], empty[slots], rawfull[], rawempty[]
+  static constexpr int nbars = 26 + 2 * kSlots + 2 * kRaw;
   static constexpr int seg = bars + nbars * 8;  // segment ring
   static constexpr int misc = seg + 4 * 64;     // tmem slot, abort, line start, flags, drain counts
   static constexpr int ml = misc + 192;         // at a unit's end: (m, l) of the odd blocks' rows [128], or the
                                                 // warps' sums of few-row units [2 groups][16 rows][4 warps]
   static constexpr int mx = ml + 1024;          // the warps' maxima of few-row units [2 groups][16][4]
-  static constexpr int mb = mx + 1024;          // the odd blocks' maxima of few-row units [16]
-  static constexpr int total = mb + 128;
+  static constexpr int mb = mx + (kHeld ? 64 : 1024);  // the odd blocks' maxima of few-row units [16]
+  static constexpr int total = mb + (kHeld ? 0 : 128);
+  static_assert(total <= 227 * 1024, "shared memory of an SM");
   // where warpgroup x's P of a few-row unit in Q region `reg` is: Q takes the first 4 KiB of each 64-dim half
   static __device__ __forceinline__ int few_p(int reg, int x) {
     return D == 128 ? q + reg * kItem + 4096 + x * kPgBox : p + x * kFewP;
@@ -108,6 +125,7 @@ struct PgSeg {
   int few;                   // one tile of at most 16 rows
   int slot, c0, nc;          // partial slot, first CTA and number of CTAs of the unit
   int region;                // Q region of a single tile, or -1: both tiles
+  int request;
 };
 static_assert(sizeof(PgSeg) <= 64, "segment ring entry");
 
@@ -151,6 +169,23 @@ __device__ __forceinline__ void tmem_wait_ld64(uint32_t* r) {
 }
 __device__ __forceinline__ PgReq pg_request(const PagedAttnArgs& a, int i) {
   return pg_make_request(a.s, ld_i32(a.b.cu + i), ld_i32(a.b.cu + i + 1), ld_i32(a.b.kv_len + i), (int)a.b.tokens, a.room);
+}
+template <bool kHeld>
+__device__ __forceinline__ PgReq pg_own_request(const PagedAttnArgs& a, int i) {
+  PgReq r = pg_request(a, i);
+  if (kHeld && r.n < a.least) r.n = r.pairs = 0;  // another kernel's
+  return r;
+}
+// Two codes of a row as a pair of 16-bit elements, times the row's power of two: exact.
+template <typename T>
+__device__ __forceinline__ uint32_t pg_widen(uint32_t codes, __half2 scale) {
+  const __half2 h = __hmul2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)codes, __NV_E4M3)), scale);
+  if constexpr (Elem<T>::kBf16) {
+    const float2 f = __half22float2(h);
+    return Elem<T>::pack(f.x, f.y);
+  } else {
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
 }
 
 // Joins a cut few-row unit's pieces (rows of D floats) in the order of their keys: four warps, a row per D / 4
@@ -216,9 +251,9 @@ __device__ __forceinline__ void pg_join_few(const PagedAttnArgs& a, const PgSeg&
 
 // A K or V block in shared memory: the halves of 64 dims, in each the rows of 128 bytes, 8 to a group; or, merged,
 // the groups and in each the halves, so that a page's whole rows are one box of a copy.
-template <typename T, int D, bool kMerged>
+template <typename T, int D, bool kMerged, bool kHeld>
 __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {
-  using Lay = PgLayout<D>;
+  using Lay = PgLayout<D, kHeld>;
   constexpr int kHalves = D / 64, kSlots = Lay::kSlots;
   constexpr uint32_t kGroup = kMerged ? 2048 : 1024, kHalf = kMerged ? 1024 : kPgBox;  // bytes from one to the next
   grid_dep_wait();
@@ -244,6 +279,10 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
   const uint32_t sload_b = bars + 200;
   auto full = [&](int s) { return bars + 208 + 8u * s; };
   auto empty = [&](int s) { return bars + 208 + 8u * (kSlots + s); };
+  // the ring that the copies fill
+  constexpr int kCopied = kHeld ? Lay::kRaw : kSlots;
+  auto copied = [&](int s) { return kHeld ? bars + 208 + 8u * (2 * kSlots + s) : full(s); };
+  auto copied_empty = [&](int s) { return kHeld ? bars + 208 + 8u * (2 * kSlots + kCopied + s) : empty(s); };
   PgSeg* segs = reinterpret_cast<PgSeg*>(smem + Lay::seg);
   int* misc = reinterpret_cast<int*>(smem + Lay::misc);
   int* abort = misc + 1;
@@ -265,11 +304,15 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
     mbar_init(sload_a(1), 4);
     for (int k = 0; k < 4; ++k) {
       mbar_init(segfull(k), 1);
-      mbar_init(segempty(k), 9);  // the MMA warp and eight softmax warps
+      mbar_init(segempty(k), kHeld ? 11 : 9);  // the MMA warp, eight softmax warps, those that widen
     }
     for (int s = 0; s < kSlots; ++s) {
-      mbar_init(full(s), 1);
+      mbar_init(full(s), kHeld ? 2 : 1);
       mbar_init(empty(s), 1);
+    }
+    for (int s = 0; s < Lay::kRaw; ++s) {
+      mbar_init(copied(s), 1);
+      mbar_init(copied_empty(s), 2);
     }
     fence_mbar_init();
     for (int m = 1; m < 12; ++m) misc[m] = 0;  // (the scan comes after them)
@@ -284,7 +327,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
   PgReq r = {};
   bool cut = false, tiles = false, longer = false;
   for (int i = i0; i < i1; ++i) {
-    r = pg_request(a, i);
+    r = pg_own_request<kHeld>(a, i);
     tiles |= r.n > a.s.tpf;
     cut |= r.kv != r.pos0 + r.n && r.n > 0;
     mine += a.b.nkv * pg_sum_cost(a.s, r);
@@ -338,7 +381,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
     int64_t w = begin - before;
     int i = i0;
     if (per > 1) {
-      for (r = pg_request(a, i);; r = pg_request(a, ++i)) {
+      for (r = pg_own_request<kHeld>(a, i);; r = pg_own_request<kHeld>(a, ++i)) {
         const int64_t c = a.b.nkv * (whole ? r.pairs : pg_sum_cost(a.s, r));
         if (w < c) break;
         w -= c;
@@ -364,9 +407,9 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
     int64_t at = begin;
     int i = misc[2], k = misc[3], h = misc[4], o = misc[5];
     // a lane's copy: a page of the block, and a half of its dims unless they are merged
-    constexpr int copies = kMerged ? 1 : kHalves;
+    constexpr int copies = kMerged || kHeld ? 1 : kHalves, row_bytes = kHeld ? D : D * 2;
     const int boxes = (kPgKeys >> a.b.page_shift) * copies;
-    const int box_bytes = a.b.page_size * (D * 2) / copies, my_page = lane / copies, my_half = lane % copies;
+    const int box_bytes = a.b.page_size * row_bytes / copies, my_page = lane / copies, my_half = lane % copies;
     int seg = 0, items = 0, slot = 0, next_region = 0, qfills[2] = {0, 0};
     uint32_t phase = 1;  // of empty(slot): a ring's first round passes at once
     bool ok = true;
@@ -427,6 +470,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
           s->c0 = c0;
           s->nc = c1 - c0 + 1;
           s->region = two ? -1 : ra;
+          s->request = i;
           mbar_arrive(segfull(seg));
         }
         for (int x = 0; x <= (two ? 1 : 0); ++x) ++qfills[two ? x : ra];
@@ -441,22 +485,24 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
             flag_error(a.b.err, QD_DEVERR_PAGE);
             page = -1;  // outside the tensor map: the copy fills zeros
           }
-          const uint32_t at_page = sb + Lay::kv + my_half * kPgBox + my_page * box_bytes;
+          const uint32_t at_page = sb + (kHeld ? Lay::raw : Lay::kv) + my_half * kPgBox + my_page * box_bytes;
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {
-            const bool got = mbar_wait_abort(empty(slot), phase, a.b.err, kErrWaitEmpty, abort);
+            const bool got = mbar_wait_abort(copied_empty(slot), phase, a.b.err, kErrWaitEmpty, abort);
             if (!__all_sync(0xffffffffu, got)) {
               ok = false;
               break;
             }
             if (lane == 0) {
-              mbar_arrive_expect_tx(full(slot), n_need * box_bytes);
+              mbar_arrive_expect_tx(copied(slot), n_need * box_bytes);
               misc[8] = ++items;
             }
             __syncwarp();
-            if (need)
+            if (need && kHeld)
+              pg_tma_4d(at_page + slot * Lay::kRawItem, kv ? &a.tv : &a.tk, 0, 0, h, page, copied(slot), pol);
+            else if (need)
               pg_tma_5d(at_page + slot * Lay::kItem, kv ? &a.tv : &a.tk, my_half, h * a.head_groups, page, full(slot), pol);
-            if (++slot == kSlots) {
+            if (++slot == kCopied) {
               slot = 0;
               phase ^= 1;
             }
@@ -470,7 +516,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
         h = 0;
         if (++k == r.pairs) {
           k = 0;
-          do r = pg_request(a, ++i);
+          do r = pg_own_request<kHeld>(a, ++i);
           while (r.pairs == 0);
         }
       }
@@ -506,8 +552,9 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
       int slot;
       uint32_t phase;
     };
-    auto ahead = [&](int n) {  // the item n places on
+    auto ahead = [&](int n) {  // the item n <= 4 places on
       const int t = slot + n;
+      if (kSlots < 5 && t >= 2 * kSlots) return Ring{t - 2 * kSlots, phase};
       return t >= kSlots ? Ring{t - kSlots, phase ^ 1u} : Ring{t, phase};
     };
     auto advance = [&](int n) {
@@ -563,6 +610,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
     };
     // `rows` of V are keys; the ones past them hold anything and are zeroed (the whole warp comes here)
     auto zero_v = [&](int rows, Ring v) {
+      if constexpr (kHeld) return;  // (they come as zeros)
       if (leader) wait(full(v.slot), v.phase);
       __syncwarp();
       char* const vt = smem + Lay::kv + v.slot * Lay::kItem;
@@ -683,7 +731,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
       if (g.nb == 0) break;
       if (g.region < 0)
         pair_unit(g);
-      else if (g.few)
+      else if (g.few && !kHeld)
         single_unit(g, c1);
       else
         single_unit(g, c0);
@@ -692,6 +740,100 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
     if (leader)  // no MMA may still run when its memory is given back
       for (int x = 0; x < 2; ++x)
         if (pc[x] > 0) mbar_wait(odone(x), (pc[x] - 1) & 1, a.b.err, kErrDrain);
+  } else if constexpr (kHeld) {
+    // ------------------------------------------------------------ blocks of 8 bits to 16: a warp each half of the rows
+    constexpr int kOwn = 2;  // rows of a lane
+    const int row0 = (warp - 10) * 64 + lane;
+    int items = 0;  // blocks of K and V so far
+    bool ok = true;
+    auto wait = [&](uint32_t bar, int parity, int code) {
+      if (ok) ok = mbar_wait_abort(bar, parity & 1, a.b.err, code, abort);
+      ok = __all_sync(0xffffffffu, ok);
+    };
+#pragma unroll 1
+    for (int seg = 0;; ++seg) {
+      wait(segfull(seg), seg >> 2, kErrWaitFull);
+      if (!ok) break;
+      const int head = segs[seg & 3].head, kv = segs[seg & 3].kv, j0 = segs[seg & 3].j0, nb = segs[seg & 3].nb;
+      const int32_t* const table = a.b.table + segs[seg & 3].request * a.b.ld_table;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(segempty(seg));
+      if (nb == 0) break;
+      // this lane's pages of block j (-1: none, or past the last key), and its rows' powers of two (0: none)
+      auto page_of = [&](int j, int o) {
+        const int64_t key = (int64_t)j * kPgKeys + row0 + 32 * o;
+        const int page = j < j0 + nb && key < kv ? ld_i32(table + (key >> a.b.page_shift)) : -1;
+        return page < a.b.n_pages ? page : -1;
+      };
+      auto scale_of = [&](const uint8_t* scale, int page, int o) {
+        return page < 0 ? 0 : (int)__ldcg(scale + page * a.ss_page + head * a.ss_head + ((row0 + 32 * o) & (a.b.page_size - 1)));
+      };
+      int page[kOwn], ks[kOwn], vs[kOwn];
+#pragma unroll
+      for (int o = 0; o < kOwn; ++o) page[o] = page_of(j0, o);
+#pragma unroll
+      for (int o = 0; o < kOwn; ++o) {
+        ks[o] = scale_of(a.k_scale, page[o], o);
+        vs[o] = scale_of(a.v_scale, page[o], o);
+      }
+#pragma unroll 1
+      for (int j = j0; j < j0 + nb && ok; ++j) {
+        int next[kOwn], next_ks[kOwn], next_vs[kOwn];  // under way while this block is widened
+#pragma unroll
+        for (int o = 0; o < kOwn; ++o) next[o] = page_of(j + 1, o);
+#pragma unroll
+        for (int is_v = 0; is_v < 2; ++is_v, ++items) {
+          const int from = items % Lay::kRaw, to = items % kSlots;
+          wait(copied(from), items / Lay::kRaw, kErrWaitFull);
+          wait(empty(to), items / kSlots + 1, kErrWaitEmpty);  // (a ring's first round passes at once)
+          if (!ok) break;
+#pragma unroll
+          for (int o = 0; o < kOwn; ++o) {
+            const int row = row0 + 32 * o, b = is_v ? vs[o] : ks[o];
+            const bool dead = page[o] < 0;
+            const __half2 scale = __float2half2_rn(__uint_as_float((uint32_t)b << 23));
+            const char* const src = smem + Lay::raw + from * Lay::kRawItem + row * D;
+            char* const dst = smem + Lay::kv + to * Lay::kItem + row * 128;
+            const int sw = D == 128 ? row & 7 : (row >> 1) & 3;
+#pragma unroll 2
+            for (int c = 0; c < D / 16; ++c) {
+              const uint4 u = *reinterpret_cast<const uint4*>(src + ((c ^ sw) << 4));
+              uint32_t w[8];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const uint32_t four = (&u.x)[k];
+                w[2 * k] = dead ? 0u : pg_widen<T>(four & 0xffffu, scale);
+                w[2 * k + 1] = dead ? 0u : pg_widen<T>(four >> 16, scale);
+              }
+              char* const half = dst + (c >> 2) * kPgBox;
+              const int c8 = (2 * c) & 7;
+              *reinterpret_cast<uint4*>(half + ((c8 ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+              *reinterpret_cast<uint4*>(half + (((c8 + 1) ^ (row & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(copied_empty(from));
+            mbar_arrive(full(to));
+          }
+          if (is_v == 0)
+#pragma unroll
+            for (int o = 0; o < kOwn; ++o) {
+              next_ks[o] = scale_of(a.k_scale, next[o], o);
+              next_vs[o] = scale_of(a.v_scale, next[o], o);
+            }
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int o = 0; o < kOwn; ++o) {
+          page[o] = next[o];
+          ks[o] = next_ks[o];
+          vs[o] = next_vs[o];
+        }
+      }
+      if (!ok) break;
+    }
   }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPgSoftmaxRegs));
@@ -906,7 +1048,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
       const bool idle = (r & ~31) >= rows;  // no row of this warp is a token's
       float m_used = -INFINITY, l = 0.f;
       const int jf = two ? 0 : x;
-      if (g.few) {
+      if (g.few && !kHeld) {
         if (rows <= 4)
           few_rows(Const<4>(), g, rows, joined);
         else
@@ -1185,8 +1327,8 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
   if (warp == 9) tmem_dealloc(tmem, 512);
   if (tid == 0) {  // no bulk copy may still be writing shared memory when the CTA exits
     const int n = misc[8];
-    for (int it = max(n - kSlots, 0); it < n; ++it)
-      if (!mbar_wait(full(it % kSlots), (it / kSlots) & 1, a.b.err, kErrDrain)) break;
+    for (int it = max(n - kCopied, 0); it < n; ++it)
+      if (!mbar_wait(copied(it % kCopied), (it / kCopied) & 1, a.b.err, kErrDrain)) break;
     for (int x = 0; x < 2; ++x)
       if (misc[6 + x] > 0) mbar_wait(qfull(x), (misc[6 + x] - 1) & 1, a.b.err, kErrDrain);
   }
@@ -1194,9 +1336,61 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
 
 template <typename T>
 static const void* attn_kernel(int head_dim, bool merged) {
-  return head_dim == 64 ? (const void*)paged_attn_kernel<T, 64, false>
-         : merged       ? (const void*)paged_attn_kernel<T, 128, true>
-                        : (const void*)paged_attn_kernel<T, 128, false>;
+  return head_dim == 64 ? (const void*)paged_attn_kernel<T, 64, false, false>
+         : merged       ? (const void*)paged_attn_kernel<T, 128, true, false>
+                        : (const void*)paged_attn_kernel<T, 128, false, false>;
+}
+
+// The maps of q: a tile's rows are token-major, its KV head's query heads inner.
+static int map_queries(PagedAttnArgs& a, PFN_cuTensorMapEncodeTiled_v12000 encode, const void* q, int64_t ldq, int dtype,
+                       int head_dim) {
+  const CUtensorMapDataType type = dtype == QD_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  const cuuint64_t dims[4] = {(cuuint64_t)head_dim, (cuuint64_t)a.s.group, (cuuint64_t)a.b.nkv, (cuuint64_t)a.b.tokens};
+  const cuuint64_t strides[3] = {(cuuint64_t)head_dim * 2, (cuuint64_t)a.s.group * head_dim * 2, (cuuint64_t)ldq * 2};
+  const cuuint32_t toks[3] = {(cuuint32_t)a.s.tpt, (cuuint32_t)(a.s.tpf > 0 ? a.s.tpf : 1), 1};
+  CUtensorMap* const maps[3] = {&a.tq, &a.tqf, &a.tq1};
+  for (int m = 0; m < 3; ++m) {
+    const cuuint32_t box[4] = {64, (cuuint32_t)a.s.group, 1, toks[m]};
+    if (encode(maps[m], type, 4, const_cast<void*>(q), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return set_error(QD_ERR_CUDA, "cuTensorMapEncodeTiled failed for q");
+  }
+  return QD_OK;
+}
+
+int launch_tiles8(const Paged8Call& c, int least) {
+  const PFN_cuTensorMapEncodeTiled_v12000 encode = tensor_map_encoder();
+  if (!encode) return set_error(QD_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  PagedAttnArgs a = {};
+  a.b = c.b;
+  a.s = pg_shape(a.b.nq, a.b.nkv);
+  a.s.tpf = 0;  // all units are of tiles here
+  a.room = (int)std::min((int64_t)a.b.max_pages * a.b.page_size, (int64_t)kPgMaxKeys);
+  a.inv_group = 65536 / a.s.group + 1;
+  const int rq = map_queries(a, encode, c.q, c.ldq, c.dtype, c.head_dim);
+  if (rq != QD_OK) return rq;
+  const int rp = map_pools8(c, encode, &a.tk, &a.tv);
+  if (rp != QD_OK) return rp;
+  a.out = static_cast<char*>(c.out);
+  a.lse = c.lse;
+  a.ldo = c.ldo;
+  a.ld_lse = c.ld_lse;
+  a.scale_log2 = c.scale * 1.4426950408889634f;
+  a.tickets = static_cast<int*>(c.scratch);
+  a.partials = reinterpret_cast<float*>(static_cast<char*>(c.scratch) + paged_attn_plan(c.grid, c.head_dim).off_partials);
+  a.k_scale = static_cast<const uint8_t*>(c.k_scale);
+  a.v_scale = static_cast<const uint8_t*>(c.v_scale);
+  a.ss_page = c.ss_page;
+  a.ss_head = c.ss_head;
+  a.least = least;
+  const bool bf = c.dtype == QD_BF16, wide = c.head_dim == 128;
+  const void* fn = bf ? (wide ? (const void*)paged_attn_kernel<__nv_bfloat16, 128, false, true> : (const void*)paged_attn_kernel<__nv_bfloat16, 64, false, true>)
+                      : (wide ? (const void*)paged_attn_kernel<__half, 128, false, true> : (const void*)paged_attn_kernel<__half, 64, false, true>);
+  const int smem = wide ? PgLayout<128, true>::total : PgLayout<64, true>::total;
+  const int rs = set_max_dynamic_smem(fn, smem);
+  if (rs != QD_OK) return rs;
+  return launch_kernel(fn, dim3((unsigned)c.grid), dim3(kPgThreads), smem, c.pdl, c.stream, &a);
 }
 
 }  // namespace qd
@@ -1243,21 +1437,8 @@ extern "C" int qd_paged_attn(const void* q, int64_t ldq, int dtype, int64_t toke
   a.room = (int)std::min((int64_t)max_pages * page_size, (int64_t)kPgMaxKeys);
   a.inv_group = 65536 / a.s.group + 1;  // exact: the excess is below 128 / 65536, a fraction's distance to 1 at least 1 / 128
   const CUtensorMapDataType type = dtype == QD_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  const cuuint32_t estr[4] = {1, 1, 1, 1};
-  auto map4 = [&](CUtensorMap* m, const void* base, const cuuint64_t* dims, const cuuint64_t* strides,
-                  const cuuint32_t* box) {
-    return encode(m, type, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-  };
-  {  // a tile's rows are token-major, its KV head's query heads inner
-    const cuuint64_t dims[4] = {(cuuint64_t)head_dim, (cuuint64_t)a.s.group, (cuuint64_t)nkv_heads, (cuuint64_t)tokens};
-    const cuuint64_t strides[3] = {(cuuint64_t)head_dim * 2, (cuuint64_t)a.s.group * head_dim * 2, (cuuint64_t)ldq * 2};
-    const cuuint32_t box[4] = {64, (cuuint32_t)a.s.group, 1, (cuuint32_t)a.s.tpt}, box1[4] = {64, (cuuint32_t)a.s.group, 1, 1};
-    const cuuint32_t boxf[4] = {64, (cuuint32_t)a.s.group, 1, (cuuint32_t)(a.s.tpf > 0 ? a.s.tpf : 1)};
-    if (!map4(&a.tq, q, dims, strides, box) || !map4(&a.tqf, q, dims, strides, boxf) || !map4(&a.tq1, q, dims, strides, box1))
-      return set_error(QD_ERR_CUDA, "cuTensorMapEncodeTiled failed for q");
-  }
+  const int rq = map_queries(a, encode, q, ldq, dtype, head_dim);
+  if (rq != QD_OK) return rq;
   // Pages of 16 rows are merged: half the copies (64 decoding requests 71 us, 84 apart). Larger pages are not: the
   // products read the interleaved rows slower (a chunk of 2048 after 8192 keys 349 us, 341 apart).
   const bool merged = page_size == 16 && head_dim == 128;
@@ -1282,7 +1463,7 @@ extern "C" int qd_paged_attn(const void* q, int64_t ldq, int dtype, int64_t toke
   a.tickets = static_cast<int*>(scratch);
   a.partials = reinterpret_cast<float*>(static_cast<char*>(scratch) + plan.off_partials);
   const void* fn = dtype == QD_BF16 ? attn_kernel<__nv_bfloat16>(head_dim, merged) : attn_kernel<__half>(head_dim, merged);
-  const int smem = head_dim == 128 ? PgLayout<128>::total : PgLayout<64>::total;
+  const int smem = head_dim == 128 ? PgLayout<128, false>::total : PgLayout<64, false>::total;
   const int rs = set_max_dynamic_smem(fn, smem);
   if (rs != QD_OK) return rs;
   return launch_kernel(fn, dim3((unsigned)grid), dim3(kPgThreads), smem, pdl, stream, &a);

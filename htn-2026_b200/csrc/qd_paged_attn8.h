@@ -1,6 +1,7 @@
 // The two kernels of the attention over pages of 8 bits, for requests of few rows and of tiles of them.
 #pragma once
 
+#include "qd_host.h"
 #include "qd_paged_dev.cuh"
 #include "qd_paged_line.h"
 
@@ -32,5 +33,9 @@ struct Paged8Call {
 // The requests of at most 16 query rows a KV head (of none, where a group of heads is larger). `alone`: there is no
 // other launch for the rest, whose rows are left as they are and flagged.
 int launch_few8(const Paged8Call& c, bool alone);
+// The requests of `least` tokens and more, in tiles of 128 query rows.
+int launch_tiles8(const Paged8Call& c, int least);
+// Maps of the values: a box is a page of a KV head, its rows of head_dim bytes swizzled over as many.
+int map_pools8(const Paged8Call& c, PFN_cuTensorMapEncodeTiled_v12000 encode, CUtensorMap* tk, CUtensorMap* tv);
 
 }  // namespace qd
