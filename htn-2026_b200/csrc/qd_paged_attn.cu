@@ -33,10 +33,12 @@
 // from cu_tokens and kv_len itself: no planning launch, and no length is needed on the host.
 //
 // Pages of 8 bits (kHeld): requests of few rows have a kernel of their own (qd_paged_few8.cu), which reads the codes as
-// they are. Tiles get 16-bit operands: two warps that have nothing else to do widen each block from a ring of raw blocks
-// into the ring of K and V blocks (a code times a power of two is exact in both 16-bit types), so that the products, the
-// softmax and P are those of 16-bit pages; a block of two tiles takes the tensor cores and the softmax longer than it
-// takes the two warps. Rows past the last key, and of pages that are not there, are written as zeros.
+// they are. Tiles get FP16 operands, whatever the type of q: a code times its power of two is exact in FP16, and two
+// instructions a pair of codes make it, where BF16 takes five. Two warps that have nothing else to do widen each block in
+// its slot; a raw row lands where the row's last 64 dims will be, so a lane that has read its row may write it at once.
+// Rows past the last key, and of pages that are not there, are written as zeros. The same warps turn BF16 queries into
+// FP16, a power of two of each row (its largest to 2^14) taken out and multiplied onto the scores. P' = 2^7 P: with up to
+// 2^15, FP16 holds what weighs 2^-31 of a row's largest.
 //
 // Measured, 32 query and 8 KV heads of 128 in BF16: 8 single tokens over up to 41 k keys 183 us (HBM: 6.3 TB/s); 64
 // single tokens over 1 to 1.5 k keys 72 us (4.7 TB/s: each CTA's start and end); one token over 1 k keys 12.3 us in a
@@ -48,7 +50,9 @@
 #include <cuda_fp8.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <climits>
+#include <type_traits>
 
 #include "qd_host.h"
 #include "qd_paged_attn8.h"
@@ -63,9 +67,12 @@ namespace qd {
 constexpr int kPgThreads = 384;
 // registers per thread after the start: 2 * 224 + 56 = 3 * 168, what the launch gave the three warpgroups
 constexpr int kPgSoftmaxRegs = 224, kPgOtherRegs = 56;
+constexpr int kPgHeldSoftmaxRegs = 208, kPgHeldOtherRegs = 88;  // 2 * 208 + 88 = 504 too
+static_assert(2 * kPgSoftmaxRegs + kPgOtherRegs <= 3 * 168 && 2 * kPgHeldSoftmaxRegs + kPgHeldOtherRegs <= 3 * 168, "what the launch gave");
 constexpr int kPgBox = 128 * 128;  // [128 rows][64 dims] of 16 bits
 constexpr int kFewP = 2 * kFewRows * 128;  // its P: 2 halves of 64 keys x 16 rows of 128 B
 constexpr int kPgManyUnits = 1 << 20;  // above any grid (whose scratch would be 280 GB); 384 of them fit 32 bits
+constexpr int kPgHeldBias = 7;  // pages of 8 bits: P' = 2^7 P
 constexpr int kPgWhole = 8;   // key blocks up to which units of tiles are left whole, when there are CTAs for all
 
 struct alignas(64) PagedAttnArgs {
@@ -92,23 +99,22 @@ struct alignas(64) PagedAttnArgs {
 template <int D, bool kHeld>
 struct PgLayout {
   static constexpr int kItem = D / 64 * kPgBox;  // a K or V block, and a Q tile
-  static constexpr int kSlots = kHeld ? (D == 128 ? 3 : 6) : D == 128 ? 5 : 10;
-  static_assert(kSlots >= 3, "a pair of tiles holds K and V of a block and the next K");
-  static constexpr int kRawItem = kPgKeys * D, kRaw = kHeld ? (D == 128 ? 4 : 8) : 0;  // blocks of 8 bits
+  static constexpr int kSlots = D == 128 ? 5 : 10;
+  static constexpr int raw = (D / 64 - 1) * kPgBox;  // of a slot: where its rows of 8 bits come
   static constexpr int q = 0;
   static constexpr int kv = q + 2 * kItem;
-  static constexpr int raw = kv + kSlots * kItem;
-  static constexpr int p = raw + kRaw * kRawItem;  // P of few-row units (head_dim 128: in their Q region)
+  static constexpr int p = kv + kSlots * kItem;  // P of few-row units (head_dim 128: in their Q region)
   static constexpr int bars = p + (D == 64 && !kHeld ? 2 * kFewP : 0);
   // qfull[2], qempty[2], sfull[2], pfull[2], odone[2], ofree[2], group[2], segfull[4], segempty[4], join,
-  // sload A odd, A even, B, full[slots], empty[slots], rawfull[], rawempty[]
-  static constexpr int nbars = 26 + 2 * kSlots + 2 * kRaw;
+  // sload A odd, A even, B, full[slots], empty[slots], and for 8 bits copied[slots], qready[4]
+  static constexpr int nbars = 26 + (kHeld ? 3 : 2) * kSlots + (kHeld ? 4 : 0);
   static constexpr int seg = bars + nbars * 8;  // segment ring
   static constexpr int misc = seg + 4 * 64;     // tmem slot, abort, line start, flags, drain counts
   static constexpr int ml = misc + 192;         // at a unit's end: (m, l) of the odd blocks' rows [128], or the
                                                 // warps' sums of few-row units [2 groups][16 rows][4 warps]
-  static constexpr int mx = ml + 1024;          // the warps' maxima of few-row units [2 groups][16][4]
-  static constexpr int mb = mx + (kHeld ? 64 : 1024);  // the odd blocks' maxima of few-row units [16]
+  // the warps' maxima of few-row units [2 groups][16][4]; of pages of 8 bits the queries' exponents [segment][2 tiles][128]
+  static constexpr int mx = ml + 1024;
+  static constexpr int mb = mx + 1024;  // the odd blocks' maxima of few-row units [16]
   static constexpr int total = mb + (kHeld ? 0 : 128);
   static_assert(total <= 227 * 1024, "shared memory of an SM");
   // where warpgroup x's P of a few-row unit in Q region `reg` is: Q takes the first 4 KiB of each 64-dim half
@@ -176,16 +182,10 @@ __device__ __forceinline__ PgReq pg_own_request(const PagedAttnArgs& a, int i) {
   if (kHeld && r.n < a.least) r.n = r.pairs = 0;  // another kernel's
   return r;
 }
-// Two codes of a row as a pair of 16-bit elements, times the row's power of two: exact.
-template <typename T>
+// Two codes of a row as FP16, times the row's power of two: exact.
 __device__ __forceinline__ uint32_t pg_widen(uint32_t codes, __half2 scale) {
   const __half2 h = __hmul2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)codes, __NV_E4M3)), scale);
-  if constexpr (Elem<T>::kBf16) {
-    const float2 f = __half22float2(h);
-    return Elem<T>::pack(f.x, f.y);
-  } else {
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 // Joins a cut few-row unit's pieces (rows of D floats) in the order of their keys: four warps, a row per D / 4
@@ -255,6 +255,7 @@ template <typename T, int D, bool kMerged, bool kHeld>
 __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {
   using Lay = PgLayout<D, kHeld>;
   constexpr int kHalves = D / 64, kSlots = Lay::kSlots;
+  using U = typename std::conditional<kHeld, __half, T>::type;  // of the operands
   constexpr uint32_t kGroup = kMerged ? 2048 : 1024, kHalf = kMerged ? 1024 : kPgBox;  // bytes from one to the next
   grid_dep_wait();
   extern __shared__ __align__(1024) char smem[];
@@ -279,10 +280,10 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
   const uint32_t sload_b = bars + 200;
   auto full = [&](int s) { return bars + 208 + 8u * s; };
   auto empty = [&](int s) { return bars + 208 + 8u * (kSlots + s); };
-  // the ring that the copies fill
-  constexpr int kCopied = kHeld ? Lay::kRaw : kSlots;
-  auto copied = [&](int s) { return kHeld ? bars + 208 + 8u * (2 * kSlots + s) : full(s); };
-  auto copied_empty = [&](int s) { return kHeld ? bars + 208 + 8u * (2 * kSlots + kCopied + s) : empty(s); };
+  auto copied = [&](int s) { return kHeld ? bars + 208 + 8u * (2 * kSlots + s) : full(s); };  // by the copies alone
+  auto qready = [&](int s) { return bars + 208 + 8u * (3 * kSlots + (s & 3)); };
+  constexpr float kBias = kHeld ? kPgHeldBias : 0;
+  constexpr bool kTurn = kHeld && Elem<T>::kBf16;  // queries of BF16 to FP16
   PgSeg* segs = reinterpret_cast<PgSeg*>(smem + Lay::seg);
   int* misc = reinterpret_cast<int*>(smem + Lay::misc);
   int* abort = misc + 1;
@@ -303,16 +304,14 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
     mbar_init(join, 4);
     mbar_init(sload_a(1), 4);
     for (int k = 0; k < 4; ++k) {
+      if (kHeld) mbar_init(qready(k), 2);
       mbar_init(segfull(k), 1);
       mbar_init(segempty(k), kHeld ? 11 : 9);  // the MMA warp, eight softmax warps, those that widen
     }
     for (int s = 0; s < kSlots; ++s) {
       mbar_init(full(s), kHeld ? 2 : 1);
+      if (kHeld) mbar_init(copied(s), 1);
       mbar_init(empty(s), 1);
-    }
-    for (int s = 0; s < Lay::kRaw; ++s) {
-      mbar_init(copied(s), 1);
-      mbar_init(copied_empty(s), 2);
     }
     fence_mbar_init();
     for (int m = 1; m < 12; ++m) misc[m] = 0;  // (the scan comes after them)
@@ -400,14 +399,14 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
   auto tO = [&](int x) { return tmem + 256u + 128u * x; };
 
   if (warp >= 8) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPgOtherRegs));
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kHeld ? kPgHeldOtherRegs : kPgOtherRegs));
   if (warp == 8) {
     // ------------------------------------------------------------ producer: all lanes walk the line
     const uint64_t pol = policy_evict_normal();
     int64_t at = begin;
     int i = misc[2], k = misc[3], h = misc[4], o = misc[5];
     // a lane's copy: a page of the block, and a half of its dims unless they are merged
-    constexpr int copies = kMerged || kHeld ? 1 : kHalves, row_bytes = kHeld ? D : D * 2;
+    constexpr int copies = kMerged || kHeld ? 1 : kHalves, row_bytes = kHeld ? 128 : D * 2;
     const int boxes = (kPgKeys >> a.b.page_shift) * copies;
     const int box_bytes = a.b.page_size * row_bytes / copies, my_page = lane / copies, my_half = lane % copies;
     int seg = 0, items = 0, slot = 0, next_region = 0, qfills[2] = {0, 0};
@@ -485,10 +484,10 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
             flag_error(a.b.err, QD_DEVERR_PAGE);
             page = -1;  // outside the tensor map: the copy fills zeros
           }
-          const uint32_t at_page = sb + (kHeld ? Lay::raw : Lay::kv) + my_half * kPgBox + my_page * box_bytes;
+          const uint32_t at_page = sb + Lay::kv + (kHeld ? Lay::raw : 0) + my_half * kPgBox + my_page * box_bytes;
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {
-            const bool got = mbar_wait_abort(copied_empty(slot), phase, a.b.err, kErrWaitEmpty, abort);
+            const bool got = mbar_wait_abort(empty(slot), phase, a.b.err, kErrWaitEmpty, abort);
             if (!__all_sync(0xffffffffu, got)) {
               ok = false;
               break;
@@ -499,10 +498,10 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
             }
             __syncwarp();
             if (need && kHeld)
-              pg_tma_4d(at_page + slot * Lay::kRawItem, kv ? &a.tv : &a.tk, 0, 0, h, page, copied(slot), pol);
+              pg_tma_4d(at_page + slot * Lay::kItem, kv ? &a.tv : &a.tk, 0, 0, h, page, copied(slot), pol);
             else if (need)
               pg_tma_5d(at_page + slot * Lay::kItem, kv ? &a.tv : &a.tk, my_half, h * a.head_groups, page, full(slot), pol);
-            if (++slot == kCopied) {
+            if (++slot == kSlots) {
               slot = 0;
               phase ^= 1;
             }
@@ -529,7 +528,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
     }
   } else if (warp == 9) {
     // ------------------------------------------------------------ MMA: one elected lane waits and issues
-    constexpr uint32_t kTypes = (7u << 7) | (7u << 10), kind = Elem<T>::kBf16 ? (1u << 7) | (1u << 10) : 0u;
+    constexpr uint32_t kTypes = (7u << 7) | (7u << 10), kind = Elem<U>::kBf16 ? (1u << 7) | (1u << 10) : 0u;
     constexpr uint32_t id_s = (umma_idesc_bf16(kPgKeys) & ~kTypes) | kind;
     constexpr uint32_t id_o = (umma_idesc_bf16(D, false, true) & ~kTypes) | kind;
     constexpr uint32_t id_sf = (umma_idesc_bf16(kFewRows) & ~kTypes) | kind;
@@ -552,9 +551,8 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
       int slot;
       uint32_t phase;
     };
-    auto ahead = [&](int n) {  // the item n <= 4 places on
+    auto ahead = [&](int n) {  // the item n places on
       const int t = slot + n;
-      if (kSlots < 5 && t >= 2 * kSlots) return Ring{t - 2 * kSlots, phase};
       return t >= kSlots ? Ring{t - kSlots, phase ^ 1u} : Ring{t, phase};
     };
     auto advance = [&](int n) {
@@ -628,10 +626,14 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
     // Two tiles over the same blocks. Each tile's P goes over the other's S, which that has long loaded: so the
     // next S of a tile does not wait for its own P to be used up, and S_A runs a block ahead:
     //   S_A 0, S_B 0, S_A 1;  PV_A j, S_B j+1, PV_B j, S_A j+2
-    auto pair_unit = [&](const PgSeg& g) {
+    auto pair_unit = [&](const PgSeg& g, int seg) {
       if (leader) {
-        wait(qfull(0), quse);
-        wait(qfull(1), quse >> 1);
+        if constexpr (kTurn) {
+          wait(qready(seg), seg >> 2);
+        } else {
+          wait(qfull(0), quse);
+          wait(qfull(1), quse >> 1);
+        }
         wait_pv(0);
         wait_pv(1);
         issue_s(c0, c0, 0, ahead(0));
@@ -679,11 +681,14 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
       ++units[1];
     };
     // one tile: its even blocks in S_A, O_A, its odd ones in S_B, O_B; K_j+2 is asked for after V_j
-    auto single_unit = [&](const PgSeg& g, auto fewc) {
+    auto single_unit = [&](const PgSeg& g, auto fewc, int seg) {
       constexpr bool few = decltype(fewc)::value != 0;
       const int reg = g.region;
       if (leader) {
-        wait(qfull(reg), quse >> reg);
+        if constexpr (kTurn)
+          wait(qready(seg), seg >> 2);
+        else
+          wait(qfull(reg), quse >> reg);
         wait_pv(0);
         wait_pv(1);
         issue_s(c0, fewc, reg, ahead(0));
@@ -730,11 +735,11 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
       if (lane == 0) mbar_arrive(segempty(seg));
       if (g.nb == 0) break;
       if (g.region < 0)
-        pair_unit(g);
+        pair_unit(g, seg);
       else if (g.few && !kHeld)
-        single_unit(g, c1);
+        single_unit(g, c1, seg);
       else
-        single_unit(g, c0);
+        single_unit(g, c0, seg);
       if (!__all_sync(0xffffffffu, ok)) break;
     }
     if (leader)  // no MMA may still run when its memory is given back
@@ -744,7 +749,8 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
     // ------------------------------------------------------------ blocks of 8 bits to 16: a warp each half of the rows
     constexpr int kOwn = 2;  // rows of a lane
     const int row0 = (warp - 10) * 64 + lane;
-    int items = 0;  // blocks of K and V so far
+    int items = 0;      // blocks of K and V so far
+    uint32_t quse = 0;  // bit r: the phase of qfull(r)
     bool ok = true;
     auto wait = [&](uint32_t bar, int parity, int code) {
       if (ok) ok = mbar_wait_abort(bar, parity & 1, a.b.err, code, abort);
@@ -754,89 +760,126 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
     for (int seg = 0;; ++seg) {
       wait(segfull(seg), seg >> 2, kErrWaitFull);
       if (!ok) break;
-      const int head = segs[seg & 3].head, kv = segs[seg & 3].kv, j0 = segs[seg & 3].j0, nb = segs[seg & 3].nb;
-      const int32_t* const table = a.b.table + segs[seg & 3].request * a.b.ld_table;
+      const PgSeg g = segs[seg & 3];
       __syncwarp();
       if (lane == 0) mbar_arrive(segempty(seg));
-      if (nb == 0) break;
-      // this lane's pages of block j (-1: none, or past the last key), and its rows' powers of two (0: none)
+      if (g.nb == 0) break;
+      const int32_t* const table = a.b.table + g.request * a.b.ld_table;
+      // this lane's pages of block j (-1: none, or past the last key), and its rows' powers of two
       auto page_of = [&](int j, int o) {
         const int64_t key = (int64_t)j * kPgKeys + row0 + 32 * o;
-        const int page = j < j0 + nb && key < kv ? ld_i32(table + (key >> a.b.page_shift)) : -1;
+        const int page = j < g.j0 + g.nb && key < g.kv ? ld_i32(table + (key >> a.b.page_shift)) : -1;
         return page < a.b.n_pages ? page : -1;
       };
       auto scale_of = [&](const uint8_t* scale, int page, int o) {
-        return page < 0 ? 0 : (int)__ldcg(scale + page * a.ss_page + head * a.ss_head + ((row0 + 32 * o) & (a.b.page_size - 1)));
+        return page < 0 ? 0 : (int)__ldcg(scale + page * a.ss_page + g.head * a.ss_head + ((row0 + 32 * o) & (a.b.page_size - 1)));
       };
-      int page[kOwn], ks[kOwn], vs[kOwn];
+      int page[kOwn], sc[kOwn];  // of the next block; sc: K's byte, and V's above it
+      auto scales = [&]() {
 #pragma unroll
-      for (int o = 0; o < kOwn; ++o) page[o] = page_of(j0, o);
+        for (int o = 0; o < kOwn; ++o) sc[o] = scale_of(a.k_scale, page[o], o) | scale_of(a.v_scale, page[o], o) << 8;
+      };
 #pragma unroll
-      for (int o = 0; o < kOwn; ++o) {
-        ks[o] = scale_of(a.k_scale, page[o], o);
-        vs[o] = scale_of(a.v_scale, page[o], o);
+      for (int o = 0; o < kOwn; ++o) page[o] = page_of(g.j0, o);
+      scales();
+      if constexpr (kTurn) {  // the queries, once they have come: rows of both tiles
+        const bool two = g.region < 0;
+        if (two) {
+          wait(qfull(0), quse, kErrWaitFull);
+          wait(qfull(1), quse >> 1, kErrWaitFull);
+        } else {
+          wait(qfull(g.region), quse >> g.region, kErrWaitFull);
+        }
+        if (!ok) break;
+        quse ^= two ? 3u : 1u << g.region;
+        signed char* const exps = reinterpret_cast<signed char*>(smem + Lay::mx) + (seg & 3) * 256;
+#pragma unroll 1
+        for (int i = row0; i < (two ? 256 : 128); i += i & 32 ? 96 : 32) {  // this lane's two rows of each
+          const int x = i >> 7, row = i & 127;
+          if (row >= min(a.s.tpt, g.ntok - x * a.s.tpt) * a.s.group) continue;
+          char* const at = smem + Lay::q + (two ? x : g.region) * Lay::kItem + row * 128;
+          float most = 0.f;
+#pragma unroll
+          for (int c = 0; c < D / 8; ++c) {
+            const uint4 u = *reinterpret_cast<const uint4*>(at + (c >> 3) * kPgBox + (((c & 7) ^ (row & 7)) << 4));
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float2 f = Elem<T>::unpack((&u.x)[k]);
+              const float fx = fabsf(f.x), fy = fabsf(f.y);
+              most = fmaxf(most, fmaxf(fx <= FLT_MAX ? fx : 0.f, fy <= FLT_MAX ? fy : 0.f));
+            }
+          }
+          const int e = max((int)(__float_as_uint(most) >> 23) - 127 - 14, -110);  // the largest comes to [2^14, 2^15)
+          const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+          for (int c = 0; c < D / 8; ++c) {
+            uint4* const chunk = reinterpret_cast<uint4*>(at + (c >> 3) * kPgBox + (((c & 7) ^ (row & 7)) << 4));
+            uint4 u = *chunk;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float2 f = Elem<T>::unpack((&u.x)[k]);
+              (&u.x)[k] = Elem<__half>::pack(f.x * inv, f.y * inv);
+            }
+            *chunk = u;
+          }
+          exps[i] = (signed char)e;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(qready(seg));
       }
 #pragma unroll 1
-      for (int j = j0; j < j0 + nb && ok; ++j) {
-        int next[kOwn], next_ks[kOwn], next_vs[kOwn];  // under way while this block is widened
+      for (int j = g.j0; j < g.j0 + g.nb && ok; ++j) {
+        int next[kOwn];
+        const int sc0 = sc[0], sc1 = sc[1];
+        const bool dead0 = page[0] < 0, dead1 = page[1] < 0;
 #pragma unroll
         for (int o = 0; o < kOwn; ++o) next[o] = page_of(j + 1, o);
-#pragma unroll
+#pragma unroll 1
         for (int is_v = 0; is_v < 2; ++is_v, ++items) {
-          const int from = items % Lay::kRaw, to = items % kSlots;
-          wait(copied(from), items / Lay::kRaw, kErrWaitFull);
-          wait(empty(to), items / kSlots + 1, kErrWaitEmpty);  // (a ring's first round passes at once)
+          const int slot = items % kSlots;
+          wait(copied(slot), items / kSlots, kErrWaitFull);
           if (!ok) break;
 #pragma unroll
           for (int o = 0; o < kOwn; ++o) {
-            const int row = row0 + 32 * o, b = is_v ? vs[o] : ks[o];
-            const bool dead = page[o] < 0;
-            const __half2 scale = __float2half2_rn(__uint_as_float((uint32_t)b << 23));
-            const char* const src = smem + Lay::raw + from * Lay::kRawItem + row * D;
-            char* const dst = smem + Lay::kv + to * Lay::kItem + row * 128;
-            const int sw = D == 128 ? row & 7 : (row >> 1) & 3;
-#pragma unroll 2
+            const int row = row0 + 32 * o;
+            const bool dead = o ? dead1 : dead0;
+            const uint32_t byte = ((o ? sc1 : sc0) >> (8 * is_v)) & 255;
+            const __half2 scale = __float2half2_rn(__uint_as_float(byte << 23));
+            char* const dst = smem + Lay::kv + slot * Lay::kItem + row * 128;
+            const uint4* const src = reinterpret_cast<const uint4*>(dst + Lay::raw);
+            uint4 u[D / 16];
+#pragma unroll
             for (int c = 0; c < D / 16; ++c) {
-              const uint4 u = *reinterpret_cast<const uint4*>(src + ((c ^ sw) << 4));
+              u[c] = src[c ^ (row & 7)];
+              if (dead) u[c] = make_uint4(0u, 0u, 0u, 0u);
+            }
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) {
               uint32_t w[8];
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
-                const uint32_t four = (&u.x)[k];
-                w[2 * k] = dead ? 0u : pg_widen<T>(four & 0xffffu, scale);
-                w[2 * k + 1] = dead ? 0u : pg_widen<T>(four >> 16, scale);
+                w[2 * k] = pg_widen((&u[c].x)[k] & 0xffffu, scale);
+                w[2 * k + 1] = pg_widen((&u[c].x)[k] >> 16, scale);
               }
-              char* const half = dst + (c >> 2) * kPgBox;
-              const int c8 = (2 * c) & 7;
-              *reinterpret_cast<uint4*>(half + ((c8 ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-              *reinterpret_cast<uint4*>(half + (((c8 + 1) ^ (row & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
+              uint4* const half = reinterpret_cast<uint4*>(dst + (c >> 2) * kPgBox);
+              half[((2 * c) & 7) ^ (row & 7)] = make_uint4(w[0], w[1], w[2], w[3]);
+              half[((2 * c + 1) & 7) ^ (row & 7)] = make_uint4(w[4], w[5], w[6], w[7]);
             }
           }
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(copied_empty(from));
-            mbar_arrive(full(to));
-          }
-          if (is_v == 0)
-#pragma unroll
-            for (int o = 0; o < kOwn; ++o) {
-              next_ks[o] = scale_of(a.k_scale, next[o], o);
-              next_vs[o] = scale_of(a.v_scale, next[o], o);
-            }
+          if (lane == 0) mbar_arrive(full(slot));
         }
-        if (!ok) break;
 #pragma unroll
-        for (int o = 0; o < kOwn; ++o) {
-          page[o] = next[o];
-          ks[o] = next_ks[o];
-          vs[o] = next_vs[o];
-        }
+        for (int o = 0; o < kOwn; ++o) page[o] = next[o];
+        scales();  // (under way while the next block's copies are waited for)
       }
       if (!ok) break;
     }
   }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPgSoftmaxRegs));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kHeld ? kPgHeldSoftmaxRegs : kPgSoftmaxRegs));
     // ------------------------------------------------------------ softmax and epilogue: warpgroup x = tile x
     const int x = warp >> 2, r = 32 * (warp & 3) + lane;  // (r: the row, no longer the request)
     const uint32_t lane_off = (uint32_t)(32 * (warp & 3)) << 16;
@@ -1034,16 +1077,30 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
       if (!ok) break;
       const PgSeg g = segs[seg & 3];
       __syncwarp();
-      if (lane == 0) mbar_arrive(segempty(seg));
+      const bool two = g.region < 0, joined = !two && g.nb > 1;
+      const bool none = g.nb == 0 || (x == 1 && !two && !joined);  // the end, or one tile and one block
+      if (lane == 0 && (!kTurn || none)) mbar_arrive(segempty(seg));
       if (g.nb == 0) break;
       blocks += g.nb;
-      const bool two = g.region < 0, joined = !two && g.nb > 1;
-      if (x == 1 && !two && !joined) continue;  // one tile, one block
+      if (none) continue;
       const int t0 = two ? x * a.s.tpt : 0;       // this tile's first token
       const int ntok = min(a.s.tpt, g.ntok - t0), rows = ntok * a.s.group;
       const int my_tok = (r * a.inv_group) >> 16, tok = g.row0 + t0 + my_tok;
       const int head = g.head * a.s.group + r - my_tok * a.s.group;
       // keys this row sees: up to its own position (MMA rows past the last token hold anything)
+      float turned = 1.f;  // the scores' factor, with the power of two that was taken out of the query
+      auto scale_log2 = [&]() {
+        if constexpr (kTurn) return turned;
+        return a.scale_log2;
+      };
+      if constexpr (kTurn) {
+        wait(qready(seg), seg >> 2);
+        if (!ok) break;
+        const int e = reinterpret_cast<const signed char*>(smem + Lay::mx)[(seg & 3) * 256 + (two ? x * 128 : 0) + r];
+        turned = r < rows ? a.scale_log2 * __uint_as_float((uint32_t)(127 + e) << 23) : a.scale_log2;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(segempty(seg));
+      }
       const int lim = r < rows ? min(g.kv, g.pos0 + t0 + my_tok + 1) : INT_MAX;
       const bool idle = (r & ~31) >= rows;  // no row of this warp is a token's
       float m_used = -INFINITY, l = 0.f;
@@ -1094,7 +1151,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
               for (int c = 0; c < 4; ++c)
                 m4[c] = pg_max3(m4[c], __uint_as_float(v[e + 2 * c]), __uint_as_float(v[e + 2 * c + 1]));
           }
-          m_new = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * a.scale_log2;
+          m_new = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * scale_log2();
           if (r >= rows) m_new = -INFINITY;  // what a row holds that is no token's must not move its warp's maxima
         }
         if (two) {
@@ -1124,15 +1181,15 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
           }
         }
         if (!idle) {
-          const float nm = m_used == -INFINITY ? 0.f : -m_used;  // a row that has seen no key yet: P = 0
+          const float nm = m_used == -INFINITY ? 0.f : kBias - m_used;  // a row that has seen no key yet: P = 0
           float ls[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int c = 0; c < 64; ++c) {  // P pair c = keys 2c, 2c + 1, rounded (the operand's type), over the scores
-            const float p0 = pg_ex2(fmaf(__uint_as_float(sv[2 * c]), a.scale_log2, nm));
-            const float p1 = pg_ex2(fmaf(__uint_as_float(sv[2 * c + 1]), a.scale_log2, nm));
+            const float p0 = pg_ex2(fmaf(__uint_as_float(sv[2 * c]), scale_log2(), nm));
+            const float p1 = pg_ex2(fmaf(__uint_as_float(sv[2 * c + 1]), scale_log2(), nm));
             ls[(2 * c) & 3] += p0;
             ls[(2 * c + 1) & 3] += p1;
-            sv[c] = Elem<T>::pack(p0, p1);
+            sv[c] = Elem<U>::pack(p0, p1);
           }
           l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
           if (two) {  // over the other tile's S, once that has loaded it (B: the one A is ahead with, whose
@@ -1298,7 +1355,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
               if (c8[i] == 0 && a.lse) {
                 const int rt = (row[i] * a.inv_group) >> 16;
                 a.lse[(g.row0 + t0 + rt) * a.ld_lse + g.head * a.s.group + row[i] - rt * a.s.group] =
-                    pg_lse(M[i], L[i]);
+                    pg_lse(M[i] - kBias, L[i]);
               }
             }
           }
@@ -1313,7 +1370,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
         store_rows();
         if (!ok) break;
         if (g.whole && r < rows && a.lse)
-          a.lse[tok * a.ld_lse + head] = pg_lse(m_used, l);
+          a.lse[tok * a.ld_lse + head] = pg_lse(m_used - kBias, l);
       }
       fence_proxy_async_smem();  // the slot's next contents come by TMA
       meet();
@@ -1327,8 +1384,8 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
   if (warp == 9) tmem_dealloc(tmem, 512);
   if (tid == 0) {  // no bulk copy may still be writing shared memory when the CTA exits
     const int n = misc[8];
-    for (int it = max(n - kCopied, 0); it < n; ++it)
-      if (!mbar_wait(copied(it % kCopied), (it / kCopied) & 1, a.b.err, kErrDrain)) break;
+    for (int it = max(n - kSlots, 0); it < n; ++it)
+      if (!mbar_wait(copied(it % kSlots), (it / kSlots) & 1, a.b.err, kErrDrain)) break;
     for (int x = 0; x < 2; ++x)
       if (misc[6 + x] > 0) mbar_wait(qfull(x), (misc[6 + x] - 1) & 1, a.b.err, kErrDrain);
   }
@@ -1370,7 +1427,7 @@ int launch_tiles8(const Paged8Call& c, int least) {
   a.inv_group = 65536 / a.s.group + 1;
   const int rq = map_queries(a, encode, c.q, c.ldq, c.dtype, c.head_dim);
   if (rq != QD_OK) return rq;
-  const int rp = map_pools8(c, encode, &a.tk, &a.tv);
+  const int rp = map_pools8(c, encode, 128, &a.tk, &a.tv);  // (heads of 64: rows of 128 bytes, the rest zeros)
   if (rp != QD_OK) return rp;
   a.out = static_cast<char*>(c.out);
   a.lse = c.lse;

@@ -35,7 +35,7 @@ struct Paged8Call {
 int launch_few8(const Paged8Call& c, bool alone);
 // The requests of `least` tokens and more, in tiles of 128 query rows.
 int launch_tiles8(const Paged8Call& c, int least);
-// Maps of the values: a box is a page of a KV head, its rows of head_dim bytes swizzled over as many.
-int map_pools8(const Paged8Call& c, PFN_cuTensorMapEncodeTiled_v12000 encode, CUtensorMap* tk, CUtensorMap* tv);
+// Maps of the values: a box is a page of a KV head as rows of `row` bytes (head_dim or 128), swizzled over as many.
+int map_pools8(const Paged8Call& c, PFN_cuTensorMapEncodeTiled_v12000 encode, int row, CUtensorMap* tk, CUtensorMap* tv);
 
 }  // namespace qd

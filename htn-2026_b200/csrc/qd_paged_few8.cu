@@ -823,15 +823,15 @@ __global__ void __launch_bounds__(kF8Threads, kF8Resident) paged_few8_kernel(con
   }
 }
 
-int map_pools8(const Paged8Call& c, PFN_cuTensorMapEncodeTiled_v12000 encode, CUtensorMap* tk, CUtensorMap* tv) {
+int map_pools8(const Paged8Call& c, PFN_cuTensorMapEncodeTiled_v12000 encode, int row, CUtensorMap* tk, CUtensorMap* tv) {
   const int D = c.head_dim;
   const PagedBatch& b = c.b;
   const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)b.page_size, (cuuint64_t)b.nkv, (cuuint64_t)b.n_pages};
   const cuuint64_t strides[3] = {(cuuint64_t)D, (cuuint64_t)b.ps_head, (cuuint64_t)b.ps_page};
-  const cuuint32_t box[4] = {(cuuint32_t)D, (cuuint32_t)b.page_size, 1, 1}, one[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {(cuuint32_t)row, (cuuint32_t)b.page_size, 1, 1}, one[4] = {1, 1, 1, 1};
   for (int v = 0; v < 2; ++v)
     if (encode(v ? tv : tk, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(v ? c.v_pages : c.k_pages), dims, strides,
-               box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+               box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, row == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
       return set_error(QD_ERR_CUDA, "cuTensorMapEncodeTiled failed for the pools");
   return QD_OK;
@@ -845,7 +845,7 @@ int launch_few8(const Paged8Call& c, bool alone) {
   const PFN_cuTensorMapEncodeTiled_v12000 encode = tensor_map_encoder();
   if (!encode) return set_error(QD_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
   const int D = c.head_dim;
-  const int rp = map_pools8(c, encode, &a.tk, &a.tv);
+  const int rp = map_pools8(c, encode, c.head_dim, &a.tk, &a.tv);
   if (rp != QD_OK) return rp;
   a.q = static_cast<const char*>(c.q);
   a.k_scale = static_cast<const uint8_t*>(c.k_scale);
