@@ -34,7 +34,7 @@
 //
 // Pages of 8 bits (kHeld): requests of few rows have a kernel of their own (qd_paged_few8.cu), which reads the codes as
 // they are. Tiles get FP16 operands, whatever the type of q: a code times its power of two is exact in FP16, and two
-// instructions a pair of codes make it, where BF16 takes five. Two warps that have nothing else to do widen each block in
+// instructions a pair of codes make it, where BF16 takes five. Four warps, one to each scheduler, widen each block in
 // its slot; a raw row lands where the row's last 64 dims will be, so a lane that has read its row may write it at once.
 // Rows past the last key, and of pages that are not there, are written as zeros. The same warps turn BF16 queries into
 // FP16, a power of two of each row (its largest to 2^14) taken out and multiplied onto the scores. P' = 2^7 P: with up to
@@ -63,12 +63,12 @@
 
 namespace qd {
 
-// warps 0-3 softmax A, 4-7 softmax B, 8 producer, 9 MMA, 10-11 only start up, or widen pages of 8 bits
-constexpr int kPgThreads = 384;
+// warps 0-3 softmax A, 4-7 softmax B, 8 producer, 9 MMA, 10-11 only start up; for pages of 8 bits 12-15 widen
+constexpr int pg_threads(bool held) { return held ? 512 : 384; }
 // registers per thread after the start: 2 * 224 + 56 = 3 * 168, what the launch gave the three warpgroups
 constexpr int kPgSoftmaxRegs = 224, kPgOtherRegs = 56;
-constexpr int kPgHeldSoftmaxRegs = 208, kPgHeldOtherRegs = 88;  // 2 * 208 + 88 = 504 too
-static_assert(2 * kPgSoftmaxRegs + kPgOtherRegs <= 3 * 168 && 2 * kPgHeldSoftmaxRegs + kPgHeldOtherRegs <= 3 * 168, "what the launch gave");
+constexpr int kPgHeldSoftmaxRegs = 200, kPgHeldOtherRegs = 56;  // 2 * 200 + 2 * 56 = 4 * 128
+static_assert(2 * kPgSoftmaxRegs + kPgOtherRegs <= 3 * 168 && 2 * kPgHeldSoftmaxRegs + 2 * kPgHeldOtherRegs <= 4 * 128, "what the launch gave");
 constexpr int kPgBox = 128 * 128;  // [128 rows][64 dims] of 16 bits
 constexpr int kFewP = 2 * kFewRows * 128;  // its P: 2 halves of 64 keys x 16 rows of 128 B
 constexpr int kPgManyUnits = 1 << 20;  // above any grid (whose scratch would be 280 GB); 384 of them fit 32 bits
@@ -103,20 +103,25 @@ struct PgLayout {
   static constexpr int raw = (D / 64 - 1) * kPgBox;  // of a slot: where its rows of 8 bits come
   static constexpr int q = 0;
   static constexpr int kv = q + 2 * kItem;
-  static constexpr int p = kv + kSlots * kItem;  // P of few-row units (head_dim 128: in their Q region)
+  static constexpr int sc = kv + kSlots * kItem;   // heads of 64: the slots' powers of two
+  static constexpr int p = sc + (kHeld && D == 64 ? kSlots * 128 : 0);  // P of few-row units (head_dim 128: in their Q region)
   static constexpr int bars = p + (D == 64 && !kHeld ? 2 * kFewP : 0);
   // qfull[2], qempty[2], sfull[2], pfull[2], odone[2], ofree[2], group[2], segfull[4], segempty[4], join,
   // sload A odd, A even, B, full[slots], empty[slots], and for 8 bits copied[slots], qready[4]
   static constexpr int nbars = 26 + (kHeld ? 3 : 2) * kSlots + (kHeld ? 4 : 0);
   static constexpr int seg = bars + nbars * 8;  // segment ring
   static constexpr int misc = seg + 4 * 64;     // tmem slot, abort, line start, flags, drain counts
-  static constexpr int ml = misc + 192;         // at a unit's end: (m, l) of the odd blocks' rows [128], or the
+  static constexpr int ml = misc + (kHeld ? 256 : 192);         // at a unit's end: (m, l) of the odd blocks' rows [128], or the
                                                 // warps' sums of few-row units [2 groups][16 rows][4 warps]
   // the warps' maxima of few-row units [2 groups][16][4]; of pages of 8 bits the queries' exponents [segment][2 tiles][128]
   static constexpr int mx = ml + 1024;
   static constexpr int mb = mx + 1024;  // the odd blocks' maxima of few-row units [16]
   static constexpr int total = mb + (kHeld ? 0 : 128);
   static_assert(total <= 227 * 1024, "shared memory of an SM");
+  // the power of two of a row of 8 bits: with heads of 128 in what its widened row will take
+  static __device__ __forceinline__ unsigned char* scale_at(char* smem, int slot, int row) {
+    return reinterpret_cast<unsigned char*>(smem) + (D == 128 ? kv + slot * kItem + row * 128 : sc + slot * 128 + row);
+  }
   // where warpgroup x's P of a few-row unit in Q region `reg` is: Q takes the first 4 KiB of each 64-dim half
   static __device__ __forceinline__ int few_p(int reg, int x) {
     return D == 128 ? q + reg * kItem + 4096 + x * kPgBox : p + x * kFewP;
@@ -131,7 +136,6 @@ struct PgSeg {
   int few;                   // one tile of at most 16 rows
   int slot, c0, nc;          // partial slot, first CTA and number of CTAs of the unit
   int region;                // Q region of a single tile, or -1: both tiles
-  int request;
 };
 static_assert(sizeof(PgSeg) <= 64, "segment ring entry");
 
@@ -252,8 +256,9 @@ __device__ __forceinline__ void pg_join_few(const PagedAttnArgs& a, const PgSeg&
 // A K or V block in shared memory: the halves of 64 dims, in each the rows of 128 bytes, 8 to a group; or, merged,
 // the groups and in each the halves, so that a page's whole rows are one box of a copy.
 template <typename T, int D, bool kMerged, bool kHeld>
-__global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {
+__global__ void __launch_bounds__(pg_threads(kHeld), 1) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {
   using Lay = PgLayout<D, kHeld>;
+  constexpr int kPgThreads = pg_threads(kHeld), kWide = 4;  // (warps that widen)
   constexpr int kHalves = D / 64, kSlots = Lay::kSlots;
   using U = typename std::conditional<kHeld, __half, T>::type;  // of the operands
   constexpr uint32_t kGroup = kMerged ? 2048 : 1024, kHalf = kMerged ? 1024 : kPgBox;  // bytes from one to the next
@@ -288,7 +293,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
   int* misc = reinterpret_cast<int*>(smem + Lay::misc);
   int* abort = misc + 1;
   int64_t* scan = reinterpret_cast<int64_t*>(misc + 12);  // the warps' totals: places, and units
-  int* scan_u = misc + 36;
+  int* scan_u = misc + 12 + 2 * (kPgThreads / 32);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int x = 0; x < 2; ++x) {
@@ -304,12 +309,12 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
     mbar_init(join, 4);
     mbar_init(sload_a(1), 4);
     for (int k = 0; k < 4; ++k) {
-      if (kHeld) mbar_init(qready(k), 2);
+      if (kHeld) mbar_init(qready(k), kWide);
       mbar_init(segfull(k), 1);
-      mbar_init(segempty(k), kHeld ? 11 : 9);  // the MMA warp, eight softmax warps, those that widen
+      mbar_init(segempty(k), kHeld ? 9 + kWide : 9);  // the MMA warp, eight softmax warps, those that widen
     }
     for (int s = 0; s < kSlots; ++s) {
-      mbar_init(full(s), kHeld ? 2 : 1);
+      mbar_init(full(s), kHeld ? kWide : 1);
       if (kHeld) mbar_init(copied(s), 1);
       mbar_init(empty(s), 1);
     }
@@ -429,6 +434,18 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
       const int j1 = whole ? nblk : (max(o + take - fixed, 0) + wt - 1) / wt;
       if (j1 > j0) {
         int page = page_of(j0);
+        // pages of 8 bits: the powers of two of this lane's four keys, K's and V's (0: no such key), a block ahead
+        uint32_t four[2];
+        auto load_four = [&](int j) {
+          const int64_t key = (int64_t)j * kPgKeys + 4 * lane;
+          const int pg = __shfl_sync(0xffffffffu, page, (4 * lane) >> a.b.page_shift);
+          const bool in = key < r.kv && pg >= 0 && pg < a.b.n_pages;
+          const int64_t from = pg * a.ss_page + h * a.ss_head + (key & (a.b.page_size - 1));
+          const uint32_t keep = in && key + 4 > r.kv ? 0xffffffffu >> (8 * (key + 4 - r.kv)) : 0xffffffffu;
+          four[0] = in ? __ldcg(reinterpret_cast<const uint32_t*>(a.k_scale + from)) & keep : 0u;
+          four[1] = in ? __ldcg(reinterpret_cast<const uint32_t*>(a.v_scale + from)) & keep : 0u;
+        };
+        if constexpr (kHeld) load_four(j0);
         const int64_t first = at - o + fixed;  // place of the unit's first block
         const int t0 = k * 2 * a.s.tpt, ntok = min(2 * a.s.tpt, r.n - t0);
         const bool two = ntok > a.s.tpt, few = ntok <= a.s.tpf;
@@ -469,7 +486,6 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
           s->c0 = c0;
           s->nc = c1 - c0 + 1;
           s->region = two ? -1 : ra;
-          s->request = i;
           mbar_arrive(segfull(seg));
         }
         for (int x = 0; x <= (two ? 1 : 0); ++x) ++qfills[two ? x : ra];
@@ -493,7 +509,10 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
               break;
             }
             if (lane == 0) {
-              mbar_arrive_expect_tx(copied(slot), n_need * box_bytes);
+              if constexpr (kHeld)
+                mbar_expect_tx(copied(slot), n_need * box_bytes);
+              else
+                mbar_arrive_expect_tx(full(slot), n_need * box_bytes);
               misc[8] = ++items;
             }
             __syncwarp();
@@ -501,12 +520,20 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
               pg_tma_4d(at_page + slot * Lay::kItem, kv ? &a.tv : &a.tk, 0, 0, h, page, copied(slot), pol);
             else if (need)
               pg_tma_5d(at_page + slot * Lay::kItem, kv ? &a.tv : &a.tk, my_half, h * a.head_groups, page, full(slot), pol);
+            if constexpr (kHeld) {  // (the copies do not wait for these)
+#pragma unroll
+              for (int b = 0; b < 4; ++b) *Lay::scale_at(smem, slot, 4 * lane + b) = (unsigned char)(four[kv] >> (8 * b));
+              __syncwarp();
+              if (lane == 0) mbar_arrive(copied(slot));
+            }
             if (++slot == kSlots) {
               slot = 0;
               phase ^= 1;
             }
           }
           page = next;
+          if constexpr (kHeld)
+            if (j + 1 < j1) load_four(j + 1);
         }
       }
       at += take;
@@ -745,12 +772,12 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
     if (leader)  // no MMA may still run when its memory is given back
       for (int x = 0; x < 2; ++x)
         if (pc[x] > 0) mbar_wait(odone(x), (pc[x] - 1) & 1, a.b.err, kErrDrain);
-  } else if constexpr (kHeld) {
-    // ------------------------------------------------------------ blocks of 8 bits to 16: a warp each half of the rows
-    constexpr int kOwn = 2;  // rows of a lane
-    const int row0 = (warp - 10) * 64 + lane;
-    int items = 0;      // blocks of K and V so far
-    uint32_t quse = 0;  // bit r: the phase of qfull(r)
+  } else if (kHeld && warp >= 12) {
+    if constexpr (kHeld) {
+    // ------------------------------------------------------------ blocks of 8 bits to 16: a row a lane
+    const int row = (warp - 12) * 32 + lane;
+    int slot = 0;
+    uint32_t phase = 0, quse = 0;  // of copied(slot); bit r: the phase of qfull(r)
     bool ok = true;
     auto wait = [&](uint32_t bar, int parity, int code) {
       if (ok) ok = mbar_wait_abort(bar, parity & 1, a.b.err, code, abort);
@@ -764,24 +791,6 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
       __syncwarp();
       if (lane == 0) mbar_arrive(segempty(seg));
       if (g.nb == 0) break;
-      const int32_t* const table = a.b.table + g.request * a.b.ld_table;
-      // this lane's pages of block j (-1: none, or past the last key), and its rows' powers of two
-      auto page_of = [&](int j, int o) {
-        const int64_t key = (int64_t)j * kPgKeys + row0 + 32 * o;
-        const int page = j < g.j0 + g.nb && key < g.kv ? ld_i32(table + (key >> a.b.page_shift)) : -1;
-        return page < a.b.n_pages ? page : -1;
-      };
-      auto scale_of = [&](const uint8_t* scale, int page, int o) {
-        return page < 0 ? 0 : (int)__ldcg(scale + page * a.ss_page + g.head * a.ss_head + ((row0 + 32 * o) & (a.b.page_size - 1)));
-      };
-      int page[kOwn], sc[kOwn];  // of the next block; sc: K's byte, and V's above it
-      auto scales = [&]() {
-#pragma unroll
-        for (int o = 0; o < kOwn; ++o) sc[o] = scale_of(a.k_scale, page[o], o) | scale_of(a.v_scale, page[o], o) << 8;
-      };
-#pragma unroll
-      for (int o = 0; o < kOwn; ++o) page[o] = page_of(g.j0, o);
-      scales();
       if constexpr (kTurn) {  // the queries, once they have come: rows of both tiles
         const bool two = g.region < 0;
         if (two) {
@@ -794,8 +803,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
         quse ^= two ? 3u : 1u << g.region;
         signed char* const exps = reinterpret_cast<signed char*>(smem + Lay::mx) + (seg & 3) * 256;
 #pragma unroll 1
-        for (int i = row0; i < (two ? 256 : 128); i += i & 32 ? 96 : 32) {  // this lane's two rows of each
-          const int x = i >> 7, row = i & 127;
+        for (int x = 0; x < (two ? 2 : 1); ++x) {
           if (row >= min(a.s.tpt, g.ntok - x * a.s.tpt) * a.s.group) continue;
           char* const at = smem + Lay::q + (two ? x : g.region) * Lay::kItem + row * 128;
           float most = 0.f;
@@ -822,60 +830,46 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_attn_kernel(const __grid_
             }
             *chunk = u;
           }
-          exps[i] = (signed char)e;
+          exps[x * 128 + row] = (signed char)e;
         }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(qready(seg));
       }
 #pragma unroll 1
-      for (int j = g.j0; j < g.j0 + g.nb && ok; ++j) {
-        int next[kOwn];
-        const int sc0 = sc[0], sc1 = sc[1];
-        const bool dead0 = page[0] < 0, dead1 = page[1] < 0;
+      for (int n = 0; n < 2 * g.nb; ++n) {
+        wait(copied(slot), phase, kErrWaitFull);
+        if (!ok) break;
+        char* const dst = smem + Lay::kv + slot * Lay::kItem + row * 128;
+        const uint4* const src = reinterpret_cast<const uint4*>(dst + Lay::raw);
+        const uint32_t byte = *Lay::scale_at(smem, slot, row);
+        uint4 u[D / 16];
 #pragma unroll
-        for (int o = 0; o < kOwn; ++o) next[o] = page_of(j + 1, o);
-#pragma unroll 1
-        for (int is_v = 0; is_v < 2; ++is_v, ++items) {
-          const int slot = items % kSlots;
-          wait(copied(slot), items / kSlots, kErrWaitFull);
-          if (!ok) break;
+        for (int c = 0; c < D / 16; ++c) u[c] = src[c ^ (row & 7)];
+        const __half2 scale = __float2half2_rn(__uint_as_float(byte << 23));
 #pragma unroll
-          for (int o = 0; o < kOwn; ++o) {
-            const int row = row0 + 32 * o;
-            const bool dead = o ? dead1 : dead0;
-            const uint32_t byte = ((o ? sc1 : sc0) >> (8 * is_v)) & 255;
-            const __half2 scale = __float2half2_rn(__uint_as_float(byte << 23));
-            char* const dst = smem + Lay::kv + slot * Lay::kItem + row * 128;
-            const uint4* const src = reinterpret_cast<const uint4*>(dst + Lay::raw);
-            uint4 u[D / 16];
+        for (int c = 0; c < D / 16; ++c) {
+          if (byte == 0) u[c] = make_uint4(0u, 0u, 0u, 0u);
+          uint32_t w[8];
 #pragma unroll
-            for (int c = 0; c < D / 16; ++c) {
-              u[c] = src[c ^ (row & 7)];
-              if (dead) u[c] = make_uint4(0u, 0u, 0u, 0u);
-            }
-#pragma unroll
-            for (int c = 0; c < D / 16; ++c) {
-              uint32_t w[8];
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                w[2 * k] = pg_widen((&u[c].x)[k] & 0xffffu, scale);
-                w[2 * k + 1] = pg_widen((&u[c].x)[k] >> 16, scale);
-              }
-              uint4* const half = reinterpret_cast<uint4*>(dst + (c >> 2) * kPgBox);
-              half[((2 * c) & 7) ^ (row & 7)] = make_uint4(w[0], w[1], w[2], w[3]);
-              half[((2 * c + 1) & 7) ^ (row & 7)] = make_uint4(w[4], w[5], w[6], w[7]);
-            }
+          for (int k = 0; k < 4; ++k) {
+            w[2 * k] = pg_widen((&u[c].x)[k] & 0xffffu, scale);
+            w[2 * k + 1] = pg_widen((&u[c].x)[k] >> 16, scale);
           }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(full(slot));
+          uint4* const half = reinterpret_cast<uint4*>(dst + (c >> 2) * kPgBox);
+          half[((2 * c) & 7) ^ (row & 7)] = make_uint4(w[0], w[1], w[2], w[3]);
+          half[((2 * c + 1) & 7) ^ (row & 7)] = make_uint4(w[4], w[5], w[6], w[7]);
         }
-#pragma unroll
-        for (int o = 0; o < kOwn; ++o) page[o] = next[o];
-        scales();  // (under way while the next block's copies are waited for)
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full(slot));
+        if (++slot == kSlots) {
+          slot = 0;
+          phase ^= 1;
+        }
       }
       if (!ok) break;
+    }
     }
   }
   } else {
@@ -1447,7 +1441,7 @@ int launch_tiles8(const Paged8Call& c, int least) {
   const int smem = wide ? PgLayout<128, true>::total : PgLayout<64, true>::total;
   const int rs = set_max_dynamic_smem(fn, smem);
   if (rs != QD_OK) return rs;
-  return launch_kernel(fn, dim3((unsigned)c.grid), dim3(kPgThreads), smem, c.pdl, c.stream, &a);
+  return launch_kernel(fn, dim3((unsigned)c.grid), dim3(pg_threads(true)), smem, c.pdl, c.stream, &a);
 }
 
 }  // namespace qd
@@ -1523,5 +1517,5 @@ extern "C" int qd_paged_attn(const void* q, int64_t ldq, int dtype, int64_t toke
   const int smem = head_dim == 128 ? PgLayout<128, false>::total : PgLayout<64, false>::total;
   const int rs = set_max_dynamic_smem(fn, smem);
   if (rs != QD_OK) return rs;
-  return launch_kernel(fn, dim3((unsigned)grid), dim3(kPgThreads), smem, pdl, stream, &a);
+  return launch_kernel(fn, dim3((unsigned)grid), dim3(pg_threads(false)), smem, pdl, stream, &a);
 }
