@@ -40,6 +40,10 @@
 // FP16, a power of two of each row (its largest to 2^14) taken out and multiplied onto the scores. P' = 2^7 P: with up to
 // 2^15, FP16 holds what weighs 2^-31 of a row's largest.
 //
+// Shared beginnings (kShared): the rows of work are not the requests but PgShared entries, a group's tokens over the keys
+// that its requests have in common and each request's over its own; see qd_prefix_attn.cu. The results of both go to
+// fp32 rows, to be joined afterwards.
+//
 // Measured, 32 query and 8 KV heads of 128 in BF16: 8 single tokens over up to 41 k keys 183 us (HBM: 6.3 TB/s); 64
 // single tokens over 1 to 1.5 k keys 72 us (4.7 TB/s: each CTA's start and end); one token over 1 k keys 12.3 us in a
 // graph, 14.5 with the keys not in L2 (latency; a call takes the host 11.9); 2048 tokens after 8192 keys 340 to 368 us
@@ -94,6 +98,9 @@ struct alignas(64) PagedAttnArgs {
   const uint8_t *k_scale, *v_scale;
   int64_t ss_page, ss_head;
   int least;
+  // shared beginnings: the rows of work, and the results' two layers of [tokens][query heads] rows of D, and of lse
+  const PgShared* shared;
+  float *rows, *rows_lse;
 };
 
 template <int D, bool kHeld>
@@ -136,6 +143,7 @@ struct PgSeg {
   int few;                   // one tile of at most 16 rows
   int slot, c0, nc;          // partial slot, first CTA and number of CTAs of the unit
   int region;                // Q region of a single tile, or -1: both tiles
+  int layer;                 // shared beginnings: of the fp32 rows that it goes to, or -1: out
 };
 static_assert(sizeof(PgSeg) <= 64, "segment ring entry");
 
@@ -180,11 +188,35 @@ __device__ __forceinline__ void tmem_wait_ld64(uint32_t* r) {
 __device__ __forceinline__ PgReq pg_request(const PagedAttnArgs& a, int i) {
   return pg_make_request(a.s, ld_i32(a.b.cu + i), ld_i32(a.b.cu + i + 1), ld_i32(a.b.kv_len + i), (int)a.b.tokens, a.room);
 }
-template <bool kHeld>
+template <bool kHeld, bool kShared>
 __device__ __forceinline__ PgReq pg_own_request(const PagedAttnArgs& a, int i) {
-  PgReq r = pg_request(a, i);
-  if (kHeld && r.n < a.least) r.n = r.pairs = 0;  // another kernel's
-  return r;
+  if constexpr (kShared) {
+    const int4 u = __ldcg(reinterpret_cast<const int4*>(a.shared + i));
+    PgReq r;
+    r.row0 = u.x;
+    r.n = u.y;
+    r.pos0 = u.z;
+    r.kv = u.w;
+    r.pairs = (r.n + 2 * a.s.tpt - 1) / (2 * a.s.tpt);
+    r.jb = __ldcg(&a.shared[i].jb);
+    return r;
+  } else {
+    PgReq r = pg_request(a, i);
+    if (kHeld && r.n < a.least) r.n = r.pairs = 0;  // another kernel's
+    return r;
+  }
+}
+// Where a row's results go, in elements of T or of fp32.
+template <int D, bool kShared>
+__device__ __forceinline__ int64_t pg_row_at(const PagedAttnArgs& a, int layer, int tok, int head) {
+  return kShared && layer >= 0 ? ((layer * a.b.tokens + tok) * a.b.nq + head) * D : tok * a.ldo + (int64_t)head * D;
+}
+template <bool kShared>
+__device__ __forceinline__ void pg_store_lse(const PagedAttnArgs& a, int layer, int tok, int head, float lse) {
+  if (kShared && layer >= 0)
+    a.rows_lse[(layer * a.b.tokens + tok) * a.b.nq + head] = lse;
+  else if (a.lse)
+    a.lse[tok * a.ld_lse + head] = lse;
 }
 // Two codes of a row as FP16, times the row's power of two: exact.
 __device__ __forceinline__ uint32_t pg_widen(uint32_t codes, __half2 scale) {
@@ -194,7 +226,7 @@ __device__ __forceinline__ uint32_t pg_widen(uint32_t codes, __half2 scale) {
 
 // Joins a cut few-row unit's pieces (rows of D floats) in the order of their keys: four warps, a row per D / 4
 // lanes, kRows such rows at a time with kPieces pieces' loads in flight for each.
-template <typename T, int D, int kRows, int kPieces>
+template <typename T, int D, int kRows, int kPieces, bool kShared>
 __device__ __forceinline__ void pg_join_few(const PagedAttnArgs& a, const PgSeg& g, int r, int rows) {
   constexpr int kAt = 128 / (D / 4);  // rows under way per step of kRows
   const int c4 = r % (D / 4), first = r / (D / 4);
@@ -244,10 +276,13 @@ __device__ __forceinline__ void pg_join_few(const PagedAttnArgs& a, const PgSeg&
       if (row < rows) {
         const float inv = pg_inverse(L[i]);
         const int tok = (row * a.inv_group) >> 16, t2 = g.row0 + tok, h2 = g.head * a.s.group + row - tok * a.s.group;
-        *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + t2 * a.ldo + (int64_t)h2 * D + 4 * c4) =
-            make_uint2(Elem<T>::pack(acc[i].x * inv, acc[i].y * inv), Elem<T>::pack(acc[i].z * inv, acc[i].w * inv));
-        if (c4 == 0 && a.lse)
-          a.lse[t2 * a.ld_lse + h2] = pg_lse(M[i], L[i]);
+        const int64_t at = pg_row_at<D, kShared>(a, g.layer, t2, h2) + 4 * c4;
+        if (kShared && g.layer >= 0)
+          *reinterpret_cast<float4*>(a.rows + at) = make_float4(acc[i].x * inv, acc[i].y * inv, acc[i].z * inv, acc[i].w * inv);
+        else
+          *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + at) =
+              make_uint2(Elem<T>::pack(acc[i].x * inv, acc[i].y * inv), Elem<T>::pack(acc[i].z * inv, acc[i].w * inv));
+        if (c4 == 0) pg_store_lse<kShared>(a, g.layer, t2, h2, pg_lse(M[i], L[i]));
       }
     }
   }
@@ -255,7 +290,7 @@ __device__ __forceinline__ void pg_join_few(const PagedAttnArgs& a, const PgSeg&
 
 // A K or V block in shared memory: the halves of 64 dims, in each the rows of 128 bytes, 8 to a group; or, merged,
 // the groups and in each the halves, so that a page's whole rows are one box of a copy.
-template <typename T, int D, bool kMerged, bool kHeld>
+template <typename T, int D, bool kMerged, bool kHeld, bool kShared>
 __global__ void __launch_bounds__(pg_threads(kHeld), 1) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {
   using Lay = PgLayout<D, kHeld>;
   constexpr int kPgThreads = pg_threads(kHeld), kWide = 4;  // (warps that widen)
@@ -331,9 +366,9 @@ __global__ void __launch_bounds__(pg_threads(kHeld), 1) paged_attn_kernel(const 
   PgReq r = {};
   bool cut = false, tiles = false, longer = false;
   for (int i = i0; i < i1; ++i) {
-    r = pg_own_request<kHeld>(a, i);
+    r = pg_own_request<kHeld, kShared>(a, i);
     tiles |= r.n > a.s.tpf;
-    cut |= r.kv != r.pos0 + r.n && r.n > 0;
+    cut |= !kShared && r.kv != r.pos0 + r.n && r.n > 0;
     mine += a.b.nkv * pg_sum_cost(a.s, r);
     mine_u = (int)min(mine_u + (int64_t)a.b.nkv * r.pairs, (int64_t)kPgManyUnits);
     longer |= r.pairs && pg_blocks(a.s, r, r.pairs - 1) > kPgWhole;
@@ -385,7 +420,7 @@ __global__ void __launch_bounds__(pg_threads(kHeld), 1) paged_attn_kernel(const 
     int64_t w = begin - before;
     int i = i0;
     if (per > 1) {
-      for (r = pg_own_request<kHeld>(a, i);; r = pg_own_request<kHeld>(a, ++i)) {
+      for (r = pg_own_request<kHeld, kShared>(a, i);; r = pg_own_request<kHeld, kShared>(a, ++i)) {
         const int64_t c = a.b.nkv * (whole ? r.pairs : pg_sum_cost(a.s, r));
         if (w < c) break;
         w -= c;
@@ -419,11 +454,19 @@ __global__ void __launch_bounds__(pg_threads(kHeld), 1) paged_attn_kernel(const 
     bool ok = true;
     r = *reinterpret_cast<const PgReq*>(smem + Lay::mx);
     __syncwarp();
+    int table_row = 0, layer = -1;  // of the current row of work
+    auto take_shared = [&]() {
+      if constexpr (kShared) {
+        table_row = __ldcg(&a.shared[i].table_row);
+        layer = __ldcg(&a.shared[i].layer);
+      }
+    };
+    if (begin < end) take_shared();
     // this lane's page of block j of the current request; -2: no box (past the last key)
     auto page_of = [&](int j) {
-      const int key = j * kPgKeys + (my_page << a.b.page_shift);
+      const int key = (kShared ? r.jb + j : j) * kPgKeys + (my_page << a.b.page_shift);
       if (lane >= boxes || key >= r.kv) return -2;
-      return max(ld_i32(a.b.table + i * a.b.ld_table + (key >> a.b.page_shift)), -1);
+      return max(ld_i32(a.b.table + (kShared ? table_row : i) * a.b.ld_table + (key >> a.b.page_shift)), -1);
     };
     while (at < end && ok) {
       const int nblk = pg_blocks(a.s, r, k), wt = pg_weight(a.s, r, k), fixed = pg_fixed(a.s, r, k);
@@ -478,7 +521,8 @@ __global__ void __launch_bounds__(pg_threads(kHeld), 1) paged_attn_kernel(const 
           s->pos0 = r.pos0 + t0;
           s->kv = r.kv;
           s->head = h;
-          s->j0 = j0;
+          s->j0 = kShared ? r.jb + j0 : j0;
+          if constexpr (kShared) s->layer = layer;
           s->nb = j1 - j0;
           s->whole = j0 == 0 && j1 == nblk;
           s->few = few;
@@ -542,8 +586,9 @@ __global__ void __launch_bounds__(pg_threads(kHeld), 1) paged_attn_kernel(const 
         h = 0;
         if (++k == r.pairs) {
           k = 0;
-          do r = pg_own_request<kHeld>(a, ++i);
+          do r = pg_own_request<kHeld, kShared>(a, ++i);
           while (r.pairs == 0);
+          take_shared();
         }
       }
     }
@@ -1035,13 +1080,12 @@ __global__ void __launch_bounds__(pg_threads(kHeld), 1) paged_attn_kernel(const 
           M = mn;
         }
         const int tok = (lane * a.inv_group) >> 16, hq = g.head * a.s.group + lane - tok * a.s.group;
-        row_at = (g.row0 + tok) * a.ldo + (int64_t)hq * D;
+        row_at = pg_row_at<D, kShared>(a, g.layer, g.row0 + tok, hq);
         if (g.whole) {
           const float inv = pg_inverse(L);
           fa *= inv;
           fb *= inv;
-          if (wg == 0 && a.lse)
-            a.lse[(g.row0 + tok) * a.ld_lse + hq] = pg_lse(M, L);
+          if (wg == 0) pg_store_lse<kShared>(a, g.layer, g.row0 + tok, hq, pg_lse(M, L));
         } else if (wg == 0) {
           __stcg(part_m(g.slot, lane), make_float2(M, L));
         }
@@ -1053,10 +1097,12 @@ __global__ void __launch_bounds__(pg_threads(kHeld), 1) paged_attn_kernel(const 
         const int64_t to = __shfl_sync(0xffffffffu, row_at, c);
         if (joined) v = fmaf(__uint_as_float(ob[c]), f, v);
         if (c < rows && r < D) {
-          if (g.whole)
-            reinterpret_cast<uint16_t*>(a.out)[to + r] = (uint16_t)Elem<T>::pack(v, 0.f);
-          else
+          if (!g.whole)
             __stcg(part_o(g.slot, c) + r, v);
+          else if (kShared && g.layer >= 0)
+            a.rows[to + r] = v;
+          else
+            reinterpret_cast<uint16_t*>(a.out)[to + r] = (uint16_t)Elem<T>::pack(v, 0.f);
         }
       }
       tc_fence_before();
@@ -1108,9 +1154,9 @@ __global__ void __launch_bounds__(pg_threads(kHeld), 1) paged_attn_kernel(const 
         if (x == 1 || g.whole) continue;
         if (is_last(g)) {
           if (rows <= 4)
-            pg_join_few<T, D, 1, 4>(a, g, r, rows);
+            pg_join_few<T, D, 1, 4, kShared>(a, g, r, rows);
           else
-            pg_join_few<T, D, 2, 2>(a, g, r, rows);
+            pg_join_few<T, D, 2, 2, kShared>(a, g, r, rows);
         }
         if (!ok) break;
         continue;
@@ -1251,10 +1297,23 @@ __global__ void __launch_bounds__(pg_threads(kHeld), 1) paged_attn_kernel(const 
           *reinterpret_cast<uint4*>(to) = v;
         }
       };
+      const bool wide = kShared && g.layer >= 0;  // fp32 rows
+      constexpr int kPass = Lay::kItem / 512, kQuads = kPass / 4;  // their dims that fit the slot at a time, by fours
+      auto store_wide = [&](int pass) {
+        meet();
+#pragma unroll 1
+        for (int i = r; i < rows * kQuads; i += 128) {
+          const int row = i / kQuads, c = i % kQuads, rt = (row * a.inv_group) >> 16;
+          const float4 v = *reinterpret_cast<const float4*>(stage + row * (kPass * 4) + ((c ^ (row & 7)) << 4));
+          *reinterpret_cast<float4*>(a.rows + pg_row_at<D, kShared>(a, g.layer, g.row0 + t0 + rt, g.head * a.s.group + row - rt * a.s.group) +
+                                     pass * kPass + 4 * c) = v;
+        }
+        meet();
+      };
       const float norm = !g.whole ? 1.f : pg_inverse(l);  // a piece's rows stay as they are
       fa *= norm;
       fb *= norm;
-      if (!idle) {
+      if (!idle || wide) {
 #pragma unroll 1
         for (int c4 = 0; c4 < D / 32; ++c4) {
           uint32_t o[32];
@@ -1268,7 +1327,14 @@ __global__ void __launch_bounds__(pg_threads(kHeld), 1) paged_attn_kernel(const 
             for (int e = 0; e < 32; ++e)
               o[e] = __float_as_uint(fmaf(__uint_as_float(ob[e]), fb, __uint_as_float(o[e])));
           }
-          if (g.whole) {
+          if (g.whole && wide) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+              *reinterpret_cast<uint4*>(stage + r * (kPass * 4) + (((8 * c4 % kQuads + c) ^ (r & 7)) << 4)) =
+                  make_uint4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+            if ((c4 + 1) * 32 % kPass == 0) store_wide((c4 + 1) * 32 / kPass - 1);
+            if (!ok) break;
+          } else if (g.whole) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[e] = Elem<T>::pack(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1]));
 #pragma unroll
@@ -1341,16 +1407,19 @@ __global__ void __launch_bounds__(pg_threads(kHeld), 1) paged_attn_kernel(const 
             for (int i = 0; i < kI; ++i) {
               if (e0 + 128 * i >= items) break;
               const float inv = pg_inverse(L[i]);
-              uint32_t w[4];
+              const int rt = (row[i] * a.inv_group) >> 16, t2 = g.row0 + t0 + rt, h2 = g.head * a.s.group + row[i] - rt * a.s.group;
+              if (wide) {
+                float4* const to = reinterpret_cast<float4*>(a.rows + pg_row_at<D, kShared>(a, g.layer, t2, h2) + 8 * c8[i]);
+                to[0] = make_float4(acc[i][0] * inv, acc[i][1] * inv, acc[i][2] * inv, acc[i][3] * inv);
+                to[1] = make_float4(acc[i][4] * inv, acc[i][5] * inv, acc[i][6] * inv, acc[i][7] * inv);
+              } else {
+                uint32_t w[4];
 #pragma unroll
-              for (int d = 0; d < 4; ++d) w[d] = Elem<T>::pack(acc[i][2 * d] * inv, acc[i][2 * d + 1] * inv);
-              *reinterpret_cast<uint4*>(stage + row[i] * (2 * D) + ((c8[i] ^ (row[i] & 7)) << 4)) =
-                  make_uint4(w[0], w[1], w[2], w[3]);
-              if (c8[i] == 0 && a.lse) {
-                const int rt = (row[i] * a.inv_group) >> 16;
-                a.lse[(g.row0 + t0 + rt) * a.ld_lse + g.head * a.s.group + row[i] - rt * a.s.group] =
-                    pg_lse(M[i] - kBias, L[i]);
+                for (int d = 0; d < 4; ++d) w[d] = Elem<T>::pack(acc[i][2 * d] * inv, acc[i][2 * d + 1] * inv);
+                *reinterpret_cast<uint4*>(stage + row[i] * (2 * D) + ((c8[i] ^ (row[i] & 7)) << 4)) =
+                    make_uint4(w[0], w[1], w[2], w[3]);
               }
+              if (c8[i] == 0) pg_store_lse<kShared>(a, g.layer, t2, h2, pg_lse(M[i] - kBias, L[i]));
             }
           }
         };
@@ -1361,10 +1430,9 @@ __global__ void __launch_bounds__(pg_threads(kHeld), 1) paged_attn_kernel(const 
       }
       if (!ok) break;
       if (out_rows) {
-        store_rows();
+        if (!wide) store_rows();
         if (!ok) break;
-        if (g.whole && r < rows && a.lse)
-          a.lse[tok * a.ld_lse + head] = pg_lse(m_used - kBias, l);
+        if (g.whole && r < rows) pg_store_lse<kShared>(a, g.layer, tok, head, pg_lse(m_used - kBias, l));
       }
       fence_proxy_async_smem();  // the slot's next contents come by TMA
       meet();
@@ -1385,11 +1453,11 @@ __global__ void __launch_bounds__(pg_threads(kHeld), 1) paged_attn_kernel(const 
   }
 }
 
-template <typename T>
+template <typename T, bool kShared>
 static const void* attn_kernel(int head_dim, bool merged) {
-  return head_dim == 64 ? (const void*)paged_attn_kernel<T, 64, false, false>
-         : merged       ? (const void*)paged_attn_kernel<T, 128, true, false>
-                        : (const void*)paged_attn_kernel<T, 128, false, false>;
+  return head_dim == 64 ? (const void*)paged_attn_kernel<T, 64, false, false, kShared>
+         : merged       ? (const void*)paged_attn_kernel<T, 128, true, false, kShared>
+                        : (const void*)paged_attn_kernel<T, 128, false, false, kShared>;
 }
 
 // The maps of q: a tile's rows are token-major, its KV head's query heads inner.
@@ -1436,8 +1504,8 @@ int launch_tiles8(const Paged8Call& c, int least) {
   a.ss_head = c.ss_head;
   a.least = least;
   const bool bf = c.dtype == QD_BF16, wide = c.head_dim == 128;
-  const void* fn = bf ? (wide ? (const void*)paged_attn_kernel<__nv_bfloat16, 128, false, true> : (const void*)paged_attn_kernel<__nv_bfloat16, 64, false, true>)
-                      : (wide ? (const void*)paged_attn_kernel<__half, 128, false, true> : (const void*)paged_attn_kernel<__half, 64, false, true>);
+  const void* fn = bf ? (wide ? (const void*)paged_attn_kernel<__nv_bfloat16, 128, false, true, false> : (const void*)paged_attn_kernel<__nv_bfloat16, 64, false, true, false>)
+                      : (wide ? (const void*)paged_attn_kernel<__half, 128, false, true, false> : (const void*)paged_attn_kernel<__half, 64, false, true, false>);
   const int smem = wide ? PgLayout<128, true>::total : PgLayout<64, true>::total;
   const int rs = set_max_dynamic_smem(fn, smem);
   if (rs != QD_OK) return rs;
@@ -1460,32 +1528,19 @@ extern "C" int qd_paged_attn_plan(int nq_heads, int nkv_heads, int head_dim, int
   return QD_OK;
 }
 
-extern "C" int qd_paged_attn(const void* q, int64_t ldq, int dtype, int64_t tokens, int nq_heads, int nkv_heads,
-                             int head_dim, const void* k_pages, const void* v_pages, int64_t n_pages, int page_size,
-                             int64_t ps_page, int64_t ps_head, const int32_t* cu_tokens, const int32_t* kv_len,
-                             int batch, const int32_t* page_table, int64_t ld_table, int max_pages, float scale,
-                             void* out, int64_t ldo, float* lse, int64_t ld_lse, int grid, void* scratch,
-                             int64_t scratch_bytes, int* err, int pdl, cudaStream_t stream) {
-  PagedAttnArgs a = {};
-  const int rc = paged_batch_check("paged attention", dtype, tokens, nq_heads, nkv_heads, head_dim, k_pages, v_pages,
-                                   n_pages, page_size, ps_page, ps_head, cu_tokens, kv_len, batch, page_table,
-                                   ld_table, max_pages, err, &a.b);
-  if (rc != QD_OK) return rc;
-  if ((tokens > 0 && (!q || !out)) || !aligned16(q) || !aligned16(out) || ldq % 8 || ldo % 8 || ldq < (int64_t)nq_heads * head_dim ||
-      ldo < (int64_t)nq_heads * head_dim || (lse && ld_lse < nq_heads) || !(scale > 0.f))
-    return set_error(QD_ERR_ARG, "paged attention: q / out / lse null, misaligned or with a bad stride (%lld, %lld, %lld), or scale %g",
-                     (long long)ldq, (long long)ldo, (long long)ld_lse, (double)scale);
-  const PagedAttnPlan plan = paged_attn_plan(grid < 1 ? 1 : grid, head_dim);
-  if (grid < 1 || !scratch || scratch_bytes < plan.bytes || (reinterpret_cast<uintptr_t>(scratch) & 31))
-    return set_error(QD_ERR_SCRATCH, "paged attention: grid %d needs %lld B of 32-byte aligned scratch (have %lld)", grid,
-                     (long long)plan.bytes, (long long)scratch_bytes);
-  if (ps_head % (8 * head_dim))
-    return set_error(QD_ERR_ARG, "paged attention: head stride %lld (whole groups of 8 rows)", (long long)ps_head);
-  if (tokens == 0) return QD_OK;
+namespace qd {
+
+// One launch over checked arguments: over the batch's requests, or over `shared` entries.
+static int launch_attn(PagedAttnArgs& a, const void* q, int64_t ldq, int dtype, int head_dim, const void* k_pages,
+                       const void* v_pages, float scale, void* out, int64_t ldo, float* lse, int64_t ld_lse, int grid,
+                       void* scratch, int pdl, cudaStream_t stream) {
+  const int page_size = a.b.page_size, nkv_heads = a.b.nkv;
+  const int64_t ps_head = a.b.ps_head, ps_page = a.b.ps_page, n_pages = a.b.n_pages;
+  const PagedAttnPlan plan = paged_attn_plan(grid, head_dim);
   const PFN_cuTensorMapEncodeTiled_v12000 encode = tensor_map_encoder();
   if (!encode) return set_error(QD_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
-  a.s = pg_shape(nq_heads, nkv_heads);
-  a.room = (int)std::min((int64_t)max_pages * page_size, (int64_t)kPgMaxKeys);
+  a.s = pg_shape(a.b.nq, nkv_heads);
+  a.room = pg_room(a.b);
   a.inv_group = 65536 / a.s.group + 1;  // exact: the excess is below 128 / 65536, a fraction's distance to 1 at least 1 / 128
   const CUtensorMapDataType type = dtype == QD_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const int rq = map_queries(a, encode, q, ldq, dtype, head_dim);
@@ -1513,9 +1568,50 @@ extern "C" int qd_paged_attn(const void* q, int64_t ldq, int dtype, int64_t toke
   a.scale_log2 = scale * 1.4426950408889634f;
   a.tickets = static_cast<int*>(scratch);
   a.partials = reinterpret_cast<float*>(static_cast<char*>(scratch) + plan.off_partials);
-  const void* fn = dtype == QD_BF16 ? attn_kernel<__nv_bfloat16>(head_dim, merged) : attn_kernel<__half>(head_dim, merged);
+  const bool bf = dtype == QD_BF16;
+  const void* fn = a.shared ? (bf ? attn_kernel<__nv_bfloat16, true>(head_dim, merged) : attn_kernel<__half, true>(head_dim, merged))
+                            : (bf ? attn_kernel<__nv_bfloat16, false>(head_dim, merged) : attn_kernel<__half, false>(head_dim, merged));
   const int smem = head_dim == 128 ? PgLayout<128, false>::total : PgLayout<64, false>::total;
   const int rs = set_max_dynamic_smem(fn, smem);
   if (rs != QD_OK) return rs;
   return launch_kernel(fn, dim3((unsigned)grid), dim3(pg_threads(false)), smem, pdl, stream, &a);
+}
+
+int launch_shared(const PagedBatch& b, const PgShared* shared, int entries, float* rows, float* rows_lse, const void* q,
+                  int64_t ldq, int dtype, int head_dim, const void* k_pages, const void* v_pages, float scale, void* out,
+                  int64_t ldo, float* lse, int64_t ld_lse, int grid, void* scratch, int pdl, cudaStream_t stream) {
+  PagedAttnArgs a = {};
+  a.b = b;
+  a.b.batch = entries;
+  a.shared = shared;
+  a.rows = rows;
+  a.rows_lse = rows_lse;
+  return launch_attn(a, q, ldq, dtype, head_dim, k_pages, v_pages, scale, out, ldo, lse, ld_lse, grid, scratch, pdl, stream);
+}
+
+}  // namespace qd
+
+extern "C" int qd_paged_attn(const void* q, int64_t ldq, int dtype, int64_t tokens, int nq_heads, int nkv_heads,
+                             int head_dim, const void* k_pages, const void* v_pages, int64_t n_pages, int page_size,
+                             int64_t ps_page, int64_t ps_head, const int32_t* cu_tokens, const int32_t* kv_len,
+                             int batch, const int32_t* page_table, int64_t ld_table, int max_pages, float scale,
+                             void* out, int64_t ldo, float* lse, int64_t ld_lse, int grid, void* scratch,
+                             int64_t scratch_bytes, int* err, int pdl, cudaStream_t stream) {
+  PagedAttnArgs a = {};
+  const int rc = paged_batch_check("paged attention", dtype, tokens, nq_heads, nkv_heads, head_dim, k_pages, v_pages,
+                                   n_pages, page_size, ps_page, ps_head, cu_tokens, kv_len, batch, page_table,
+                                   ld_table, max_pages, err, &a.b);
+  if (rc != QD_OK) return rc;
+  if ((tokens > 0 && (!q || !out)) || !aligned16(q) || !aligned16(out) || ldq % 8 || ldo % 8 || ldq < (int64_t)nq_heads * head_dim ||
+      ldo < (int64_t)nq_heads * head_dim || (lse && ld_lse < nq_heads) || !(scale > 0.f))
+    return set_error(QD_ERR_ARG, "paged attention: q / out / lse null, misaligned or with a bad stride (%lld, %lld, %lld), or scale %g",
+                     (long long)ldq, (long long)ldo, (long long)ld_lse, (double)scale);
+  const PagedAttnPlan plan = paged_attn_plan(grid < 1 ? 1 : grid, head_dim);
+  if (grid < 1 || !scratch || scratch_bytes < plan.bytes || (reinterpret_cast<uintptr_t>(scratch) & 31))
+    return set_error(QD_ERR_SCRATCH, "paged attention: grid %d needs %lld B of 32-byte aligned scratch (have %lld)", grid,
+                     (long long)plan.bytes, (long long)scratch_bytes);
+  if (ps_head % (8 * head_dim))
+    return set_error(QD_ERR_ARG, "paged attention: head stride %lld (whole groups of 8 rows)", (long long)ps_head);
+  if (tokens == 0) return QD_OK;
+  return launch_attn(a, q, ldq, dtype, head_dim, k_pages, v_pages, scale, out, ldo, lse, ld_lse, grid, scratch, pdl, stream);
 }

@@ -18,7 +18,25 @@ inline PagedAttnPlan paged_attn_plan(int grid, int head_dim) {
   return p;
 }
 
-// A checked call.
+// positions in a row of the page table, as many as are attended to
+inline int pg_room(const PagedBatch& b) {
+  const int64_t room = (int64_t)b.max_pages * b.page_size;
+  return room < kPgMaxKeys ? (int)room : kPgMaxKeys;
+}
+
+// A row of work of the attention over shared beginnings: token rows row0 .. row0 + n - 1, the first at position pos0, over
+// the keys from block jb to kv of the page table's row table_row. layer: the fp32 rows that the results go to (0: of keys
+// that are shared, 1: of a request's own), or -1: straight out.
+struct alignas(16) PgShared {
+  int row0, n, pos0, kv;
+  int jb, table_row, layer, pad;
+};
+// The 16-bit attention over `entries` such rows of work; rows and rows_lse: 2 layers of [tokens][nq] rows.
+int launch_shared(const PagedBatch& b, const PgShared* shared, int entries, float* rows, float* rows_lse, const void* q,
+                  int64_t ldq, int dtype, int head_dim, const void* k_pages, const void* v_pages, float scale, void* out,
+                  int64_t ldo, float* lse, int64_t ld_lse, int grid, void* scratch, int pdl, cudaStream_t stream);
+
+// A checked call over pages of 8 bits.
 struct Paged8Call {
   PagedBatch b;
   const void *q, *k_pages, *v_pages, *k_scale, *v_scale;

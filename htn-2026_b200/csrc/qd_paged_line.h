@@ -57,6 +57,7 @@ inline PgShape pg_shape(int nq, int nkv) {
 struct PgReq {
   int row0, n, pos0, kv;  // token rows, the first one's position, keys (cut to `room`)
   int pairs;              // tile pairs
+  int jb;                 // key blocks before its first: of keys that other rows of work cover
 };
 // Token rows begin .. end - 1 of `tokens`; `room` positions in a row of the page table, at most kPgMaxKeys.
 QD_LINE_FN PgReq pg_make_request(const PgShape& s, int begin, int end, int kv_len, int tokens, int room) {
@@ -68,13 +69,14 @@ QD_LINE_FN PgReq pg_make_request(const PgShape& s, int begin, int end, int kv_le
   r.pos0 = kv - r.n;
   r.kv = pg_min(kv, room);
   r.pairs = (r.n + 2 * s.tpt - 1) / (2 * s.tpt);
+  r.jb = 0;
   return r;
 }
 // key blocks of tile pair k: up to its last token's position (at least one, so that rows without keys are
 // written too)
 QD_LINE_FN int pg_blocks(const PgShape& s, const PgReq& r, int k) {
   const int keys = pg_min(r.kv, r.pos0 + pg_min(r.n, (k + 1) * 2 * s.tpt));
-  return pg_max((keys + kPgKeys - 1) / kPgKeys, 1);
+  return pg_max((keys + kPgKeys - 1) / kPgKeys - r.jb, 1);
 }
 // places of a key block of tile pair k
 QD_LINE_FN int pg_weight(const PgShape& s, const PgReq& r, int k) {
@@ -100,7 +102,7 @@ QD_LINE_FN int64_t pg_sum_cost(const PgShape& s, const PgReq& r) {
       const int64_t cnt = q + (j <= rest);
       sum += cnt * ((r.pos0 + 2 * s.tpt * j + kPgKeys - 1) / kPgKeys) + s.period_blocks * (cnt * (cnt - 1) / 2);
     }
-    return (int64_t)kPgUnitCost * m + kPgPairCost * sum + pg_cost(s, r, m);
+    return (int64_t)kPgUnitCost * m + kPgPairCost * (sum - (int64_t)m * r.jb) + pg_cost(s, r, m);
   }
 #pragma unroll 1
   for (int k = 0; k < r.pairs; ++k) sum += pg_cost(s, r, k);

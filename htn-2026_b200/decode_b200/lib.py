@@ -126,6 +126,11 @@ PROTOTYPES = {
                               c_int, c_int64, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int, c_float,
                               c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p, c_int64, c_void_p, c_int,
                               c_void_p]),
+    "qd_prefix_attn_plan": (c_int, [c_int, c_int, c_int, c_int64, c_int, c_int, P_INT, P_I64]),
+    "qd_prefix_attn": (c_int, [c_void_p, c_int64, c_int, c_int64, c_int, c_int, c_int, c_void_p, c_void_p, c_int64,
+                               c_int, c_int64, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int, c_void_p,
+                               c_void_p, c_int, c_float, c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p, c_int64,
+                               c_void_p, c_int, c_void_p]),
     "qd_paged_attn8_plan": (c_int, [c_int, c_int, c_int, c_int, P_INT, P_I64]),
     "qd_paged_attn8": (c_int, [c_void_p, c_int64, c_int, c_int64, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p,
                                c_void_p, c_int64, c_int, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int,

@@ -185,6 +185,47 @@ class PagedAttention:
         return out
 
 
+class PrefixAttention(PagedAttention):
+    """`PagedAttention` of requests that begin with the same pages in groups, whose common positions are read once for
+    all of a group's tokens (qd_prefix_attn), for calls of up to max_tokens tokens and max_requests requests."""
+
+    def __init__(self, nq: int, nkv: int, head_dim: int, device, max_tokens: int, max_requests: int, dtype=torch.bfloat16,
+                 grid: int = 0):
+        assert dtype in TYPES, f"expected BF16 or FP16, got {dtype}"
+        self.nq, self.nkv, self.head_dim, self.dtype = nq, nkv, head_dim, dtype
+        g, nbytes = ctypes.c_int(0), ctypes.c_int64(0)
+        L.call("qd_prefix_attn_plan", nq, nkv, head_dim, max_tokens, max_requests, grid, ctypes.byref(g), ctypes.byref(nbytes))
+        self.grid = g.value
+        self.scratch = torch.zeros((nbytes.value,), dtype=torch.uint8, device=device)
+        self.scratch_bytes = nbytes.value
+        self.scale = 1.0 / math.sqrt(head_dim)
+
+    def __call__(self, q, k_pages, v_pages, cu_tokens, kv_len, page_table, cu_groups, prefix_len, out, lse=None,
+                 scale: float | None = None, err=None, pdl: bool = True):
+        """As PagedAttention's. Requests cu_groups[g] .. cu_groups[g + 1] - 1 have their first prefix_len[g] positions in
+        the same pages (int32 [groups + 1] and [groups], on the device)."""
+        nq, D, dtype, dev = self.nq, self.head_dim, self.dtype, q.get_device()
+        pool, ps, batch, ld_table, max_pages = _check_batch(dev, dtype, k_pages, v_pages, cu_tokens, kv_len, page_table, err)
+        tokens, groups = q.shape[0], prefix_len.shape[0]
+        assert q.dtype is dtype and out.dtype is dtype and out.get_device() == dev and self.scratch.get_device() == dev
+        assert pool[1] == self.nkv and pool[3] == D
+        assert cu_groups.dtype is I32 and cu_groups.get_device() == dev and cu_groups.shape == (groups + 1,) and cu_groups.is_contiguous()
+        assert prefix_len.dtype is I32 and prefix_len.get_device() == dev and prefix_len.is_contiguous()
+        ldq, ldo = _rows(q, tokens, nq, D), _rows(out, tokens, nq, D)
+        lse_ptr, ld_lse = None, 0
+        if lse is not None:
+            assert lse.dtype is F32 and lse.get_device() == dev and lse.shape == (tokens, nq)
+            ld_lse, step = lse.stride()
+            assert step == 1 or nq == 1
+            lse_ptr, ld_lse = lse.data_ptr(), max(ld_lse, nq) if tokens <= 1 else ld_lse
+        L.call("qd_prefix_attn", q.data_ptr(), ldq, TYPES[dtype], tokens, nq, self.nkv, D, k_pages.data_ptr(),
+               v_pages.data_ptr(), pool[0], pool[2], ps[0], ps[1], cu_tokens.data_ptr(), kv_len.data_ptr(), batch,
+               page_table.data_ptr(), ld_table, max_pages, cu_groups.data_ptr(), prefix_len.data_ptr(), groups,
+               self.scale if scale is None else scale, out.data_ptr(), ldo, lse_ptr, ld_lse, self.grid,
+               self.scratch.data_ptr(), self.scratch_bytes, None if err is None else err.data_ptr(), pdl, _raw_stream(dev))
+        return out
+
+
 class PagedAttention8(PagedAttention):
     """`PagedAttention` over pages of 8 bits (`new_pools8`; qd_paged_attn8)."""
 

@@ -469,6 +469,25 @@ int qd_paged_attn(const void* q, int64_t ldq, int dtype, int64_t tokens, int nq_
                   float* lse, int64_t ld_lse, int grid, void* scratch, int64_t scratch_bytes, int* err, int pdl,
                   cudaStream_t stream);
 
+/* qd_prefix_attn is qd_paged_attn for requests that begin alike in groups: requests cu_groups[g] ..
+ * cu_groups[g + 1] - 1 (device int32 [n_groups + 1], ascending; requests outside any group stand alone) have their first
+ * prefix_len[g] positions in the same pages, which every one of their page table rows names (device int32 [n_groups]; the
+ * caller's promise: they are read through the first request's row). The results are qd_paged_attn's, up to the order of
+ * the fp32 sums; those positions are read once for all of the group's tokens instead of once per request. Read once are
+ * whole blocks of 128 positions that lie before every new token of the group, where that saves more than it costs; the
+ * rest is read as by qd_paged_attn. Pools are of 16 bits. qd_prefix_attn_plan gives the grid and the size of the scratch
+ * (32-byte aligned) for calls of up to max_tokens tokens and max_requests requests; it is to be zero before its first
+ * call, and after one that ended early, as for qd_paged_attn. */
+int qd_prefix_attn_plan(int nq_heads, int nkv_heads, int head_dim, int64_t max_tokens, int max_requests, int grid_hint,
+                        int* grid, int64_t* scratch_bytes);
+int qd_prefix_attn(const void* q, int64_t ldq, int dtype, int64_t tokens, int nq_heads, int nkv_heads, int head_dim,
+                   const void* k_pages, const void* v_pages, int64_t n_pages, int page_size, int64_t ps_page,
+                   int64_t ps_head, const int32_t* cu_tokens, const int32_t* kv_len, int batch,
+                   const int32_t* page_table, int64_t ld_table, int max_pages, const int32_t* cu_groups,
+                   const int32_t* prefix_len, int n_groups, float scale, void* out, int64_t ldo, float* lse,
+                   int64_t ld_lse, int grid, void* scratch, int64_t scratch_bytes, int* err, int pdl,
+                   cudaStream_t stream);
+
 /* ---------------------------------------------------------------- paged K/V cache of 8 bits
  * Pages that hold a position of a KV head in head_dim + 1 bytes: head_dim values of E4M3 (4 bits of exponent, 3 of
  * mantissa, largest 448) in pools [n_pages][nkv_heads][page_size][head_dim], and one byte e + 127 in pools
