@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __gr
         x[8 + k] = q * cs[k] + p * sn[k];
       }
     }
-    if constexpr (kHeld) {
+    if (kHeld && h0 + unit * kHeads - lane / kLanes + kHeads > a.b.nq) {  // (some head of the warp's is K or V)
       if (is_v) unpack();  // V goes in as it was
       float most = 0.f;
 #pragma unroll

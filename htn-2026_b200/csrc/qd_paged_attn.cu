@@ -42,7 +42,9 @@
 //
 // Shared beginnings (kShared): the rows of work are not the requests but PgShared entries, a group's tokens over the keys
 // that its requests have in common and each request's over its own; see qd_prefix_attn.cu. The results of both go to
-// fp32 rows, to be joined afterwards.
+// fp32 rows, to be joined afterwards, and the pieces of a cut unit of common keys stay where they are, to be joined with
+// them: by the whole GPU, where the CTA that ends last would read 128 KB a piece (64 tokens after 4096 keys, 14 pieces: 73
+// us, 45 of them that).
 //
 // Measured, 32 query and 8 KV heads of 128 in BF16: 8 single tokens over up to 41 k keys 183 us (HBM: 6.3 TB/s); 64
 // single tokens over 1 to 1.5 k keys 72 us (4.7 TB/s: each CTA's start and end); one token over 1 k keys 12.3 us in a
@@ -101,6 +103,7 @@ struct alignas(64) PagedAttnArgs {
   // shared beginnings: the rows of work, and the results' two layers of [tokens][query heads] rows of D, and of lse
   const PgShared* shared;
   float *rows, *rows_lse;
+  PgUnit* units;  // of common keys: [first token row][KV heads]
 };
 
 template <int D, bool kHeld>
@@ -529,6 +532,8 @@ __global__ void __launch_bounds__(pg_threads(kHeld), 1) paged_attn_kernel(const 
           s->slot = 2 * cta + (j0 > 0 ? 0 : 1);
           s->c0 = c0;
           s->nc = c1 - c0 + 1;
+          if (kShared && layer == 0)
+            a.units[(int64_t)(r.row0 + t0) * a.b.nkv + h] = PgUnit{c0, j0 == 0 && j1 == nblk ? 0 : c1 - c0 + 1};
           s->region = two ? -1 : ra;
           mbar_arrive(segfull(seg));
         }
@@ -1151,7 +1156,7 @@ __global__ void __launch_bounds__(pg_threads(kHeld), 1) paged_attn_kernel(const 
         else
           few_rows(Const<kFewRows>(), g, rows, joined);
         if (!ok) break;
-        if (x == 1 || g.whole) continue;
+        if (x == 1 || g.whole || (kShared && g.layer == 0)) continue;
         if (is_last(g)) {
           if (rows <= 4)
             pg_join_few<T, D, 1, 4, kShared>(a, g, r, rows);
@@ -1355,7 +1360,7 @@ __global__ void __launch_bounds__(pg_threads(kHeld), 1) paged_attn_kernel(const 
         if (joined) mbar_arrive(ofree(1));
       }
       bool out_rows = g.whole;
-      if (!g.whole && is_last(g)) {  // join the pieces in the order of their keys
+      if (!g.whole && !(kShared && g.layer == 0) && is_last(g)) {  // join the pieces in the order of their keys
         out_rows = true;
         // kP pieces of 4 / kP times 8 dims of a row at a time: 8 loads in flight, none twice where a unit is cut once
         // (16 in flight spill)
@@ -1577,7 +1582,7 @@ static int launch_attn(PagedAttnArgs& a, const void* q, int64_t ldq, int dtype, 
   return launch_kernel(fn, dim3((unsigned)grid), dim3(pg_threads(false)), smem, pdl, stream, &a);
 }
 
-int launch_shared(const PagedBatch& b, const PgShared* shared, int entries, float* rows, float* rows_lse, const void* q,
+int launch_shared(const PagedBatch& b, const PgShared* shared, int entries, float* rows, float* rows_lse, PgUnit* units, const void* q,
                   int64_t ldq, int dtype, int head_dim, const void* k_pages, const void* v_pages, float scale, void* out,
                   int64_t ldo, float* lse, int64_t ld_lse, int grid, void* scratch, int pdl, cudaStream_t stream) {
   PagedAttnArgs a = {};
@@ -1586,6 +1591,7 @@ int launch_shared(const PagedBatch& b, const PgShared* shared, int entries, floa
   a.shared = shared;
   a.rows = rows;
   a.rows_lse = rows_lse;
+  a.units = units;
   return launch_attn(a, q, ldq, dtype, head_dim, k_pages, v_pages, scale, out, ldo, lse, ld_lse, grid, scratch, pdl, stream);
 }
 

@@ -10,14 +10,14 @@
 //          query heads a KV head are a pair of tiles there, so a block of common keys is read, and multiplied, once for
 //          all, and both kinds of work fill the SMs together. The results go to fp32 rows, two layers of them, as a second
 //          rounding to 16 bits would cost as much as the last.
-//   merge  joins the layers' rows, a warp for 8 heads of a token.
+//   merge  joins the layers' rows and the pieces that units of common keys were cut into, a warp for 2 heads of a token.
 // A group is taken apart again (its requests read all keys, straight to out) where sharing would not pay: see the plan.
 #include "qd_host.h"
 #include "qd_paged_attn8.h"
 
 namespace qd {
 
-constexpr int kPlanThreads = 1024, kMergeWarps = 8, kMergeHeads = 8;
+constexpr int kPlanThreads = 1024, kMergeWarps = 8, kMergeHeads = 2, kMergePieces = 4;
 
 struct PrefixPlanArgs {
   PagedBatch b;
@@ -82,73 +82,113 @@ __global__ void __launch_bounds__(kPlanThreads) prefix_plan_kernel(const __grid_
         if (request(i).n > 0) {
           a.shared[a.n_groups + i].jb = blocks;
           a.shared[a.n_groups + i].layer = 1;
+          a.shared[a.n_groups + i].group = g;
         }
   }
 }
 
 struct PrefixMergeArgs {
   PagedBatch b;
-  const PgShared* requests;
-  const float *rows, *rows_lse;
+  PgShape s;
+  const PgShared *groups, *requests;
+  const PgUnit* units;
+  const float *partials, *rows, *rows_lse;
   char* out;
   float* lse;
   int64_t ldo, ld_lse;
+  int grid;  // of the attention
 };
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kMergeWarps * 32) prefix_merge_kernel(const __grid_constant__ PrefixMergeArgs a) {
   constexpr int kOwn = D / 32;  // dims of a lane
+  using Vec = typename std::conditional<D == 128, float4, float2>::type;
   grid_dep_wait();
   grid_dep_launch();
   const int lane = threadIdx.x & 31, per = (a.b.nq + kMergeHeads - 1) / kMergeHeads;
   const int64_t w = (int64_t)blockIdx.x * kMergeWarps + (threadIdx.x >> 5), t = w / per;
   if (t >= a.b.tokens) return;
-  const int h0 = (int)(w - t * per) * kMergeHeads, heads = min(a.b.nq - h0, kMergeHeads);
+  const int h0 = (int)(w - t * per) * kMergeHeads;
   const int i = warp_find_request(a.b.cu, a.b.batch, (int)t, lane);
-  if (i >= a.b.batch || ld_i32(&a.requests[i].layer) != 1) return;
-  const int64_t row = t * a.b.nq + h0, layer = a.b.tokens * a.b.nq;
-  using Vec = typename std::conditional<D == 128, float4, float2>::type;
-  Vec c[kMergeHeads], o[kMergeHeads];
-  float zc[kMergeHeads], zo[kMergeHeads];
-#pragma unroll
-  for (int k = 0; k < kMergeHeads; ++k) {  // (past the last head: that one again)
-    const int64_t at = row + min(k, heads - 1);
-    c[k] = __ldcs(reinterpret_cast<const Vec*>(a.rows + at * D) + lane);
-    o[k] = __ldcs(reinterpret_cast<const Vec*>(a.rows + (layer + at) * D) + lane);
-    zc[k] = __ldcs(a.rows_lse + at);
-    zo[k] = __ldcs(a.rows_lse + layer + at);
-  }
+  if (i >= a.b.batch || a.requests[i].layer != 1) return;
+  const PgShared group = a.groups[a.requests[i].group];
+  // the token's unit of common keys, and where in it its rows are
+  const int at = max((int)t - group.row0, 0), pair = at / (2 * a.s.tpt), in_pair = at - pair * 2 * a.s.tpt;
+  const int x = in_pair >= a.s.tpt ? 1 : 0, first = min(group.row0 + pair * 2 * a.s.tpt, (int)a.b.tokens - 1);
+  const bool few = min(2 * a.s.tpt, group.n - pair * 2 * a.s.tpt) <= a.s.tpf;
+  const float2* const pm = reinterpret_cast<const float2*>(a.partials + (int64_t)2 * a.grid * 2 * 128 * D);
+  const int64_t layer = a.b.tokens * a.b.nq;
 #pragma unroll
   for (int k = 0; k < kMergeHeads; ++k) {
-    if (k >= heads) break;
-    const float m = fmaxf(zc[k], zo[k]), base = m == -INFINITY ? 0.f : m;
-    const float ec = expf(zc[k] - base), eo = expf(zo[k] - base), sum = ec + eo, inv = sum == 0.f ? 0.f : 1.f / sum;
-    const float* const x = reinterpret_cast<const float*>(&c[k]);
-    const float* const y = reinterpret_cast<const float*>(&o[k]);
-    uint32_t v[kOwn / 2];
+    const int h = h0 + k;
+    if (h >= a.b.nq) return;
+    const int kvh = h / a.s.group, row = (in_pair - x * a.s.tpt) * a.s.group + h - kvh * a.s.group;
+    const int64_t out_row = t * a.b.nq + h;
+    PgUnit unit = a.units[(int64_t)first * a.b.nkv + kvh];
+    if (unit.cta < 0 || unit.pieces < 0 || unit.pieces > a.grid - unit.cta) unit.pieces = 0;  // (groups that overlap)
+    // the sum of what there is, each part with its weight 2^(m - M); the own part first
+    float acc[kOwn], M = a.rows_lse[layer + out_row] * 1.4426950408889634f, L = M == -INFINITY ? 0.f : 1.f;
+    auto take = [&](const Vec& v, float* f) {
+      const float* const e = reinterpret_cast<const float*>(&v);
 #pragma unroll
-    for (int d = 0; d < kOwn / 2; ++d)
-      v[d] = Elem<T>::pack((x[2 * d] * ec + y[2 * d] * eo) * inv, (x[2 * d + 1] * ec + y[2 * d + 1] * eo) * inv);
-    T* const to = reinterpret_cast<T*>(a.out) + t * a.ldo + (int64_t)(h0 + k) * D + lane * kOwn;
+      for (int d = 0; d < kOwn; ++d) f[d] = e[d];
+    };
+    auto add = [&](const Vec& v, float m, float l) {  // v: the sum of 2^(score - m) V, l of 2^(score - m)
+      if (l == 0.f) return;                           // (no key seen)
+      const float mn = fmaxf(M, m), fa = M == -INFINITY && L == 0.f ? 0.f : exp2f(M - mn), fb = exp2f(m - mn);
+      const float* const e = reinterpret_cast<const float*>(&v);
+      M = mn;
+      L = L * fa + l * fb;
+#pragma unroll
+      for (int d = 0; d < kOwn; ++d) acc[d] = acc[d] * fa + e[d] * fb;
+    };
+    take(__ldcs(reinterpret_cast<const Vec*>(a.rows + (layer + out_row) * D) + lane), acc);
+    if (unit.pieces == 0) {
+      const float z = a.rows_lse[out_row] * 1.4426950408889634f;
+      add(__ldcs(reinterpret_cast<const Vec*>(a.rows + out_row * D) + lane), z, z == -INFINITY ? 0.f : 1.f);
+    }
+#pragma unroll 1
+    for (int q0 = 0; q0 < unit.pieces; q0 += kMergePieces) {
+      float2 ml[kMergePieces];
+      Vec v[kMergePieces];
+#pragma unroll
+      for (int q = 0; q < kMergePieces; ++q) {
+        const int qq = min(q0 + q, unit.pieces - 1);  // past the last piece: the last again, not counted
+        const int64_t tile = (int64_t)(2 * (unit.cta + qq) + (qq == 0 ? 1 : 0)) * 2 + x;
+        ml[q] = pm[tile * 128 + row];
+        // few rows: [row][D]; tiles: [D / 4][128 rows][4], of which neighbouring heads share the sectors
+        v[q] = few ? reinterpret_cast<const Vec*>(a.partials + (tile * 128 + row) * D)[lane]
+                   : *reinterpret_cast<const Vec*>(a.partials + ((tile * (D / 4) + lane * kOwn / 4) * 128 + row) * 4 + lane * kOwn % 4);
+      }
+#pragma unroll
+      for (int q = 0; q < kMergePieces; ++q)
+        if (q0 + q < unit.pieces) add(v[q], ml[q].x, ml[q].y);
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    uint32_t o[kOwn / 2];
+#pragma unroll
+    for (int d = 0; d < kOwn / 2; ++d) o[d] = Elem<T>::pack(acc[2 * d] * inv, acc[2 * d + 1] * inv);
+    T* const to = reinterpret_cast<T*>(a.out) + t * a.ldo + (int64_t)h * D + lane * kOwn;
     if constexpr (D == 128)
-      *reinterpret_cast<uint2*>(to) = make_uint2(v[0], v[1]);
+      *reinterpret_cast<uint2*>(to) = make_uint2(o[0], o[1]);
     else
-      *reinterpret_cast<uint32_t*>(to) = v[0];
-    if (lane == 0 && a.lse) a.lse[t * a.ld_lse + h0 + k] = sum == 0.f ? -INFINITY : base + logf(sum);
+      *reinterpret_cast<uint32_t*>(to) = o[0];
+    if (lane == 0 && a.lse) a.lse[t * a.ld_lse + h] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
   }
 }
 
 // After the attention's own scratch: the rows of work, and the two layers.
 struct PrefixPlan {
-  int64_t off_shared, off_rows, off_lse, bytes;
+  int64_t off_shared, off_rows, off_lse, off_units, bytes;
 };
-static PrefixPlan prefix_plan(int grid, int head_dim, int nq, int64_t tokens, int64_t entries) {
+static PrefixPlan prefix_plan(int grid, int head_dim, int nq, int nkv, int64_t tokens, int64_t entries) {
   auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
   PrefixPlan p;
   p.off_shared = up(paged_attn_plan(grid, head_dim).bytes);
   p.off_rows = p.off_shared + up(entries * (int64_t)sizeof(PgShared));
   p.off_lse = p.off_rows + up(2 * tokens * nq * head_dim * 4);
-  p.bytes = p.off_lse + up(2 * tokens * nq * 4);
+  p.off_units = p.off_lse + up(2 * tokens * nq * 4);
+  p.bytes = p.off_units + up(tokens * nkv * (int64_t)sizeof(PgUnit));
   return p;
 }
 
@@ -162,7 +202,7 @@ extern "C" int qd_prefix_attn_plan(int nq_heads, int nkv_heads, int head_dim, in
   if (rc != QD_OK) return rc;
   if (max_tokens < 0 || max_tokens > INT32_MAX || max_requests < 0)
     return set_error(QD_ERR_ARG, "prefix attention plan: %lld tokens, %d requests", (long long)max_tokens, max_requests);
-  *scratch_bytes = prefix_plan(*grid, head_dim, nq_heads, max_tokens, 2 * (int64_t)max_requests).bytes;
+  *scratch_bytes = prefix_plan(*grid, head_dim, nq_heads, nkv_heads, max_tokens, 2 * (int64_t)max_requests).bytes;
   return QD_OK;
 }
 
@@ -186,7 +226,7 @@ extern "C" int qd_prefix_attn(const void* q, int64_t ldq, int dtype, int64_t tok
     return set_error(QD_ERR_ARG, "%s: head stride %lld (whole groups of 8 rows)", what, (long long)ps_head);
   if (n_groups < 0 || n_groups > batch || (n_groups > 0 && tokens > 0 && (!cu_groups || !prefix_len)))
     return set_error(QD_ERR_ARG, "%s: %d groups of %d requests, or null groups", what, n_groups, batch);
-  const PrefixPlan plan = prefix_plan(grid < 1 ? 1 : grid, head_dim, nq_heads, tokens, (int64_t)batch + n_groups);
+  const PrefixPlan plan = prefix_plan(grid < 1 ? 1 : grid, head_dim, nq_heads, nkv_heads, tokens, (int64_t)batch + n_groups);
   if (grid < 1 || !scratch || scratch_bytes < plan.bytes || (reinterpret_cast<uintptr_t>(scratch) & 31))
     return set_error(QD_ERR_SCRATCH, "%s: grid %d, %lld tokens, %d requests and %d groups need %lld B of 32-byte aligned scratch (have %lld)",
                      what, grid, (long long)tokens, batch, n_groups, (long long)plan.bytes, (long long)scratch_bytes);
@@ -201,10 +241,13 @@ extern "C" int qd_prefix_attn(const void* q, int64_t ldq, int dtype, int64_t tok
   float *const rows = reinterpret_cast<float*>(base + plan.off_rows), *const rows_lse = reinterpret_cast<float*>(base + plan.off_lse);
   const int rp = launch_kernel((const void*)prefix_plan_kernel, dim3(1), dim3(kPlanThreads), 0, pdl, stream, &p);
   if (rp != QD_OK) return rp;
-  const int ra = launch_shared(p.b, p.shared, batch + n_groups, rows, rows_lse, q, ldq, dtype, head_dim, k_pages, v_pages, scale,
+  PgUnit* const units = reinterpret_cast<PgUnit*>(base + plan.off_units);
+  const int ra = launch_shared(p.b, p.shared, batch + n_groups, rows, rows_lse, units, q, ldq, dtype, head_dim, k_pages, v_pages, scale,
                                out, ldo, lse, ld_lse, grid, scratch, pdl, stream);
   if (ra != QD_OK || n_groups == 0) return ra;
-  PrefixMergeArgs m = {p.b, p.shared + n_groups, rows, rows_lse, static_cast<char*>(out), lse, ldo, ld_lse};
+  const float* const partials = reinterpret_cast<const float*>(base + paged_attn_plan(grid, head_dim).off_partials);
+  PrefixMergeArgs m = {p.b, p.s, p.shared, p.shared + n_groups, units, partials, rows, rows_lse, static_cast<char*>(out),
+                       lse, ldo, ld_lse, grid};
   const int64_t warps = tokens * ((nq_heads + kMergeHeads - 1) / kMergeHeads), ctas = (warps + kMergeWarps - 1) / kMergeWarps;
   if (ctas > INT32_MAX) return set_error(QD_ERR_UNSUPPORTED, "%s: %lld tokens", what, (long long)tokens);
   const bool bf = dtype == QD_BF16;

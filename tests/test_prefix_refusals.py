@@ -41,7 +41,7 @@ def test_prefix_plan(lib):  # noqa: F811
     rc, grid, small = _plan(lib, 32, 8, 128, 64, 64, 5)
     assert rc == 0 and grid == 5
     rc, _, large = _plan(lib, 32, 8, 128, 2048, 64, 5)
-    assert rc == 0 and large - small == 2 * (2048 - 64) * 32 * (128 + 1) * 4
+    assert rc == 0 and large - small == (2048 - 64) * (2 * 32 * (128 + 1) * 4 + 8 * 8)
     assert _plan(lib, 32, 8, 128, 1 << 31, 64, 0)[0] == 1 and _plan(lib, 32, 8, 128, -1, 64, 0)[0] == 1
     assert _plan(lib, 32, 8, 128, 64, -1, 0)[0] == 1 and _plan(lib, 32, 7, 128, 64, 64, 0)[0] == 4
     # scratch for fewer tokens, or requests, than a call has
