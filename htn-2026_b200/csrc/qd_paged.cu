@@ -44,21 +44,22 @@ __device__ __forceinline__ int row_exponent(float most) {
   const int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
   return min(max(e, kHeldLeastExp), kHeldMostExp);
 }
-// Two values over the row's power of two as E4M3: beyond +-448 (where the exponent was cut) +-448, infinities as NaN.
+// Two values over the row's power of two as E4M3: beyond +-448 (where the exponent was cut) +-448.
 __device__ __forceinline__ uint32_t held_pair(float a, float b, float inv) {
-  const float nan = __uint_as_float(0x7fffffffu);
-  return __nv_cvt_float2_to_fp8x2(make_float2(fabsf(a) <= FLT_MAX ? a * inv : nan, fabsf(b) <= FLT_MAX ? b * inv : nan),
-                                  __NV_SATFINITE, __NV_E4M3);
+  return __nv_cvt_float2_to_fp8x2(make_float2(a * inv, b * inv), __NV_SATFINITE, __NV_E4M3);
 }
 
 constexpr int kAppendThreads = 128;
+// CTAs an SM, which is 72 registers a thread: 16-bit pages need no more, and into 8-bit pages 13,808 tokens take 83 us,
+// where 96 registers without a spill take 102 (a warp waits for its loads most of the time)
+constexpr int kAppendResident = 7;
 
 // kUnits: groups of heads of one token that a warp takes, all their loads in flight before the first is used.
 // 13,808 prompt tokens of 48 heads of 128 take 71 us, 5.1 TB/s over the 364 MB that have to move (a copy
 // reaches 6.5); 64 single tokens 3.0 us and one 2.2 us in a graph, of which the launch is most (a call takes the
 // host 11.8).
 template <typename T, int D, int kUnits, bool kHeld>
-__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __grid_constant__ AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, kAppendResident) paged_append_kernel(const __grid_constant__ AppendArgs a) {
   constexpr int kLanes = D / 16, kHeads = 32 / kLanes;  // lanes per head, heads per unit
   grid_dep_wait();
   grid_dep_launch();
@@ -141,7 +142,9 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __gr
       }
     };
     unpack();
-    if (a.q_norm) {  // every lane takes part in the sum; V heads do not use it
+    // (of 8-bit rows, whose instructions come on top of these, a warp's V heads alone need neither norm nor rotation)
+    const bool plain = kHeld && h0 + unit * kHeads - lane / kLanes >= a.b.nq + a.b.nkv;
+    if (a.q_norm && !plain) {  // every lane takes part in the sum; V heads do not use it
       float sq = 0.f;
 #pragma unroll
       for (int k = 0; k < 16; ++k) sq = fmaf(x[k], x[k], sq);
@@ -159,7 +162,7 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __gr
         x[8 + 2 * k + 1] *= rstd * q.y;
       }
     }
-    if (turned) {
+    if (turned && !plain) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const float p = x[k], q = x[8 + k];
@@ -168,12 +171,21 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __gr
       }
     }
     if (kHeld && h0 + unit * kHeads - lane / kLanes + kHeads > a.b.nq) {  // (some head of the warp's is K or V)
-      if (is_v) unpack();  // V goes in as it was
-      float most = 0.f;
+      if (is_v && !plain) unpack();  // V goes in as it was
+      auto largest = [&]() {  // of the row (NaN is passed over)
+        float m = 0.f;
 #pragma unroll
-      for (int k = 0; k < 16; ++k) most = fmaxf(most, fabsf(x[k]) <= FLT_MAX ? fabsf(x[k]) : 0.f);
+        for (int k = 0; k < 16; ++k) m = fmaxf(m, fabsf(x[k]));
 #pragma unroll
-      for (int o = kLanes / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        for (int o = kLanes / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        return m;
+      };
+      float most = largest();
+      if (__any_sync(0xffffffffu, most > FLT_MAX)) {  // infinities are held as NaN, and are not what a row is measured by
+#pragma unroll
+        for (int k = 0; k < 16; ++k) x[k] = fabsf(x[k]) <= FLT_MAX ? x[k] : __uint_as_float(0x7fffffffu);
+        most = largest();
+      }
       if (h >= heads || !dst) continue;
       if (h >= a.b.nq) {
         const int e = row_exponent(most);

@@ -40,6 +40,7 @@ QD_LINE_FN T pg_max(T x, T y) {
 struct PgShape {
   int nkv, group, tpt, tpf;   // heads per KV head; tokens per tile and per 16 rows (0: a group is larger)
   int period, period_blocks;  // ceil sums over tile pairs repeat every `period` pairs, `period_blocks` blocks on
+  int few_cost;               // a few-row unit's fixed cost
 };
 inline PgShape pg_shape(int nq, int nkv) {
   PgShape s;
@@ -50,6 +51,7 @@ inline PgShape pg_shape(int nq, int nkv) {
   const int pair = 2 * s.tpt, two = pair & -pair, g = two < kPgKeys ? two : kPgKeys;  // g = gcd(pair, 128)
   s.period = kPgKeys / g;
   s.period_blocks = pair / g;
+  s.few_cost = 0;
   return s;
 }
 
@@ -85,7 +87,7 @@ QD_LINE_FN int pg_weight(const PgShape& s, const PgReq& r, int k) {
 }
 // and of its fixed cost
 QD_LINE_FN int pg_fixed(const PgShape& s, const PgReq& r, int k) {
-  return r.n - k * 2 * s.tpt > s.tpf ? kPgUnitCost : 0;
+  return r.n - k * 2 * s.tpt > s.tpf ? kPgUnitCost : s.few_cost;
 }
 QD_LINE_FN int pg_cost(const PgShape& s, const PgReq& r, int k) {
   return pg_fixed(s, r, k) + pg_weight(s, r, k) * pg_blocks(s, r, k);
