@@ -1502,7 +1502,7 @@ int launch_tiles8(const Paged8Call& c, int least) {
   a.ld_lse = c.ld_lse;
   a.scale_log2 = c.scale * 1.4426950408889634f;
   a.tickets = static_cast<int*>(c.scratch);
-  a.partials = reinterpret_cast<float*>(static_cast<char*>(c.scratch) + paged_attn_plan(c.grid, c.head_dim).off_partials);
+  a.partials = reinterpret_cast<float*>(static_cast<char*>(c.scratch) + paged8_plan(c.grid, c.head_dim).off_tiles);
   a.k_scale = static_cast<const uint8_t*>(c.k_scale);
   a.v_scale = static_cast<const uint8_t*>(c.v_scale);
   a.ss_page = c.ss_page;

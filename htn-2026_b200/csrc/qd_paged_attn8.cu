@@ -1,15 +1,18 @@
 // Causal grouped-query attention of a ragged batch's new tokens over cache pages of 8 bits: the entry points. Requests of
 // at most 16 query rows a KV head (single tokens) run in qd_paged_few8.cu, the others in tiles of 128 rows in
 // qd_paged_attn.cu. Two launches, since what bounds them differs (the memory, and the tensor cores with the softmax) and
-// with it all of their shared memory and warps; a caller that knows that there are no longer requests saves the second
-// (some 3 us). The second waits for the first, so they can share the scratch.
+// with it all of their shared memory and warps. The second does not wait for the first, which waits for what came before
+// both, but for its end: it fills the SMs that the first leaves. A caller that knows that there are no longer requests
+// saves a launch.
 #include "qd_paged_attn8.h"
 
 using namespace qd;
 
 extern "C" int qd_paged_attn8_plan(int nq_heads, int nkv_heads, int head_dim, int grid_hint, int* grid,
                                    int64_t* scratch_bytes) {
-  return qd_paged_attn_plan(nq_heads, nkv_heads, head_dim, grid_hint, grid, scratch_bytes);
+  const int rc = qd_paged_attn_plan(nq_heads, nkv_heads, head_dim, grid_hint, grid, scratch_bytes);
+  if (rc == QD_OK) *scratch_bytes = paged8_plan(*grid, head_dim).bytes;
+  return rc;
 }
 
 extern "C" int qd_paged_attn8(const void* q, int64_t ldq, int dtype, int64_t tokens, int nq_heads, int nkv_heads,
@@ -29,7 +32,7 @@ extern "C" int qd_paged_attn8(const void* q, int64_t ldq, int dtype, int64_t tok
       ldq < (int64_t)nq_heads * head_dim || ldo < (int64_t)nq_heads * head_dim || (lse && ld_lse < nq_heads) || !(scale > 0.f))
     return set_error(QD_ERR_ARG, "%s: q / out / lse null, misaligned or with a bad stride (%lld, %lld, %lld), or scale %g",
                      what, (long long)ldq, (long long)ldo, (long long)ld_lse, (double)scale);
-  const int64_t need = paged_attn_plan(grid < 1 ? 1 : grid, head_dim).bytes;
+  const int64_t need = paged8_plan(grid < 1 ? 1 : grid, head_dim).bytes;
   if (grid < 1 || !scratch || scratch_bytes < need || (reinterpret_cast<uintptr_t>(scratch) & 31))
     return set_error(QD_ERR_SCRATCH, "%s: grid %d needs %lld B of 32-byte aligned scratch (have %lld)", what, grid,
                      (long long)need, (long long)scratch_bytes);
@@ -55,9 +58,9 @@ extern "C" int qd_paged_attn8(const void* q, int64_t ldq, int dtype, int64_t tok
   c.stream = stream;
   const int few = kFewRows / (nq_heads / nkv_heads);  // tokens of a request of few rows
   const bool only_few = (max_new > 0 && max_new <= few) || tokens <= few;
-  if (few > 0) {
-    const int rf = launch_few8(c, only_few);
-    if (rf != QD_OK || only_few) return rf;
+  if (!only_few || few == 0) {
+    const int rt = launch_tiles8(c, few + 1);
+    if (rt != QD_OK || few == 0) return rt;
   }
-  return launch_tiles8(c, few + 1);
+  return launch_few8(c, !only_few);
 }

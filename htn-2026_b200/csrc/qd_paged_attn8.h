@@ -18,6 +18,21 @@ inline PagedAttnPlan paged_attn_plan(int grid, int head_dim) {
   return p;
 }
 
+// Of the attention over pages of 8 bits, whose two kernels may run at once: the tickets of both ([grid][2] each), then the
+// pieces of each.
+constexpr int kF8Resident = 2;  // CTAs an SM of the kernel for few rows
+struct Paged8Plan {
+  int64_t off_few_tickets, off_tiles, off_few, bytes;
+};
+inline Paged8Plan paged8_plan(int grid, int head_dim) {
+  Paged8Plan p;
+  p.off_few_tickets = (int64_t)grid * 2 * 4;
+  p.off_tiles = ((int64_t)grid * 4 * 4 + 255) / 256 * 256;
+  p.off_few = p.off_tiles + (int64_t)2 * grid * 2 * 128 * (head_dim * 4 + 8);
+  p.bytes = p.off_few + (int64_t)2 * grid * kF8Resident * kFewRows * (head_dim * 4 + 8);
+  return p;
+}
+
 // positions in a row of the page table, as many as are attended to
 inline int pg_room(const PagedBatch& b) {
   const int64_t room = (int64_t)b.max_pages * b.page_size;
@@ -53,9 +68,9 @@ struct Paged8Call {
   void* scratch;
   cudaStream_t stream;
 };
-// The requests of at most 16 query rows a KV head (of none, where a group of heads is larger). `alone`: there is no
-// other launch for the rest, whose rows are left as they are and flagged.
-int launch_few8(const Paged8Call& c, bool alone);
+// The requests of at most 16 query rows a KV head (of none, where a group of heads is larger). `beside`: launch_tiles8
+// came right before, for the rest; without it their rows are left as they are and flagged.
+int launch_few8(const Paged8Call& c, bool beside);
 // The requests of `least` tokens and more, in tiles of 128 query rows.
 int launch_tiles8(const Paged8Call& c, int least);
 // Maps of the values: a box is a page of a KV head as rows of `row` bytes (head_dim or 128), swizzled over as many.

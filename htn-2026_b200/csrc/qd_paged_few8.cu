@@ -34,7 +34,6 @@
 namespace qd {
 
 constexpr int kF8Threads = 256;  // warps 0-3 softmax, 4 producer, 5 MMA, 6 the line and the queries, 7 the scales
-constexpr int kF8Resident = 2;   // CTAs an SM
 constexpr int kF8Scales = 8;     // blocks whose scales are in shared memory
 constexpr int kF8Unit = 2;       // blocks' time that a unit's start and end take
 constexpr int kF8Bias = 7;       // P' is up to 2^(8 + 7): the upper end of E5M2's range
@@ -75,6 +74,7 @@ struct alignas(64) Few8Args {
   int room;       // positions in a row of the page table, kPgMaxKeys at most
   int inv_group;  // row / group = row * inv_group >> 16
   int alone;      // no other kernel takes the requests of more tokens
+  int beside;     // the kernel before is the one for those: nothing of it is waited for but its end
   float scale_log2;
   float* partials;  // [2 * grid slots][16 rows][D], then the rows' (m, l)
   int* tickets;     // [grid]
@@ -252,7 +252,8 @@ __global__ void __launch_bounds__(kF8Threads, kF8Resident) paged_few8_kernel(con
     for (int m = 1; m < 16; ++m) misc[m] = 0;
   }
   if (warp == 5) tmem_alloc(smem_u32(misc), 256);
-  grid_dep_wait();
+  // (the kernel before it waited for what came before both)
+  if (!a.beside) grid_dep_wait();
   {  // the page table on its way to L2 while the lengths are read: a line per thread of the grid
     const int lines = (a.b.max_pages + 31) / 32;
     const int64_t at = (int64_t)blockIdx.x * kF8Threads + tid, row = at / lines;
@@ -815,6 +816,7 @@ __global__ void __launch_bounds__(kF8Threads, kF8Resident) paged_few8_kernel(con
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (a.beside) grid_dep_wait();  // whoever waits for this kernel waits for both
   if (warp == 5) tmem_dealloc(tmem, 256);
   if (tid == 0) {  // no copy may still be writing shared memory when the CTA exits
     const int n = misc[8];
@@ -837,7 +839,7 @@ int map_pools8(const Paged8Call& c, PFN_cuTensorMapEncodeTiled_v12000 encode, in
   return QD_OK;
 }
 
-int launch_few8(const Paged8Call& c, bool alone) {
+int launch_few8(const Paged8Call& c, bool beside) {
   const PagedBatch& b = c.b;
   Few8Args a = {};
   a.b = b;
@@ -859,10 +861,12 @@ int launch_few8(const Paged8Call& c, bool alone) {
   a.ss_head = c.ss_head;
   a.room = (int)std::min((int64_t)b.max_pages * b.page_size, (int64_t)kPgMaxKeys);
   a.inv_group = 65536 / a.s.group + 1;
-  a.alone = alone;
+  a.alone = !beside;
+  a.beside = beside;
   a.scale_log2 = c.scale * 1.4426950408889634f;
-  a.tickets = static_cast<int*>(c.scratch);
-  a.partials = reinterpret_cast<float*>(static_cast<char*>(c.scratch) + paged_attn_plan(c.grid, D).off_partials);
+  const Paged8Plan plan = paged8_plan(c.grid, c.head_dim);
+  a.tickets = reinterpret_cast<int*>(static_cast<char*>(c.scratch) + plan.off_few_tickets);
+  a.partials = reinterpret_cast<float*>(static_cast<char*>(c.scratch) + plan.off_few);
   const bool bf = c.dtype == QD_BF16;
   const void* fn = bf ? (D == 128 ? (const void*)paged_few8_kernel<__nv_bfloat16, 128> : (const void*)paged_few8_kernel<__nv_bfloat16, 64>)
                       : (D == 128 ? (const void*)paged_few8_kernel<__half, 128> : (const void*)paged_few8_kernel<__half, 64>);

@@ -231,6 +231,9 @@ class PagedAttention8(PagedAttention):
 
     PLAN = "qd_paged_attn8_plan"
 
+    def reset(self) -> None:
+        self.scratch[:16 * self.grid].zero_()  # (two kernels' counts)
+
     def __call__(self, q, k_pages, v_pages, k_scale, v_scale, cu_tokens, kv_len, page_table, out, lse=None,
                  scale: float | None = None, max_new: int | None = None, err=None, pdl: bool = True):
         """As PagedAttention's. max_new: no request of this call has more new tokens (1 for a step of single tokens)."""

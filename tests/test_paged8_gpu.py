@@ -344,6 +344,40 @@ def test_attention8_flags_what_it_cannot_reach():
     assert bool(((out.double().cpu() - ref).abs() <= tol).all()), "a request cut to its table row uses the row's keys"
 
 
+def test_attention8_scratch_is_made_ready_again():
+    """A call that ends early leaves counts in the scratch, as they are set here; after reset() the object answers as a
+    new one does."""
+    b = R8.Batch8([(1, 2900), (70, 1333), (1, 5)], 8, 2, 128, 32, seed=1, device=DEV)
+    handle = _paged().PagedAttention8(8, 2, 128, DEV)
+    first, _ = _attend8(b, handle)
+    handle.scratch[:16 * handle.grid] = 1
+    handle.reset()
+    out, lse = _attend8(b, handle)
+    _check(b, out, lse)
+    assert torch.equal(out, first)
+
+
+@pytest.mark.parametrize("pdl", [True, False])
+def test_attention8_calls_in_a_row_on_what_the_last_one_wrote(pdl):
+    """Queries written by the kernel before, and results read by the kernel after, with both kernels at work: neither starts
+    before what it reads is there, nor does a later call overtake an earlier one's kernels."""
+    b = R8.Batch8([(1, 3000), (60, 900), (1, 700), (2, 90)], 8, 2, 128, 32, seed=7, device=DEV)
+    handle = _paged().PagedAttention8(8, 2, 128, DEV)
+    pools = [b.on(n) for n in ("k_pages", "v_pages", "k_scale", "v_scale")]
+    cu, kv_len, table, q0 = b.on("cu"), b.on("kv_len"), b.on("table"), b.on("q")
+    want, _ = _attend8(b, handle)
+    q, out, sums = torch.zeros_like(q0), torch.empty_like(q0), []
+    for k in range(6):
+        q.zero_()
+        handle(q, *pools, cu, kv_len, table, out, pdl=pdl)
+        q.copy_(q0)
+        handle(q, *pools, cu, kv_len, table, out, pdl=pdl)
+        sums.append(out.clone())
+        out.fill_(math.nan)
+    torch.cuda.synchronize()
+    assert all(torch.equal(s, want) for s in sums)
+
+
 def test_attention8_in_a_graph_follows_the_lengths():
     P = _paged()
     b = R8.Batch8([(1, 400), (20, 300)], 4, 1, 128, 16, seed=12, device=DEV)
