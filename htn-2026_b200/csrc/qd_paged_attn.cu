@@ -78,6 +78,11 @@ static_assert(2 * kPgSoftmaxRegs + kPgOtherRegs <= 3 * 168 && 2 * kPgHeldSoftmax
 constexpr int kPgBox = 128 * 128;  // [128 rows][64 dims] of 16 bits
 constexpr int kFewP = 2 * kFewRows * 128;  // its P: 2 halves of 64 keys x 16 rows of 128 B
 constexpr int kPgManyUnits = 1 << 20;  // above any grid (whose scratch would be 280 GB); 384 of them fit 32 bits
+// Pages of 8 bits: units are left whole if the longest takes no more than the SMs' even share of all work, the other
+// kernel's too, and this, about what storing and joining pieces takes. 30 single tokens and 2 chunks of 251 after up to 2 k
+// keys (64 units of 16 blocks): 95 us whole, with the single tokens on the SMs that have none, 129 cut; the chunks alone 67
+// and 90; with 40 places for 60 chunks after up to 3 k keys are cut, 153 us, 121 whole.
+constexpr int kPgHeldJoin = 60;
 constexpr int kPgHeldBias = 7;  // pages of 8 bits: P' = 2^7 P
 constexpr int kPgWhole = 8;   // key blocks up to which units of tiles are left whole, when there are CTAs for all
 
@@ -368,8 +373,15 @@ __global__ void __launch_bounds__(pg_threads(kHeld), 1) paged_attn_kernel(const 
   const int i0 = min(tid * per, a.b.batch), i1 = min(i0 + per, a.b.batch);
   PgReq r = {};
   bool cut = false, tiles = false, longer = false;
+  int longest = 0;     // pages of 8 bits: places of the longest unit, and of the other kernel's work
+  int64_t beside = 0;
   for (int i = i0; i < i1; ++i) {
     r = pg_own_request<kHeld, kShared>(a, i);
+    if constexpr (kHeld) {
+      const PgReq f = pg_request(a, i);
+      if (f.n > 0 && r.n == 0) beside += (int64_t)a.b.nkv * pg_blocks(a.s, f, 0);  // (about a place each)
+      for (int k = pg_max(r.pairs - 2, 0); k < r.pairs; ++k) longest = max(longest, pg_cost(a.s, r, k));
+    }
     tiles |= r.n > a.s.tpf;
     cut |= !kShared && r.kv != r.pos0 + r.n && r.n > 0;
     mine += a.b.nkv * pg_sum_cost(a.s, r);
@@ -392,6 +404,17 @@ __global__ void __launch_bounds__(pg_threads(kHeld), 1) paged_attn_kernel(const 
     scan[warp] = incl;
     scan_u[warp] = incl_u;
   }
+  int* const warp_longest = reinterpret_cast<int*>(smem + Lay::ml);
+  int64_t* const warp_beside = reinterpret_cast<int64_t*>(smem + Lay::ml + 64);
+  if constexpr (kHeld) {
+    longest = __reduce_max_sync(0xffffffffu, longest);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) beside += __shfl_xor_sync(0xffffffffu, beside, o);
+    if (lane == 0) {
+      warp_longest[warp] = longest;
+      warp_beside[warp] = beside;
+    }
+  }
   tc_fence_before();
   tiles = __syncthreads_or(tiles);
   longer = __syncthreads_or(longer);
@@ -401,6 +424,15 @@ __global__ void __launch_bounds__(pg_threads(kHeld), 1) paged_attn_kernel(const 
 #pragma unroll
   for (int w = 0; w < kPgThreads / 32; ++w) units += scan_u[w];
   // Units of tiles that are few and short are not cut: a place each, and a CTA each
+  if constexpr (kHeld) {
+    int64_t all = 0;
+#pragma unroll
+    for (int w = 0; w < kPgThreads / 32; ++w) {
+      longest = max(longest, warp_longest[w]);
+      all += scan[w] + warp_beside[w];
+    }
+    longer = longest > all / (int)gridDim.x + kPgHeldJoin;
+  }
   const bool whole = tiles && !longer && units <= (int)gridDim.x;
   if (whole) {
     mine = mine_u;
