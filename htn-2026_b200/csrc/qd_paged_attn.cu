@@ -38,7 +38,8 @@
 // its slot; a raw row lands where the row's last 64 dims will be, so a lane that has read its row may write it at once.
 // Rows past the last key, and of pages that are not there, are written as zeros. The same warps turn BF16 queries into
 // FP16, a power of two of each row (its largest to 2^14) taken out and multiplied onto the scores. P' = 2^7 P: with up to
-// 2^15, FP16 holds what weighs 2^-31 of a row's largest.
+// 2^15, FP16 holds what weighs 2^-31 of a row's largest. 2048 tokens after 8192 keys take 475 to 489 us (0.39 of the BF16
+// peak); the same pipeline without the widening 374, and with 208 registers for the softmax 328.
 //
 // Shared beginnings (kShared): the rows of work are not the requests but PgShared entries, a group's tokens over the keys
 // that its requests have in common and each request's over its own; see qd_prefix_attn.cu. The results of both go to
