@@ -44,8 +44,8 @@
 // Shared beginnings (kShared): the rows of work are not the requests but PgShared entries, a group's tokens over the keys
 // that its requests have in common and each request's over its own; see qd_prefix_attn.cu. The results of both go to
 // fp32 rows, to be joined afterwards, and the pieces of a cut unit of common keys stay where they are, to be joined with
-// them: by the whole GPU, where the CTA that ends last would read 128 KB a piece (64 tokens after 4096 keys, 14 pieces: 73
-// us, 45 of them that).
+// them by the whole GPU, where the CTA that ends last would read 128 KB a piece (a chunk of 64 tokens after 4032 keys, of
+// which a unit is cut into 14 pieces, takes 73 us without).
 //
 // Measured, 32 query and 8 KV heads of 128 in BF16: 8 single tokens over up to 41 k keys 183 us (HBM: 6.3 TB/s); 64
 // single tokens over 1 to 1.5 k keys 72 us (4.7 TB/s: each CTA's start and end); one token over 1 k keys 12.3 us in a
@@ -566,7 +566,7 @@ __global__ void __launch_bounds__(pg_threads(kHeld), 1) paged_attn_kernel(const 
           s->c0 = c0;
           s->nc = c1 - c0 + 1;
           if (kShared && layer == 0)
-            a.units[(int64_t)(r.row0 + t0) * a.b.nkv + h] = PgUnit{c0, j0 == 0 && j1 == nblk ? 0 : c1 - c0 + 1};
+            a.units[(int64_t)(r.row0 + t0) * a.b.nkv + h] = PgUnit{c0, j0 == 0 && j1 == nblk ? 0 : (c1 - c0 + 1) | (few ? PgUnit::kFew : 0)};
           s->region = two ? -1 : ra;
           mbar_arrive(segfull(seg));
         }

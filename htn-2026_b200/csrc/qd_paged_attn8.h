@@ -44,12 +44,13 @@ inline int pg_room(const PagedBatch& b) {
 // that are shared, 1: of a request's own), or -1: straight out.
 struct alignas(16) PgShared {
   int row0, n, pos0, kv;
-  int jb, table_row, layer, group;  // (group: a request's, where layer is 1)
+  int jb, table_row, layer, group_row0;  // (the last: a request's, where layer is 1)
 };
 // A unit of common keys, known by its first token row and KV head: its first CTA and the number of its pieces in the
 // scratch (0: it was not cut, and is in the rows). Piece p has slot 2 (cta + p) + (p == 0).
-struct PgUnit {
-  int cta, pieces;
+struct alignas(8) PgUnit {
+  int cta, pieces;  // (kFew: the pieces are of few rows)
+  static constexpr int kFew = 1 << 30;
 };
 // The 16-bit attention over `entries` such rows of work; rows and rows_lse: 2 layers of [tokens][nq] rows.
 int launch_shared(const PagedBatch& b, const PgShared* shared, int entries, float* rows, float* rows_lse, PgUnit* units,

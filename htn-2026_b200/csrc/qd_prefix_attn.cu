@@ -10,9 +10,9 @@
 //          query heads a KV head are a pair of tiles there, so a block of common keys is read, and multiplied, once for
 //          all, and both kinds of work fill the SMs together. The results go to fp32 rows, two layers of them, as a second
 //          rounding to 16 bits would cost as much as the last.
-//   merge  joins the layers' rows and the pieces that units of common keys were cut into, a warp for 2 heads of a token.
-// Measured, 32 query and 8 KV heads of 128: 64 users, 4 k common and up to 1 k own keys each, 84 us, of which the plan is 3.5
-// and the merge 5 (dependent loads); 4 documents of 16 k keys with 4 answers each 79 us. The floors are 36 and 38; the rest
+//   merge  joins the layers' rows and the pieces that units of common keys were cut into, a warp per token and head.
+// Measured, 32 query and 8 KV heads of 128: 64 users, 4 k common and up to 1 k own keys each, 81 us, of which the plan is 3.5
+// and the merge some 3 (dependent loads); 4 documents of 16 k keys with 4 answers each 76 us. The floors are 36 and 38; the rest
 // is what the attention kernel loses on short units.
 // A group is taken apart again (its requests read all keys, straight to out) where sharing would not pay: see the plan.
 #include "qd_host.h"
@@ -20,7 +20,7 @@
 
 namespace qd {
 
-constexpr int kPlanThreads = 1024, kMergeWarps = 8, kMergeHeads = 2, kMergePieces = 4;
+constexpr int kPlanThreads = 1024, kMergeWarps = 8, kMergePieces = 4;
 
 struct PrefixPlanArgs {
   PagedBatch b;
@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(kPlanThreads) prefix_plan_kernel(const __grid_
         if (request(i).n > 0) {
           a.shared[a.n_groups + i].jb = blocks;
           a.shared[a.n_groups + i].layer = 1;
-          a.shared[a.n_groups + i].group = g;
+          a.shared[a.n_groups + i].group_row0 = first;
         }
   }
 }
@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(kPlanThreads) prefix_plan_kernel(const __grid_
 struct PrefixMergeArgs {
   PagedBatch b;
   PgShape s;
-  const PgShared *groups, *requests;
+  const PgShared* requests;
   const PgUnit* units;
   const float *partials, *rows, *rows_lse;
   char* out;
@@ -108,76 +108,71 @@ __global__ void __launch_bounds__(kMergeWarps * 32) prefix_merge_kernel(const __
   using Vec = typename std::conditional<D == 128, float4, float2>::type;
   grid_dep_wait();
   grid_dep_launch();
-  const int lane = threadIdx.x & 31, per = (a.b.nq + kMergeHeads - 1) / kMergeHeads;
-  const int64_t w = (int64_t)blockIdx.x * kMergeWarps + (threadIdx.x >> 5), t = w / per;
+  const int lane = threadIdx.x & 31;
+  const int64_t w = (int64_t)blockIdx.x * kMergeWarps + (threadIdx.x >> 5), t = w / a.b.nq;
   if (t >= a.b.tokens) return;
-  const int h0 = (int)(w - t * per) * kMergeHeads;
+  const int h = (int)(w - t * a.b.nq), kvh = h / a.s.group;
   const int i = warp_find_request(a.b.cu, a.b.batch, (int)t, lane);
-  if (i >= a.b.batch || a.requests[i].layer != 1) return;
-  const PgShared group = a.groups[a.requests[i].group];
-  // the token's unit of common keys, and where in it its rows are
-  const int at = max((int)t - group.row0, 0), pair = at / (2 * a.s.tpt), in_pair = at - pair * 2 * a.s.tpt;
-  const int x = in_pair >= a.s.tpt ? 1 : 0, first = min(group.row0 + pair * 2 * a.s.tpt, (int)a.b.tokens - 1);
-  const bool few = min(2 * a.s.tpt, group.n - pair * 2 * a.s.tpt) <= a.s.tpf;
+  if (i >= a.b.batch) return;
+  const PgShared request = a.requests[i];
+  if (request.layer != 1) return;
+  // the token's unit of common keys, and where in it its row is
+  const int at = max((int)t - request.group_row0, 0), in_pair = at % (2 * a.s.tpt);
+  const int x = in_pair >= a.s.tpt ? 1 : 0, row = (in_pair - x * a.s.tpt) * a.s.group + h - kvh * a.s.group;
   const float2* const pm = reinterpret_cast<const float2*>(a.partials + (int64_t)2 * a.grid * 2 * 128 * D);
-  const int64_t layer = a.b.tokens * a.b.nq;
+  const int64_t layer = a.b.tokens * a.b.nq, out_row = t * a.b.nq + h;
+  const PgUnit unit = a.units[((int)t - in_pair < 0 ? 0 : (int)t - in_pair) * (int64_t)a.b.nkv + kvh];
+  const bool few = unit.pieces & PgUnit::kFew;
+  int pieces = unit.pieces & ~PgUnit::kFew;
+  if (unit.cta < 0 || pieces < 0 || pieces > a.grid - unit.cta) pieces = 0;  // (groups that overlap)
+  // the sum of what there is, each part with its weight 2^(m - M); the own part first
+  float acc[kOwn], M = a.rows_lse[layer + out_row] * 1.4426950408889634f, L = M == -INFINITY ? 0.f : 1.f;
+  auto take = [&](const Vec& v, float* f) {
+    const float* const e = reinterpret_cast<const float*>(&v);
 #pragma unroll
-  for (int k = 0; k < kMergeHeads; ++k) {
-    const int h = h0 + k;
-    if (h >= a.b.nq) return;
-    const int kvh = h / a.s.group, row = (in_pair - x * a.s.tpt) * a.s.group + h - kvh * a.s.group;
-    const int64_t out_row = t * a.b.nq + h;
-    PgUnit unit = a.units[(int64_t)first * a.b.nkv + kvh];
-    if (unit.cta < 0 || unit.pieces < 0 || unit.pieces > a.grid - unit.cta) unit.pieces = 0;  // (groups that overlap)
-    // the sum of what there is, each part with its weight 2^(m - M); the own part first
-    float acc[kOwn], M = a.rows_lse[layer + out_row] * 1.4426950408889634f, L = M == -INFINITY ? 0.f : 1.f;
-    auto take = [&](const Vec& v, float* f) {
-      const float* const e = reinterpret_cast<const float*>(&v);
+    for (int d = 0; d < kOwn; ++d) f[d] = e[d];
+  };
+  auto add = [&](const Vec& v, float m, float l) {  // v: the sum of 2^(score - m) V, l of 2^(score - m)
+    if (l == 0.f) return;                           // (no key seen)
+    const float mn = fmaxf(M, m), fa = M == -INFINITY && L == 0.f ? 0.f : exp2f(M - mn), fb = exp2f(m - mn);
+    const float* const e = reinterpret_cast<const float*>(&v);
+    M = mn;
+    L = L * fa + l * fb;
 #pragma unroll
-      for (int d = 0; d < kOwn; ++d) f[d] = e[d];
-    };
-    auto add = [&](const Vec& v, float m, float l) {  // v: the sum of 2^(score - m) V, l of 2^(score - m)
-      if (l == 0.f) return;                           // (no key seen)
-      const float mn = fmaxf(M, m), fa = M == -INFINITY && L == 0.f ? 0.f : exp2f(M - mn), fb = exp2f(m - mn);
-      const float* const e = reinterpret_cast<const float*>(&v);
-      M = mn;
-      L = L * fa + l * fb;
-#pragma unroll
-      for (int d = 0; d < kOwn; ++d) acc[d] = acc[d] * fa + e[d] * fb;
-    };
-    take(__ldcs(reinterpret_cast<const Vec*>(a.rows + (layer + out_row) * D) + lane), acc);
-    if (unit.pieces == 0) {
-      const float z = a.rows_lse[out_row] * 1.4426950408889634f;
-      add(__ldcs(reinterpret_cast<const Vec*>(a.rows + out_row * D) + lane), z, z == -INFINITY ? 0.f : 1.f);
-    }
-#pragma unroll 1
-    for (int q0 = 0; q0 < unit.pieces; q0 += kMergePieces) {
-      float2 ml[kMergePieces];
-      Vec v[kMergePieces];
-#pragma unroll
-      for (int q = 0; q < kMergePieces; ++q) {
-        const int qq = min(q0 + q, unit.pieces - 1);  // past the last piece: the last again, not counted
-        const int64_t tile = (int64_t)(2 * (unit.cta + qq) + (qq == 0 ? 1 : 0)) * 2 + x;
-        ml[q] = pm[tile * 128 + row];
-        // few rows: [row][D]; tiles: [D / 4][128 rows][4], of which neighbouring heads share the sectors
-        v[q] = few ? reinterpret_cast<const Vec*>(a.partials + (tile * 128 + row) * D)[lane]
-                   : *reinterpret_cast<const Vec*>(a.partials + ((tile * (D / 4) + lane * kOwn / 4) * 128 + row) * 4 + lane * kOwn % 4);
-      }
-#pragma unroll
-      for (int q = 0; q < kMergePieces; ++q)
-        if (q0 + q < unit.pieces) add(v[q], ml[q].x, ml[q].y);
-    }
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    uint32_t o[kOwn / 2];
-#pragma unroll
-    for (int d = 0; d < kOwn / 2; ++d) o[d] = Elem<T>::pack(acc[2 * d] * inv, acc[2 * d + 1] * inv);
-    T* const to = reinterpret_cast<T*>(a.out) + t * a.ldo + (int64_t)h * D + lane * kOwn;
-    if constexpr (D == 128)
-      *reinterpret_cast<uint2*>(to) = make_uint2(o[0], o[1]);
-    else
-      *reinterpret_cast<uint32_t*>(to) = o[0];
-    if (lane == 0 && a.lse) a.lse[t * a.ld_lse + h] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
+    for (int d = 0; d < kOwn; ++d) acc[d] = acc[d] * fa + e[d] * fb;
+  };
+  take(__ldcs(reinterpret_cast<const Vec*>(a.rows + (layer + out_row) * D) + lane), acc);
+  if (pieces == 0) {
+    const float z = a.rows_lse[out_row] * 1.4426950408889634f;
+    add(__ldcs(reinterpret_cast<const Vec*>(a.rows + out_row * D) + lane), z, z == -INFINITY ? 0.f : 1.f);
   }
+#pragma unroll 1
+  for (int q0 = 0; q0 < pieces; q0 += kMergePieces) {
+    float2 ml[kMergePieces];
+    Vec v[kMergePieces];
+#pragma unroll
+    for (int q = 0; q < kMergePieces; ++q) {
+      const int qq = min(q0 + q, pieces - 1);  // past the last piece: the last again, not counted
+      const int64_t tile = (int64_t)(2 * (unit.cta + qq) + (qq == 0 ? 1 : 0)) * 2 + x;
+      ml[q] = pm[tile * 128 + row];
+      // few rows: [row][D]; tiles: [D / 4][128 rows][4], of which neighbouring heads share the sectors
+      v[q] = few ? reinterpret_cast<const Vec*>(a.partials + (tile * 128 + row) * D)[lane]
+                 : *reinterpret_cast<const Vec*>(a.partials + ((tile * (D / 4) + lane * kOwn / 4) * 128 + row) * 4 + lane * kOwn % 4);
+    }
+#pragma unroll
+    for (int q = 0; q < kMergePieces; ++q)
+      if (q0 + q < pieces) add(v[q], ml[q].x, ml[q].y);
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  uint32_t o[kOwn / 2];
+#pragma unroll
+  for (int d = 0; d < kOwn / 2; ++d) o[d] = Elem<T>::pack(acc[2 * d] * inv, acc[2 * d + 1] * inv);
+  T* const to = reinterpret_cast<T*>(a.out) + t * a.ldo + (int64_t)h * D + lane * kOwn;
+  if constexpr (D == 128)
+    *reinterpret_cast<uint2*>(to) = make_uint2(o[0], o[1]);
+  else
+    *reinterpret_cast<uint32_t*>(to) = o[0];
+  if (lane == 0 && a.lse) a.lse[t * a.ld_lse + h] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
 }
 
 // After the attention's own scratch: the rows of work, and the two layers.
@@ -249,9 +244,9 @@ extern "C" int qd_prefix_attn(const void* q, int64_t ldq, int dtype, int64_t tok
                                out, ldo, lse, ld_lse, grid, scratch, pdl, stream);
   if (ra != QD_OK || n_groups == 0) return ra;
   const float* const partials = reinterpret_cast<const float*>(base + paged_attn_plan(grid, head_dim).off_partials);
-  PrefixMergeArgs m = {p.b, p.s, p.shared, p.shared + n_groups, units, partials, rows, rows_lse, static_cast<char*>(out),
+  PrefixMergeArgs m = {p.b, p.s, p.shared + n_groups, units, partials, rows, rows_lse, static_cast<char*>(out),
                        lse, ldo, ld_lse, grid};
-  const int64_t warps = tokens * ((nq_heads + kMergeHeads - 1) / kMergeHeads), ctas = (warps + kMergeWarps - 1) / kMergeWarps;
+  const int64_t warps = tokens * nq_heads, ctas = (warps + kMergeWarps - 1) / kMergeWarps;
   if (ctas > INT32_MAX) return set_error(QD_ERR_UNSUPPORTED, "%s: %lld tokens", what, (long long)tokens);
   const bool bf = dtype == QD_BF16;
   const void* fn = head_dim == 128 ? (bf ? (const void*)prefix_merge_kernel<__nv_bfloat16, 128> : (const void*)prefix_merge_kernel<__half, 128>)
