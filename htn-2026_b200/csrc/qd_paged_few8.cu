@@ -110,13 +110,10 @@ __device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint32_t a_lo, uint32_t
 constexpr uint32_t f8_idesc(int n, bool a_mn, bool b_e5m2) {
   return (1u << 4) | ((b_e5m2 ? 1u : 0u) << 10) | ((a_mn ? 1u : 0u) << 15) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
-// N columns of this thread's lane of tensor memory, in steps of 16, waited for
-template <int N>
+// 16 columns of this thread's lane of tensor memory, waited for
 __device__ __forceinline__ void f8_load(uint32_t taddr, uint32_t* r) {
-#pragma unroll
-  for (int i = 0; i < N; i += 16) tmem_ld16_raw(taddr + i, r + i);
-#pragma unroll
-  for (int i = 0; i < N; i += 16) tmem_wait_ld16(r + i);
+  tmem_ld16_raw(taddr, r);
+  tmem_wait_ld16(r);
 }
 constexpr int f8_cols(int n) { return (n + 15) / 16 * 16; }
 // The sums of kC rows' terms, each `step` of the one before it: column c + t kC is row c's term t.
@@ -124,7 +121,7 @@ template <int kC, int kTerms>
 __device__ __forceinline__ void f8_terms(uint32_t taddr, float step, float* v) {
   if constexpr (kC < 16) {  // all in one load
     uint32_t u[16];
-    f8_load<16>(taddr, u);
+    f8_load(taddr, u);
 #pragma unroll
     for (int c = 0; c < kC; ++c) {
       v[c] = __uint_as_float(u[c + (kTerms - 1) * kC]);
@@ -135,7 +132,7 @@ __device__ __forceinline__ void f8_terms(uint32_t taddr, float step, float* v) {
 #pragma unroll
     for (int t = kTerms - 1; t >= 0; --t) {
       uint32_t u[16];
-      f8_load<16>(taddr + t * kC, u);
+      f8_load(taddr + t * kC, u);
 #pragma unroll
       for (int c = 0; c < kC; ++c) v[c] = t == kTerms - 1 ? __uint_as_float(u[c]) : fmaf(v[c], step, __uint_as_float(u[c]));
     }
@@ -712,7 +709,7 @@ __global__ void __launch_bounds__(kF8Threads, kF8Resident) paged_few8_kernel(con
 #pragma unroll 1
             for (int i = 0; i < f8_cols(kC * kTP); i += 16) {
               uint32_t o[16];
-              f8_load<16>(tO + lane_off + i, o);
+              f8_load(tO + lane_off + i, o);
 #pragma unroll
               for (int c = 0; c < 16; ++c)
                 o[c] = __float_as_uint(__uint_as_float(o[c]) * __shfl_sync(0xffffffffu, alpha, c & (kC - 1)));

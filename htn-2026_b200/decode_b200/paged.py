@@ -252,7 +252,7 @@ class PagedAttention8(PagedAttention):
             lse_ptr, ld_lse = lse.data_ptr(), max(ld_lse, nq) if tokens <= 1 else ld_lse
         L.call("qd_paged_attn8", q.data_ptr(), ldq, TYPES[dtype], tokens, nq, self.nkv, D, k_pages.data_ptr(),
                v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pool[0], pool[2], ps[0], ps[1], ss_page, ss_head,
-               cu_tokens.data_ptr(), kv_len.data_ptr(), batch, page_table.data_ptr(), ld_table, max_pages, max_new or 0,
+               cu_tokens.data_ptr(), kv_len.data_ptr(), batch, page_table.data_ptr(), ld_table, max_pages, min(max_new or 0, tokens),
                self.scale if scale is None else scale, out.data_ptr(), ldo, lse_ptr, ld_lse, self.grid,
                self.scratch.data_ptr(), self.scratch_bytes, None if err is None else err.data_ptr(), pdl, _raw_stream(dev))
         return out

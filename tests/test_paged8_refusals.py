@@ -134,3 +134,17 @@ def test_new_pools8_and_what_they_hold():
     for dtype in (torch.float32, torch.bfloat16, torch.float16):
         x = paged.held_values(k, ks, dtype)
         assert x.dtype == dtype and float(x[0, 0, 0, 0]) == 57344.0 and float(x[0, 0, 1, 0]) == 2.0 ** -24
+
+
+def test_max_new_does_not_wrap(caller, monkeypatch):
+    """A bound larger than 32 bits is no bound, and not a small one."""
+    from decode_b200 import paged
+
+    run, _ = caller
+    seen = []
+    monkeypatch.setattr(paged.L, "call", lambda name, *a: seen.append(a))
+    for given in (None, 0, 1, 5, 2 ** 32 + 1):
+        t = _stands()["attn"]
+        t["max_new"] = given
+        run("attn", t)
+    assert [a[23] for a in seen] == [0, 0, 1, 5, 5], "never more than the call's tokens"
