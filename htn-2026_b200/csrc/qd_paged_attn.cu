@@ -84,6 +84,9 @@ constexpr int kPgManyUnits = 1 << 20;  // above any grid (whose scratch would be
 // keys (64 units of 16 blocks): 95 us whole, with the single tokens on the SMs that have none, 129 cut; the chunks alone 67
 // and 90; with 40 places for 60 chunks after up to 3 k keys are cut, 153 us, 121 whole.
 constexpr int kPgHeldJoin = 60;
+// A unit of U places in p pieces takes U / p places and, at the CTA that joins them, about 8 places a piece: shortest with
+// sqrt(8 U) places a piece (34 tokens after 4 k keys, 1 KV head: 57 us, 77 with 12).
+constexpr float kPgHeldPiece = 8.f;
 constexpr int kPgHeldBias = 7;  // pages of 8 bits: P' = 2^7 P
 constexpr int kPgWhole = 8;   // key blocks up to which units of tiles are left whole, when there are CTAs for all
 
@@ -449,7 +452,10 @@ __global__ void __launch_bounds__(pg_threads(kHeld), 1) paged_attn_kernel(const 
   // With little work the first CTAs take kPgPiece places each (a block, if all units have few rows), the rest
   // nothing: joining the pieces of a tile of 128 rows costs about as much as some blocks of keys. No CTA takes
   // less than a block, so that every one between the first and the last of a cut unit has some of it.
-  const PgLine line = pg_line(total, (int)gridDim.x, whole ? 1 : tiles ? kPgPiece : kPgBlockCost);
+  int least = whole ? 1 : tiles ? kPgPiece : kPgBlockCost;
+  if constexpr (kHeld)
+    if (!whole) least = max(least, (int)sqrtf(kPgHeldPiece * longest));
+  const PgLine line = pg_line(total, (int)gridDim.x, least);
   const int cta = blockIdx.x;
   const int64_t begin = cta < line.ctas ? line.begin(cta) : 0, end = cta < line.ctas ? line.begin(cta + 1) : 0;
   if (begin < end && begin >= before && begin < before + mine) {

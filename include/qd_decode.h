@@ -511,7 +511,8 @@ int qd_paged_rope_append8(const void* qkv, int64_t ldqkv, int dtype, int64_t tok
 /* qd_paged_attn8 is qd_paged_attn over such pages: q and out are of `dtype`, scores, softmax statistics and sums fp32.
  * max_new > 0 says that no request has more new tokens than this (a step of single tokens: 1), which saves a launch
  * for requests of more; the rows of one that has more all the same may be left as they were, with QD_DEVERR_POS
- * flagged. A row that sees a code of NaN in a K row, or whose request has one in a V row that it sees, has NaN there.
+ * flagged. A row that sees a code of NaN in a K row is NaN, and so is its lse; one in a V row is NaN in its dim of the rows
+ * that see it, and may reach the rows before it in the same chunk (0 x NaN), as what is not finite does in 16 bits.
  * Grid and scratch as for qd_paged_attn (qd_paged_attn8_plan), of which the first 16 * grid bytes are what is zeroed again
  * after a call that ended early. */
 int qd_paged_attn8_plan(int nq_heads, int nkv_heads, int head_dim, int grid_hint, int* grid, int64_t* scratch_bytes);
