@@ -254,7 +254,9 @@ __global__ void __launch_bounds__(kF8Threads, kF8Resident) paged_few8_kernel(con
     for (int m = 1; m < 16; ++m) misc[m] = 0;
   }
   if (warp == 5) tmem_alloc(smem_u32(misc), 256);
-  // (the kernel before it waited for what came before both)
+  // Beside the tiles' kernel nothing is waited for here: its CTAs had all waited for what came before both when they let
+  // this one start, so those writes are in L2. What lies in an SM's L1 may be older (the queries of the call before, in
+  // the same buffer), so all that is read ahead of the wait at the end bypasses L1: ld.cg, and copies, which do.
   if (!a.beside) grid_dep_wait();
   {  // the page table on its way to L2 while the lengths are read: a line per thread of the grid
     const int lines = (a.b.max_pages + 31) / 32;
@@ -569,7 +571,7 @@ __global__ void __launch_bounds__(kF8Threads, kF8Resident) paged_few8_kernel(con
         for (int y = 0; y < kAhead; ++y) {
           const int c = min(c0 + y * kAt + lane / kLanes, rows - 1);  // (past the last row: that one again)
           const int tok = (c * a.inv_group) >> 16, hq = g.head * a.s.group + c - tok * a.s.group;
-          u[y] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + (g.row0 + tok) * a.ldq + (int64_t)hq * D + 8 * sub);
+          u[y] = __ldcg(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + (g.row0 + tok) * a.ldq + (int64_t)hq * D + 8 * sub));
         }
 #pragma unroll
         for (int y = 0; y < kAhead; ++y) {
