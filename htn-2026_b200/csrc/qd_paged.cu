@@ -183,8 +183,9 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendResident) paged_append_
       };
       float most = largest();
       if (__any_sync(0xffffffffu, most > FLT_MAX)) {  // infinities are held as NaN, and are not what a row is measured by
+        const float top = h < a.b.nq ? INFINITY : FLT_MAX;  // (queries are not held, and keep theirs)
 #pragma unroll
-        for (int k = 0; k < 16; ++k) x[k] = fabsf(x[k]) <= FLT_MAX ? x[k] : __uint_as_float(0x7fffffffu);
+        for (int k = 0; k < 16; ++k) x[k] = fabsf(x[k]) <= top ? x[k] : __uint_as_float(0x7fffffffu);
         most = largest();
       }
       if (h >= heads || !dst) continue;
