@@ -54,16 +54,19 @@ __global__ void __launch_bounds__(kPlanThreads) prefix_plan_kernel(const __grid_
   for (int g = warp; g < a.n_groups; g += kPlanThreads / 32) {
     const int lo = min(max(ld_i32(a.cu_groups + g), 0), batch), hi = min(max(ld_i32(a.cu_groups + g + 1), lo), batch);
     int least = INT32_MAX, some = 0, first = INT32_MAX, last = 0;  // first new position; requests with tokens; token rows
+    int reader = INT32_MAX;  // the first request with tokens: a row of the page table without any may hold anything
     int64_t apart = 0;  // places of a block of common keys, if each request reads it
     for (int i = lo + lane; i < hi; i += 32) {
       const PgReq r = request(i);
       if (r.n == 0) continue;
+      reader = min(reader, i);
       least = min(least, r.pos0);
       first = min(first, r.row0);
       last = max(last, r.row0 + r.n);
       apart += block_weight(a.s, r.n);
       ++some;
     }
+    reader = __reduce_min_sync(0xffffffffu, reader);
     least = __reduce_min_sync(0xffffffffu, least);
     first = __reduce_min_sync(0xffffffffu, first);
     last = __reduce_max_sync(0xffffffffu, last);
@@ -79,7 +82,7 @@ __global__ void __launch_bounds__(kPlanThreads) prefix_plan_kernel(const __grid_
     const int pairs = (n + 2 * a.s.tpt - 1) / (2 * a.s.tpt);
     if (blocks * (apart - block_weight(a.s, n)) <= 2 * kPgUnitCost * (int64_t)pairs) blocks = 0;
     if (lane == 0)
-      a.shared[g] = blocks ? PgShared{first, n, blocks * kPgKeys - 1, blocks * kPgKeys, 0, lo, 0, 0} : PgShared{};
+      a.shared[g] = blocks ? PgShared{first, n, blocks * kPgKeys - 1, blocks * kPgKeys, 0, reader, 0, 0} : PgShared{};
     if (blocks)
       for (int i = lo + lane; i < hi; i += 32)
         if (request(i).n > 0) {

@@ -471,11 +471,11 @@ int qd_paged_attn(const void* q, int64_t ldq, int dtype, int64_t tokens, int nq_
 
 /* qd_prefix_attn is qd_paged_attn for requests that begin alike in groups: requests cu_groups[g] ..
  * cu_groups[g + 1] - 1 (device int32 [n_groups + 1], ascending; requests outside any group stand alone) have their first
- * prefix_len[g] positions in the same pages, which every one of their page table rows names (device int32 [n_groups]; the
- * caller's promise: they are read through the first request's row). The results are qd_paged_attn's, up to the order of
- * the fp32 sums; those positions are read once for all of the group's tokens instead of once per request. Read once are
- * whole blocks of 128 positions that lie before every new token of the group, where that saves more than it costs; the
- * rest is read as by qd_paged_attn. Pools are of 16 bits. qd_prefix_attn_plan gives the grid and the size of the scratch
+ * prefix_len[g] positions in the same pages, which the page table rows of those that have new tokens name (device int32
+ * [n_groups]; the caller's promise: they are read through the first of these rows). The results are qd_paged_attn's, up
+ * to the order of the fp32 sums; those positions are read once for all of the group's tokens instead of once per request.
+ * Read once are whole blocks of 128 positions that lie before every new token of the group, where that saves more than it
+ * costs; the rest is read as by qd_paged_attn. Pools are of 16 bits. qd_prefix_attn_plan gives the grid and the size of the scratch
  * (32-byte aligned) for calls of up to max_tokens tokens and max_requests requests; it is to be zero before its first
  * call, and after one that ended early, as for qd_paged_attn. */
 int qd_prefix_attn_plan(int nq_heads, int nkv_heads, int head_dim, int64_t max_tokens, int max_requests, int grid_hint,
