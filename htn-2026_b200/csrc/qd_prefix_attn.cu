@@ -232,6 +232,9 @@ extern "C" int qd_prefix_attn(const void* q, int64_t ldq, int dtype, int64_t tok
     return set_error(QD_ERR_SCRATCH, "%s: grid %d, %lld tokens, %d requests and %d groups need %lld B of 32-byte aligned scratch (have %lld)",
                      what, grid, (long long)tokens, batch, n_groups, (long long)plan.bytes, (long long)scratch_bytes);
   if (tokens == 0) return QD_OK;
+  const int64_t merge_ctas = (tokens * nq_heads + kMergeWarps - 1) / kMergeWarps;
+  if (merge_ctas > INT32_MAX || (int64_t)batch + n_groups > INT32_MAX)
+    return set_error(QD_ERR_UNSUPPORTED, "%s: %lld tokens, %d requests and %d groups", what, (long long)tokens, batch, n_groups);
   char* const base = static_cast<char*>(scratch);
   p.s = pg_shape(nq_heads, nkv_heads);
   p.cu_groups = cu_groups;
@@ -249,10 +252,8 @@ extern "C" int qd_prefix_attn(const void* q, int64_t ldq, int dtype, int64_t tok
   const float* const partials = reinterpret_cast<const float*>(base + paged_attn_plan(grid, head_dim).off_partials);
   PrefixMergeArgs m = {p.b, p.s, p.shared + n_groups, units, partials, rows, rows_lse, static_cast<char*>(out),
                        lse, ldo, ld_lse, grid};
-  const int64_t warps = tokens * nq_heads, ctas = (warps + kMergeWarps - 1) / kMergeWarps;
-  if (ctas > INT32_MAX) return set_error(QD_ERR_UNSUPPORTED, "%s: %lld tokens", what, (long long)tokens);
   const bool bf = dtype == QD_BF16;
   const void* fn = head_dim == 128 ? (bf ? (const void*)prefix_merge_kernel<__nv_bfloat16, 128> : (const void*)prefix_merge_kernel<__half, 128>)
                                    : (bf ? (const void*)prefix_merge_kernel<__nv_bfloat16, 64> : (const void*)prefix_merge_kernel<__half, 64>);
-  return launch_kernel(fn, dim3((unsigned)ctas), dim3(kMergeWarps * 32), 0, pdl, stream, &m);
+  return launch_kernel(fn, dim3((unsigned)merge_ctas), dim3(kMergeWarps * 32), 0, pdl, stream, &m);
 }
