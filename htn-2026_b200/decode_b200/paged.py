@@ -203,14 +203,14 @@ class PrefixAttention(PagedAttention):
     def __call__(self, q, k_pages, v_pages, cu_tokens, kv_len, page_table, cu_groups, prefix_len, out, lse=None,
                  scale: float | None = None, err=None, pdl: bool = True):
         """As PagedAttention's. Requests cu_groups[g] .. cu_groups[g + 1] - 1 have their first prefix_len[g] positions in
-        the same pages (int32 [groups + 1] and [groups], on the device)."""
+        the same pages, which the table rows of those with new tokens name (int32 [groups + 1] and [groups], on the device)."""
         nq, D, dtype, dev = self.nq, self.head_dim, self.dtype, q.get_device()
         pool, ps, batch, ld_table, max_pages = _check_batch(dev, dtype, k_pages, v_pages, cu_tokens, kv_len, page_table, err)
         tokens, groups = q.shape[0], prefix_len.shape[0]
         assert q.dtype is dtype and out.dtype is dtype and out.get_device() == dev and self.scratch.get_device() == dev
         assert pool[1] == self.nkv and pool[3] == D
         assert cu_groups.dtype is I32 and cu_groups.get_device() == dev and cu_groups.shape == (groups + 1,) and cu_groups.is_contiguous()
-        assert prefix_len.dtype is I32 and prefix_len.get_device() == dev and prefix_len.is_contiguous()
+        assert prefix_len.dtype is I32 and prefix_len.get_device() == dev and prefix_len.numel() == groups and prefix_len.is_contiguous()
         ldq, ldo = _rows(q, tokens, nq, D), _rows(out, tokens, nq, D)
         lse_ptr, ld_lse = None, 0
         if lse is not None:
