@@ -50,15 +50,16 @@ __device__ __forceinline__ uint32_t held_pair(float a, float b, float inv) {
 }
 
 constexpr int kAppendThreads = 128;
-// CTAs an SM, which is 72 registers a thread: 16-bit pages need no more, and into 8-bit pages 13,808 tokens take 83 us,
-// where 96 registers without a spill take 102 (a warp waits for its loads most of the time)
+// CTAs an SM, which is 72 registers a thread: 16-bit pages need no more, and into 8-bit pages 14,771 tokens take 83 to 88
+// us, where 96 registers without a spill take 102 (a warp waits for its loads most of the time). In twos the 8-bit
+// instances spill: 96 bytes stored and 132 loaded in the code of a BF16 thread, 108 and 176 in FP16's
 constexpr int kAppendResident = 7;
 
 // kUnits: groups of heads of one token that a warp takes, all their loads in flight before the first is used.
-// 13,808 prompt tokens of 48 heads of 128 take 71 us, 5.1 TB/s over the 364 MB that have to move (a copy
+// 14,771 prompt tokens of 48 heads of 128 take 69 to 73 us, 5.0 to 5.2 TB/s over the 364 MB that have to move (a copy
 // reaches 6.5); 64 single tokens 3.0 us and one 2.2 us in a graph, of which the launch is most (a call takes the
-// host 11.8). Into 8-bit pages the prompts take 83 us (4.0 TB/s over 334 MB): the rows' maxima and codes add a third to
-// the instructions, and there are 28 warps an SM to wait for loads.
+// host 11.8). Into 8-bit pages the prompts take 83 to 88 us (3.8 to 4.0 TB/s over 334 MB): the rows' maxima and codes add
+// a third to the instructions, and there are 28 warps an SM to wait for loads.
 template <typename T, int D, int kUnits, bool kHeld>
 __global__ void __launch_bounds__(kAppendThreads, kAppendResident) paged_append_kernel(const __grid_constant__ AppendArgs a) {
   constexpr int kLanes = D / 16, kHeads = 32 / kLanes;  // lanes per head, heads per unit
@@ -310,7 +311,7 @@ static int launch_append(const char* what, const void* qkv, int64_t ldqkv, int d
   a.rot_half = rot_half;
   a.eps = eps;
   // Two groups of heads a warp once there are warps enough to fill the SMs without: 64 tokens of 48 heads (768
-  // groups of 4) take 3.0 us one by one and 3.3 in twos, 256 tokens 6.7 and 4.2, 13,808 tokens 85 and 71.
+  // groups of 4) take 3.0 us one by one and 3.3 in twos, 256 tokens 6.7 and 4.2, 14,771 tokens 85 and 71.
   const int group = 512 / head_dim;
   const bool two = tokens * ((heads + group - 1) / group) > 2048;
   const int per = (heads + group * (two ? 2 : 1) - 1) / (group * (two ? 2 : 1));

@@ -52,8 +52,9 @@
 // graph, 14.5 with the keys not in L2 (latency; a call takes the host 11.9); 2048 tokens after 8192 keys 340 to 368 us
 // (0.50 to 0.54 of the BF16 peak: a pair's block of 128 keys takes some 4000 cycles, 2048 of them products, since each
 // tile's softmax and products wait for one another). Heads of 64 in FP16, 14 over 2: the 64 single tokens 33 us, the 8
-// long ones 51. At 168 registers a thread the instances spill: 168 bytes stored and 456 loaded in the code of a
-// thread with heads of 128 (156 and 428 with pages of 16 rows), 120 and 356 with heads of 64.
+// long ones 51. At 168 registers a thread the instances spill: 188 bytes stored and 436 loaded in the code of a
+// thread with heads of 128 (176 and 416 with pages of 16 rows), 144 and 288 with heads of 64; those of shared beginnings
+// 256 and 648 (244 and 620), 220 and 580; those of 8-bit pages, at 128 registers, 232 to 248 and 396 to 428.
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -80,9 +81,10 @@ constexpr int kPgBox = 128 * 128;  // [128 rows][64 dims] of 16 bits
 constexpr int kFewP = 2 * kFewRows * 128;  // its P: 2 halves of 64 keys x 16 rows of 128 B
 constexpr int kPgManyUnits = 1 << 20;  // above any grid (whose scratch would be 280 GB); 384 of them fit 32 bits
 // Pages of 8 bits: units are left whole if the longest takes no more than the SMs' even share of all work, the other
-// kernel's too, and this, about what storing and joining pieces takes. 30 single tokens and 2 chunks of 251 after up to 2 k
-// keys (64 units of 16 blocks): 95 us whole, with the single tokens on the SMs that have none, 129 cut; the chunks alone 67
-// and 90; with 40 places for 60 chunks after up to 3 k keys are cut, 153 us, 121 whole.
+// kernel's too, and this. 30 single tokens and 2 chunks of 251 after up to 2 k keys (64 units of 16 blocks): 95 us whole,
+// 129 cut; the chunks alone 67 and 90; with 40 places for 60 chunks after up to 3 k keys are cut, 153 us, 121 whole. (Beside
+// single tokens these times hold more than what storing and joining pieces takes: the kernel for few rows starts its first
+// CTAs on the SMs that have no unit, the others when this one has ended.)
 constexpr int kPgHeldJoin = 60;
 // A unit of U places in p pieces takes U / p places and, at the CTA that joins them, about 8 places a piece: shortest with
 // sqrt(8 U) places a piece (34 tokens after 4 k keys, 1 KV head: 57 us, 77 with 12).

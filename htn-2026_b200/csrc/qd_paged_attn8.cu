@@ -2,8 +2,9 @@
 // at most 16 query rows a KV head (single tokens) run in qd_paged_few8.cu, the others in tiles of 128 rows in
 // qd_paged_attn.cu. Two launches, since what bounds them differs (the memory, and the tensor cores with the softmax) and
 // with it all of their shared memory and warps. The second does not wait for the first, which waits for what came before
-// both, but for its end: it fills the SMs that the first leaves. A caller that knows that there are no longer requests
-// saves a launch.
+// both, but for its end: its first CTAs run on the SMs that the first leaves, and keep them until the first has ended, so
+// the rest of them, which find no room, come after it. A caller that knows that there are no longer requests saves a
+// launch.
 #include "qd_paged_attn8.h"
 
 using namespace qd;

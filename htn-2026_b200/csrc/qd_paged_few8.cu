@@ -23,10 +23,10 @@
 // scores of the next two blocks are always under way, across the units too. Pieces of a cut unit are left in the scratch
 // and joined in the order of their keys by the CTA that ends last.
 //
-// Measured, 32 query and 8 KV heads of 128 in BF16: 8 single tokens over up to 41 k keys 94 us (6.2 TB/s, 0.95 of a copy's
-// rate); 64 over 1 to 1.5 k keys 39.6 us (4.3 TB/s: start 4 us, unit ends and the pieces' joins 2 us each); one over 1 k keys
-// 11.0 us in a graph. A block of 128 keys takes a CTA 0.8 us when its data is there, of which S, the maxima, P and the
-// barriers between are a quarter each; two CTAs need one every 1.5 us.
+// Measured, 32 query and 8 KV heads of 128 in BF16: 8 single tokens over up to 41 k keys 94 to 98 us (6.0 to 6.2 TB/s,
+// 0.92 to 0.95 of a copy's rate); 64 over 1 to 1.5 k keys 40 us (4.3 TB/s: start 4 us, unit ends and the pieces' joins 2 us
+// each); one over 1 k keys 11.0 us in a graph. A block of 128 keys takes a CTA 0.8 us when its data is there, of which S, the
+// maxima, P and the barriers between are a quarter each; two CTAs need one every 1.5 us.
 #include <cuda_fp8.h>
 
 #include <algorithm>

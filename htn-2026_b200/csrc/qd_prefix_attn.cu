@@ -11,9 +11,9 @@
 //          all, and both kinds of work fill the SMs together. The results go to fp32 rows, two layers of them, as a second
 //          rounding to 16 bits would cost as much as the last.
 //   merge  joins the layers' rows and the pieces that units of common keys were cut into, a warp per token and head.
-// Measured, 32 query and 8 KV heads of 128: 64 users, 4 k common and up to 1 k own keys each, 81 us, of which the plan is 3.5
-// and the merge some 3 (dependent loads); 4 documents of 16 k keys with 4 answers each 76 us. The floors are 36 and 38; the rest
-// is what the attention kernel loses on short units.
+// Measured, 32 query and 8 KV heads of 128: 64 users, 4 k common and up to 1 k own keys each, 78 to 84 us, of which the
+// plan is 3.5 and the merge some 3 (dependent loads); 4 documents of 16 k keys with 4 answers each 76 to 79 us. The floors
+// are 36 and 38; the rest is what the attention kernel loses on short units.
 // A group is taken apart again (its requests read all keys, straight to out) where sharing would not pay: see the plan.
 #include "qd_host.h"
 #include "qd_paged_attn8.h"

@@ -144,7 +144,7 @@ QD_OK, QD_ERR_ARG, QD_ERR_SCRATCH, QD_ERR_CUDA, QD_ERR_UNSUPPORTED = 0, 1, 2, 3,
 QD_EPI_STORE, QD_EPI_RES, QD_EPI_SWIGLU, QD_EPI_SWIGLU_PACKED, QD_EPI_RES_SUMS, QD_EPI_STORE_SUMS = 0, 1, 2, 3, 4, 5
 DEVERR = {1: "wait for a weight block timed out", 2: "wait for a free ring slot timed out",
           4: "drain of in-flight copies timed out", 8: "token id out of range",
-          16: "decode position outside the cache", 32: "a wait for another CTA's results timed out",
+          16: "decode position outside the cache, or a request of more new tokens than max_new", 32: "a wait for another CTA's results timed out",
           64: "dynamic shared memory misaligned (kernel did nothing)",
           128: "page outside the pool, or a request longer than its page table row"}
 QD_BF16, QD_FP16, QD_FP32 = 0, 1, 2
